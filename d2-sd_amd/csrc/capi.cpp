@@ -1138,4 +1138,271 @@ int d2sd_paged_kv_append(const d2sd_kv_append_args* a, d2sd_stream_t stream) {
   return e == hipSuccess ? D2SD_OK : fail_hip(e, "paged_kv_append launch");
 }
 
+// Rotary embedding of queries and keys at their positions.
+int d2sd_rotary_embedding(const d2sd_rotary_args* a, d2sd_stream_t stream) {
+  g_last_error.clear();
+  if (!a) return fail(D2SD_ERR_INVALID_ARG, "rotary_embedding: null args");
+  if (a->num_tokens < 0 || a->num_qo_heads < 0 || a->num_kv_heads < 0)
+    return fail(D2SD_ERR_INVALID_ARG, "rotary_embedding: negative count");
+  if (a->head_dim <= 0 || a->head_dim % 2 != 0 || a->head_dim > 2 * d2sd::kRotaryMaxPairs)
+    return fail(D2SD_ERR_UNSUPPORTED, "rotary_embedding: head_dim must be even and at most 256");
+  if (a->num_pairs < 1 || 2 * a->num_pairs > a->head_dim)
+    return fail(D2SD_ERR_INVALID_ARG, "rotary_embedding: 2 * num_pairs must be in [2, head_dim]");
+  if (a->num_tokens == 0 || a->num_qo_heads + a->num_kv_heads == 0) return D2SD_OK;
+  if (!a->positions || !a->inv_freq || (a->num_qo_heads > 0 && (!a->q || !a->q_out)) ||
+      (a->num_kv_heads > 0 && (!a->k || !a->k_out)))
+    return fail(D2SD_ERR_INVALID_ARG, "rotary_embedding: null pointer");
+  if (!std::isfinite(a->scale)) return fail(D2SD_ERR_INVALID_ARG, "rotary_embedding: scale must be finite");
+  const bool q_in = a->q == a->q_out, k_in = a->k == a->k_out;
+  if ((q_in && (a->q_stride_n != a->qo_stride_n || a->q_stride_h != a->qo_stride_h)) ||
+      (k_in && (a->k_stride_n != a->ko_stride_n || a->k_stride_h != a->ko_stride_h)))
+    return fail(D2SD_ERR_INVALID_ARG, "rotary_embedding: in place needs the same strides");
+  d2sd::RotaryParams p{};
+  p.q = a->q;
+  p.k = a->k;
+  p.q_out = a->q_out;
+  p.k_out = a->k_out;
+  p.q_stride_n = a->q_stride_n;
+  p.q_stride_h = a->q_stride_h;
+  p.k_stride_n = a->k_stride_n;
+  p.k_stride_h = a->k_stride_h;
+  p.qo_stride_n = a->qo_stride_n;
+  p.qo_stride_h = a->qo_stride_h;
+  p.ko_stride_n = a->ko_stride_n;
+  p.ko_stride_h = a->ko_stride_h;
+  p.positions = a->positions;
+  p.inv_freq = a->inv_freq;
+  p.scale = a->scale;
+  p.num_tokens = a->num_tokens;
+  p.num_qo_heads = a->num_qo_heads;
+  p.num_kv_heads = a->num_kv_heads;
+  p.head_dim = a->head_dim;
+  p.pairs = a->num_pairs;
+  p.pos64 = a->positions_64 ? 1 : 0;
+  p.inverse = a->inverse ? 1 : 0;
+  p.copy_rest = (a->num_qo_heads > 0 && !q_in) || (a->num_kv_heads > 0 && !k_in);
+  hipError_t e = d2sd::launch_rotary(p, a->interleaved != 0, (hipStream_t)stream);
+  return e == hipSuccess ? D2SD_OK : fail_hip(e, "rotary_embedding launch");
+}
+
+namespace {
+
+// log2 of a power of two, or -1
+int log2_of(int n) {
+  int lg = 0;
+  while (lg < 30 && (1 << lg) < n) ++lg;
+  return n > 0 && (1 << lg) == n ? lg : -1;
+}
+
+int check_cache(const d2sd_paged_cache& c, const char* who) {
+  const std::string at = std::string(who) + ": ";
+  if (c.format < D2SD_CACHE_BF16 || c.format > D2SD_CACHE_MXFP4)
+    return fail(D2SD_ERR_INVALID_ARG, at + "unknown cache format");
+  if (c.num_pages <= 0 || c.num_kv_heads <= 0)
+    return fail(D2SD_ERR_INVALID_ARG, at + "num_pages and num_kv_heads must be positive");
+  if (log2_of(c.page_size) < 0) return fail(D2SD_ERR_INVALID_ARG, at + "page_size must be a power of two");
+  if (c.head_dim <= 0 || c.head_dim % 32 != 0 || c.head_dim > 256)
+    return fail(D2SD_ERR_UNSUPPORTED, at + "head_dim must be a multiple of 32 up to 256");
+  if (!c.k || !c.v) return fail(D2SD_ERR_INVALID_ARG, at + "null pool");
+  if (c.format != D2SD_CACHE_BF16 && (!c.k_scale || !c.v_scale))
+    return fail(D2SD_ERR_INVALID_ARG, at + "quantised caches need k_scale and v_scale");
+  const int64_t unit = c.format == D2SD_CACHE_BF16 ? 8 : 16;  // elements of 16 bytes
+  for (int64_t st : {c.stride_page, c.stride_head, c.stride_tok})
+    if (st < 0 || st % unit != 0)
+      return fail(D2SD_ERR_INVALID_ARG, at + "cache strides must be multiples of 16 bytes");
+  if (!aligned16(c.k) || !aligned16(c.v)) return fail(D2SD_ERR_INVALID_ARG, at + "pools must be 16-byte aligned");
+  if (c.format >= D2SD_CACHE_MXFP8)
+    for (int64_t st : {c.scale_stride_page, c.scale_stride_head, c.scale_stride_tok})
+      if (st < 0) return fail(D2SD_ERR_INVALID_ARG, at + "scale strides must not be negative");
+  return D2SD_OK;
+}
+
+int cache_params(const d2sd_cache_io_args* a, const char* who, d2sd::CacheParams& p) {
+  if (!a) return fail(D2SD_ERR_INVALID_ARG, std::string(who) + ": null args");
+  if (int rc = check_cache(a->cache, who)) return rc;
+  const std::string at = std::string(who) + ": ";
+  if (a->num_items < 0) return fail(D2SD_ERR_INVALID_ARG, at + "negative count");
+  if (a->num_items > 0 && (!a->items || !a->kv_len || !a->page_table || !a->k || !a->v))
+    return fail(D2SD_ERR_INVALID_ARG, at + "null pointer");
+  if (!aligned16(a->k) || !aligned16(a->v) || !aligned16(a->items))
+    return fail(D2SD_ERR_INVALID_ARG, at + "k, v and items must be 16-byte aligned");
+  if (!stride_ok(a->stride_n) || !stride_ok(a->stride_h) || a->stride_n < 0 || a->stride_h < 0)
+    return fail(D2SD_ERR_INVALID_ARG, at + "strides must be multiples of 8 elements");
+  const d2sd_paged_cache& c = a->cache;
+  p = d2sd::CacheParams{};
+  p.items = a->items;
+  p.kv_len = a->kv_len;
+  p.page_table = a->page_table;
+  p.k = a->k;
+  p.v = a->v;
+  p.stride_n = a->stride_n;
+  p.stride_h = a->stride_h;
+  p.ks = {c.k, c.k_scale};
+  p.vs = {c.v, c.v_scale};
+  p.stride_page = c.stride_page;
+  p.stride_head = c.stride_head;
+  p.stride_tok = c.stride_tok;
+  p.scale_stride_page = c.scale_stride_page;
+  p.scale_stride_head = c.scale_stride_head;
+  p.scale_stride_tok = c.scale_stride_tok;
+  p.num_items = a->num_items;
+  p.num_kv_heads = c.num_kv_heads;
+  p.head_dim = c.head_dim;
+  p.log2_page = log2_of(c.page_size);
+  p.num_pages = c.num_pages;
+  return D2SD_OK;
+}
+
+}  // namespace
+
+int d2sd_cache_write(const d2sd_cache_io_args* a, d2sd_stream_t stream) {
+  g_last_error.clear();
+  d2sd::CacheParams p;
+  if (int rc = cache_params(a, "cache_write", p)) return rc;
+  hipError_t e = d2sd::launch_cache_write(p, a->cache.format, (hipStream_t)stream);
+  return e == hipSuccess ? D2SD_OK : fail_hip(e, "cache_write launch");
+}
+
+int d2sd_cache_read(const d2sd_cache_io_args* a, d2sd_stream_t stream) {
+  g_last_error.clear();
+  d2sd::CacheParams p;
+  if (int rc = cache_params(a, "cache_read", p)) return rc;
+  hipError_t e = d2sd::launch_cache_read(p, a->cache.format, (hipStream_t)stream);
+  return e == hipSuccess ? D2SD_OK : fail_hip(e, "cache_read launch");
+}
+
+int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t host_plan_ints,
+                    d2sd_chunk_plan_info* info) {
+  g_last_error.clear();
+  try {
+    if (!d || !info) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: null argument");
+    *info = d2sd_chunk_plan_info{};
+    if (d->num_reqs < 0) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: negative num_reqs");
+    if (d->num_reqs > 0 && (!d->qo_indptr || !d->kv_len || !d->page_indptr))
+      return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: null pointer");
+    if (d->head_dim != 64 && d->head_dim != 128)
+      return fail(D2SD_ERR_UNSUPPORTED, "chunk_plan: head_dim must be 64 or 128");
+    if (d->num_kv_heads <= 0 || d->num_qo_heads <= 0 || d->num_qo_heads % d->num_kv_heads != 0)
+      return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: num_qo_heads must be a positive multiple of num_kv_heads");
+    if (d->format < D2SD_CACHE_BF16 || d->format > D2SD_CACHE_MXFP4)
+      return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: unknown cache format");
+    const int lg = log2_of(d->page_size);
+    if (lg < 0) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: page_size must be a power of two");
+    if (d->window_left < -1) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: window_left must be >= -1");
+    if (d->max_splits < 0 || d->num_cus < 0) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: negative count");
+    const int group = d->num_qo_heads / d->num_kv_heads;
+    if (d->num_reqs > 0 && (d->qo_indptr[0] != 0 || d->page_indptr[0] < 0))
+      return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: qo_indptr starts at 0, page_indptr at 0 or above");
+    for (int r = 0; r < d->num_reqs; ++r) {
+      const int64_t n = (int64_t)d->qo_indptr[r + 1] - d->qo_indptr[r];
+      const int64_t pages = (int64_t)d->page_indptr[r + 1] - d->page_indptr[r];
+      if (n < 0 || pages < 0 || d->kv_len[r] < 0)
+        return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: indptrs must not decrease, lengths must not be negative");
+      if (d->kv_len[r] > (pages << lg))
+        return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: request " + std::to_string(r) + " has no pages for its cache");
+      if ((pages << lg) > (int64_t)INT32_MAX - 64 || n * group > (int64_t)INT32_MAX)
+        return fail(D2SD_ERR_UNSUPPORTED, "chunk_plan: request " + std::to_string(r) + " is too long");
+    }
+    d2sd::ChunkPlanInput in{};
+    in.num_reqs = d->num_reqs;
+    in.qo_indptr = d->qo_indptr;
+    in.kv_len = d->kv_len;
+    in.page_indptr = d->page_indptr;
+    in.num_qo_heads = d->num_qo_heads;
+    in.num_kv_heads = d->num_kv_heads;
+    in.head_dim = d->head_dim;
+    in.format = d->format;
+    in.window_left = d->window_left;
+    in.num_cus = d->num_cus > 0 ? d->num_cus : device_num_cus();
+    in.max_splits = d->max_splits;
+    d2sd::ChunkPlanOutput out;
+    d2sd::plan_chunk(in, out);
+    constexpr size_t item_ints = sizeof(d2sd::ChunkItem) / 4, merge_ints = sizeof(d2sd::ChunkMerge) / 4;
+    const size_t ints = out.items.size() * item_ints + out.merges.size() * merge_ints;
+    if (ints > (size_t)INT32_MAX || out.partial_rows > (long long)INT32_MAX)
+      return fail(D2SD_ERR_UNSUPPORTED, "chunk_plan: the batch is too large for one plan");
+    info->num_items = (int)out.items.size();
+    info->num_merges = (int)out.merges.size();
+    info->plan_ints = (int)ints;
+    info->total_q = d->num_reqs > 0 ? d->qo_indptr[d->num_reqs] : 0;
+    info->num_reqs = d->num_reqs;
+    info->num_qo_heads = d->num_qo_heads;
+    info->num_kv_heads = d->num_kv_heads;
+    info->head_dim = d->head_dim;
+    info->format = d->format;
+    info->page_size = d->page_size;
+    info->window_left = d->window_left;
+    info->num_page_entries = d->num_reqs > 0 ? d->page_indptr[d->num_reqs] : 0;
+    info->workspace_bytes = (size_t)out.partial_rows * (d->head_dim + 1) * sizeof(float);
+    if (!host_plan) return D2SD_OK;
+    if (host_plan_ints < ints)
+      return fail(D2SD_ERR_WORKSPACE, "chunk_plan: host_plan too small (need " + std::to_string(ints) + " ints)");
+    if (!out.items.empty()) std::memcpy(host_plan, out.items.data(), out.items.size() * sizeof(d2sd::ChunkItem));
+    if (!out.merges.empty())
+      std::memcpy(host_plan + out.items.size() * item_ints, out.merges.data(),
+                  out.merges.size() * sizeof(d2sd::ChunkMerge));
+    return D2SD_OK;
+  } catch (const std::exception& e) {
+    return fail(D2SD_ERR_INVALID_ARG, std::string("chunk_plan: ") + e.what());
+  }
+}
+
+int d2sd_chunk_run(const d2sd_chunk_plan_info* info, const d2sd_chunk_run_args* a, d2sd_stream_t stream) {
+  g_last_error.clear();
+  if (!info || !a) return fail(D2SD_ERR_INVALID_ARG, "chunk_run: null argument");
+  if (info->num_items == 0) return D2SD_OK;
+  if (int rc = check_cache(a->cache, "chunk_run")) return rc;
+  const d2sd_paged_cache& c = a->cache;
+  if (c.format != info->format || c.page_size != info->page_size || c.num_kv_heads != info->num_kv_heads ||
+      c.head_dim != info->head_dim)
+    return fail(D2SD_ERR_INVALID_ARG, "chunk_run: the cache is not the one planned for");
+  if (!a->plan || !a->kv_len || !a->page_table || !a->q || !a->out || !a->lse)
+    return fail(D2SD_ERR_INVALID_ARG, "chunk_run: null pointer");
+  if (!aligned16(a->q) || !aligned16(a->out) || !stride_ok(a->q_stride_n) || !stride_ok(a->q_stride_h) ||
+      !stride_ok(a->o_stride_n) || !stride_ok(a->o_stride_h))
+    return fail(D2SD_ERR_INVALID_ARG, "chunk_run: q and out need 16-byte rows");
+  if (!(a->sm_scale > 0.f) || !std::isfinite(a->sm_scale))
+    return fail(D2SD_ERR_INVALID_ARG, "chunk_run: sm_scale must be positive and finite");
+  if (info->workspace_bytes > 0 && (!a->workspace || !aligned16(a->workspace)))
+    return fail(D2SD_ERR_INVALID_ARG, "chunk_run: a 16-byte aligned workspace is required");
+  if (a->workspace_bytes < info->workspace_bytes)
+    return fail(D2SD_ERR_WORKSPACE, "chunk_run: workspace too small (need " + std::to_string(info->workspace_bytes) +
+                                        " bytes)");
+  const int64_t unit = c.format == D2SD_CACHE_BF16 ? 2 : 1;
+  d2sd::ChunkParams p{};
+  p.q = a->q;
+  p.q_stride_n = a->q_stride_n;
+  p.q_stride_h = a->q_stride_h;
+  p.o = a->out;
+  p.o_stride_n = a->o_stride_n;
+  p.o_stride_h = a->o_stride_h;
+  p.lse = a->lse;
+  p.lse_stride_n = a->lse_stride_n;
+  p.items = (const d2sd::ChunkItem*)a->plan;
+  p.merges = (const d2sd::ChunkMerge*)(a->plan + (size_t)info->num_items * (sizeof(d2sd::ChunkItem) / 4));
+  p.kv_len = a->kv_len;
+  p.page_table = a->page_table;
+  p.ks = {c.k, c.k_scale};
+  p.vs = {c.v, c.v_scale};
+  p.stride_page = c.stride_page * unit;
+  p.stride_head = c.stride_head * unit;
+  p.stride_tok = c.stride_tok * unit;
+  p.scale_stride_page = c.scale_stride_page;
+  p.scale_stride_head = c.scale_stride_head;
+  p.scale_stride_tok = c.scale_stride_tok;
+  const size_t partial_rows = info->workspace_bytes / ((size_t)(info->head_dim + 1) * sizeof(float));
+  p.part_o = (float*)a->workspace;
+  p.part_lse = p.part_o ? p.part_o + partial_rows * info->head_dim : nullptr;
+  p.sinks = a->sinks;
+  p.sm_scale = a->sm_scale;
+  p.group = info->num_qo_heads / info->num_kv_heads;
+  p.window_left = info->window_left;
+  p.log2_page = log2_of(c.page_size);
+  p.num_pages = c.num_pages;
+  p.lse_base2 = a->lse_base2 ? 1 : 0;
+  hipError_t e = d2sd::launch_chunk_attention(p, info->head_dim, info->format, info->num_items, info->num_merges,
+                                              (hipStream_t)stream);
+  return e == hipSuccess ? D2SD_OK : fail_hip(e, "chunk_run launch");
+}
+
 }  // extern "C"

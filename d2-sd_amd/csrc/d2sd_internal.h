@@ -235,6 +235,103 @@ struct QkRopeParams {
 };
 
 // ---------------------------------------------------------------------------
+// Rotary embedding at positions (rotary.hip).
+// ---------------------------------------------------------------------------
+constexpr int kRotaryMaxPairs = 128;      // rotated pairs of a head
+constexpr int kRotaryManyTokens = 1024;   // from here on a wave takes all heads of its token
+struct RotaryParams {
+  const void* q;             // bf16 [tokens, Hq, D], head_dim contiguous
+  const void* k;             // bf16 [tokens, Hkv, D]
+  void* q_out;               // may be q
+  void* k_out;               // may be k
+  long long q_stride_n, q_stride_h, k_stride_n, k_stride_h;      // elements
+  long long qo_stride_n, qo_stride_h, ko_stride_n, ko_stride_h;
+  const void* positions;     // [tokens] int32, or int64 (pos64)
+  const double* inv_freq;    // [pairs] radians per position
+  float scale;               // factor on cos and sin
+  int num_tokens, num_qo_heads, num_kv_heads, head_dim;
+  int pairs;                 // rotated pairs: dims [0, 2 pairs) of a head
+  int pos64, inverse;
+  int copy_rest;             // the dims behind the rotated ones are copied too (not in place)
+  int runs, heads_per_run;   // launcher: waves of a token, heads of a wave
+};
+
+// ---------------------------------------------------------------------------
+// Paged KV cache of a ragged batch (paged_cache.hip).
+// ---------------------------------------------------------------------------
+enum : int { CACHE_BF16 = 0, CACHE_FP8 = 1, CACHE_MXFP8 = 2, CACHE_MXFP4 = 3 };
+constexpr int kReadTokens = 16;  // cached tokens per workgroup of the read back
+struct CacheSide {               // keys or values
+  void* codes;
+  void* scale;                   // fp32 [Hkv] (fp8) or bytes (mx formats)
+};
+// Up to kReadTokens cached tokens of one request (32 bytes)
+struct CacheReadItem {
+  int req, count;
+  int first, from_end;           // cache position of the first one; from_end: it is cache length - first
+  int row;                       // its row of the contiguous keys and values
+  int page_begin, page_end;      // the request's entries of the page table
+  int pad;
+};
+struct CacheParams {
+  const void* items;             // write: int4 per token; read: CacheReadItem
+  const int* kv_len;             // [requests] current cache lengths, the new tokens included
+  const int* page_table;
+  void* k;                       // contiguous bf16 rows [tokens, Hkv, D]
+  void* v;
+  long long stride_n, stride_h;  // elements
+  CacheSide ks, vs;
+  long long stride_page, stride_head, stride_tok;                    // code elements (mxfp4: bytes)
+  long long scale_stride_page, scale_stride_head, scale_stride_tok;  // bytes (mx formats)
+  int num_items, num_kv_heads, head_dim, log2_page, num_pages;
+};
+
+// ---------------------------------------------------------------------------
+// Attention of each request's newest tokens over its paged cache
+// (chunk_attention.hip).
+// ---------------------------------------------------------------------------
+constexpr int kChunkWaves = 8;      // waves of a workgroup
+constexpr int kChunkRows = 256;     // packed rows of a tile item (32 per wave)
+constexpr int kTokenRows = 32;      // packed rows a token item holds at most (all waves share them)
+constexpr int kChunkMaxSplits = 64;
+enum : int { CHUNK_TILE = 0, CHUNK_TOKEN = 1 };
+struct ChunkItem {                  // one workgroup (64 bytes)
+  int req, kvh;
+  int q0, nq;                       // the request's first query row and query count
+  int row0, nrows;                  // packed rows [row0, row0 + nrows): row = token * group + head
+  int page_begin, page_end;         // the request's entries of the page table
+  int chunk, nchunks;               // key chunk of its rows' visible keys
+  int slot;                         // first partial row (nchunks > 1)
+  int kind;                         // CHUNK_TILE / CHUNK_TOKEN
+  int pad[4];
+};
+struct ChunkMerge {                 // 32 bytes: rows merged by one workgroup
+  int q0, kvh, row0, nrows;
+  int slot, stride, nchunks;        // chunk c's partial of row i: slot + c * stride + i
+  int pad;
+};
+struct ChunkParams {
+  const void* q;
+  long long q_stride_n, q_stride_h;  // elements
+  void* o;
+  long long o_stride_n, o_stride_h;
+  float* lse;                        // [rows, Hq]
+  long long lse_stride_n;
+  const ChunkItem* items;
+  const ChunkMerge* merges;
+  const int* kv_len;
+  const int* page_table;
+  CacheSide ks, vs;
+  long long stride_page, stride_head, stride_tok;                    // bytes
+  long long scale_stride_page, scale_stride_head, scale_stride_tok;  // bytes
+  float* part_o;                     // [partial row][D]
+  float* part_lse;                   // [partial row], base 2; -inf: no key
+  const float* sinks;                // nullable, [Hq]
+  float sm_scale;
+  int group, window_left, log2_page, num_pages, lse_base2;
+};
+
+// ---------------------------------------------------------------------------
 // Candidate-tree build (tree_build.hip).
 // ---------------------------------------------------------------------------
 constexpr int kTreeMaxRows = 65;  // DFlash row + at most 64 boundaries

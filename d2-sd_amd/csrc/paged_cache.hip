@@ -1,0 +1,268 @@
+// gfx950 kernels of the paged KV cache of a ragged batch: the new tokens' keys
+// and values quantised into their pages (write), and cached tokens read back
+// as contiguous bf16 (read).
+//
+// Formats.  bf16; fp8: e4m3fn(x / scale[head]), the quotient correctly rounded
+// in fp32; mxfp8 / mxfp4: blocks of 32 head dims, each a power-of-two scale 2^e
+// (byte e + 127) and elements RNE(x 2^-e) in e4m3 or e2m1 (two to a byte, the
+// even element low).  e is the smallest exponent with amax <= M 2^e, M = 448
+// or 6: with amax = f 2^k, 1 <= f < 2, it is k - kM + (f > fM) for
+// M = fM 2^kM, integer arithmetic on amax's bits, so that the codes follow from
+// the inputs alone, whatever the order of work.  e stays at or above -117,
+// where the smallest element (2^-9 2^e) is a normal bf16, and at or below 119
+// (mxfp8) or 125 (mxfp4), where the largest is finite; there elements saturate.
+// x 2^-e is exact and every element times 2^e is a bf16 value, so reading back
+// is exact.  A block that holds an infinity or NaN gets the scale byte 255 and
+// reads back as NaN.
+//
+// Both kernels move data once: bound by HBM (or, for a step's few tokens, by
+// the chain token -> cache length -> page id -> store).  A thread carries 8
+// elements: a 16-byte bf16 load or store against 8 bytes (fp8, mxfp8) or 4
+// (mxfp4) of codes; the four threads of a block of 32 find its amax by DPP.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "d2sd_internal.h"
+#include "kernel_common.h"
+#include "plan.h"
+
+namespace d2sd {
+
+namespace {
+
+constexpr int kReadUnroll = 4;
+
+// 2^(byte - 127); byte 255 stands for NaN, byte 0 for 2^-127
+__device__ __forceinline__ float block_scale(unsigned byte) {
+  const unsigned bits = byte == 255u ? 0x7FC00000u : byte == 0u ? 0x00400000u : byte << 23;
+  return __uint_as_float(bits);
+}
+
+// e4m3fn byte pairs of f0..f3, |f| <= 448, rounded to nearest even
+__device__ __forceinline__ unsigned fp8x4(float f0, float f1, float f2, float f3) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(f0, f1, 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(f2, f3, w, true);
+  return (unsigned)w;
+}
+
+// e2m1 code of f, |f| <= 6, ties to the even code: below 2 the step is 1/2,
+// below 4 it is 1, below 6 it is 2, and codes count the steps.
+__device__ __forceinline__ unsigned fp4_code(float f) {
+  const float a = fabsf(f);
+  const float r = a < 2.f ? rintf(2.f * a) : a < 4.f ? rintf(a) + 2.f : rintf(0.5f * a) + 4.f;
+  return (unsigned)r | (__float_as_uint(f) >> 31 << 3);
+}
+
+__device__ __forceinline__ void expand8(const u32x4& u, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = bf16_lo(u[i]);
+    x[2 * i + 1] = bf16_hi(u[i]);
+  }
+}
+
+// Maximum over the four threads of a block (threads 4b .. 4b + 3 of a wave).
+__device__ __forceinline__ unsigned quad_max(unsigned v) {
+  v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));  // quad_perm [1,0,3,2]
+  return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));  // [2,3,0,1]
+}
+
+// One 8-element piece of a new row into its cache row.  Threads that share a
+// block call it together; `on` says whether this thread stores.
+template <int FMT>
+__device__ __forceinline__ void store_piece(const CacheSide& s, int fmt_head, long long row, long long srow, int d,
+                                            const u32x4& val) {
+  if constexpr (FMT == CACHE_BF16) {
+    *(u32x4*)((uint16_t*)s.codes + row + d) = val;
+  } else {
+    float x[8];
+    expand8(val, x);
+    if constexpr (FMT == CACHE_FP8) {
+      const float sc = ((const float*)s.scale)[fmt_head];
+      u32x2 b;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float q[4];
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float r = __fdiv_rn(x[4 * i + e], sc);
+          bad = bad || isnan(r);
+          q[e] = fminf(fmaxf(r, -448.f), 448.f);
+        }
+        b[i] = fp8x4(q[0], q[1], q[2], q[3]);
+        if (bad) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (isnan(__fdiv_rn(x[4 * i + e], sc))) b[i] |= 0x7Fu << (8 * e);
+        }
+      }
+      *(u32x2*)((uint8_t*)s.codes + row + d) = b;
+    } else {
+      constexpr bool FP4 = FMT == CACHE_MXFP4;
+      unsigned amax = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) amax = max(amax, max(val[i] << 16 & 0x7FFF0000u, val[i] & 0x7FFF0000u));
+      amax = quad_max(amax);
+      const bool finite = amax < 0x7F800000u;
+      // amax = f 2^k: k + 127 in bits 30..23, f's fraction below (a subnormal's
+      // k reads as -127, below the range all the same)
+      constexpr unsigned FM = FP4 ? 0x00400000u : 0x00600000u;  // fraction bits of 1.5, 1.75
+      constexpr int KM = FP4 ? 2 : 8, TOP = FP4 ? 125 : 119;
+      int e = (int)(amax >> 23) - 127 - KM + ((amax & 0x007FFFFFu) > FM ? 1 : 0);
+      e = min(max(e, -117), TOP);
+      const float inv = __uint_as_float((unsigned)(127 - e) << 23);
+      constexpr float M = FP4 ? 6.f : 448.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = finite ? fminf(fmaxf(x[i] * inv, -M), M) : 0.f;
+      if constexpr (FP4) {
+        unsigned w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w |= fp4_code(x[i]) << (4 * i);
+        *(unsigned*)((uint8_t*)s.codes + row + d / 2) = w;
+      } else {
+        *(u32x2*)((uint8_t*)s.codes + row + d) =
+            (u32x2){fp8x4(x[0], x[1], x[2], x[3]), fp8x4(x[4], x[5], x[6], x[7])};
+      }
+      if ((d & 31) == 0) ((uint8_t*)s.scale)[srow + d / 32] = (uint8_t)(finite ? e + 127 : 255);
+    }
+  }
+}
+
+// Block t: new token t, all heads, keys then values.  tokens[t] = (request,
+// tokens from it to its request's end, first page table entry, page table end).
+template <int FMT>
+__global__ __launch_bounds__(256) void cache_write_kernel(const CacheParams p) {
+  const int t = blockIdx.x;
+  const int4 w = ((const int4*)p.items)[t];
+  const int cpr = p.head_dim / 8, nch = p.num_kv_heads * cpr;
+  // the rows' loads first: they do not wait for the place they go to
+  auto source = [&](int c) {
+    const bool is_v = c >= nch;
+    const int cc = is_v ? c - nch : c, h = cc / cpr, d = 8 * (cc - h * cpr);
+    return *(const u32x4*)((const uint16_t*)(is_v ? p.v : p.k) + (long long)t * p.stride_n + (long long)h * p.stride_h + d);
+  };
+  int c = threadIdx.x;
+  u32x4 val = c < 2 * nch ? source(c) : u32x4{};
+  const int pos = p.kv_len[w.x] - w.y;
+  const int at = w.z + (pos >> p.log2_page);
+  if (pos < 0 || at >= w.w) return;  // before the cache's start, or no page is reserved for it
+  const int page = p.page_table[at];
+  if (page < 0 || page >= p.num_pages) return;
+  const int slot = pos & ((1 << p.log2_page) - 1);
+  for (; c < 2 * nch; c += blockDim.x) {
+    const bool is_v = c >= nch;
+    const int cc = is_v ? c - nch : c, h = cc / cpr, d = 8 * (cc - h * cpr);
+    const CacheSide& s = is_v ? p.vs : p.ks;
+    store_piece<FMT>(s, h, page * p.stride_page + h * p.stride_head + slot * p.stride_tok,
+                     page * p.scale_stride_page + h * p.scale_stride_head + slot * p.scale_stride_tok, d, val);
+    if (c + (int)blockDim.x < 2 * nch) val = source(c + blockDim.x);
+  }
+}
+
+// 8 cached elements as bf16.
+template <int FMT>
+__device__ __forceinline__ u32x4 load_piece(const CacheSide& s, int h, long long row, long long srow, int d) {
+  if constexpr (FMT == CACHE_BF16) {
+    return *(const u32x4*)((const uint16_t*)s.codes + row + d);
+  } else if constexpr (FMT == CACHE_FP8) {
+    const u32x2 b = *(const u32x2*)((const uint8_t*)s.codes + row + d);
+    const float sc = ((const float*)s.scale)[h];
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const u32x2 v = fp8x4_to_bf16x4(b[i]);
+      o[2 * i] = pack_bf16x2(bf16_lo(v[0]) * sc, bf16_hi(v[0]) * sc);
+      o[2 * i + 1] = pack_bf16x2(bf16_lo(v[1]) * sc, bf16_hi(v[1]) * sc);
+    }
+    return o;
+  } else {
+    const float sc = block_scale(((const uint8_t*)s.scale)[srow + d / 32]);
+    u32x4 o;
+    if constexpr (FMT == CACHE_MXFP8) {
+      const u32x2 b = *(const u32x2*)((const uint8_t*)s.codes + row + d);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        o[2 * i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[i], sc, false));
+        o[2 * i + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b[i], sc, true));
+      }
+    } else {
+      const unsigned b = *(const unsigned*)((const uint8_t*)s.codes + row + d / 2);
+      o[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(b, sc, 0));
+      o[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(b, sc, 1));
+      o[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(b, sc, 2));
+      o[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(b, sc, 3));
+    }
+    return o;
+  }
+}
+
+// Block i: up to kReadTokens cached tokens of one request, all heads, keys then
+// values.  items[i] = (request | token count << 24.., see CacheReadItem).
+template <int FMT>
+__global__ __launch_bounds__(256) void cache_read_kernel(const CacheParams p) {
+  const CacheReadItem w = ((const CacheReadItem*)p.items)[blockIdx.x];
+  const int len = p.kv_len[w.req];
+  const int pos0 = w.from_end ? len - w.first : w.first;  // cache position of the item's first token
+  const int cpr = p.head_dim / 8, row_ch = p.num_kv_heads * cpr, nch = w.count * row_ch;
+  for (int c0 = threadIdx.x; c0 < 2 * nch; c0 += kReadUnroll * blockDim.x) {
+    u32x4 val[kReadUnroll];
+    long long dst[kReadUnroll];
+    bool on[kReadUnroll];
+#pragma unroll
+    for (int u = 0; u < kReadUnroll; ++u) {
+      const int c = c0 + u * (int)blockDim.x;
+      const bool is_v = c >= nch;
+      const int cc = is_v ? c - nch : c;
+      const int i = cc / row_ch, r = cc - i * row_ch, h = r / cpr, d = 8 * (r - h * cpr);
+      const int pos = pos0 + i, at = w.page_begin + (pos >> p.log2_page);
+      on[u] = c < 2 * nch && pos >= 0 && pos < len && at < w.page_end;
+      const int page = on[u] ? p.page_table[at] : 0;
+      on[u] = on[u] && page >= 0 && page < p.num_pages;
+      dst[u] = (long long)(w.row + i) * p.stride_n + (long long)h * p.stride_h + d;
+      val[u] = u32x4{};
+      if (on[u]) {
+        const int slot = pos & ((1 << p.log2_page) - 1);
+        val[u] = load_piece<FMT>(is_v ? p.vs : p.ks, h,
+                                 page * p.stride_page + h * p.stride_head + slot * p.stride_tok,
+                                 page * p.scale_stride_page + h * p.scale_stride_head + slot * p.scale_stride_tok, d);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kReadUnroll; ++u)
+      if (on[u]) *(u32x4*)((uint16_t*)(c0 + u * (int)blockDim.x >= nch ? p.v : p.k) + dst[u]) = val[u];
+  }
+}
+
+}  // namespace
+
+hipError_t launch_cache_write(const CacheParams& p, int format, hipStream_t s) {
+  if (p.num_items <= 0) return hipSuccess;
+  const dim3 grid((unsigned)p.num_items);
+  const int pieces = 2 * p.num_kv_heads * (p.head_dim / 8);
+  const dim3 block((unsigned)std::min(256, (pieces + 63) / 64 * 64));
+  switch (format) {
+    case CACHE_BF16: hipLaunchKernelGGL(cache_write_kernel<CACHE_BF16>, grid, block, 0, s, p); break;
+    case CACHE_FP8: hipLaunchKernelGGL(cache_write_kernel<CACHE_FP8>, grid, block, 0, s, p); break;
+    case CACHE_MXFP8: hipLaunchKernelGGL(cache_write_kernel<CACHE_MXFP8>, grid, block, 0, s, p); break;
+    case CACHE_MXFP4: hipLaunchKernelGGL(cache_write_kernel<CACHE_MXFP4>, grid, block, 0, s, p); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_cache_read(const CacheParams& p, int format, hipStream_t s) {
+  if (p.num_items <= 0) return hipSuccess;
+  const dim3 grid((unsigned)p.num_items), block(256);
+  switch (format) {
+    case CACHE_BF16: hipLaunchKernelGGL(cache_read_kernel<CACHE_BF16>, grid, block, 0, s, p); break;
+    case CACHE_FP8: hipLaunchKernelGGL(cache_read_kernel<CACHE_FP8>, grid, block, 0, s, p); break;
+    case CACHE_MXFP8: hipLaunchKernelGGL(cache_read_kernel<CACHE_MXFP8>, grid, block, 0, s, p); break;
+    case CACHE_MXFP4: hipLaunchKernelGGL(cache_read_kernel<CACHE_MXFP4>, grid, block, 0, s, p); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace d2sd

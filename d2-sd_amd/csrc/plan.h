@@ -87,6 +87,34 @@ hipError_t launch_d3_tree_build(const TreeBuildParams& p, hipStream_t s);
 // ---- QK RMSNorm + RoPE (qk_rope.hip) ----
 hipError_t launch_qk_norm_rope(const QkRopeParams& p, hipStream_t s);
 
+// ---- rotary embedding at positions (rotary.hip) ----
+hipError_t launch_rotary(RotaryParams p, bool interleaved, hipStream_t s);
+
+// ---- paged KV cache of a ragged batch (paged_cache.hip); format: CACHE_* ----
+hipError_t launch_cache_write(const CacheParams& p, int format, hipStream_t s);
+hipError_t launch_cache_read(const CacheParams& p, int format, hipStream_t s);
+
+// ---- attention of new tokens over the paged cache (chunk_attention.hip, chunk_plan.cpp) ----
+struct ChunkPlanInput {
+  int num_reqs;
+  const int* qo_indptr;    // host [num_reqs + 1]
+  const int* kv_len;       // host [num_reqs]: longest cache of each request, its new tokens included
+  const int* page_indptr;  // host [num_reqs + 1]
+  int num_qo_heads, num_kv_heads, head_dim;
+  int format;              // CACHE_*
+  int window_left;
+  int num_cus;
+  int max_splits;          // 0: up to kChunkMaxSplits
+};
+struct ChunkPlanOutput {
+  std::vector<ChunkItem> items;
+  std::vector<ChunkMerge> merges;
+  long long partial_rows;
+};
+void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out);
+hipError_t launch_chunk_attention(const ChunkParams& p, int head_dim, int format, int nitems, int nmerges,
+                                  hipStream_t s);
+
 // ---- greedy acceptance walk (accept.hip) ----
 hipError_t launch_greedy_accept(const AcceptParams& p, bool bf16, hipStream_t s);
 // vocabulary chunks per node of the argmax pass

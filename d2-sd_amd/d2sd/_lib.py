@@ -20,6 +20,10 @@ D2SD_MASK_CAUSAL = 1
 D2SD_MASK_TREE = 2
 D2SD_DTYPE_BF16 = 0
 D2SD_DTYPE_F32 = 1
+D2SD_CACHE_BF16 = 0
+D2SD_CACHE_FP8 = 1
+D2SD_CACHE_MXFP8 = 2
+D2SD_CACHE_MXFP4 = 3
 
 # Every symbol include/d2sd.h declares.
 EXPORTED_SYMBOLS = (
@@ -45,6 +49,11 @@ EXPORTED_SYMBOLS = (
     "d2sd_sample_accept",
     "d2sd_qk_norm_rope",
     "d2sd_d3_tree_build",
+    "d2sd_rotary_embedding",
+    "d2sd_cache_write",
+    "d2sd_cache_read",
+    "d2sd_chunk_plan",
+    "d2sd_chunk_run",
 )
 
 
@@ -243,9 +252,133 @@ class SampleAcceptArgs(C.Structure):
     ]
 
 
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("k_out", C.c_void_p),
+        ("q_stride_n", C.c_int64),
+        ("q_stride_h", C.c_int64),
+        ("k_stride_n", C.c_int64),
+        ("k_stride_h", C.c_int64),
+        ("qo_stride_n", C.c_int64),
+        ("qo_stride_h", C.c_int64),
+        ("ko_stride_n", C.c_int64),
+        ("ko_stride_h", C.c_int64),
+        ("positions", C.c_void_p),
+        ("inv_freq", C.c_void_p),
+        ("scale", C.c_float),
+        ("num_tokens", C.c_int),
+        ("num_qo_heads", C.c_int),
+        ("num_kv_heads", C.c_int),
+        ("head_dim", C.c_int),
+        ("num_pairs", C.c_int),
+        ("positions_64", C.c_int),
+        ("interleaved", C.c_int),
+        ("inverse", C.c_int),
+    ]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("stride_page", C.c_int64),
+        ("stride_head", C.c_int64),
+        ("stride_tok", C.c_int64),
+        ("scale_stride_page", C.c_int64),
+        ("scale_stride_head", C.c_int64),
+        ("scale_stride_tok", C.c_int64),
+        ("format", C.c_int),
+        ("num_pages", C.c_int),
+        ("page_size", C.c_int),
+        ("num_kv_heads", C.c_int),
+        ("head_dim", C.c_int),
+    ]
+
+
+class CacheIoArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("items", C.c_void_p),
+        ("kv_len", C.c_void_p),
+        ("page_table", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("stride_n", C.c_int64),
+        ("stride_h", C.c_int64),
+        ("num_items", C.c_int),
+    ]
+
+
+class ChunkPlanDesc(C.Structure):
+    _fields_ = [
+        ("num_reqs", C.c_int),
+        ("qo_indptr", C.POINTER(C.c_int32)),
+        ("kv_len", C.POINTER(C.c_int32)),
+        ("page_indptr", C.POINTER(C.c_int32)),
+        ("num_qo_heads", C.c_int),
+        ("num_kv_heads", C.c_int),
+        ("head_dim", C.c_int),
+        ("format", C.c_int),
+        ("page_size", C.c_int),
+        ("window_left", C.c_int),
+        ("num_cus", C.c_int),
+        ("max_splits", C.c_int),
+    ]
+
+
+class ChunkPlanInfo(C.Structure):
+    _fields_ = [
+        ("num_items", C.c_int),
+        ("num_merges", C.c_int),
+        ("plan_ints", C.c_int),
+        ("total_q", C.c_int),
+        ("num_reqs", C.c_int),
+        ("num_qo_heads", C.c_int),
+        ("num_kv_heads", C.c_int),
+        ("head_dim", C.c_int),
+        ("format", C.c_int),
+        ("page_size", C.c_int),
+        ("window_left", C.c_int),
+        ("num_page_entries", C.c_int),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class ChunkRunArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("plan", C.c_void_p),
+        ("kv_len", C.c_void_p),
+        ("page_table", C.c_void_p),
+        ("q", C.c_void_p),
+        ("q_stride_n", C.c_int64),
+        ("q_stride_h", C.c_int64),
+        ("out", C.c_void_p),
+        ("o_stride_n", C.c_int64),
+        ("o_stride_h", C.c_int64),
+        ("lse", C.c_void_p),
+        ("lse_stride_n", C.c_int64),
+        ("sinks", C.c_void_p),
+        ("sm_scale", C.c_float),
+        ("lse_base2", C.c_int),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
 # int32 entries per attention item / merge item in the host plan
 PLAN_ITEM_INTS = 16
 PLAN_MERGE_INTS = 8
+# the same of a chunk attention plan
+CHUNK_ITEM_INTS = 16
+CHUNK_MERGE_INTS = 8
+# cached tokens of one d2sd_cache_span
+READ_TOKENS = 16
 
 
 def _load() -> C.CDLL:
@@ -299,6 +432,16 @@ def _load() -> C.CDLL:
     lib.d2sd_d3_tree_build.argtypes = [C.POINTER(TreeArgs), vp]
     lib.d2sd_qk_norm_rope.restype = i32
     lib.d2sd_qk_norm_rope.argtypes = [C.POINTER(QkRopeArgs), vp]
+    lib.d2sd_rotary_embedding.restype = i32
+    lib.d2sd_rotary_embedding.argtypes = [C.POINTER(RotaryArgs), vp]
+    for name in ("d2sd_cache_write", "d2sd_cache_read"):
+        fn = getattr(lib, name)
+        fn.restype = i32
+        fn.argtypes = [C.POINTER(CacheIoArgs), vp]
+    lib.d2sd_chunk_plan.restype = i32
+    lib.d2sd_chunk_plan.argtypes = [C.POINTER(ChunkPlanDesc), C.POINTER(C.c_int32), sz, C.POINTER(ChunkPlanInfo)]
+    lib.d2sd_chunk_run.restype = i32
+    lib.d2sd_chunk_run.argtypes = [C.POINTER(ChunkPlanInfo), C.POINTER(ChunkRunArgs), vp]
     return lib
 
 

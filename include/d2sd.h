@@ -508,6 +508,184 @@ typedef struct {
 
 int d2sd_sample_accept(const d2sd_sample_accept_args* args, d2sd_stream_t stream);
 
+/* ----------------------------------------------------------------------
+ * Rotary embedding of queries and keys at their positions.
+ * No table of cosines: qk_norm_rope above takes the reference's bf16 table
+ * (generation/verification.py:113-123); this call takes positions and
+ * frequencies and computes the angles itself (in turns, 64-bit products,
+ * 32-bit sines), so positions may be far and differ per token.
+ * Head dims [0, 2 * num_pairs) of every head are rotated in pairs
+ *   half layout (interleaved = 0): (x[i], x[i + num_pairs])
+ *   interleaved = 1:               (x[2i], x[2i + 1])
+ *   (a, b) -> scale * (a cos t - b sin t, b cos t + a sin t),
+ *   t = positions[token] * inv_freq[i]   (inverse = 1: -t)
+ * with 32-bit products rounded to bf16 once; the other dims pass through.
+ * q_out / k_out may equal q / k with the same strides (in place) or lie
+ * apart; anything in between is undefined.  |position| < 2^31 * 2^20.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  const void* q;               /* bf16 [tokens, Hq, D]; may be NULL with num_qo_heads 0 */
+  const void* k;               /* bf16 [tokens, Hkv, D]; may be NULL with num_kv_heads 0 */
+  void* q_out;
+  void* k_out;
+  int64_t q_stride_n, q_stride_h, k_stride_n, k_stride_h; /* elements; head_dim contiguous */
+  int64_t qo_stride_n, qo_stride_h, ko_stride_n, ko_stride_h;
+  const void* positions;       /* device [tokens] int32, or int64 (positions_64) */
+  const double* inv_freq;      /* device [num_pairs], radians per position */
+  float scale;
+  int num_tokens;
+  int num_qo_heads;
+  int num_kv_heads;
+  int head_dim;                /* even, <= 256 */
+  int num_pairs;               /* 2 * num_pairs <= head_dim */
+  int positions_64;
+  int interleaved;
+  int inverse;
+} d2sd_rotary_args;
+
+int d2sd_rotary_embedding(const d2sd_rotary_args* args, d2sd_stream_t stream);
+
+/* ----------------------------------------------------------------------
+ * Paged KV cache of a ragged batch: write, read back, attention.
+ *
+ * A cache row is one token's head.  Formats:
+ *   D2SD_CACHE_BF16   bf16
+ *   D2SD_CACHE_FP8    e4m3fn(clamp(x / scale[kv head], +-448)), scales fp32, positive
+ *                     (D2SD_KV_FP8_E4M3 of d2sd_cascade_run and the KV commit)
+ *   D2SD_CACHE_MXFP8  blocks of 32 head dims: a scale byte b (2^(b - 127);
+ *   D2SD_CACHE_MXFP4  255: NaN) and elements e4m3fn, or e2m1 with the even
+ *                     element in the low nibble.  Writing takes the smallest
+ *                     exponent with amax <= 448 * 2^e (6 * 2^e), at least
+ *                     -117 and at most 119 (125), and rounds to nearest even,
+ *                     saturating; a block with an infinity or NaN becomes NaN.
+ * Codes of page p, slot s, kv head h start at element
+ *   p * stride_page + h * stride_head + s * stride_tok   (bf16: elements of 2
+ * bytes; else bytes); block scales at the scale strides (bytes), one byte per
+ * 32 head dims.  Strides and pointers: codes on 16-byte boundaries.
+ *
+ * The batch: request r has cache positions [0, kv_len[r]), position t in page
+ * page_table[page_indptr[r] + t / page_size]; kv_len is read from the device
+ * by every call (the new tokens included), so that one captured call replays
+ * while caches grow, up to the pages a request has.  Entries outside
+ * [0, num_pages) are skipped by writes and reads and clamped by the attention.
+ * ---------------------------------------------------------------------- */
+#define D2SD_CACHE_BF16 0
+#define D2SD_CACHE_FP8 1
+#define D2SD_CACHE_MXFP8 2
+#define D2SD_CACHE_MXFP4 3
+typedef struct {
+  void* k;
+  void* v;
+  void* k_scale;   /* fp8: fp32 [Hkv]; mx: bytes; bf16: NULL */
+  void* v_scale;
+  int64_t stride_page, stride_head, stride_tok;
+  int64_t scale_stride_page, scale_stride_head, scale_stride_tok; /* mx formats */
+  int format;
+  int num_pages;
+  int page_size;     /* power of two */
+  int num_kv_heads;
+  int head_dim;      /* multiple of 32, <= 256 (attention: 64 or 128) */
+} d2sd_paged_cache;
+
+/* One new token of a write: request, tokens from it to its request's end
+ * (1 for the last), and the request's entries of the page table. */
+typedef struct {
+  int32_t req, back, page_begin, page_end;
+} d2sd_cache_token;
+/* Up to 16 cached tokens of one request for a read: cache positions
+ * first .. first + count - 1 (from_end: kv_len[req] - first ..), rows
+ * row .. row + count - 1 of k and v. */
+typedef struct {
+  int32_t req, count, first, from_end, row, page_begin, page_end, reserved;
+} d2sd_cache_span;
+
+typedef struct {
+  d2sd_paged_cache cache;
+  const void* items;         /* device [num_items]: d2sd_cache_token (write; token i is row i of
+                                k and v) or d2sd_cache_span (read) */
+  const int32_t* kv_len;     /* device [requests] */
+  const int32_t* page_table; /* device */
+  void* k;                   /* bf16 [rows, Hkv, D], head_dim contiguous, 16-byte rows: read by
+                                the write, written by the read */
+  void* v;
+  int64_t stride_n, stride_h; /* elements, of k and v */
+  int num_items;
+} d2sd_cache_io_args;
+
+/* Writes new keys and values into their pages.  A slot that two tokens of one
+ * call share holds one of them or a mixture of both.  Tokens without a page
+ * are skipped. */
+int d2sd_cache_write(const d2sd_cache_io_args* args, d2sd_stream_t stream);
+/* Reads cached tokens as bf16 (fp8: code * scale, rounded once; the other
+ * formats exactly).  Rows of tokens the cache does not hold stay as they are. */
+int d2sd_cache_read(const d2sd_cache_io_args* args, d2sd_stream_t stream);
+
+/* Attention of each request's newest tokens over its cache, which already
+ * holds them.  Query i of request r (row qo_indptr[r] + i of q) sits at
+ * position kv_len[r] - n_r + i and sees keys j <= its position, with
+ * window_left >= 0 only those with j >= position - window_left.  A row that
+ * sees no key gets output 0 and lse -inf.  sinks as in d2sd_cascade_run.
+ * plan() as d2sd_cascade_plan: it takes the longest caches the calls will see
+ * (kv_len on the host, with the pages to hold them) and fills a work list that
+ * the caller uploads; run() is one launch, and a second that joins partial
+ * states where keys were split (info.num_merges > 0).  run() allocates nothing
+ * and does not synchronise; calls that may overlap need workspaces of their
+ * own.  K and V of the tokens a request sees must be finite (a NaN or infinity
+ * reaches every row whose 64-key tile holds it); anything may lie elsewhere. */
+typedef struct {
+  int num_reqs;
+  const int32_t* qo_indptr;   /* host [num_reqs + 1], from 0 */
+  const int32_t* kv_len;      /* host [num_reqs]: longest cache, new tokens included */
+  const int32_t* page_indptr; /* host [num_reqs + 1] */
+  int num_qo_heads;
+  int num_kv_heads;
+  int head_dim;               /* 64 or 128 */
+  int format;                 /* D2SD_CACHE_* */
+  int page_size;
+  int window_left;            /* -1: all keys up to the position */
+  int num_cus;                /* 0: query the device */
+  int max_splits;             /* 0: default cap */
+} d2sd_chunk_plan_desc;
+
+typedef struct {
+  int num_items;
+  int num_merges;
+  int plan_ints;
+  int total_q;
+  int num_reqs;
+  int num_qo_heads;
+  int num_kv_heads;
+  int head_dim;
+  int format;
+  int page_size;
+  int window_left;
+  int num_page_entries;  /* page_table entries the plan may read */
+  size_t workspace_bytes;
+} d2sd_chunk_plan_info;
+
+int d2sd_chunk_plan(const d2sd_chunk_plan_desc* desc, int32_t* host_plan, size_t host_plan_ints,
+                    d2sd_chunk_plan_info* info);
+
+typedef struct {
+  d2sd_paged_cache cache;
+  const int32_t* plan;       /* device copy of the host plan */
+  const int32_t* kv_len;     /* device [num_reqs] */
+  const int32_t* page_table; /* device, >= info.num_page_entries */
+  const void* q;             /* bf16 [total_q, Hq, D] */
+  int64_t q_stride_n, q_stride_h;
+  void* out;                 /* bf16 [total_q, Hq, D] */
+  int64_t o_stride_n, o_stride_h;
+  float* lse;                /* [total_q, Hq] */
+  int64_t lse_stride_n;
+  const float* sinks;        /* nullable, [Hq] */
+  float sm_scale;            /* > 0 */
+  int lse_base2;
+  void* workspace;           /* >= info.workspace_bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} d2sd_chunk_run_args;
+
+int d2sd_chunk_run(const d2sd_chunk_plan_info* info, const d2sd_chunk_run_args* args, d2sd_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
