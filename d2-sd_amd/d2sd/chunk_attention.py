@@ -25,8 +25,10 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .graph import keep_alive
+from .graph import _CAPTURING, keep_alive
 from .paged import KV_FORMATS, PagedBatch, PagedKVCache, _device
+
+_attention, _attention_out = (torch.ops.d2sd.chunk_attention.default, torch.ops.d2sd.chunk_attention_out.default)
 
 
 class PagedChunkAttention:
@@ -78,12 +80,7 @@ class PagedChunkAttention:
         self.plan_dev = torch.from_numpy(self.plan_host).to(batch.device)
         self.kv_format, self.sm_scale, self.lse_base2 = kv_format, scale, bool(lse_base2)
         self.num_qo_heads, self.num_kv_heads, self.head_dim = num_qo_heads, num_kv_heads, head_dim
-        a = _lib.ChunkRunArgs()
-        a.plan = self.plan_dev.data_ptr()
-        a.kv_len, a.page_table = batch.kv_len.data_ptr(), batch.page_table.data_ptr()
-        a.sinks = sinks.data_ptr() if sinks is not None else None
-        a.sm_scale, a.lse_base2 = scale, int(self.lse_base2)
-        self._args = a
+        self._info = torch.frombuffer(bytearray(bytes(info)), dtype=torch.uint8)
         return self
 
     def workspace(self) -> torch.Tensor:
@@ -103,43 +100,22 @@ class PagedChunkAttention:
         batch = self.batch
         if batch is None:
             raise RuntimeError("run() before plan()")
-        T, hq, d, dev = batch.total_q, self.num_qo_heads, self.head_dim, batch.device
         cache._check_batch(batch)
-        if cache.kv_format != self.kv_format or cache.num_kv_heads != self.num_kv_heads or cache.head_dim != d:
-            raise ValueError("the cache's format, heads or head_dim are not those planned")
-        if q.dtype != torch.bfloat16:
-            raise TypeError(f"q must be bfloat16 (got {q.dtype})")
-        if q.dim() != 3 or q.shape[0] < T or q.shape[1] != hq or q.shape[2] != d or q.stride(2) != 1 or q.device != dev:
-            raise ValueError(f"q must be [>= {T}, {hq}, {d}] on the batch's device with a contiguous head_dim")
-        n = q.shape[0]
-        if out is None:
-            out = torch.empty((n, hq, d), dtype=torch.bfloat16, device=dev)
-            if n > T:
-                out[T:].zero_()
-        elif out.dtype != torch.bfloat16 or out.shape != q.shape or out.stride(2) != 1 or out.device != dev:
-            raise ValueError("out must be bf16 like q, with a contiguous head_dim")
-        if lse is None:
-            lse = torch.empty((n, hq), dtype=torch.float32, device=dev)
-            if n > T:
-                lse[T:].fill_(-float("inf"))
-        elif lse.dtype != torch.float32 or lse.shape != (n, hq) or lse.stride(1) != 1 or lse.device != dev:
-            raise ValueError("lse must be float32 [rows of q, Hq] with contiguous heads")
-        ws = int(self.info.workspace_bytes)
-        if ws and workspace is None:
-            workspace = torch.empty(ws, dtype=torch.uint8, device=dev)
-        elif ws and (workspace.device != dev or not workspace.is_contiguous() or workspace.nbytes < ws):
-            raise ValueError(f"workspace must be {ws} contiguous bytes on the batch's device (workspace())")
-        a = _lib.ChunkRunArgs.from_buffer_copy(self._args)
-        a.cache = cache._cache
-        a.q, a.out, a.lse = q.data_ptr(), out.data_ptr(), lse.data_ptr()
-        a.q_stride_n, a.q_stride_h = q.stride(0), q.stride(1)
-        a.o_stride_n, a.o_stride_h = out.stride(0), out.stride(1)
-        a.lse_stride_n = lse.stride(0)
-        if ws:
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.nbytes
-        with torch.cuda.device(dev):
-            check(lib.d2sd_chunk_run(C.byref(self.info), C.byref(a),
-                                     C.c_void_p(torch.cuda.current_stream().cuda_stream)), "chunk_run")
-        keep_alive(self.plan_dev, batch.kv_len, batch.page_table, self.sinks, q, out, lse, workspace, cache.k_pool,
-                   cache.v_pool, cache.k_scale, cache.v_scale)
+        if cache.kv_format != self.kv_format:
+            raise ValueError(f"the plan is for a {self.kv_format} cache, not {cache.kv_format}")
+        rest = (self._info, self.plan_dev, batch.kv_len, batch.page_table, *cache._pools, self.sinks, self.sm_scale,
+                self.lse_base2)
+        if workspace is None and self.info.workspace_bytes and _CAPTURING:
+            workspace = self.workspace()  # the graph holds it
+        if out is None and lse is None:
+            out, lse = _attention(q, workspace, *rest)
+        else:
+            if out is None:
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                out[batch.total_q:].zero_()
+            if lse is None:
+                lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+                lse[batch.total_q:].fill_(-float("inf"))
+            _attention_out(q, out, lse, workspace, *rest)
+        keep_alive(self.plan_dev, batch.kv_len, batch.page_table, self.sinks, q, out, lse, workspace, *cache._pools[:4])
         return out, lse

@@ -24,16 +24,15 @@ or infinity reads back as NaN.
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import check, lib
 from .graph import capturing, keep_alive
 
+_write, _read, _read_out = (getattr(torch.ops.d2sd, n).default for n in ("cache_write", "cache_read", "cache_read_out"))
 KV_FORMATS = {"bf16": _lib.D2SD_CACHE_BF16, "fp8": _lib.D2SD_CACHE_FP8, "mxfp8": _lib.D2SD_CACHE_MXFP8,
               "mxfp4": _lib.D2SD_CACHE_MXFP4}
 _BLOCK = 32
@@ -170,7 +169,6 @@ class PagedKVCache:
         tok, head = (2, 1) if kv_layout == "HND" else (1, 2)
         P, hkv = k_pool.shape[tok], k_pool.shape[head]
         d = k_pool.shape[3] * (2 if kv_format == "mxfp4" else 1)
-        c = _lib.PagedCache()
         if kv_format == "bf16":
             if k_scale is not None or v_scale is not None:
                 raise ValueError("a bf16 cache has no scales")
@@ -186,19 +184,12 @@ class PagedKVCache:
                         or t.device != k_pool.device:
                     raise ValueError(f"{name} must be {list(shape)} on the pools' device, contiguous in its last "
                                      "dimension, both alike")
-            c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-            if mx:
-                c.scale_stride_page, c.scale_stride_head, c.scale_stride_tok = (
-                    k_scale.stride(0), k_scale.stride(head), k_scale.stride(tok))
         if P & (P - 1) or P == 0:
             raise ValueError("page_size must be a power of two")
         if d % _BLOCK or not 0 < d <= 256:
             raise ValueError("head_dim must be a multiple of 32 up to 256")
-        c.k, c.v = k_pool.data_ptr(), v_pool.data_ptr()
-        c.stride_page, c.stride_head, c.stride_tok = k_pool.stride(0), k_pool.stride(head), k_pool.stride(tok)
-        c.format, c.num_pages, c.page_size = KV_FORMATS[kv_format], k_pool.shape[0], P
-        c.num_kv_heads, c.head_dim = hkv, d
-        self._cache = c
+        # what every operator over the cache takes of it
+        self._pools = (k_pool, v_pool, k_scale, v_scale, KV_FORMATS[kv_format], kv_layout == "NHD")
         self.k_pool, self.v_pool, self.k_scale, self.v_scale = k_pool, v_pool, k_scale, v_scale
         self.kv_format, self.kv_layout, self.device = kv_format, kv_layout, k_pool.device
         self.num_pages, self.page_size, self.num_kv_heads, self.head_dim = k_pool.shape[0], P, hkv, d
@@ -226,27 +217,6 @@ class PagedKVCache:
     def _check_batch(self, batch: PagedBatch) -> None:
         if batch.page_size != self.page_size:
             raise ValueError(f"the batch's page_size {batch.page_size} is not the cache's {self.page_size}")
-        if batch.device != self.device:
-            raise ValueError("the batch and the cache are on different devices")
-
-    def _io(self, fn: str, k: torch.Tensor, v: torch.Tensor, rows: int, items: torch.Tensor, n: int,
-            batch: PagedBatch) -> None:
-        for name, t in (("k", k), ("v", v)):
-            if t.dtype != torch.bfloat16:
-                raise TypeError(f"{name} must be bfloat16 (got {t.dtype})")
-            if t.dim() != 3 or t.shape[0] < rows or t.shape[1] != self.num_kv_heads or t.shape[2] != self.head_dim \
-                    or t.stride(2) != 1 or t.stride() != k.stride() or t.device != self.device:
-                raise ValueError(f"{name} must be [>= {rows}, {self.num_kv_heads}, {self.head_dim}] on the cache's "
-                                 "device with a contiguous head_dim, k and v of the same strides")
-        a = _lib.CacheIoArgs()
-        a.cache = self._cache
-        a.items, a.num_items = items.data_ptr(), n
-        a.kv_len, a.page_table = batch.kv_len.data_ptr(), batch.page_table.data_ptr()
-        a.k, a.v = k.data_ptr(), v.data_ptr()
-        a.stride_n, a.stride_h = k.stride(0), k.stride(1)
-        with torch.cuda.device(self.device):
-            check(getattr(lib, fn)(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)), fn[5:])
-        keep_alive(k, v, items, batch.kv_len, batch.page_table, self.k_pool, self.v_pool, self.k_scale, self.v_scale)
 
     def write(self, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch) -> None:
         """Writes the batch's new tokens, rows of k and v [total_q, Hkv, D]
@@ -255,7 +225,8 @@ class PagedKVCache:
         outside the pool are skipped.  Two tokens of one call must not share a
         slot."""
         self._check_batch(batch)
-        self._io("d2sd_cache_write", k, v, batch.total_q, batch._tokens, batch.total_q, batch)
+        _write(k, v, batch._tokens, batch.total_q, batch.kv_len, batch.page_table, *self._pools)
+        keep_alive(k, v, batch._tokens, batch.kv_len, batch.page_table, *self._pools[:4])
 
     def read(self, batch: PagedBatch, new_only: bool = False,
              out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -267,10 +238,13 @@ class PagedKVCache:
         (k, v) of any token and head strides, alike."""
         self._check_batch(batch)
         rows = batch.total_q if new_only else batch.total_kv
+        if new_only not in batch._reads:
+            batch.prepare_read(new_only)
+        items = batch._reads[new_only]
         if out is None:
-            k, v = torch.empty((2, rows, self.num_kv_heads, self.head_dim), dtype=torch.bfloat16, device=self.device)
+            out = _read(rows, items, items.shape[0], batch.kv_len, batch.page_table, *self._pools)
         else:
             k, v = out
-        items = batch.prepare_read(new_only)._reads[new_only]
-        self._io("d2sd_cache_read", k, v, rows, items, items.shape[0], batch)
-        return k, v
+            _read_out(k, v, rows, items, items.shape[0], batch.kv_len, batch.page_table, *self._pools)
+        keep_alive(*out, items, batch.kv_len, batch.page_table, *self._pools[:4])
+        return out

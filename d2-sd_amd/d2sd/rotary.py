@@ -9,15 +9,15 @@ cos and sin are 32-bit and the result is rounded to bf16 once.
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 from typing import Mapping, Optional, Tuple
 
 import torch
 
-from . import _lib
-from ._lib import check, lib
+from . import _lib  # noqa: F401  (registers torch.ops.d2sd)
 from .graph import keep_alive
+
+_rotary = torch.ops.d2sd.rotary_embedding.default
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[Mapping] = None,
@@ -120,51 +120,9 @@ def rotary_embedding(q: Optional[torch.Tensor], k: Optional[torch.Tensor], posit
     multiplied by `scale`; inverse turns back (the gradient of the rotation,
     or keys moved to other positions).  In place, or into out = (q_out, k_out)
     of the same shapes.  Returns (q, k) or out."""
-    given = [(n, t) for n, t in (("q", q), ("k", k)) if t is not None]
-    if not given:
-        raise ValueError("rotary_embedding needs q or k")
-    dev, n, d = given[0][1].device, given[0][1].shape[0], given[0][1].shape[-1]
-    a = _lib.RotaryArgs()
     outs = (q, k) if out is None else tuple(out)
     if len(outs) != 2:
         raise ValueError("out must be (q_out, k_out)")
-    for (name, t), y in zip((("q", q), ("k", k)), outs):
-        if t is None:
-            if y is not None:
-                raise ValueError(f"out has a {name} but {name} is None")
-            continue
-        if y is None:
-            raise ValueError(f"out lacks a tensor for {name}")
-        for what, x in ((name, t), (f"{name}_out", y)):
-            if x.dtype != torch.bfloat16:
-                raise TypeError(f"{what} must be bfloat16 (got {x.dtype})")
-            if x.dim() != 3 or x.shape[0] != n or x.shape[2] != d or x.shape != t.shape or (d > 1 and x.stride(2) != 1):
-                raise ValueError(f"{what} must be [tokens, heads, head_dim] with a contiguous head_dim")
-            if not x.is_cuda or x.device != dev:
-                raise ValueError("q, k and out must be tensors of one ROCm device")
-    if positions.dtype not in (torch.int32, torch.int64) or inv_freq.dtype != torch.float64:
-        raise TypeError("positions must be int32 or int64, inv_freq float64")
-    if positions.dim() != 1 or positions.shape[0] != n or not positions.is_contiguous() or positions.device != dev:
-        raise ValueError("positions must be a contiguous [tokens] tensor on q's device")
-    if inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.device != dev:
-        raise ValueError("inv_freq must be a contiguous 1-D tensor on q's device")
-    if q is not None:
-        a.q, a.q_out = q.data_ptr(), outs[0].data_ptr()
-        a.q_stride_n, a.q_stride_h = q.stride(0), q.stride(1)
-        a.qo_stride_n, a.qo_stride_h = outs[0].stride(0), outs[0].stride(1)
-        a.num_qo_heads = q.shape[1]
-    if k is not None:
-        a.k, a.k_out = k.data_ptr(), outs[1].data_ptr()
-        a.k_stride_n, a.k_stride_h = k.stride(0), k.stride(1)
-        a.ko_stride_n, a.ko_stride_h = outs[1].stride(0), outs[1].stride(1)
-        a.num_kv_heads = k.shape[1]
-    a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
-    a.scale = scale
-    a.num_tokens, a.head_dim, a.num_pairs = n, d, inv_freq.shape[0]
-    a.positions_64 = positions.dtype == torch.int64
-    a.interleaved, a.inverse = bool(interleaved), bool(inverse)
-    with torch.cuda.device(dev):
-        check(lib.d2sd_rotary_embedding(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)),
-              "rotary_embedding")
+    _rotary(q, k, positions, inv_freq, outs[0], outs[1], interleaved, scale, inverse)
     keep_alive(q, k, positions, inv_freq, *outs)
     return outs
