@@ -1332,6 +1332,7 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t ho
     info->format = d->format;
     info->page_size = d->page_size;
     info->window_left = d->window_left;
+    info->tokens_only = out.tokens_only ? 1 : 0;
     info->num_page_entries = d->num_reqs > 0 ? d->page_indptr[d->num_reqs] : 0;
     info->workspace_bytes = (size_t)out.partial_rows * (d->head_dim + 1) * sizeof(float);
     if (!host_plan) return D2SD_OK;
@@ -1384,12 +1385,16 @@ int d2sd_chunk_run(const d2sd_chunk_plan_info* info, const d2sd_chunk_run_args* 
   p.page_table = a->page_table;
   p.ks = {c.k, c.k_scale};
   p.vs = {c.v, c.v_scale};
-  p.stride_page = c.stride_page * unit;
+  const int64_t most = (int64_t)1 << 32;  // the kernel multiplies 32-bit strides
+  if (c.stride_page >= most / unit || c.stride_tok >= most / unit / c.page_size ||
+      (c.format >= D2SD_CACHE_MXFP8 && (c.scale_stride_page >= most || c.scale_stride_tok >= most / c.page_size)))
+    return fail(D2SD_ERR_UNSUPPORTED, "chunk_run: pages of 4 GiB and more");
+  p.stride_page = (unsigned)(c.stride_page * unit);
   p.stride_head = c.stride_head * unit;
-  p.stride_tok = c.stride_tok * unit;
-  p.scale_stride_page = c.scale_stride_page;
+  p.stride_tok = (unsigned)(c.stride_tok * unit);
+  p.scale_stride_page = (unsigned)c.scale_stride_page;
   p.scale_stride_head = c.scale_stride_head;
-  p.scale_stride_tok = c.scale_stride_tok;
+  p.scale_stride_tok = (unsigned)c.scale_stride_tok;
   const size_t partial_rows = info->workspace_bytes / ((size_t)(info->head_dim + 1) * sizeof(float));
   p.part_o = (float*)a->workspace;
   p.part_lse = p.part_o ? p.part_o + partial_rows * info->head_dim : nullptr;
@@ -1400,7 +1405,7 @@ int d2sd_chunk_run(const d2sd_chunk_plan_info* info, const d2sd_chunk_run_args* 
   p.log2_page = log2_of(c.page_size);
   p.num_pages = c.num_pages;
   p.lse_base2 = a->lse_base2 ? 1 : 0;
-  hipError_t e = d2sd::launch_chunk_attention(p, info->head_dim, info->format, info->num_items, info->num_merges,
+  hipError_t e = d2sd::launch_chunk_attention(p, info->head_dim, info->format, info->tokens_only != 0, info->num_items, info->num_merges,
                                               (hipStream_t)stream);
   return e == hipSuccess ? D2SD_OK : fail_hip(e, "chunk_run launch");
 }

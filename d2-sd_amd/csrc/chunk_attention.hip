@@ -8,7 +8,7 @@
 // for a chunk of a prompt, a single token, or a batch of both, over a cache in
 // bf16, fp8 (one scale per kv head) or the block formats mxfp8 and mxfp4.
 //
-//   chunk_attn_kernel   one workgroup of 8 waves per work item: packed rows of
+//   chunk_attn_kernel   one workgroup of 4 waves per work item: packed rows of
 //                       one (request, kv head) against a chunk of their visible
 //                       keys, with a running maximum and sum (one pass over the
 //                       cache), state in registers
@@ -27,7 +27,7 @@
 //    stages tiles of 64 keys through registers into LDS (two buffers, one
 //    barrier a tile).  Bound by MFMA beside the softmax's vector instructions.
 //  * token items (up to 32 rows: decoding): all waves share the rows, and wave w
-//    takes every 8th tile of 32 keys.  Keys go from the cache straight to the
+//    takes every 4th tile of 32 keys.  Keys go from the cache straight to the
 //    MFMA operand: the sum over head dims may run in any order, so lane l takes
 //    the contiguous half l / 32 of key l % 32's dims.  Values pass through the
 //    wave's own LDS to be read transposed.  No barrier until the waves' states
@@ -178,6 +178,15 @@ struct ValueRead {
   }
 };
 
+// Byte offset of a cache row / its block scales (head 0) in page `page`: strides
+// below 2^32, one 32 x 32 -> 64-bit multiply each.
+__device__ __forceinline__ unsigned long long row_offset(const ChunkParams& p, unsigned page, unsigned slot) {
+  return (unsigned long long)page * p.stride_page + slot * p.stride_tok;
+}
+__device__ __forceinline__ unsigned long long scale_offset(const ChunkParams& p, unsigned page, unsigned slot) {
+  return (unsigned long long)page * p.scale_stride_page + slot * p.scale_stride_tok;
+}
+
 template <int D>
 __device__ __forceinline__ lds_char* lds_piece(lds_char* tile, int row, int chunk) {
   return tile + row * D * 2 + 16 * (chunk ^ chunk_swizzle<D>(row));
@@ -193,8 +202,6 @@ struct RowOut {
   }
 };
 
-__device__ __forceinline__ float natural(const ChunkParams& p, float lse2) { return lse2 * kLn2; }
-
 __device__ __forceinline__ float sink_factor(const ChunkParams& p, int head, float lse2) {
   if (!p.sinks) return 1.f;
   return 1.f / (1.f + __builtin_amdgcn_exp2f((p.sinks[head] - lse2 * kLn2) * kLog2e));
@@ -203,9 +210,8 @@ __device__ __forceinline__ float sink_factor(const ChunkParams& p, int head, flo
 // ---- tile items ----
 template <int D, int FMT>
 __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem& w, lds_char* lds) {
-  constexpr int MT = D / 32, KS = D / 16, EPT = D / 8, ROW = Format<D, FMT>::ROW, TB = 64 * D * 2;
+  constexpr int MT = D / 32, KS = D / 16, ROW = Format<D, FMT>::ROW, TB = 64 * D * 2;
   constexpr bool MX = Format<D, FMT>::MX;
-  constexpr int WORDS = ROW / 8 / 4;  // words of codes per thread and tile (keys; as many for values)
   const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
 
   const Span all = item_span(p, w, w.row0 / p.group, (w.row0 + w.nrows - 1) / p.group);
@@ -235,15 +241,41 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
   }
   const float slack = c > 0.f ? kRescaleSlack / c : 0.f;
 
-  // staging: thread tid carries 1/8 of key row tid / 8
-  const int srow = tid >> 3, spart = tid & 7;
-  const char* kb_ = (const char*)p.ks.codes + w.kvh * p.stride_head + spart * (ROW / 8);
-  const char* vb_ = (const char*)p.vs.codes + w.kvh * p.stride_head + spart * (ROW / 8);
-  const long long shead = w.kvh * p.scale_stride_head + spart * EPT / 32;
-  auto page_of = [&](int tile) -> int {
-    const int key = min(max(64 * tile + srow, all.lo), all.hi - 1);
-    return min((unsigned)p.page_table[w.page_begin + (key >> p.log2_page)], (unsigned)p.num_pages - 1u);
+  // staging of a tile's keys (then values) into chunk-swizzled bf16 rows
+  // (a page id is clamped where it is used: clamped where it is loaded, the
+  // wait for it would be a wait for all the tile's loads before it)
+  auto page_of = [&](int key) -> unsigned { return (unsigned)p.page_table[w.page_begin + (key >> p.log2_page)]; };
+  const unsigned last_page = (unsigned)p.num_pages - 1u;
+  auto key_of = [&](int tile, int row_) -> int { return min(max(64 * tile + row_, all.lo), all.hi - 1); };
+  const int pmask = (1 << p.log2_page) - 1;
+  // bf16: a wave copies 64 / W rows straight into LDS, 1 KB (1024 / ROW rows) at a time
+  constexpr int RPC = 1024 / (2 * D), NC = 64 / kChunkWaves / RPC;  // rows per copy, copies per wave
+  const int crow = wv * (64 / kChunkWaves) + lane / (D / 8);  // of copy 0
+  const char* kcopy = (const char*)p.ks.codes + w.kvh * p.stride_head;
+  const char* vcopy = (const char*)p.vs.codes + w.kvh * p.stride_head;
+  unsigned pages[NC];
+  auto pages_of = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) pages[i] = page_of(key_of(tile, crow + RPC * i));
   };
+  const unsigned lds0 = lds_address((const void*)lds);
+  auto copy = [&](int tile, unsigned at) {  // pages: of this tile
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int r = crow + RPC * i;
+      const unsigned long long off = row_offset(p, min(pages[i], last_page), key_of(tile, r) & pmask) +
+                                     16 * ((lane % (D / 8)) ^ chunk_swizzle<D>(r));
+      const unsigned dst = at + (wv * (64 / kChunkWaves) + RPC * i) * D * 2;
+      dma16(kcopy + off, dst);
+      dma16(vcopy + off, dst + TB);
+    }
+  };
+  // quantised: thread tid carries 1 / TPR of row tid / TPR through registers
+  constexpr int TPR = kChunkWaves, EPT = D / TPR, WORDS = FMT == CACHE_BF16 ? 1 : ROW / TPR / 4;
+  const int srow = tid / TPR, spart = tid % TPR;
+  const char* kpart = kcopy + spart * (ROW / TPR);
+  const char* vpart = vcopy + spart * (ROW / TPR);
+  const long long shead = w.kvh * p.scale_stride_head + spart * EPT / 32;
   unsigned kw[WORDS], vw[WORDS];
   unsigned ksc = 0, vsc = 0;
   auto load_words = [](unsigned (&d)[WORDS], const char* s) {
@@ -261,30 +293,26 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
       d[0] = *(const unsigned*)s;
     }
   };
-  auto fetch = [&](int tile, int page) {
-    const int key = min(max(64 * tile + srow, all.lo), all.hi - 1);
-    const int slot = key & ((1 << p.log2_page) - 1);
-    const long long off = page * p.stride_page + slot * p.stride_tok;
-    load_words(kw, kb_ + off);
-    load_words(vw, vb_ + off);
+  auto fetch = [&](int tile, unsigned page) {
+    const unsigned pg = min(page, last_page), slot = key_of(tile, srow) & pmask;
+    const unsigned long long off = row_offset(p, pg, slot);
+    load_words(kw, kpart + off);
+    load_words(vw, vpart + off);
     if constexpr (MX) {
-      const long long so = page * p.scale_stride_page + slot * p.scale_stride_tok + shead;
+      const unsigned long long so = scale_offset(p, pg, slot) + shead;
       ksc = ((const uint8_t*)p.ks.scale)[so];
       vsc = ((const uint8_t*)p.vs.scale)[so];
     }
   };
   auto put = [&](lds_char* tile, const unsigned (&d)[WORDS], unsigned sc) {
-    const float f = MX ? block_scale(sc) : 1.f;
+    if constexpr (FMT != CACHE_BF16) {
+      const float f = MX ? block_scale(sc) : 1.f;
 #pragma unroll
-    for (int i = 0; i < EPT / 8; ++i) {
-      bf16x8 v;
-      if constexpr (FMT == CACHE_BF16)
-        v = __builtin_bit_cast(bf16x8, (u32x4){d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]});
-      else if constexpr (FMT == CACHE_MXFP4)
-        v = expand<FMT>(d[i], 0u, f);
-      else
-        v = expand<FMT>(d[2 * i], d[2 * i + 1], f);
-      *(__attribute__((address_space(3))) bf16x8*)lds_piece<D>(tile, srow, spart * (EPT / 8) + i) = v;
+      for (int i = 0; i < EPT / 8; ++i) {
+        const bf16x8 v = FMT == CACHE_MXFP4 ? expand<FMT>(d[i % WORDS], 0u, f)
+                                            : expand<FMT>(d[2 * i % WORDS], d[(2 * i + 1) % WORDS], f);
+        *(__attribute__((address_space(3))) bf16x8*)lds_piece<D>(tile, srow, spart * (EPT / 8) + i) = v;
+      }
     }
   };
 
@@ -297,39 +325,66 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
   for (int ks = 0; ks < KS; ++ks) koff[ks] = (l32 * D + 8 * ((2 * ks + hh) ^ chunk_swizzle<D>(l32))) * 2;
   const ValueRead<D> vread(lane);
 
-  int page = 0;
+  // Two buffers of (K, V).  bf16: tile t + 1 is on its way while tile t is
+  // worked on.  Quantised: tile t + 2 is, and t + 1 is expanded into LDS.
+  unsigned page = 0;
   if (tb < te) {
-    fetch(tb, page_of(tb));
-    put(lds, kw, ksc);
-    put(lds + TB, vw, vsc);
-    if (tb + 1 < te) {
-      fetch(tb + 1, page_of(tb + 1));
-      page = page_of(min(tb + 2, te - 1));
+    if constexpr (FMT == CACHE_BF16) {
+      pages_of(tb);
+      copy(tb, lds0);
+      pages_of(min(tb + 1, te - 1));
+      wait_vmcnt<0>();
+    } else {
+      fetch(tb, page_of(key_of(tb, srow)));
+      put(lds, kw, ksc);
+      put(lds + TB, vw, vsc);
+      if (tb + 1 < te) {
+        fetch(tb + 1, page_of(key_of(tb + 1, srow)));
+        page = page_of(key_of(min(tb + 2, te - 1), srow));
+      }
     }
     __syncthreads();
   }
   for (int t = tb; t < te; ++t) {
-    lds_char* kt = lds + ((t - tb) & 1) * 2 * TB;
+    const int cur = ((t - tb) & 1) * 2 * TB, nxt = 2 * TB - cur;
+    lds_char* kt = lds + cur;
     lds_char* vt = kt + TB;
-    lds_char* nx = lds + ((t - tb + 1) & 1) * 2 * TB;
+    if constexpr (FMT == CACHE_BF16) {
+      if (t + 1 < te) {
+        copy(t + 1, lds0 + nxt);
+        pages_of(min(t + 2, te - 1));
+      }
+    }
     const int kb = 64 * t;
     const bool on = wave_on && kb < own.hi && kb + 64 > own.lo;
     f32x16 s[2];
     if (on) {
+      // operands are read AHEAD steps before their product
+      constexpr int AHEAD = 3;
+      bf16x8 kf[KS][2];
+      auto kread = [&](int ks) {
+        kf[ks][0] = *(const __attribute__((address_space(3))) bf16x8*)(kt + koff[ks]);
+        kf[ks][1] = *(const __attribute__((address_space(3))) bf16x8*)(kt + koff[ks] + 32 * D * 2);
+      };
+#pragma unroll
+      for (int ks = 0; ks < AHEAD; ++ks) kread(ks);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const bf16x8 a0 = *(const __attribute__((address_space(3))) bf16x8*)(kt + koff[ks]);
-        const bf16x8 a1 = *(const __attribute__((address_space(3))) bf16x8*)(kt + koff[ks] + 32 * D * 2);
-        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, qf[ks], ks ? s[0] : f32x16{}, 0, 0, 0);
-        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, qf[ks], ks ? s[1] : f32x16{}, 0, 0, 0);
+        if (ks + AHEAD < KS) kread(ks + AHEAD);
+        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks][0], qf[ks], ks ? s[0] : f32x16{}, 0, 0, 0);
+        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks][1], qf[ks], ks ? s[1] : f32x16{}, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (t + 1 < te) {
-      put(nx, kw, ksc);
-      put(nx + TB, vw, vsc);
-      if (t + 2 < te) {
-        fetch(t + 2, page);
-        page = page_of(min(t + 3, te - 1));
+    if constexpr (FMT != CACHE_BF16) {
+      if (t + 1 < te) {
+        put(lds + nxt, kw, ksc);
+        put(lds + nxt + TB, vw, vsc);
+        if (t + 2 < te) {
+          fetch(t + 2, page);
+          page = page_of(key_of(min(t + 3, te - 1), srow));
+        }
       }
     }
     if (on) {
@@ -346,6 +401,7 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
           o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vread(vt, mt, j), pb, o[mt], 0, 0, 0);
       }
     }
+    if constexpr (FMT == CACHE_BF16) wait_vmcnt<0>();  // this wave's copies of the next tile have landed
     __syncthreads();
   }
 
@@ -381,29 +437,37 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
 }
 
 // ---- token items ----
-template <int D, int FMT>
+// RB row blocks of 16 packed rows, shared by all waves; v_mfma_f32_16x16x32_bf16:
+// lane l holds row l % 16 of a block, and of a 16-key block the scores of keys
+// 4 (l / 16) .. + 3.  PF tiles of 32 keys are in flight per wave.
+template <int D, int FMT, int W, int RB, int PF>
 __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem& w, lds_char* lds, float* stats) {
-  constexpr int MT = D / 32, KS = D / 16, ROW = Format<D, FMT>::ROW;
+  constexpr int MT = D / 16, KS = D / 32, ROW = Format<D, FMT>::ROW;
   constexpr bool MX = Format<D, FMT>::MX;
-  constexpr int PPR = ROW / 16;    // 16-byte pieces of a row
-  constexpr int NP = PPR / 2;      // pieces per lane and tile of 32 keys (keys; as many for values)
-  constexpr int VB = 32 * D * 2;   // bytes of a wave's value tile
-  const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
+  constexpr int NK = ROW / 64;                  // 16-byte pieces of a lane's quarter of a key row
+  constexpr int KW = NK > 0 ? 4 : ROW / 16;     // words of a piece (half pieces where a quarter row is 8 bytes)
+  constexpr int NKP = NK > 0 ? NK : 1;
+  constexpr int PPR = ROW / 16;                 // 16-byte pieces of a row
+  constexpr int NV = PPR / 2;                   // value pieces per lane and tile
+  constexpr int VB = 32 * D * 2;                // bytes of a wave's value tile
+  const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
 
   const Span all = item_span(p, w, w.row0 / p.group, (w.row0 + w.nrows - 1) / p.group);
   const int tile0 = all.lo >> 5, ntiles_all = all.hi > all.lo ? ((all.hi + 31) >> 5) - tile0 : 0;
   const int tb = tile0 + (int)((long long)ntiles_all * w.chunk / w.nchunks);
   const int te = tile0 + (int)((long long)ntiles_all * (w.chunk + 1) / w.nchunks);
 
-  const int row = min(l32, w.nrows - 1);
-  const int pos = all.pos0 + (w.row0 + row) / p.group;
-  const int row_lo = p.window_left >= 0 ? max(pos - p.window_left, 0) : 0;
-  bf16x8 qf[KS];
-  {
-    const RowOut at(p, w, row);
-    const bf16_t* qp = (const bf16_t*)p.q + (long long)at.token * p.q_stride_n + (long long)at.head * p.q_stride_h + hh * (D / 2);
+  int pos[RB], row_lo[RB];
+  bf16x8 qf[RB][KS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const bf16x8*)(qp + 8 * ks);
+  for (int rb = 0; rb < RB; ++rb) {
+    const int row = min(16 * rb + l16, w.nrows - 1);
+    const RowOut at(p, w, row);
+    pos[rb] = all.pos0 + (w.row0 + row) / p.group;
+    row_lo[rb] = p.window_left >= 0 ? max(pos[rb] - p.window_left, 0) : 0;
+    const bf16_t* qp = (const bf16_t*)p.q + (long long)at.token * p.q_stride_n + (long long)at.head * p.q_stride_h + g4 * (D / 4);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[rb][ks] = *(const bf16x8*)(qp + 8 * ks);
   }
   float c = p.sm_scale * kLog2e, vscale = 1.f;
   if constexpr (FMT == CACHE_FP8) {
@@ -412,147 +476,238 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
   }
   const float slack = c > 0.f ? kRescaleSlack / c : 0.f;
 
-  const char* kbase = (const char*)p.ks.codes + w.kvh * p.stride_head + hh * (ROW / 2);
-  const char* vbase = (const char*)p.vs.codes + w.kvh * p.stride_head;
+  // keys go straight to the operand (the sum over head dims may run in any
+  // order: lane l takes quarter l / 16 of key l % 16's dims), values through
+  // the wave's LDS
+  const char* kbase = (const char*)p.ks.codes + w.kvh * p.stride_head + g4 * (ROW / 4);
+  const char* vbase = (const char*)p.vs.codes + w.kvh * p.stride_head + 16 * (lane % PPR);
   const long long shead = w.kvh * p.scale_stride_head;
+  const uint8_t* ksbase = (const uint8_t*)p.ks.scale + shead + g4 * (D / 4) / 32;
+  const uint8_t* vsbase = (const uint8_t*)p.vs.scale + shead + (FMT == CACHE_MXFP4 ? lane % PPR : lane % PPR / 2);
   const int pmask = (1 << p.log2_page) - 1;
+  const unsigned last_page = (unsigned)p.num_pages - 1u;  // (clamped where used, as above)
   auto key_at = [&](int tile, int i) -> int { return min(max(32 * tile + i, all.lo), all.hi - 1); };
-  auto page_at = [&](int key) -> int {
-    return min((unsigned)p.page_table[w.page_begin + (key >> p.log2_page)], (unsigned)p.num_pages - 1u);
-  };
-  u32x4 kr[NP], vr[NP];
-  unsigned ksc = 0, vsc[NP];
-  // page: the page of this lane's key (l32) of the tile
-  auto fetch_k = [&](int tile, int page) {
-    const int slot = key_at(tile, l32) & pmask;
-    const char* s = kbase + page * p.stride_page + slot * p.stride_tok;
+  auto page_at = [&](int key) -> unsigned { return (unsigned)p.page_table[w.page_begin + (key >> p.log2_page)]; };
+  struct Raw {
+    unsigned k[2][NKP][KW];
+    u32x4 v[NV];
+    unsigned ksc[2], vsc[NV];
+    unsigned next;  // page of this lane's key (l % 32) of the tile after the next one to take these registers
+  } raw[PF];
+  // page: lane l's is the page of key l % 32 of the tile
+  auto fetch_k = [&](Raw& x, int tile, unsigned page) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) kr[i] = *(const u32x4*)(s + 16 * i);
-    if constexpr (MX) {
-      const uint8_t* q = (const uint8_t*)p.ks.scale + page * p.scale_stride_page + slot * p.scale_stride_tok + shead;
-      if constexpr (D == 128) ksc = q[2 * hh] | (unsigned)q[2 * hh + 1] << 8;
-      else ksc = q[hh];
-    }
-  };
-  auto fetch_v = [&](int tile, int page) {
+    for (int b = 0; b < 2; ++b) {
+      const unsigned pg = __shfl(page, 16 * b + l16), slot = key_at(tile, 16 * b + l16) & pmask;
+      const char* s = kbase + row_offset(p, pg, slot);
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int idx = 64 * i + lane, kk = idx / PPR, col = idx % PPR;
-      const int pg = __shfl(page, kk);
-      const int slot = key_at(tile, kk) & pmask;
-      vr[i] = *(const u32x4*)(vbase + pg * p.stride_page + slot * p.stride_tok + 16 * col);
-      if constexpr (MX)
-        vsc[i] = ((const uint8_t*)p.vs.scale)[pg * p.scale_stride_page + slot * p.scale_stride_tok + shead +
-                                              (FMT == CACHE_MXFP4 ? col : col / 2)];
-    }
-  };
-
-  f32x16 o[MT];
+      for (int i = 0; i < NKP; ++i) {
+        if constexpr (KW == 4) {
+          const u32x4 u = *(const u32x4*)(s + 16 * i);
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) o[mt] = f32x16{};
-  float m = -INFINITY, l = 0.f;
-  lds_char* vt = lds + wv * VB;
-  const ValueRead<D> vread(lane);
-
-  int t = tb + wv;
-  int page = 0, pnext = 0;
-  if (t < te) {
-    page = page_at(key_at(t, l32));
-    fetch_k(t, page);
-    fetch_v(t, page);
-    pnext = page_at(key_at(min(t + kChunkWaves, te - 1), l32));
-  }
-  for (; t < te; t += kChunkWaves) {
-    const int tn = min(t + kChunkWaves, te - 1);  // (the last round fetches its own tile again, unused)
-    const int pg = pnext;
-    pnext = page_at(key_at(min(t + 2 * kChunkWaves, te - 1), l32));
-    f32x16 s[1];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      bf16x8 a;
-      if constexpr (FMT == CACHE_BF16) {
-        a = __builtin_bit_cast(bf16x8, kr[ks]);
-      } else {
-        const float f = MX ? block_scale(ksc >> (8 * (ks / 4)) & 255u) : 1.f;
-        if constexpr (FMT == CACHE_MXFP4) a = expand<FMT>(kr[ks / 4][ks % 4], 0u, f);
-        else a = expand<FMT>(kr[ks / 2][2 * (ks % 2)], kr[ks / 2][2 * (ks % 2) + 1], f);
+          for (int e = 0; e < 4; ++e) x.k[b][i][e] = u[e];
+        } else {
+          const u32x2 u = *(const u32x2*)s;
+          x.k[b][i][0] = u[0], x.k[b][i][1] = u[1];
+        }
       }
-      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qf[ks], ks ? s[0] : f32x16{}, 0, 0, 0);
+      if constexpr (MX) x.ksc[b] = ksbase[scale_offset(p, pg, slot)];
     }
-    if (t + kChunkWaves < te) fetch_k(tn, pg);
-    const int kb = 32 * t;
-    if (kb < all.all_lo || kb + 32 > all.all_hi) hide(s[0], kb, row_lo, pos, hh);
+  };
+  auto fetch_v = [&](Raw& x, int tile, unsigned page) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int idx = 64 * i + lane, kk = idx / PPR, col = idx % PPR;
+    for (int i = 0; i < NV; ++i) {
+      const int kk = (64 * i + lane) / PPR;
+      const unsigned pg = __shfl(page, kk), slot = key_at(tile, kk) & pmask;
+      x.v[i] = *(const u32x4*)(vbase + row_offset(p, pg, slot));
+      if constexpr (MX) x.vsc[i] = vsbase[scale_offset(p, pg, slot)];
+    }
+  };
+
+  f32x4 o[RB][MT];
+  float m[RB], l[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) o[rb][mt] = f32x4{};
+    m[rb] = -INFINITY, l[rb] = 0.f;
+  }
+  lds_char* vt = lds + wv * VB;
+  // V^T operands: 16-lane group g reads keys 4g .. 4g + 3 (+ 16 for the second
+  // half) of 16 head dims, the keys its lanes hold probabilities of
+  auto vread = [&](int mt) -> bf16x8 {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const int r = 4 * g4 + (l16 >> 2), ch = 2 * mt + ((l16 & 3) >> 1), in = 8 * (l16 & 1);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_piece<D>(vt, r, ch) + in));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_piece<D>(vt, r + 16, ch) + in));
+    const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+    return __builtin_bit_cast(bf16x8, (u32x4){x[0], x[1], y[0], y[1]});
+  };
+  // maximum / sum over the four lanes of a row
+  auto over_row = [&](float x, auto&& f) -> float {
+    x = f(x, __shfl_xor(x, 16));
+    return f(x, __shfl_xor(x, 32));
+  };
+
+  auto step = [&](Raw& x, int t) {
+    const int tn = t + PF * W;  // the tile that takes these registers next
+    // (page ids are loaded a round before the rows they lead to: the wait for
+    // one is a wait for every load before it)
+    const unsigned pg = min(x.next, last_page);
+    x.next = page_at(key_at(tn + PF * W, lane & 31));
+    f32x4 s[RB][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        bf16x8 a;
+        if constexpr (FMT == CACHE_BF16) {
+          a = __builtin_bit_cast(bf16x8, (u32x4){x.k[b][ks][0], x.k[b][ks][1], x.k[b][ks][2], x.k[b][ks][3]});
+        } else {
+          const float f = MX ? block_scale(x.ksc[b]) : 1.f;
+          constexpr int PER = FMT == CACHE_MXFP4 ? 1 : 2;  // words of 8 codes
+          const int w0 = PER * ks;
+          a = expand<FMT>(x.k[b][w0 / KW][w0 % KW], x.k[b][(w0 + PER - 1) / KW][(w0 + PER - 1) % KW], f);
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          s[rb][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, qf[rb][ks], ks ? s[rb][b] : f32x4{}, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int kk = (64 * i + lane) / PPR, col = lane % PPR;
       if constexpr (FMT == CACHE_BF16) {
-        *(__attribute__((address_space(3))) u32x4*)lds_piece<D>(vt, kk, col) = vr[i];
+        *(__attribute__((address_space(3))) u32x4*)lds_piece<D>(vt, kk, col) = x.v[i];
       } else {
         constexpr int CH = FMT == CACHE_MXFP4 ? 4 : 2;  // 8-element chunks of a piece
-        const float f = MX ? block_scale(vsc[i]) : 1.f;
+        const float f = MX ? block_scale(x.vsc[i]) : 1.f;
 #pragma unroll
         for (int e = 0; e < CH; ++e) {
-          const bf16x8 v = FMT == CACHE_MXFP4 ? expand<FMT>(vr[i][e], 0u, f) : expand<FMT>(vr[i][2 * e & 3], vr[i][(2 * e + 1) & 3], f);
+          const bf16x8 v = FMT == CACHE_MXFP4 ? expand<FMT>(x.v[i][e], 0u, f)
+                                              : expand<FMT>(x.v[i][2 * e & 3], x.v[i][(2 * e + 1) & 3], f);
           *(__attribute__((address_space(3))) bf16x8*)lds_piece<D>(vt, kk, CH * col + e) = v;
         }
       }
     }
-    if (t + kChunkWaves < te) fetch_v(tn, pg);
-    softmax_step<1, MT>(s, o, m, l, c, slack, hh);
-    // (LDS serves a wave's accesses in order; the fence keeps the compiler's order)
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const bf16x8 pb = p_operand(s[0], j);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vread(vt, mt, j), pb, o[mt], 0, 0, 0);
+    if (tn < te) {
+      fetch_k(x, tn, pg);
+      fetch_v(x, tn, pg);
     }
+    const int kb = 32 * t;
+    const bool edge = kb < all.all_lo || kb + 32 > all.all_hi;
+    bf16x8 pb[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = kb + 16 * (i >> 2) + 4 * g4 + (i & 3);
+          s[rb][i >> 2][i & 3] = key >= row_lo[rb] && key <= pos[rb] ? s[rb][i >> 2][i & 3] : -INFINITY;
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[rb][i >> 2][i & 3]);
+      mx = over_row(mx, [](float u, float v) { return fmaxf(u, v); });
+      if (__any(mx > m[rb] + slack)) {
+        const float mn = fmaxf(m[rb], mx);
+        const float a = m[rb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[rb] - mn) * c);
+        l[rb] *= a;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) o[rb][mt] *= a;
+        m[rb] = mn;
+      }
+      const float mc = m[rb] == -INFINITY ? 0.f : m[rb] * c;
+      u32x4 u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[rb][i >> 1][2 * (i & 1)], c, -mc));
+        const float e1 = __builtin_amdgcn_exp2f(fmaf(s[rb][i >> 1][2 * (i & 1) + 1], c, -mc));
+        l[rb] += e0 + e1;
+        u[i] = pack_bf16x2(e0, e1);
+      }
+      pb[rb] = __builtin_bit_cast(bf16x8, u);
+    }
+    // (LDS serves a wave's accesses in order; the fences keep the compiler's order)
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  }
-
-  // join the waves: every wave's m and l, then O in rounds that fit the LDS
-  // (all head dims at once for up to 16 rows, half of them for more)
-  l += xor32(l, hh);
-  float* ms = stats;
-  float* lw = stats + kChunkWaves * kTokenRows;
-  if (hh == 0) {
-    ms[wv * kTokenRows + l32] = m;
-    lw[wv * kTokenRows + l32] = l;
-  }
-  const int nr = w.nrows;
-  const int per_round = nr > 16 ? MT / 2 : MT;
-  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-  for (int mt0 = 0; mt0 < MT; mt0 += per_round) {
-    __syncthreads();  // the tiles, or the last round's states, have been read
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      if (mt < mt0 || mt >= mt0 + per_round || l32 >= nr) continue;
+      const bf16x8 a = vread(mt);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int d4 = 8 * (mt - mt0) + 2 * q + hh;
-        ((lds_f32x4*)lds)[(wv * 8 * per_round + d4) * nr + l32] =
-            (f32x4){o[mt][4 * q], o[mt][4 * q + 1], o[mt][4 * q + 2], o[mt][4 * q + 3]};
-      }
+      for (int rb = 0; rb < RB; ++rb)
+        o[rb][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[rb], o[rb][mt], 0, 0, 0);
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
+
+  const int t0 = tb + wv;
+  unsigned pages[PF];
+#pragma unroll
+  for (int i = 0; i < PF; ++i) {
+    // (keys past the range are clamped to its last one; an item without keys loads nothing)
+    if (te > tb) {
+      raw[i].next = page_at(key_at(t0 + (PF + i) * W, lane & 31));
+      pages[i] = page_at(key_at(t0 + i * W, lane & 31));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PF; ++i) {
+    const int t = t0 + i * W;
+    if (t < te) {
+      const unsigned pg = min(pages[i], last_page);
+      fetch_k(raw[i], t, pg);
+      fetch_v(raw[i], t, pg);
+    }
+  }
+  for (int t = t0; t < te; t += PF * W) {
+#pragma unroll
+    for (int i = 0; i < PF; ++i)
+      if (t + i * W < te) step(raw[i], t + i * W);
+  }
+
+  // join the waves' states through LDS
+  float* ms = stats;
+  float* lw = stats + W * kTokenRows;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const float ls = over_row(l[rb], [](float u, float v) { return u + v; });
+    if (g4 == 0) {
+      ms[wv * kTokenRows + 16 * rb + l16] = m[rb];
+      lw[wv * kTokenRows + 16 * rb + l16] = ls;
+    }
+  }
+  const int nr = w.nrows;
+  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+  // in RB rounds, each of D / RB head dims: W states of 16 RB rows fit the waves' value tiles
+  static_assert(16 * D * 4 <= VB, "the waves' states fit");
+  constexpr int MR = MT / RB;
+#pragma unroll
+  for (int rd = 0; rd < RB; ++rd) {
+    __syncthreads();  // the value tiles, or the last round's states, have been read
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+      if (16 * rb + l16 < nr)
+#pragma unroll
+        for (int mt = 0; mt < MR; ++mt)
+          ((lds_f32x4*)lds)[(wv * 4 * MR + 4 * mt + g4) * nr + 16 * rb + l16] = o[rb][rd * MR + mt];
     __syncthreads();
-    for (int i = tid; i < nr * 8 * per_round; i += 64 * kChunkWaves) {
-      const int r = i % nr, d4 = i / nr;
+    for (int i = tid; i < nr * 4 * MR; i += 64 * W) {
+      const int r = i % nr, d4 = i / nr, dd = 16 * rd * MR + 4 * d4;
       float top = -INFINITY;
 #pragma unroll
-      for (int v = 0; v < kChunkWaves; ++v) top = fmaxf(top, ms[v * kTokenRows + r]);
+      for (int v = 0; v < W; ++v) top = fmaxf(top, ms[v * kTokenRows + r]);
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
       float sum = 0.f;
 #pragma unroll
-      for (int v = 0; v < kChunkWaves; ++v) {
+      for (int v = 0; v < W; ++v) {
         const float mv = ms[v * kTokenRows + r];
         const float a = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mv - top) * c);
         sum += a * lw[v * kTokenRows + r];
-        acc += a * ((lds_f32x4*)lds)[(v * 8 * per_round + d4) * nr + r];
+        acc += a * ((lds_f32x4*)lds)[(v * 4 * MR + d4) * nr + r];
       }
       const float lse2 = sum > 0.f ? top * c + __builtin_amdgcn_logf(sum) : sum == 0.f ? -INFINITY : sum;
       float inv = sum != 0.f ? vscale / sum : 0.f;
-      const int dd = 32 * mt0 + 4 * d4;
       if (w.nchunks > 1) {
         const long long pr = w.slot + (long long)w.chunk * nr + r;
         *(f32x4*)(p.part_o + pr * D + dd) = acc * inv;
@@ -568,15 +723,31 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
   }
 }
 
-template <int D, int FMT>
-__global__ __launch_bounds__(64 * kChunkWaves) void chunk_attn_kernel(const ChunkParams p) {
-  __shared__ __align__(16) char lds[4 * 64 * D * 2];
-  __shared__ float stats[2 * kChunkWaves * kTokenRows];
+// Tiles of 32 keys a wave of a token item has in flight (more than one does
+// not help bf16, whose tiles are 16 KB)
+template <int FMT>
+constexpr int token_depth() {
+  return FMT == CACHE_BF16 ? 1 : 2;
+}
+
+// TOKENS: every item of the plan is a token item of up to 16 rows; kernels of
+// their own, with workgroups of kTokenWaves waves and more waves on a CU.
+template <int D, int FMT, bool TOKENS>
+__global__ __launch_bounds__(64 * (TOKENS ? kTokenWaves : kChunkWaves), TOKENS && FMT == CACHE_MXFP4 ? 3 : 2) void chunk_attn_kernel(const ChunkParams p) {
+  constexpr int W = TOKENS ? kTokenWaves : kChunkWaves;
+  __shared__ __align__(16) char lds[TOKENS ? W * 32 * D * 2 : 4 * 64 * D * 2];
+  __shared__ float stats[2 * W * kTokenRows];
   const ChunkItem w = p.items[blockIdx.x];
-  if (w.kind == CHUNK_TILE)
-    tile_item<D, FMT>(p, w, (lds_char*)lds);
-  else
-    token_item<D, FMT>(p, w, (lds_char*)lds, stats);
+  if constexpr (TOKENS) {
+    token_item<D, FMT, W, 1, token_depth<FMT>()>(p, w, (lds_char*)lds, stats);
+  } else {
+    if (w.kind == CHUNK_TILE)
+      tile_item<D, FMT>(p, w, (lds_char*)lds);
+    else if (w.nrows <= 16)
+      token_item<D, FMT, W, 1, token_depth<FMT>()>(p, w, (lds_char*)lds, stats);
+    else
+      token_item<D, FMT, W, 2, 1>(p, w, (lds_char*)lds, stats);
+  }
 }
 
 // Row i of a merge item from its nchunks partial states: thread (i, d4) holds
@@ -608,30 +779,37 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkParams p) {
   if (dd == 0) p.lse[token * p.lse_stride_n + head] = p.lse_base2 ? lse2 : lse2 * kLn2;
 }
 
-template <int D>
-hipError_t launch_d(const ChunkParams& p, int format, int nitems, int nmerges, hipStream_t s) {
-  const dim3 grid((unsigned)nitems), block(64 * kChunkWaves);
-  if (nitems > 0) {
-    switch (format) {
-      case CACHE_BF16: hipLaunchKernelGGL((chunk_attn_kernel<D, CACHE_BF16>), grid, block, 0, s, p); break;
-      case CACHE_FP8: hipLaunchKernelGGL((chunk_attn_kernel<D, CACHE_FP8>), grid, block, 0, s, p); break;
-      case CACHE_MXFP8: hipLaunchKernelGGL((chunk_attn_kernel<D, CACHE_MXFP8>), grid, block, 0, s, p); break;
-      case CACHE_MXFP4: hipLaunchKernelGGL((chunk_attn_kernel<D, CACHE_MXFP4>), grid, block, 0, s, p); break;
-      default: return hipErrorInvalidValue;
-    }
-  }
+template <int D, int FMT>
+hipError_t launch_f(const ChunkParams& p, bool tokens, int nitems, int nmerges, hipStream_t s) {
+  const dim3 grid((unsigned)nitems), block(64 * (tokens ? kTokenWaves : kChunkWaves));
+  if (tokens)
+    hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, true>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, false>), grid, block, 0, s, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (nmerges > 0) hipLaunchKernelGGL(chunk_merge_kernel<D>, dim3((unsigned)nmerges), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 
+template <int D>
+hipError_t launch_d(const ChunkParams& p, int format, bool tokens, int nitems, int nmerges, hipStream_t s) {
+  switch (format) {
+    case CACHE_BF16: return launch_f<D, CACHE_BF16>(p, tokens, nitems, nmerges, s);
+    case CACHE_FP8: return launch_f<D, CACHE_FP8>(p, tokens, nitems, nmerges, s);
+    case CACHE_MXFP8: return launch_f<D, CACHE_MXFP8>(p, tokens, nitems, nmerges, s);
+    case CACHE_MXFP4: return launch_f<D, CACHE_MXFP4>(p, tokens, nitems, nmerges, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
 }  // namespace
 
-hipError_t launch_chunk_attention(const ChunkParams& p, int head_dim, int format, int nitems, int nmerges,
+hipError_t launch_chunk_attention(const ChunkParams& p, int head_dim, int format, bool tokens, int nitems, int nmerges,
                                   hipStream_t s) {
-  return head_dim == 64    ? launch_d<64>(p, format, nitems, nmerges, s)
-         : head_dim == 128 ? launch_d<128>(p, format, nitems, nmerges, s)
+  if (nitems <= 0) return hipSuccess;
+  return head_dim == 64    ? launch_d<64>(p, format, tokens, nitems, nmerges, s)
+         : head_dim == 128 ? launch_d<128>(p, format, tokens, nitems, nmerges, s)
                            : hipErrorInvalidValue;
 }
 

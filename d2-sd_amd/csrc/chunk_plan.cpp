@@ -11,52 +11,71 @@ namespace d2sd {
 
 namespace {
 
-// Times of a workgroup on a CU of its own, in us (measured at D = 128; half at
-// D = 64): an item's start and end, a 64-key tile of a tile item, a round of
-// 8 x 32 keys of a token item, the share of HBM of one CU (bytes per us), a
-// partial state's extra and the merge launch.
-constexpr double kItemUs = 4.0, kTileUs = 1.4, kRoundUs = 0.8, kCuBytesPerUs = 19500.0, kMergeUs = 4.0;
-
-struct Group {
-  int req, kvh, row0, nrows, kind, units;  // units: 64-key tiles (tile items), 32-key tiles (token items)
-  double unit_us, cost;
-};
+// Measured times in us (D = 128; tiles half as long at D = 64): a workgroup's
+// start and end; a 64-key tile of a tile item; a 32-key tile of one wave of a
+// token item; a merge launch; and rates in bytes per us: what one CU reads at
+// most, what all of them read together, what a merge moves.
+constexpr double kItemUs = 5.0, kTileUs = 1.9, kTokenTileUs = 0.9, kMergeUs = 3.0;
+constexpr double kCuBytes = 57e3, kHbmBytes = 5.4e6, kMergeBytes = 3.0e6;
 
 int row_bytes(int format, int d) {
   return format == CACHE_BF16 ? 2 * d : format == CACHE_FP8 ? d : format == CACHE_MXFP8 ? d + d / 32 : d / 2 + d / 32;
 }
 
-int chunks_of(const Group& g, double limit, int max_splits) {
-  const int least = g.kind == CHUNK_TOKEN ? kChunkWaves : 4;  // units of the shortest chunk
-  const int most = std::max(1, std::min({g.units / least, max_splits, kChunkMaxSplits}));
-  const double work = g.cost - kItemUs;
-  const int want = work <= limit ? 1 : (int)std::min<double>(most, (work + limit - 1e-9) / limit);
-  return std::max(1, std::min(most, want));
-}
+struct Group {         // one row tile of a request, for every kv head
+  int req, row0, nrows, kind;
+  int units, least;    // key tiles, and those of the shortest chunk
+  double unit_us;      // of a tile, alone
+  double unit_read_us; // of that, its bytes at a workgroup's highest rate
+  double work() const { return units * unit_us; }
+  double read_us() const { return units * unit_read_us; }
+};
 
-// Time until the last workgroup ends when the longest start first, one per CU.
-double span_us(const std::vector<Group>& groups, double limit, int max_splits, int cus) {
-  std::vector<double> times;
-  bool split = false;
-  for (const Group& g : groups) {
-    const int n = chunks_of(g, limit, max_splits);
-    split = split || n > 1;
-    for (int c = 0; c < n; ++c) times.push_back((g.cost - kItemUs) / n + kItemUs);
+struct Planner {
+  const ChunkPlanInput& in;
+  std::vector<Group> groups;
+  int places = 1;      // workgroups resident on the device
+  double place_bytes = 0.0;  // highest rate of one of them
+  int most;            // chunks of a group
+
+  int chunks(const Group& g, double limit) const {
+    const int top = std::max(1, std::min(most, g.units / g.least));
+    return g.work() <= limit ? 1 : (int)std::min<double>(top, g.work() / limit + 0.999);
   }
-  std::sort(times.begin(), times.end(), std::greater<double>());
-  std::priority_queue<double, std::vector<double>, std::greater<double>> ends;
-  double last = 0.0;
-  for (double t : times) {
-    double at = 0.0;
-    if ((int)ends.size() >= cus) {
-      at = ends.top();
-      ends.pop();
+
+  // Time until the last workgroup ends when the longest start first.  Token
+  // items that read at the same time share the HBM's rate.
+  double span(double limit) const {
+    std::vector<double> times;
+    double partial = 0.0, readers = 0.0;
+    for (const Group& g : groups)
+      if (g.kind == CHUNK_TOKEN) readers += (double)chunks(g, limit) * in.num_kv_heads;
+    const double slower = std::max(1.0, std::min(readers, (double)places) * place_bytes / kHbmBytes);
+    for (const Group& g : groups) {
+      const int n = chunks(g, limit);
+      if (n > 1) partial += (double)n * g.nrows * in.num_kv_heads * in.head_dim * 8.0;  // written and read
+      const double us = g.kind == CHUNK_TOKEN ? std::max(g.work(), g.read_us() * slower) : g.work();
+      times.insert(times.end(), (size_t)n * in.num_kv_heads, us / n + kItemUs);
     }
-    ends.push(at + t);
-    last = std::max(last, at + t);
+    double last = 0.0;
+    if ((int)times.size() <= places) {
+      for (double t : times) last = std::max(last, t);
+    } else {
+      std::sort(times.begin(), times.end(), std::greater<double>());
+      std::priority_queue<double, std::vector<double>, std::greater<double>> ends;
+      for (double t : times) {
+        double at = 0.0;
+        if ((int)ends.size() >= places) {
+          at = ends.top();
+          ends.pop();
+        }
+        ends.push(at + t);
+        last = std::max(last, at + t);
+      }
+    }
+    return last + (partial > 0.0 ? kMergeUs + partial / kMergeBytes : 0.0);
   }
-  return last + (split ? kMergeUs : 0.0);
-}
+};
 
 }  // namespace
 
@@ -64,14 +83,21 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   out = ChunkPlanOutput{};
   const int group = in.num_qo_heads / in.num_kv_heads;
   const double scale = in.head_dim == 64 ? 0.5 : 1.0;
-  const int max_splits = in.max_splits > 0 ? in.max_splits : kChunkMaxSplits;
-  std::vector<Group> groups;
-  double total = 0.0, longest = 0.0;
+  out.tokens_only = true;
+  for (int r = 0; r < in.num_reqs; ++r)
+    if ((long long)(in.qo_indptr[r + 1] - in.qo_indptr[r]) * group > 16) out.tokens_only = false;
+  // (register bound: chunk_attn_kernel)
+  const int per_cu = !out.tokens_only ? 1 : in.head_dim == 64 ? 3 : in.format == CACHE_MXFP4 ? 3 : 2;
+  const int waves = out.tokens_only ? kTokenWaves : kChunkWaves;
+  Planner pl{in, {}, in.num_cus * per_cu, kCuBytes / per_cu, in.max_splits > 0 ? std::min(in.max_splits, kChunkMaxSplits) : kChunkMaxSplits};
+  double longest = 0.0, total = 0.0;
+  long long count = 0;
   for (int r = 0; r < in.num_reqs; ++r) {
     const int nq = in.qo_indptr[r + 1] - in.qo_indptr[r];
     const long long rows = (long long)nq * group;
     const int kind = rows <= kTokenRows ? CHUNK_TOKEN : CHUNK_TILE;
     const int step = kind == CHUNK_TOKEN ? kTokenRows : kChunkRows, keys_per_unit = kind == CHUNK_TOKEN ? 32 : 64;
+    const double unit_bytes = 2.0 * keys_per_unit * row_bytes(in.format, in.head_dim);
     for (long long row0 = 0; row0 < rows; row0 += step) {
       Group g{};
       g.req = r;
@@ -84,29 +110,30 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
       const long long lo = in.window_left >= 0 ? std::max(first - in.window_left, 0ll) : 0;
       g.units = hi > lo ? (int)((hi + keys_per_unit - 1) / keys_per_unit - lo / keys_per_unit) : 0;
       if (kind == CHUNK_TOKEN) {
-        const double bytes = 2.0 * 32 * row_bytes(in.format, in.head_dim);
-        g.unit_us = std::max(kRoundUs * scale / kChunkWaves, bytes / kCuBytesPerUs);
+        g.unit_read_us = unit_bytes / pl.place_bytes;
+        g.unit_us = std::max(kTokenTileUs * scale / waves, g.unit_read_us);
+        g.least = waves;
       } else {
         g.unit_us = kTileUs * scale;
+        g.least = 4;
       }
-      g.cost = kItemUs + g.units * g.unit_us;
-      for (int h = 0; h < in.num_kv_heads; ++h) {
-        g.kvh = h;
-        groups.push_back(g);
-        total += g.cost - kItemUs;
-        longest = std::max(longest, g.cost - kItemUs);
-      }
+      pl.groups.push_back(g);
+      longest = std::max(longest, g.work());
+      total += g.work() * in.num_kv_heads;
+      count += in.num_kv_heads;
     }
   }
-  // the longest chunk: the one whose schedule ends first, among no split and
-  // shares of an even load
+  // The longest chunk: of no split and of ever shorter ones, the one whose
+  // schedule ends first.  Batches of many groups need only be evened out.
   double limit = longest + 1.0;
-  if (!groups.empty()) {
-    double best = span_us(groups, limit, max_splits, in.num_cus);
-    const double even = total / in.num_cus;
-    for (double f : {1.0, 0.75, 0.5, 0.34, 0.25}) {
-      const double t = span_us(groups, even * f, max_splits, in.num_cus);
-      if (t < best) best = t, limit = even * f;
+  if (count > 0) {
+    double best = pl.span(limit);
+    const double even = total / pl.places;
+    const double shortest = count > 4ll * pl.places ? even * 0.5 : even / 16.0;
+    for (double x = longest * 0.7072; x > shortest && x > 1.0; x *= 0.7072) {
+      if (count > 4ll * pl.places && x > 2.0 * even) continue;
+      const double t = pl.span(x);
+      if (t < best * 0.99) best = t, limit = x;
     }
   }
   struct Timed {
@@ -116,11 +143,10 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   std::vector<Timed> items;
   const int merge_rows = 1024 / in.head_dim;  // rows of one merge workgroup: 256 threads, 4 head dims each
   long long slot = 0;
-  for (const Group& g : groups) {
-    const int n = chunks_of(g, limit, max_splits);
+  for (const Group& g : pl.groups) {
+    const int n = pl.chunks(g, limit);
     ChunkItem it{};
     it.req = g.req;
-    it.kvh = g.kvh;
     it.q0 = in.qo_indptr[g.req];
     it.nq = in.qo_indptr[g.req + 1] - it.q0;
     it.row0 = g.row0;
@@ -128,17 +154,20 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
     it.page_begin = in.page_indptr[g.req];
     it.page_end = in.page_indptr[g.req + 1];
     it.nchunks = n;
-    it.slot = n > 1 ? (int)slot : 0;
     it.kind = g.kind;
-    for (int c = 0; c < n; ++c) {
-      it.chunk = c;
-      items.push_back({(g.cost - kItemUs) / n, it});
-    }
-    if (n > 1) {
-      for (int i = 0; i < g.nrows; i += merge_rows)
-        out.merges.push_back(ChunkMerge{it.q0, g.kvh, g.row0 + i, std::min(merge_rows, g.nrows - i), (int)slot + i,
-                                        g.nrows, n, 0});
-      slot += (long long)n * g.nrows;
+    for (int h = 0; h < in.num_kv_heads; ++h) {
+      it.kvh = h;
+      it.slot = n > 1 ? (int)slot : 0;
+      for (int c = 0; c < n; ++c) {
+        it.chunk = c;
+        items.push_back({g.work() / n, it});
+      }
+      if (n > 1) {
+        for (int i = 0; i < g.nrows; i += merge_rows)
+          out.merges.push_back(ChunkMerge{it.q0, h, g.row0 + i, std::min(merge_rows, g.nrows - i), (int)slot + i, g.nrows,
+                                          n, 0});
+        slot += (long long)n * g.nrows;
+      }
     }
   }
   // Longest first; among equals the kv heads of one key chunk side by side, so

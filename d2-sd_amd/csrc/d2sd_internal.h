@@ -291,7 +291,8 @@ struct CacheParams {
 // (chunk_attention.hip).
 // ---------------------------------------------------------------------------
 constexpr int kChunkWaves = 8;      // waves of a workgroup
-constexpr int kChunkRows = 256;     // packed rows of a tile item (32 per wave)
+constexpr int kTokenWaves = 4;      // the same in plans of token items of up to 16 rows alone
+constexpr int kChunkRows = 32 * kChunkWaves;  // packed rows of a tile item (32 per wave)
 constexpr int kTokenRows = 32;      // packed rows a token item holds at most (all waves share them)
 constexpr int kChunkMaxSplits = 64;
 enum : int { CHUNK_TILE = 0, CHUNK_TOKEN = 1 };
@@ -322,8 +323,9 @@ struct ChunkParams {
   const int* kv_len;
   const int* page_table;
   CacheSide ks, vs;
-  long long stride_page, stride_head, stride_tok;                    // bytes
-  long long scale_stride_page, scale_stride_head, scale_stride_tok;  // bytes
+  unsigned stride_page, stride_tok;              // bytes; page_size * stride_tok < 2^32
+  unsigned scale_stride_page, scale_stride_tok;
+  long long stride_head, scale_stride_head;      // bytes
   float* part_o;                     // [partial row][D]
   float* part_lse;                   // [partial row], base 2; -inf: no key
   const float* sinks;                // nullable, [Hq]

@@ -110,9 +110,11 @@ struct ChunkPlanOutput {
   std::vector<ChunkItem> items;
   std::vector<ChunkMerge> merges;
   long long partial_rows;
+  bool tokens_only;        // every item is a token item of up to 16 rows
 };
 void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out);
-hipError_t launch_chunk_attention(const ChunkParams& p, int head_dim, int format, int nitems, int nmerges,
+// tokens: ChunkPlanOutput::tokens_only
+hipError_t launch_chunk_attention(const ChunkParams& p, int head_dim, int format, bool tokens, int nitems, int nmerges,
                                   hipStream_t s);
 
 // ---- greedy acceptance walk (accept.hip) ----
