@@ -210,7 +210,7 @@ __device__ __forceinline__ float sink_factor(const ChunkParams& p, int head, flo
 // ---- tile items ----
 template <int D, int FMT>
 __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem& w, lds_char* lds) {
-  constexpr int MT = D / 32, KS = D / 16, ROW = Format<D, FMT>::ROW, TB = 64 * D * 2;
+  constexpr int MT = D / 32, KS = D / 16, ROW = Format<D, FMT>::ROW, TB = 64 * D * 2, W = chunk_waves(D);
   constexpr bool MX = Format<D, FMT>::MX;
   const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
 
@@ -249,8 +249,8 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
   auto key_of = [&](int tile, int row_) -> int { return min(max(64 * tile + row_, all.lo), all.hi - 1); };
   const int pmask = (1 << p.log2_page) - 1;
   // bf16: a wave copies 64 / W rows straight into LDS, 1 KB (1024 / ROW rows) at a time
-  constexpr int RPC = 1024 / (2 * D), NC = 64 / kChunkWaves / RPC;  // rows per copy, copies per wave
-  const int crow = wv * (64 / kChunkWaves) + lane / (D / 8);  // of copy 0
+  constexpr int RPC = 1024 / (2 * D), NC = 64 / W / RPC;  // rows per copy, copies per wave
+  const int crow = wv * (64 / W) + lane / (D / 8);  // of copy 0
   const char* kcopy = (const char*)p.ks.codes + w.kvh * p.stride_head;
   const char* vcopy = (const char*)p.vs.codes + w.kvh * p.stride_head;
   unsigned pages[NC];
@@ -265,13 +265,13 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
       const int r = crow + RPC * i;
       const unsigned long long off = row_offset(p, min(pages[i], last_page), key_of(tile, r) & pmask) +
                                      16 * ((lane % (D / 8)) ^ chunk_swizzle<D>(r));
-      const unsigned dst = at + (wv * (64 / kChunkWaves) + RPC * i) * D * 2;
+      const unsigned dst = at + (wv * (64 / W) + RPC * i) * D * 2;
       dma16(kcopy + off, dst);
       dma16(vcopy + off, dst + TB);
     }
   };
   // quantised: thread tid carries 1 / TPR of row tid / TPR through registers
-  constexpr int TPR = kChunkWaves, EPT = D / TPR, WORDS = FMT == CACHE_BF16 ? 1 : ROW / TPR / 4;
+  constexpr int TPR = W, EPT = D / TPR, WORDS = FMT == CACHE_BF16 ? 1 : ROW / TPR / 4;
   const int srow = tid / TPR, spart = tid % TPR;
   const char* kpart = kcopy + spart * (ROW / TPR);
   const char* vpart = vcopy + spart * (ROW / TPR);
@@ -732,9 +732,16 @@ constexpr int token_depth() {
 
 // TOKENS: every item of the plan is a token item of up to 16 rows; kernels of
 // their own, with workgroups of kTokenWaves waves and more waves on a CU.
+// Waves per SIMD: what the registers allow without spilling.
 template <int D, int FMT, bool TOKENS>
-__global__ __launch_bounds__(64 * (TOKENS ? kTokenWaves : kChunkWaves), TOKENS && FMT == CACHE_MXFP4 ? 3 : 2) void chunk_attn_kernel(const ChunkParams p) {
-  constexpr int W = TOKENS ? kTokenWaves : kChunkWaves;
+constexpr int chunk_occupancy() {
+  return TOKENS ? (FMT == CACHE_MXFP4 ? 3 : 2) : D == 64 ? 3 : 2;
+}
+
+template <int D, int FMT, bool TOKENS>
+__global__ __launch_bounds__(64 * (TOKENS ? kTokenWaves : chunk_waves(D)), (chunk_occupancy<D, FMT, TOKENS>())) void
+chunk_attn_kernel(const ChunkParams p) {
+  constexpr int W = TOKENS ? kTokenWaves : chunk_waves(D);
   __shared__ __align__(16) char lds[TOKENS ? W * 32 * D * 2 : 4 * 64 * D * 2];
   __shared__ float stats[2 * W * kTokenRows];
   const ChunkItem w = p.items[blockIdx.x];
@@ -781,7 +788,7 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkParams p) {
 
 template <int D, int FMT>
 hipError_t launch_f(const ChunkParams& p, bool tokens, int nitems, int nmerges, hipStream_t s) {
-  const dim3 grid((unsigned)nitems), block(64 * (tokens ? kTokenWaves : kChunkWaves));
+  const dim3 grid((unsigned)nitems), block(64 * (tokens ? kTokenWaves : chunk_waves(D)));
   if (tokens)
     hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, true>), grid, block, 0, s, p);
   else

@@ -11,11 +11,11 @@ namespace d2sd {
 
 namespace {
 
-// Measured times in us (D = 128; tiles half as long at D = 64): a workgroup's
-// start and end; a 64-key tile of a tile item; a 32-key tile of one wave of a
-// token item; a merge launch; and rates in bytes per us: what one CU reads at
+// Measured times in us: a workgroup's start and end; a 64-key tile of a tile
+// item (D = 64: of half the rows, three workgroups on a CU); a 32-key tile of one
+// wave of a token item (half as long at D = 64); a merge launch; and rates in bytes per us: what one CU reads at
 // most, what all of them read together, what a merge moves.
-constexpr double kItemUs = 5.0, kTileUs = 1.9, kTokenTileUs = 0.9, kMergeUs = 3.0;
+constexpr double kItemUs = 5.0, kTileUs = 1.9, kTileUs64 = 2.0, kTokenTileUs = 0.9, kMergeUs = 3.0;
 constexpr double kCuBytes = 57e3, kHbmBytes = 5.4e6, kMergeBytes = 3.0e6;
 
 int row_bytes(int format, int d) {
@@ -82,13 +82,13 @@ struct Planner {
 void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   out = ChunkPlanOutput{};
   const int group = in.num_qo_heads / in.num_kv_heads;
-  const double scale = in.head_dim == 64 ? 0.5 : 1.0;
+  const double scale = in.head_dim == 64 ? 0.5 : 1.0, tile_us = in.head_dim == 64 ? kTileUs64 : kTileUs;
   out.tokens_only = true;
   for (int r = 0; r < in.num_reqs; ++r)
     if ((long long)(in.qo_indptr[r + 1] - in.qo_indptr[r]) * group > 16) out.tokens_only = false;
   // (register bound: chunk_attn_kernel)
-  const int per_cu = !out.tokens_only ? 1 : in.head_dim == 64 ? 3 : in.format == CACHE_MXFP4 ? 3 : 2;
-  const int waves = out.tokens_only ? kTokenWaves : kChunkWaves;
+  const int per_cu = in.head_dim == 64 ? 3 : !out.tokens_only ? 1 : in.format == CACHE_MXFP4 ? 3 : 2;
+  const int waves = out.tokens_only ? kTokenWaves : chunk_waves(in.head_dim);
   Planner pl{in, {}, in.num_cus * per_cu, kCuBytes / per_cu, in.max_splits > 0 ? std::min(in.max_splits, kChunkMaxSplits) : kChunkMaxSplits};
   double longest = 0.0, total = 0.0;
   long long count = 0;
@@ -96,7 +96,7 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
     const int nq = in.qo_indptr[r + 1] - in.qo_indptr[r];
     const long long rows = (long long)nq * group;
     const int kind = rows <= kTokenRows ? CHUNK_TOKEN : CHUNK_TILE;
-    const int step = kind == CHUNK_TOKEN ? kTokenRows : kChunkRows, keys_per_unit = kind == CHUNK_TOKEN ? 32 : 64;
+    const int step = kind == CHUNK_TOKEN ? kTokenRows : chunk_rows(in.head_dim), keys_per_unit = kind == CHUNK_TOKEN ? 32 : 64;
     const double unit_bytes = 2.0 * keys_per_unit * row_bytes(in.format, in.head_dim);
     for (long long row0 = 0; row0 < rows; row0 += step) {
       Group g{};
@@ -114,7 +114,7 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
         g.unit_us = std::max(kTokenTileUs * scale / waves, g.unit_read_us);
         g.least = waves;
       } else {
-        g.unit_us = kTileUs * scale;
+        g.unit_us = tile_us;
         g.least = 4;
       }
       pl.groups.push_back(g);

@@ -290,9 +290,9 @@ struct CacheParams {
 // Attention of each request's newest tokens over its paged cache
 // (chunk_attention.hip).
 // ---------------------------------------------------------------------------
-constexpr int kChunkWaves = 8;      // waves of a workgroup
+constexpr int chunk_waves(int head_dim) { return head_dim == 64 ? 4 : 8; }  // waves of a workgroup
 constexpr int kTokenWaves = 4;      // the same in plans of token items of up to 16 rows alone
-constexpr int kChunkRows = 32 * kChunkWaves;  // packed rows of a tile item (32 per wave)
+constexpr int chunk_rows(int head_dim) { return 32 * chunk_waves(head_dim); }  // packed rows of a tile item
 constexpr int kTokenRows = 32;      // packed rows a token item holds at most (all waves share them)
 constexpr int kChunkMaxSplits = 64;
 enum : int { CHUNK_TILE = 0, CHUNK_TOKEN = 1 };
