@@ -1332,7 +1332,7 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t ho
     info->format = d->format;
     info->page_size = d->page_size;
     info->window_left = d->window_left;
-    info->tokens_only = out.tokens_only ? 1 : 0;
+    info->form = out.form;
     info->num_page_entries = d->num_reqs > 0 ? d->page_indptr[d->num_reqs] : 0;
     info->workspace_bytes = (size_t)out.partial_rows * (d->head_dim + 1) * sizeof(float);
     if (!host_plan) return D2SD_OK;
@@ -1355,7 +1355,7 @@ int d2sd_chunk_run(const d2sd_chunk_plan_info* info, const d2sd_chunk_run_args* 
   if (int rc = check_cache(a->cache, "chunk_run")) return rc;
   const d2sd_paged_cache& c = a->cache;
   if (c.format != info->format || c.page_size != info->page_size || c.num_kv_heads != info->num_kv_heads ||
-      c.head_dim != info->head_dim)
+      c.head_dim != info->head_dim || info->form < 0 || info->form > d2sd::CHUNK_TOKENS)
     return fail(D2SD_ERR_INVALID_ARG, "chunk_run: the cache is not the one planned for");
   if (!a->plan || !a->kv_len || !a->page_table || !a->q || !a->out || !a->lse)
     return fail(D2SD_ERR_INVALID_ARG, "chunk_run: null pointer");
@@ -1405,7 +1405,7 @@ int d2sd_chunk_run(const d2sd_chunk_plan_info* info, const d2sd_chunk_run_args* 
   p.log2_page = log2_of(c.page_size);
   p.num_pages = c.num_pages;
   p.lse_base2 = a->lse_base2 ? 1 : 0;
-  hipError_t e = d2sd::launch_chunk_attention(p, info->head_dim, info->format, info->tokens_only != 0, info->num_items, info->num_merges,
+  hipError_t e = d2sd::launch_chunk_attention(p, info->head_dim, info->format, info->form, info->num_items, info->num_merges,
                                               (hipStream_t)stream);
   return e == hipSuccess ? D2SD_OK : fail_hip(e, "chunk_run launch");
 }

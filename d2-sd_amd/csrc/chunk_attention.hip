@@ -8,30 +8,36 @@
 // for a chunk of a prompt, a single token, or a batch of both, over a cache in
 // bf16, fp8 (one scale per kv head) or the block formats mxfp8 and mxfp4.
 //
-//   chunk_attn_kernel   one workgroup of 4 waves per work item: packed rows of
-//                       one (request, kv head) against a chunk of their visible
+//   chunk_attn_kernel   one workgroup per work item: packed rows of one
+//                       (request, kv head) against a chunk of their visible
 //                       keys, with a running maximum and sum (one pass over the
 //                       cache), state in registers
 //   chunk_merge_kernel  joins the partial states of rows whose keys were split
 //
 // Rows are packed (token, query head of the kv head) pairs, row = token * g + j,
 // so that a key is read once for all query heads that share it.  S^T = K Q^T
-// and O^T += V^T P^T run on v_mfma_f32_32x32x16_bf16: lane l holds the scores
-// and the output of row l % 32, so the softmax stays in a lane (and its partner
-// l ^ 32), and P^T goes back as an operand without leaving the registers.  Codes
-// are expanded to bf16 by the converters that apply a block's scale as they go;
-// that is exact, so quantised caches cost no accuracy beyond their own.
+// and O^T += V^T P^T: a lane holds scores and output of one row, so the softmax
+// stays in a lane and its one (tile items) or three (token items) partners, and
+// P^T goes back as an operand without leaving the registers.  Codes are expanded
+// to bf16 by the converters that apply a block's scale as they go; that is exact,
+// so quantised caches cost no accuracy beyond their own.
 //
 // Two kinds of item, by packed rows:
-//  * tile items (more than 32 rows): each wave owns 32 rows, the workgroup
-//    stages tiles of 64 keys through registers into LDS (two buffers, one
-//    barrier a tile).  Bound by MFMA beside the softmax's vector instructions.
-//  * token items (up to 32 rows: decoding): all waves share the rows, and wave w
-//    takes every 4th tile of 32 keys.  Keys go from the cache straight to the
-//    MFMA operand: the sum over head dims may run in any order, so lane l takes
-//    the contiguous half l / 32 of key l % 32's dims.  Values pass through the
-//    wave's own LDS to be read transposed.  No barrier until the waves' states
-//    are joined.  Bound by HBM.
+//  * tile items (more than 32 rows): v_mfma_f32_32x32x16_bf16; each wave owns 32
+//    rows, the workgroup stages tiles of 64 keys into LDS (bf16 straight, codes
+//    through registers; two buffers, one barrier a tile).  Bound by MFMA and the
+//    softmax's vector instructions, which the lock-step of the waves lets overlap
+//    only in part: 2 x 2048 tokens at 16384 keys, 32 heads of 128, take 0.97 to
+//    1.03 ms, 1.0 PFLOP/s, where a large library product reaches 1.36; a wave's
+//    tile is 2048 cycles of MFMA (both waves of its SIMD) in 4000.
+//  * token items (up to 32 rows: decoding): v_mfma_f32_16x16x32_bf16; all waves
+//    share the rows, and wave w of W takes every W-th tile of 32 keys.  Keys go
+//    from the cache straight to the MFMA operand: the sum over head dims may run
+//    in any order, so lane l takes the contiguous quarter l / 16 of key l % 16's
+//    dims (through LDS instead: 168 -> 233 us on 32 x 8..32k mxfp4).  Values pass
+//    through the wave's own LDS to be read transposed.  No barrier until the
+//    waves' states are joined.  Bound by HBM: 32 requests of 8..32k tokens read
+//    5.8 TB/s in bf16, 5.2 in mxfp8, 4.5 in mxfp4 (1 KB of a page at a time).
 //
 // Keys outside an item's visible range are never read: their addresses are
 // clamped to the range, so what lies behind a cache's end (or before its
@@ -208,9 +214,9 @@ __device__ __forceinline__ float sink_factor(const ChunkParams& p, int head, flo
 }
 
 // ---- tile items ----
-template <int D, int FMT>
+template <int D, int FMT, int W>
 __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem& w, lds_char* lds) {
-  constexpr int MT = D / 32, KS = D / 16, ROW = Format<D, FMT>::ROW, TB = 64 * D * 2, W = chunk_waves(D);
+  constexpr int MT = D / 32, KS = D / 16, ROW = Format<D, FMT>::ROW, TB = 64 * D * 2;
   constexpr bool MX = Format<D, FMT>::MX;
   const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
 
@@ -494,27 +500,54 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
     unsigned ksc[2], vsc[NV];
     unsigned next;  // page of this lane's key (l % 32) of the tile after the next one to take these registers
   } raw[PF];
+  // Where the rows of every load share a page and none is clamped, the page and
+  // the address stay in scalar registers and a lane adds a constant (32 requests
+  // of 8..32k tokens: bf16 475 -> 460 us, mxfp4 160 -> 156).
+  constexpr int VR = 64 / PPR;  // rows of one load of values
+  const bool shared_pages = (1 << p.log2_page) >= (VR > 16 ? VR : 16);
+  const char* kshared = (const char*)p.ks.codes + w.kvh * p.stride_head;
+  const char* vshared = (const char*)p.vs.codes + w.kvh * p.stride_head;
+  const uint8_t* ksshared = (const uint8_t*)p.ks.scale + shead;
+  const uint8_t* vsshared = (const uint8_t*)p.vs.scale + shead;
+  const unsigned klane = l16 * p.stride_tok + g4 * (ROW / 4), vlane = lane / PPR * p.stride_tok + 16 * (lane % PPR);
+  const unsigned kslane = l16 * p.scale_stride_tok + g4 * (D / 4) / 32;
+  const unsigned vslane = lane / PPR * p.scale_stride_tok + (FMT == CACHE_MXFP4 ? lane % PPR : lane % PPR / 2);
+  auto load_k = [&](unsigned (&d)[NKP][KW], const char* base, unsigned off) {
+#pragma unroll
+    for (int i = 0; i < NKP; ++i) {
+      if constexpr (KW == 4) {
+        const u32x4 u = *(const u32x4*)(base + off + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[i][e] = u[e];
+      } else {
+        const u32x2 u = *(const u32x2*)(base + off);
+        d[i][0] = u[0], d[i][1] = u[1];
+      }
+    }
+  };
   // page: lane l's is the page of key l % 32 of the tile
-  auto fetch_k = [&](Raw& x, int tile, unsigned page) {
+  auto fetch = [&](Raw& x, int tile, unsigned page) {
+    if (shared_pages && 32 * tile >= all.lo && 32 * tile + 32 <= all.hi) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const unsigned pg = __builtin_amdgcn_readlane(page, 16 * b), slot = (32 * tile + 16 * b) & pmask;
+        load_k(x.k[b], kshared + row_offset(p, pg, slot), klane);
+        if constexpr (MX) x.ksc[b] = (ksshared + scale_offset(p, pg, slot))[kslane];
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const unsigned pg = __builtin_amdgcn_readlane(page, VR * i), slot = (32 * tile + VR * i) & pmask;
+        x.v[i] = *(const u32x4*)(vshared + row_offset(p, pg, slot) + vlane);
+        if constexpr (MX) x.vsc[i] = (vsshared + scale_offset(p, pg, slot))[vslane];
+      }
+      return;
+    }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const unsigned pg = __shfl(page, 16 * b + l16), slot = key_at(tile, 16 * b + l16) & pmask;
-      const char* s = kbase + row_offset(p, pg, slot);
-#pragma unroll
-      for (int i = 0; i < NKP; ++i) {
-        if constexpr (KW == 4) {
-          const u32x4 u = *(const u32x4*)(s + 16 * i);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x.k[b][i][e] = u[e];
-        } else {
-          const u32x2 u = *(const u32x2*)s;
-          x.k[b][i][0] = u[0], x.k[b][i][1] = u[1];
-        }
-      }
+      load_k(x.k[b], kbase + row_offset(p, pg, slot), 0u);
       if constexpr (MX) x.ksc[b] = ksbase[scale_offset(p, pg, slot)];
     }
-  };
-  auto fetch_v = [&](Raw& x, int tile, unsigned page) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int kk = (64 * i + lane) / PPR;
@@ -591,8 +624,7 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
       }
     }
     if (tn < te) {
-      fetch_k(x, tn, pg);
-      fetch_v(x, tn, pg);
+      fetch(x, tn, pg);
     }
     const int kb = 32 * t;
     const bool edge = kb < all.all_lo || kb + 32 > all.all_hi;
@@ -641,7 +673,7 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
 
-  const int t0 = tb + wv;
+  const int t0 = tb + __builtin_amdgcn_readfirstlane(wv);
   unsigned pages[PF];
 #pragma unroll
   for (int i = 0; i < PF; ++i) {
@@ -656,8 +688,7 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
     const int t = t0 + i * W;
     if (t < te) {
       const unsigned pg = min(pages[i], last_page);
-      fetch_k(raw[i], t, pg);
-      fetch_v(raw[i], t, pg);
+      fetch(raw[i], t, pg);
     }
   }
   for (int t = t0; t < te; t += PF * W) {
@@ -730,18 +761,17 @@ constexpr int token_depth() {
   return FMT == CACHE_BF16 ? 1 : 2;
 }
 
-// TOKENS: every item of the plan is a token item of up to 16 rows; kernels of
-// their own, with workgroups of kTokenWaves waves and more waves on a CU.
 // Waves per SIMD: what the registers allow without spilling.
-template <int D, int FMT, bool TOKENS>
+template <int D, int FMT, int FORM>
 constexpr int chunk_occupancy() {
-  return TOKENS ? (FMT == CACHE_MXFP4 ? 3 : 2) : D == 64 ? 3 : 2;
+  return FORM == CHUNK_TOKENS ? (FMT == CACHE_MXFP4 ? 3 : 2) : D == 64 ? 3 : 2;
 }
 
-template <int D, int FMT, bool TOKENS>
-__global__ __launch_bounds__(64 * (TOKENS ? kTokenWaves : chunk_waves(D)), (chunk_occupancy<D, FMT, TOKENS>())) void
+template <int D, int FMT, int FORM>
+__global__ __launch_bounds__(64 * chunk_waves(FORM), (chunk_occupancy<D, FMT, FORM>())) void
 chunk_attn_kernel(const ChunkParams p) {
-  constexpr int W = TOKENS ? kTokenWaves : chunk_waves(D);
+  constexpr int W = chunk_waves(FORM);
+  constexpr bool TOKENS = FORM == CHUNK_TOKENS;
   __shared__ __align__(16) char lds[TOKENS ? W * 32 * D * 2 : 4 * 64 * D * 2];
   __shared__ float stats[2 * W * kTokenRows];
   const ChunkItem w = p.items[blockIdx.x];
@@ -749,7 +779,7 @@ chunk_attn_kernel(const ChunkParams p) {
     token_item<D, FMT, W, 1, token_depth<FMT>()>(p, w, (lds_char*)lds, stats);
   } else {
     if (w.kind == CHUNK_TILE)
-      tile_item<D, FMT>(p, w, (lds_char*)lds);
+      tile_item<D, FMT, W>(p, w, (lds_char*)lds);
     else if (w.nrows <= 16)
       token_item<D, FMT, W, 1, token_depth<FMT>()>(p, w, (lds_char*)lds, stats);
     else
@@ -787,12 +817,16 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkParams p) {
 }
 
 template <int D, int FMT>
-hipError_t launch_f(const ChunkParams& p, bool tokens, int nitems, int nmerges, hipStream_t s) {
-  const dim3 grid((unsigned)nitems), block(64 * (tokens ? kTokenWaves : chunk_waves(D)));
-  if (tokens)
-    hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, true>), grid, block, 0, s, p);
-  else
-    hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, false>), grid, block, 0, s, p);
+hipError_t launch_f(const ChunkParams& p, int form, int nitems, int nmerges, hipStream_t s) {
+  const dim3 grid((unsigned)nitems), block(64 * chunk_waves(form));
+  if (form == CHUNK_TOKENS) {
+    hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, CHUNK_TOKENS>), grid, block, 0, s, p);
+  } else if (form == CHUNK_WAVES4) {
+    hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, CHUNK_WAVES4>), grid, block, 0, s, p);
+  } else {
+    if constexpr (D == 64) return hipErrorInvalidValue;  // (the planner gives heads of 64 four waves)
+    else hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, CHUNK_WAVES8>), grid, block, 0, s, p);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (nmerges > 0) hipLaunchKernelGGL(chunk_merge_kernel<D>, dim3((unsigned)nmerges), dim3(256), 0, s, p);
@@ -800,23 +834,23 @@ hipError_t launch_f(const ChunkParams& p, bool tokens, int nitems, int nmerges, 
 }
 
 template <int D>
-hipError_t launch_d(const ChunkParams& p, int format, bool tokens, int nitems, int nmerges, hipStream_t s) {
+hipError_t launch_d(const ChunkParams& p, int format, int form, int nitems, int nmerges, hipStream_t s) {
   switch (format) {
-    case CACHE_BF16: return launch_f<D, CACHE_BF16>(p, tokens, nitems, nmerges, s);
-    case CACHE_FP8: return launch_f<D, CACHE_FP8>(p, tokens, nitems, nmerges, s);
-    case CACHE_MXFP8: return launch_f<D, CACHE_MXFP8>(p, tokens, nitems, nmerges, s);
-    case CACHE_MXFP4: return launch_f<D, CACHE_MXFP4>(p, tokens, nitems, nmerges, s);
+    case CACHE_BF16: return launch_f<D, CACHE_BF16>(p, form, nitems, nmerges, s);
+    case CACHE_FP8: return launch_f<D, CACHE_FP8>(p, form, nitems, nmerges, s);
+    case CACHE_MXFP8: return launch_f<D, CACHE_MXFP8>(p, form, nitems, nmerges, s);
+    case CACHE_MXFP4: return launch_f<D, CACHE_MXFP4>(p, form, nitems, nmerges, s);
     default: return hipErrorInvalidValue;
   }
 }
 
 }  // namespace
 
-hipError_t launch_chunk_attention(const ChunkParams& p, int head_dim, int format, bool tokens, int nitems, int nmerges,
+hipError_t launch_chunk_attention(const ChunkParams& p, int head_dim, int format, int form, int nitems, int nmerges,
                                   hipStream_t s) {
   if (nitems <= 0) return hipSuccess;
-  return head_dim == 64    ? launch_d<64>(p, format, tokens, nitems, nmerges, s)
-         : head_dim == 128 ? launch_d<128>(p, format, tokens, nitems, nmerges, s)
+  return head_dim == 64    ? launch_d<64>(p, format, form, nitems, nmerges, s)
+         : head_dim == 128 ? launch_d<128>(p, format, form, nitems, nmerges, s)
                            : hipErrorInvalidValue;
 }
 

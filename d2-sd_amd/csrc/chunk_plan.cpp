@@ -11,15 +11,23 @@ namespace d2sd {
 
 namespace {
 
-// Measured times in us: a workgroup's start and end; a 64-key tile of a tile
-// item (D = 64: of half the rows, three workgroups on a CU); a 32-key tile of one
-// wave of a token item (half as long at D = 64); a merge launch; and rates in bytes per us: what one CU reads at
-// most, what all of them read together, what a merge moves.
-constexpr double kItemUs = 5.0, kTileUs = 1.9, kTileUs64 = 2.0, kTokenTileUs = 0.9, kMergeUs = 3.0;
+// Measured times in us: a workgroup's start and end; a 32-key tile of one wave
+// of a token item (D = 128; half as long at D = 64); a merge launch; and rates in
+// bytes per us: what one CU reads at most, what all of them read together, what
+// a merge moves.
+constexpr double kItemUs = 5.0, kTokenTileUs = 1.2, kMergeUs = 5.0;
 constexpr double kCuBytes = 57e3, kHbmBytes = 5.4e6, kMergeBytes = 3.0e6;
 
 int row_bytes(int format, int d) {
   return format == CACHE_BF16 ? 2 * d : format == CACHE_FP8 ? d : format == CACHE_MXFP8 ? d + d / 32 : d / 2 + d / 32;
+}
+
+// A 64-key tile of a tile item, with n workgroups on its CU (D = 128: 8 waves
+// alone 2.0; 4 waves, half the rows, 1.35 alone and 2.35 of two; D = 64, 4
+// waves: 1.0, 1.5, 2.0).
+double tile_us(int form, int head_dim, double n) {
+  if (head_dim == 64) return 0.5 + 0.5 * n;
+  return form == CHUNK_WAVES8 ? 2.0 : 0.35 + n;
 }
 
 struct Group {         // one row tile of a request, for every kv head
@@ -33,28 +41,54 @@ struct Group {         // one row tile of a request, for every kv head
 
 struct Planner {
   const ChunkPlanInput& in;
+  int form;
   std::vector<Group> groups;
-  int places = 1;      // workgroups resident on the device
-  double place_bytes = 0.0;  // highest rate of one of them
-  int most;            // chunks of a group
+  int per_cu, places;   // workgroups resident on a CU, on the device
+  double place_bytes;   // highest rate of one of them
+  int most;             // chunks of a group
+  double limit = 0.0;   // the longest chunk, in us of one workgroup alone on its CU
+  double token_share = 1.0;  // of that, a token item's longest
 
-  int chunks(const Group& g, double limit) const {
-    const int top = std::max(1, std::min(most, g.units / g.least));
-    return g.work() <= limit ? 1 : (int)std::min<double>(top, g.work() / limit + 0.999);
+  Planner(const ChunkPlanInput& input, int f) : in(input), form(f) {
+    // (register bound: chunk_attn_kernel)
+    per_cu = form == CHUNK_WAVES8 ? 1 : in.head_dim == 64 ? 3 : form == CHUNK_TOKENS && in.format == CACHE_MXFP4 ? 3 : 2;
+    places = in.num_cus * per_cu;
+    place_bytes = kCuBytes / per_cu;
+    most = in.max_splits > 0 ? std::min(in.max_splits, kChunkMaxSplits) : kChunkMaxSplits;
   }
 
-  // Time until the last workgroup ends when the longest start first.  Token
-  // items that read at the same time share the HBM's rate.
-  double span(double limit) const {
+  void take(Planner&& other) {
+    form = other.form;
+    groups = std::move(other.groups);
+    limit = other.limit;
+    token_share = other.token_share;
+  }
+
+  int chunks(const Group& g) const {
+    const int top = std::max(1, std::min(most, g.units / g.least));
+    const double us = g.kind == CHUNK_TOKEN ? limit * token_share : limit;
+    return g.work() <= us ? 1 : (int)std::min<double>(top, g.work() / us + 0.999);
+  }
+
+  // Time until the last workgroup ends when the longest start first.  Tile items
+  // slow each other down on a CU; token items that read at the same time share
+  // the HBM's rate.
+  double span() const {
     std::vector<double> times;
-    double partial = 0.0, readers = 0.0;
-    for (const Group& g : groups)
-      if (g.kind == CHUNK_TOKEN) readers += (double)chunks(g, limit) * in.num_kv_heads;
-    const double slower = std::max(1.0, std::min(readers, (double)places) * place_bytes / kHbmBytes);
+    double partial = 0.0, readers = 0.0, work = 0.0, longest = 0.0;
     for (const Group& g : groups) {
-      const int n = chunks(g, limit);
+      const int n = chunks(g);
+      work += g.work() * in.num_kv_heads;
+      longest = std::max(longest, g.work() / n);
+      if (g.kind == CHUNK_TOKEN) readers += (double)n * in.num_kv_heads;
+    }
+    const double sharing = longest > 0.0 ? std::min<double>(per_cu, std::max(1.0, work / longest / in.num_cus)) : 1.0;
+    const double slower_tile = tile_us(form, in.head_dim, sharing) / tile_us(form, in.head_dim, 1.0);
+    const double slower_read = std::max(1.0, std::min(readers, (double)places) * place_bytes / kHbmBytes);
+    for (const Group& g : groups) {
+      const int n = chunks(g);
       if (n > 1) partial += (double)n * g.nrows * in.num_kv_heads * in.head_dim * 8.0;  // written and read
-      const double us = g.kind == CHUNK_TOKEN ? std::max(g.work(), g.read_us() * slower) : g.work();
+      const double us = g.kind == CHUNK_TOKEN ? std::max(g.work(), g.read_us() * slower_read) : g.work() * slower_tile;
       times.insert(times.end(), (size_t)n * in.num_kv_heads, us / n + kItemUs);
     }
     double last = 0.0;
@@ -75,6 +109,71 @@ struct Planner {
     }
     return last + (partial > 0.0 ? kMergeUs + partial / kMergeBytes : 0.0);
   }
+
+  // Row tiles, then the longest chunk: of no split and of ever shorter ones, the
+  // one whose schedule ends first.  Batches of many groups need only be evened
+  // out.  Returns its time.
+  double plan() {
+    const int group = in.num_qo_heads / in.num_kv_heads, waves = chunk_waves(form);
+    const double token_us = kTokenTileUs * (in.head_dim == 64 ? 0.5 : 1.0) / waves;
+    double longest = 0.0, total = 0.0;
+    bool tiles = false, tokens = false;
+    for (int r = 0; r < in.num_reqs; ++r) {
+      const int nq = in.qo_indptr[r + 1] - in.qo_indptr[r];
+      const long long rows = (long long)nq * group;
+      const int kind = rows <= kTokenRows ? CHUNK_TOKEN : CHUNK_TILE;
+      const int step = kind == CHUNK_TOKEN ? kTokenRows : chunk_rows(form), keys_per_unit = kind == CHUNK_TOKEN ? 32 : 64;
+      const double unit_bytes = 2.0 * keys_per_unit * row_bytes(in.format, in.head_dim);
+      for (long long row0 = 0; row0 < rows; row0 += step) {
+        Group g{};
+        g.req = r;
+        g.row0 = (int)row0;
+        g.nrows = (int)std::min<long long>(step, rows - row0);
+        g.kind = kind;
+        const long long pos0 = (long long)in.kv_len[r] - nq;
+        const long long first = pos0 + row0 / group, last = pos0 + (row0 + g.nrows - 1) / group;
+        const long long hi = std::max(last + 1, 0ll);
+        const long long lo = in.window_left >= 0 ? std::max(first - in.window_left, 0ll) : 0;
+        g.units = hi > lo ? (int)((hi + keys_per_unit - 1) / keys_per_unit - lo / keys_per_unit) : 0;
+        (kind == CHUNK_TOKEN ? tokens : tiles) = true;
+        if (kind == CHUNK_TOKEN) {
+          g.unit_read_us = unit_bytes / place_bytes;
+          g.unit_us = std::max(token_us, g.unit_read_us);
+          g.least = waves;
+        } else {
+          g.unit_us = tile_us(form, in.head_dim, 1.0);
+          g.least = 4;
+        }
+        groups.push_back(g);
+        longest = std::max(longest, g.work());
+        total += g.work() * in.num_kv_heads;
+      }
+    }
+    limit = longest + 1.0;
+    if (groups.empty()) return 0.0;
+    const bool many = (double)groups.size() * in.num_kv_heads > 4.0 * places;
+    double best = span(), best_limit = limit;
+    const double even = total / places, shortest = many ? even * 0.5 : even / 16.0;
+    for (double x = longest * 0.7072; x > shortest && x > 1.0; x *= 0.7072) {
+      if (many && x > 2.0 * even) continue;
+      limit = x;
+      const double t = span();
+      if (t < best * 0.99) best = t, best_limit = x;
+    }
+    limit = best_limit;
+    // beside tile items, shorter chunks for the token items alone (their partial
+    // states are small)
+    double best_share = 1.0;
+    if (tiles && tokens) {
+      for (double share : {0.7, 0.5, 0.35}) {
+        token_share = share;
+        const double t = span();
+        if (t < best * 0.99) best = t, best_share = share;
+      }
+    }
+    token_share = best_share;
+    return best;
+  }
 };
 
 }  // namespace
@@ -82,60 +181,19 @@ struct Planner {
 void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   out = ChunkPlanOutput{};
   const int group = in.num_qo_heads / in.num_kv_heads;
-  const double scale = in.head_dim == 64 ? 0.5 : 1.0, tile_us = in.head_dim == 64 ? kTileUs64 : kTileUs;
-  out.tokens_only = true;
+  bool tokens_only = true;
   for (int r = 0; r < in.num_reqs; ++r)
-    if ((long long)(in.qo_indptr[r + 1] - in.qo_indptr[r]) * group > 16) out.tokens_only = false;
-  // (register bound: chunk_attn_kernel)
-  const int per_cu = in.head_dim == 64 ? 3 : !out.tokens_only ? 1 : in.format == CACHE_MXFP4 ? 3 : 2;
-  const int waves = out.tokens_only ? kTokenWaves : chunk_waves(in.head_dim);
-  Planner pl{in, {}, in.num_cus * per_cu, kCuBytes / per_cu, in.max_splits > 0 ? std::min(in.max_splits, kChunkMaxSplits) : kChunkMaxSplits};
-  double longest = 0.0, total = 0.0;
-  long long count = 0;
-  for (int r = 0; r < in.num_reqs; ++r) {
-    const int nq = in.qo_indptr[r + 1] - in.qo_indptr[r];
-    const long long rows = (long long)nq * group;
-    const int kind = rows <= kTokenRows ? CHUNK_TOKEN : CHUNK_TILE;
-    const int step = kind == CHUNK_TOKEN ? kTokenRows : chunk_rows(in.head_dim), keys_per_unit = kind == CHUNK_TOKEN ? 32 : 64;
-    const double unit_bytes = 2.0 * keys_per_unit * row_bytes(in.format, in.head_dim);
-    for (long long row0 = 0; row0 < rows; row0 += step) {
-      Group g{};
-      g.req = r;
-      g.row0 = (int)row0;
-      g.nrows = (int)std::min<long long>(step, rows - row0);
-      g.kind = kind;
-      const long long pos0 = (long long)in.kv_len[r] - nq;
-      const long long first = pos0 + row0 / group, last = pos0 + (row0 + g.nrows - 1) / group;
-      const long long hi = std::max(last + 1, 0ll);
-      const long long lo = in.window_left >= 0 ? std::max(first - in.window_left, 0ll) : 0;
-      g.units = hi > lo ? (int)((hi + keys_per_unit - 1) / keys_per_unit - lo / keys_per_unit) : 0;
-      if (kind == CHUNK_TOKEN) {
-        g.unit_read_us = unit_bytes / pl.place_bytes;
-        g.unit_us = std::max(kTokenTileUs * scale / waves, g.unit_read_us);
-        g.least = waves;
-      } else {
-        g.unit_us = tile_us;
-        g.least = 4;
-      }
-      pl.groups.push_back(g);
-      longest = std::max(longest, g.work());
-      total += g.work() * in.num_kv_heads;
-      count += in.num_kv_heads;
-    }
+    if ((long long)(in.qo_indptr[r + 1] - in.qo_indptr[r]) * group > 16) tokens_only = false;
+  // Heads of 128: workgroups of 8 waves share a tile's staging among more rows
+  // (2 x 2048 tokens at 16384: 1.03 against 1.13 ms), those of 4 fill the device
+  // with fewer rows (1000 tokens at 2100: 50 us against 65 unsplit).
+  Planner pl(in, tokens_only ? CHUNK_TOKENS : CHUNK_WAVES4);
+  const double us = pl.plan();
+  if (!tokens_only && in.head_dim == 128) {
+    Planner other(in, CHUNK_WAVES8);
+    if (other.plan() < us) pl.take(std::move(other));
   }
-  // The longest chunk: of no split and of ever shorter ones, the one whose
-  // schedule ends first.  Batches of many groups need only be evened out.
-  double limit = longest + 1.0;
-  if (count > 0) {
-    double best = pl.span(limit);
-    const double even = total / pl.places;
-    const double shortest = count > 4ll * pl.places ? even * 0.5 : even / 16.0;
-    for (double x = longest * 0.7072; x > shortest && x > 1.0; x *= 0.7072) {
-      if (count > 4ll * pl.places && x > 2.0 * even) continue;
-      const double t = pl.span(x);
-      if (t < best * 0.99) best = t, limit = x;
-    }
-  }
+  out.form = pl.form;
   struct Timed {
     double us;
     ChunkItem item;
@@ -144,7 +202,7 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   const int merge_rows = 1024 / in.head_dim;  // rows of one merge workgroup: 256 threads, 4 head dims each
   long long slot = 0;
   for (const Group& g : pl.groups) {
-    const int n = pl.chunks(g, limit);
+    const int n = pl.chunks(g);
     ChunkItem it{};
     it.req = g.req;
     it.q0 = in.qo_indptr[g.req];

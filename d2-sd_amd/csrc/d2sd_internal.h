@@ -290,9 +290,11 @@ struct CacheParams {
 // Attention of each request's newest tokens over its paged cache
 // (chunk_attention.hip).
 // ---------------------------------------------------------------------------
-constexpr int chunk_waves(int head_dim) { return head_dim == 64 ? 4 : 8; }  // waves of a workgroup
-constexpr int kTokenWaves = 4;      // the same in plans of token items of up to 16 rows alone
-constexpr int chunk_rows(int head_dim) { return 32 * chunk_waves(head_dim); }  // packed rows of a tile item
+// Kernels that a plan may be for: workgroups of 8 or 4 waves, or those of plans
+// of token items of up to 16 rows alone (4 waves)
+enum ChunkForm : int { CHUNK_WAVES8 = 0, CHUNK_WAVES4 = 1, CHUNK_TOKENS = 2 };
+constexpr int chunk_waves(int form) { return form == CHUNK_WAVES8 ? 8 : 4; }
+constexpr int chunk_rows(int form) { return 32 * chunk_waves(form); }  // packed rows of a tile item (32 per wave)
 constexpr int kTokenRows = 32;      // packed rows a token item holds at most (all waves share them)
 constexpr int kChunkMaxSplits = 64;
 enum : int { CHUNK_TILE = 0, CHUNK_TOKEN = 1 };

@@ -110,11 +110,10 @@ struct ChunkPlanOutput {
   std::vector<ChunkItem> items;
   std::vector<ChunkMerge> merges;
   long long partial_rows;
-  bool tokens_only;        // every item is a token item of up to 16 rows
+  int form;                // ChunkForm: the kernel that the items are for
 };
 void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out);
-// tokens: ChunkPlanOutput::tokens_only
-hipError_t launch_chunk_attention(const ChunkParams& p, int head_dim, int format, bool tokens, int nitems, int nmerges,
+hipError_t launch_chunk_attention(const ChunkParams& p, int head_dim, int format, int form, int nitems, int nmerges,
                                   hipStream_t s);
 
 // ---- greedy acceptance walk (accept.hip) ----

@@ -345,7 +345,7 @@ class ChunkPlanInfo(C.Structure):
         ("page_size", C.c_int),
         ("window_left", C.c_int),
         ("num_page_entries", C.c_int),
-        ("tokens_only", C.c_int),
+        ("form", C.c_int),
         ("workspace_bytes", C.c_size_t),
     ]
 

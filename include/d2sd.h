@@ -660,7 +660,7 @@ typedef struct {
   int page_size;
   int window_left;
   int num_page_entries;  /* page_table entries the plan may read */
-  int tokens_only;       /* 1: no request has more than 16 (query, query head of a kv head) rows */
+  int form;              /* which of its kernels the plan is for */
   size_t workspace_bytes;
 } d2sd_chunk_plan_info;
 
