@@ -15,8 +15,9 @@
 // is exact.  A block that holds an infinity or NaN gets the scale byte 255 and
 // reads back as NaN.
 //
-// Both kernels move data once: bound by HBM (or, for a step's few tokens, by
-// the chain token -> cache length -> page id -> store).  A thread carries 8
+// Both kernels move data once: bound by HBM (16 requests, 0.26 GB read back:
+// 94 us, 4.8 TB/s, where a large copy reaches 4.96) or, for a step's few tokens,
+// by the chain token -> cache length -> page id -> store (64 tokens: 3 us).  A thread carries 8
 // elements: a 16-byte bf16 load or store against 8 bytes (fp8, mxfp8) or 4
 // (mxfp4) of codes; the four threads of a block of 32 find its amax by DPP.
 #include <hip/hip_runtime.h>
@@ -31,7 +32,12 @@ namespace d2sd {
 
 namespace {
 
-constexpr int kReadUnroll = 4;
+constexpr int kWriteTokens = 8;         // of one block, where there are many
+constexpr int kWriteManyTokens = 8192;
+// Results larger than half of the last-level cache are stored past it: nothing
+// of them would be found there by whoever reads them from their start (16
+// requests of 100..8000 tokens, 0.26 GB: 99 -> 94 us).
+constexpr long long kReadStreamBytes = 128ll << 20;
 
 // 2^(byte - 127); byte 255 stands for NaN, byte 0 for 2^-127
 __device__ __forceinline__ float block_scale(unsigned byte) {
@@ -44,14 +50,6 @@ __device__ __forceinline__ unsigned fp8x4(float f0, float f1, float f2, float f3
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(f0, f1, 0, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(f2, f3, w, true);
   return (unsigned)w;
-}
-
-// e2m1 code of f, |f| <= 6, ties to the even code: below 2 the step is 1/2,
-// below 4 it is 1, below 6 it is 2, and codes count the steps.
-__device__ __forceinline__ unsigned fp4_code(float f) {
-  const float a = fabsf(f);
-  const float r = a < 2.f ? rintf(2.f * a) : a < 4.f ? rintf(a) + 2.f : rintf(0.5f * a) + 4.f;
-  return (unsigned)r | (__float_as_uint(f) >> 31 << 3);
 }
 
 __device__ __forceinline__ void expand8(const u32x4& u, float (&x)[8]) {
@@ -118,8 +116,10 @@ __device__ __forceinline__ void store_piece(const CacheSide& s, int fmt_head, lo
       for (int i = 0; i < 8; ++i) x[i] = finite ? fminf(fmaxf(x[i] * inv, -M), M) : 0.f;
       if constexpr (FP4) {
         unsigned w = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w |= fp4_code(x[i]) << (4 * i);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], 1.f, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], 1.f, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], 1.f, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], 1.f, 3);
         *(unsigned*)((uint8_t*)s.codes + row + d / 2) = w;
       } else {
         *(u32x2*)((uint8_t*)s.codes + row + d) =
@@ -130,34 +130,70 @@ __device__ __forceinline__ void store_piece(const CacheSide& s, int fmt_head, lo
   }
 }
 
-// Block t: new token t, all heads, keys then values.  tokens[t] = (request,
-// tokens from it to its request's end, first page table entry, page table end).
-template <int FMT>
+// The places of N tokens, in scalar registers: lane i of a wave found token i's
+// page (below zero: none) and slot.  Built where all lanes are active.
+template <int N>
+struct Places {
+  int page[N], slot[N];
+  __device__ __forceinline__ Places(int pg, int sl) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      page[i] = __builtin_amdgcn_readlane(pg, i);
+      slot[i] = __builtin_amdgcn_readlane(sl, i);
+    }
+  }
+  __device__ __forceinline__ bool on(int i) const { return page[i] >= 0; }
+  __device__ __forceinline__ long long row(const CacheParams& p, int i) const {
+    return page[i] * p.stride_page + slot[i] * p.stride_tok;
+  }
+  __device__ __forceinline__ long long scale_row(const CacheParams& p, int i) const {
+    return page[i] * p.scale_stride_page + slot[i] * p.scale_stride_tok;
+  }
+};
+
+// Block b: new tokens TOK b .., all heads, keys then values.  tokens[t] =
+// (request, tokens from it to its request's end, first page table entry, page
+// table end).  A thread takes the same piece of every token: TOK = 8 keeps as
+// many loads in flight and starts fewer blocks (16.3k tokens of 8 heads of 128 in mxfp4: 35 -> 22 us, 84 MB at 3.8 TB/s),
+// TOK = 1 spreads a step's few tokens.
+template <int FMT, int TOK>
 __global__ __launch_bounds__(256) void cache_write_kernel(const CacheParams p) {
-  const int t = blockIdx.x;
-  const int4 w = ((const int4*)p.items)[t];
+  const int t0 = blockIdx.x * TOK, nt = min(TOK, p.num_items - t0);
   const int cpr = p.head_dim / 8, nch = p.num_kv_heads * cpr;
+  u32x4 val[TOK];
   // the rows' loads first: they do not wait for the place they go to
-  auto source = [&](int c) {
-    const bool is_v = c >= nch;
-    const int cc = is_v ? c - nch : c, h = cc / cpr, d = 8 * (cc - h * cpr);
-    return *(const u32x4*)((const uint16_t*)(is_v ? p.v : p.k) + (long long)t * p.stride_n + (long long)h * p.stride_h + d);
+  auto source = [&](bool is_v, int h, int d) {
+    const uint16_t* s = (const uint16_t*)(is_v ? p.v : p.k) + (long long)t0 * p.stride_n + (long long)h * p.stride_h + d;
+#pragma unroll
+    for (int i = 0; i < TOK; ++i)
+      if (i < nt) val[i] = *(const u32x4*)(s + i * p.stride_n);
   };
+  auto head_of = [&](int c) { return (c >= nch ? c - nch : c) / cpr; };
   int c = threadIdx.x;
-  u32x4 val = c < 2 * nch ? source(c) : u32x4{};
-  const int pos = p.kv_len[w.x] - w.y;
-  const int at = w.z + (pos >> p.log2_page);
-  if (pos < 0 || at >= w.w) return;  // before the cache's start, or no page is reserved for it
-  const int page = p.page_table[at];
-  if (page < 0 || page >= p.num_pages) return;
-  const int slot = pos & ((1 << p.log2_page) - 1);
-  for (; c < 2 * nch; c += blockDim.x) {
+  int h = head_of(c), d = 8 * ((c >= nch ? c - nch : c) - h * cpr);
+  if (c < 2 * nch) source(c >= nch, h, d);
+  const int lane = threadIdx.x & 63;
+  int page = -1, slot = 0;
+  if (lane < nt) {
+    const int4 w = ((const int4*)p.items)[t0 + lane];
+    const int pos = p.kv_len[w.x] - w.y;
+    const int at = w.z + (pos >> p.log2_page);
+    slot = pos & ((1 << p.log2_page) - 1);
+    // (before the cache's start, or no page is reserved for it: nothing to write)
+    if (pos >= 0 && at < w.w) page = p.page_table[at];
+    if (page >= p.num_pages) page = -1;
+  }
+  const Places<TOK> places(page, slot);
+  while (c < 2 * nch) {
     const bool is_v = c >= nch;
-    const int cc = is_v ? c - nch : c, h = cc / cpr, d = 8 * (cc - h * cpr);
     const CacheSide& s = is_v ? p.vs : p.ks;
-    store_piece<FMT>(s, h, page * p.stride_page + h * p.stride_head + slot * p.stride_tok,
-                     page * p.scale_stride_page + h * p.scale_stride_head + slot * p.scale_stride_tok, d, val);
-    if (c + (int)blockDim.x < 2 * nch) val = source(c + blockDim.x);
+    const long long row = h * p.stride_head, srow = h * p.scale_stride_head;
+#pragma unroll
+    for (int i = 0; i < TOK; ++i)
+      if (places.on(i)) store_piece<FMT>(s, h, row + places.row(p, i), srow + places.scale_row(p, i), d, val[i]);
+    c += blockDim.x;
+    h = head_of(c), d = 8 * ((c >= nch ? c - nch : c) - h * cpr);
+    if (c < 2 * nch) source(c >= nch, h, d);
   }
 }
 
@@ -199,67 +235,103 @@ __device__ __forceinline__ u32x4 load_piece(const CacheSide& s, int h, long long
 }
 
 // Block i: up to kReadTokens cached tokens of one request, all heads, keys then
-// values.  items[i] = (request | token count << 24.., see CacheReadItem).
-template <int FMT>
+// values (items[i]: CacheReadItem).  A thread takes the same piece of every
+// token, or, where a token has at most 128 pieces, of every n-th one; the tokens'
+// pages are found once, by one lane each.  One load, then its store: with 8 loads
+// in flight a thread's stores scatter over 8 rows (99 -> 117 us).
+template <int FMT, bool STREAM>
 __global__ __launch_bounds__(256) void cache_read_kernel(const CacheParams p) {
   const CacheReadItem w = ((const CacheReadItem*)p.items)[blockIdx.x];
   const int len = p.kv_len[w.req];
   const int pos0 = w.from_end ? len - w.first : w.first;  // cache position of the item's first token
-  const int cpr = p.head_dim / 8, row_ch = p.num_kv_heads * cpr, nch = w.count * row_ch;
-  for (int c0 = threadIdx.x; c0 < 2 * nch; c0 += kReadUnroll * blockDim.x) {
-    u32x4 val[kReadUnroll];
-    long long dst[kReadUnroll];
-    bool on[kReadUnroll];
-#pragma unroll
-    for (int u = 0; u < kReadUnroll; ++u) {
-      const int c = c0 + u * (int)blockDim.x;
-      const bool is_v = c >= nch;
-      const int cc = is_v ? c - nch : c;
-      const int i = cc / row_ch, r = cc - i * row_ch, h = r / cpr, d = 8 * (r - h * cpr);
-      const int pos = pos0 + i, at = w.page_begin + (pos >> p.log2_page);
-      on[u] = c < 2 * nch && pos >= 0 && pos < len && at < w.page_end;
-      const int page = on[u] ? p.page_table[at] : 0;
-      on[u] = on[u] && page >= 0 && page < p.num_pages;
-      dst[u] = (long long)(w.row + i) * p.stride_n + (long long)h * p.stride_h + d;
-      val[u] = u32x4{};
-      if (on[u]) {
-        const int slot = pos & ((1 << p.log2_page) - 1);
-        val[u] = load_piece<FMT>(is_v ? p.vs : p.ks, h,
-                                 page * p.stride_page + h * p.stride_head + slot * p.stride_tok,
-                                 page * p.scale_stride_page + h * p.scale_stride_head + slot * p.scale_stride_tok, d);
+  const int cpr = p.head_dim / 8, nch = p.num_kv_heads * cpr;
+  const int lane = threadIdx.x & 63;
+  int page = -1, slot = 0;
+  if (lane < w.count) {
+    const int pos = pos0 + lane, at = w.page_begin + (pos >> p.log2_page);
+    slot = pos & ((1 << p.log2_page) - 1);
+    if (pos >= 0 && pos < len && at < w.page_end) page = p.page_table[at];
+    if (page >= p.num_pages) page = -1;
+  }
+  auto piece = [&](int c, auto&& tokens) {
+    const bool is_v = c >= nch;
+    const int cc = is_v ? c - nch : c, h = cc / cpr, d = 8 * (cc - h * cpr);
+    const long long row = h * p.stride_head, srow = h * p.scale_stride_head;
+    uint16_t* out = (uint16_t*)(is_v ? p.v : p.k) + (long long)w.row * p.stride_n + (long long)h * p.stride_h + d;
+    tokens(is_v ? p.vs : p.ks, h, d, row, srow, out);
+  };
+  const int apart = 256 / (2 * nch);  // threads of a piece
+  if (apart > 1) {
+    const int first = threadIdx.x / (2 * nch);
+    piece(threadIdx.x - first * 2 * nch, [&](const CacheSide& s, int h, int d, long long row, long long srow, uint16_t* out) {
+      for (int i0 = 0; i0 < kReadTokens; i0 += apart) {  // (every lane stays for the shuffles)
+        const int i = i0 + first, pg = __shfl(page, i), sl = __shfl(slot, i);
+        if (first < apart && i < w.count && pg >= 0)
+          *(u32x4*)(out + i * p.stride_n) = load_piece<FMT>(s, h, row + pg * p.stride_page + sl * p.stride_tok,
+                                                            srow + pg * p.scale_stride_page + sl * p.scale_stride_tok, d);
       }
-    }
+    });
+    return;
+  }
+  const Places<kReadTokens> places(page, slot);
+  for (int c = threadIdx.x; c < 2 * nch; c += 256) {
+    piece(c, [&](const CacheSide& s, int h, int d, long long row, long long srow, uint16_t* out) {
 #pragma unroll
-    for (int u = 0; u < kReadUnroll; ++u)
-      if (on[u]) *(u32x4*)((uint16_t*)(c0 + u * (int)blockDim.x >= nch ? p.v : p.k) + dst[u]) = val[u];
+      for (int i = 0; i < kReadTokens; ++i) {
+        if (!places.on(i)) continue;
+        const u32x4 val = load_piece<FMT>(s, h, row + places.row(p, i), srow + places.scale_row(p, i), d);
+        u32x4* at = (u32x4*)(out + i * p.stride_n);
+        if constexpr (STREAM)
+          __builtin_nontemporal_store(val, at);
+        else
+          *at = val;
+      }
+    });
   }
 }
 
 }  // namespace
 
-hipError_t launch_cache_write(const CacheParams& p, int format, hipStream_t s) {
-  if (p.num_items <= 0) return hipSuccess;
-  const dim3 grid((unsigned)p.num_items);
+template <int FMT>
+static void launch_write(const CacheParams& p, hipStream_t s) {
   const int pieces = 2 * p.num_kv_heads * (p.head_dim / 8);
   const dim3 block((unsigned)std::min(256, (pieces + 63) / 64 * 64));
+  // (kWriteManyTokens: blocks of kWriteTokens still give every CU four)
+  if (p.num_items >= kWriteManyTokens)
+    hipLaunchKernelGGL((cache_write_kernel<FMT, kWriteTokens>), dim3((unsigned)((p.num_items + kWriteTokens - 1) / kWriteTokens)),
+                       block, 0, s, p);
+  else
+    hipLaunchKernelGGL((cache_write_kernel<FMT, 1>), dim3((unsigned)p.num_items), block, 0, s, p);
+}
+
+hipError_t launch_cache_write(const CacheParams& p, int format, hipStream_t s) {
+  if (p.num_items <= 0) return hipSuccess;
   switch (format) {
-    case CACHE_BF16: hipLaunchKernelGGL(cache_write_kernel<CACHE_BF16>, grid, block, 0, s, p); break;
-    case CACHE_FP8: hipLaunchKernelGGL(cache_write_kernel<CACHE_FP8>, grid, block, 0, s, p); break;
-    case CACHE_MXFP8: hipLaunchKernelGGL(cache_write_kernel<CACHE_MXFP8>, grid, block, 0, s, p); break;
-    case CACHE_MXFP4: hipLaunchKernelGGL(cache_write_kernel<CACHE_MXFP4>, grid, block, 0, s, p); break;
+    case CACHE_BF16: launch_write<CACHE_BF16>(p, s); break;
+    case CACHE_FP8: launch_write<CACHE_FP8>(p, s); break;
+    case CACHE_MXFP8: launch_write<CACHE_MXFP8>(p, s); break;
+    case CACHE_MXFP4: launch_write<CACHE_MXFP4>(p, s); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
 }
 
+template <int FMT>
+static void launch_read(const CacheParams& p, hipStream_t s) {
+  const dim3 grid((unsigned)p.num_items), block(256);
+  if (4ll * p.num_kv_heads * p.head_dim * kReadTokens * p.num_items > kReadStreamBytes)
+    hipLaunchKernelGGL((cache_read_kernel<FMT, true>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((cache_read_kernel<FMT, false>), grid, block, 0, s, p);
+}
+
 hipError_t launch_cache_read(const CacheParams& p, int format, hipStream_t s) {
   if (p.num_items <= 0) return hipSuccess;
-  const dim3 grid((unsigned)p.num_items), block(256);
   switch (format) {
-    case CACHE_BF16: hipLaunchKernelGGL(cache_read_kernel<CACHE_BF16>, grid, block, 0, s, p); break;
-    case CACHE_FP8: hipLaunchKernelGGL(cache_read_kernel<CACHE_FP8>, grid, block, 0, s, p); break;
-    case CACHE_MXFP8: hipLaunchKernelGGL(cache_read_kernel<CACHE_MXFP8>, grid, block, 0, s, p); break;
-    case CACHE_MXFP4: hipLaunchKernelGGL(cache_read_kernel<CACHE_MXFP4>, grid, block, 0, s, p); break;
+    case CACHE_BF16: launch_read<CACHE_BF16>(p, s); break;
+    case CACHE_FP8: launch_read<CACHE_FP8>(p, s); break;
+    case CACHE_MXFP8: launch_read<CACHE_MXFP8>(p, s); break;
+    case CACHE_MXFP4: launch_read<CACHE_MXFP4>(p, s); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();

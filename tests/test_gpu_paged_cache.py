@@ -211,6 +211,30 @@ def test_offsets_past_32_bits():
     assert c.k_pool.numel() > 2 ** 32
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hkv,d,layout", [(3, 96, "HND"), (1, 64, "NHD")])
+def test_prompts_of_many_tokens(fmt, hkv, d, layout):
+    """Thousands of tokens of ragged requests, one of which holds fewer tokens than it has new ones; a padded batch."""
+    g = torch.Generator().manual_seed(d)
+    P = 16
+    qo, kv = [4001, 0, 2, 4190, 40], [4001, 7, 5000, 4200, 25]
+    b, table, pi, pages = batch_of(qo, kv, P, g)
+    c = make(fmt, layout, pages, P, hkv, d, g)
+    T = b.total_q
+    x = torch.randn(T + 5, hkv, d, generator=g).to(torch.bfloat16)
+    c.write(x.to(DEV), (-x).to(DEV), b)
+    out = tuple(torch.full((T + 3, hkv, d), 9.0, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    c.read(b, new_only=True, out=out)
+    torch.cuda.synchronize()
+    lost = T - 40 + torch.arange(15)  # the last request's first tokens have no place
+    for got, pool, sc, s in ((out[0], c.k_pool, c.k_scale, 1), (out[1], c.v_pool, c.v_scale, -1)):
+        scale = sc.cpu() if fmt == "fp8" else None
+        want = po.values_ref(*po.quantise_ref(s * x[:T], fmt, scale), fmt, scale).to(torch.bfloat16)
+        want[lost] = 9.0
+        assert torch.equal(got[:T].cpu(), want)
+        assert bool((got[T:] == 9.0).all())
+
+
 def test_pools_serve_the_kv_commit_and_the_other_way_round():
     """fp8 and bf16 pools are PagedKVCommit's: the same bytes from either."""
     g = torch.Generator().manual_seed(4)
