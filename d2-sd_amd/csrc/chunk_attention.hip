@@ -27,9 +27,9 @@
 //    rows, the workgroup stages tiles of 64 keys into LDS (bf16 straight, codes
 //    through registers; two buffers, one barrier a tile).  Bound by MFMA and the
 //    softmax's vector instructions, which the lock-step of the waves lets overlap
-//    only in part: 2 x 2048 tokens at 16384 keys, 32 heads of 128, take 0.97 to
-//    1.03 ms, 1.0 PFLOP/s, where a large library product reaches 1.36; a wave's
-//    tile is 2048 cycles of MFMA (both waves of its SIMD) in 4000.
+//    only in part: 2 x 2048 tokens at 16384 keys, 32 heads of 128, take 0.96 to
+//    0.98 ms, 1.05 PFLOP/s, where a large library product reaches 1.36; a tile is
+//    2048 cycles of MFMA (of both waves of a SIMD) in 3800.
 //  * token items (up to 32 rows: decoding): v_mfma_f32_16x16x32_bf16; all waves
 //    share the rows, and wave w of W takes every W-th tile of 32 keys.  Keys go
 //    from the cache straight to the MFMA operand: the sum over head dims may run
@@ -272,8 +272,8 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
       const unsigned long long off = row_offset(p, min(pages[i], last_page), key_of(tile, r) & pmask) +
                                      16 * ((lane % (D / 8)) ^ chunk_swizzle<D>(r));
       const unsigned dst = at + (wv * (64 / W) + RPC * i) * D * 2;
-      dma16(kcopy + off, dst);
-      dma16(vcopy + off, dst + TB);
+      dma16_kept(kcopy + off, dst);
+      dma16_kept(vcopy + off, dst + TB);
     }
   };
   // quantised: thread tid carries 1 / TPR of row tid / TPR through registers
@@ -485,11 +485,12 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
   // keys go straight to the operand (the sum over head dims may run in any
   // order: lane l takes quarter l / 16 of key l % 16's dims), values through
   // the wave's LDS
-  const char* kbase = (const char*)p.ks.codes + w.kvh * p.stride_head + g4 * (ROW / 4);
-  const char* vbase = (const char*)p.vs.codes + w.kvh * p.stride_head + 16 * (lane % PPR);
-  const long long shead = w.kvh * p.scale_stride_head;
-  const uint8_t* ksbase = (const uint8_t*)p.ks.scale + shead + g4 * (D / 4) / 32;
-  const uint8_t* vsbase = (const uint8_t*)p.vs.scale + shead + (FMT == CACHE_MXFP4 ? lane % PPR : lane % PPR / 2);
+  const char* kbase = (const char*)p.ks.codes + w.kvh * p.stride_head;
+  const char* vbase = (const char*)p.vs.codes + w.kvh * p.stride_head;
+  const uint8_t* ksbase = (const uint8_t*)p.ks.scale + w.kvh * p.scale_stride_head;
+  const uint8_t* vsbase = (const uint8_t*)p.vs.scale + w.kvh * p.scale_stride_head;
+  const unsigned kcol = g4 * (ROW / 4), vcol = 16 * (lane % PPR), kscol = g4 * (D / 4) / 32;
+  const unsigned vscol = FMT == CACHE_MXFP4 ? lane % PPR : lane % PPR / 2;
   const int pmask = (1 << p.log2_page) - 1;
   const unsigned last_page = (unsigned)p.num_pages - 1u;  // (clamped where used, as above)
   auto key_at = [&](int tile, int i) -> int { return min(max(32 * tile + i, all.lo), all.hi - 1); };
@@ -505,13 +506,8 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
   // of 8..32k tokens: bf16 475 -> 460 us, mxfp4 160 -> 156).
   constexpr int VR = 64 / PPR;  // rows of one load of values
   const bool shared_pages = (1 << p.log2_page) >= (VR > 16 ? VR : 16);
-  const char* kshared = (const char*)p.ks.codes + w.kvh * p.stride_head;
-  const char* vshared = (const char*)p.vs.codes + w.kvh * p.stride_head;
-  const uint8_t* ksshared = (const uint8_t*)p.ks.scale + shead;
-  const uint8_t* vsshared = (const uint8_t*)p.vs.scale + shead;
-  const unsigned klane = l16 * p.stride_tok + g4 * (ROW / 4), vlane = lane / PPR * p.stride_tok + 16 * (lane % PPR);
-  const unsigned kslane = l16 * p.scale_stride_tok + g4 * (D / 4) / 32;
-  const unsigned vslane = lane / PPR * p.scale_stride_tok + (FMT == CACHE_MXFP4 ? lane % PPR : lane % PPR / 2);
+  const unsigned klane = l16 * p.stride_tok + kcol, vlane = lane / PPR * p.stride_tok + vcol;
+  const unsigned kslane = l16 * p.scale_stride_tok + kscol, vslane = lane / PPR * p.scale_stride_tok + vscol;
   auto load_k = [&](unsigned (&d)[NKP][KW], const char* base, unsigned off) {
 #pragma unroll
     for (int i = 0; i < NKP; ++i) {
@@ -531,29 +527,29 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const unsigned pg = __builtin_amdgcn_readlane(page, 16 * b), slot = (32 * tile + 16 * b) & pmask;
-        load_k(x.k[b], kshared + row_offset(p, pg, slot), klane);
-        if constexpr (MX) x.ksc[b] = (ksshared + scale_offset(p, pg, slot))[kslane];
+        load_k(x.k[b], kbase + row_offset(p, pg, slot), klane);
+        if constexpr (MX) x.ksc[b] = (ksbase + scale_offset(p, pg, slot))[kslane];
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const unsigned pg = __builtin_amdgcn_readlane(page, VR * i), slot = (32 * tile + VR * i) & pmask;
-        x.v[i] = *(const u32x4*)(vshared + row_offset(p, pg, slot) + vlane);
-        if constexpr (MX) x.vsc[i] = (vsshared + scale_offset(p, pg, slot))[vslane];
+        x.v[i] = *(const u32x4*)(vbase + row_offset(p, pg, slot) + vlane);
+        if constexpr (MX) x.vsc[i] = (vsbase + scale_offset(p, pg, slot))[vslane];
       }
       return;
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const unsigned pg = __shfl(page, 16 * b + l16), slot = key_at(tile, 16 * b + l16) & pmask;
-      load_k(x.k[b], kbase + row_offset(p, pg, slot), 0u);
-      if constexpr (MX) x.ksc[b] = ksbase[scale_offset(p, pg, slot)];
+      load_k(x.k[b], kbase + row_offset(p, pg, slot), kcol);
+      if constexpr (MX) x.ksc[b] = (ksbase + scale_offset(p, pg, slot))[kscol];
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int kk = (64 * i + lane) / PPR;
       const unsigned pg = __shfl(page, kk), slot = key_at(tile, kk) & pmask;
-      x.v[i] = *(const u32x4*)(vbase + row_offset(p, pg, slot));
-      if constexpr (MX) x.vsc[i] = vsbase[scale_offset(p, pg, slot)];
+      x.v[i] = *(const u32x4*)(vbase + row_offset(p, pg, slot) + vcol);
+      if constexpr (MX) x.vsc[i] = (vsbase + scale_offset(p, pg, slot))[vscol];
     }
   };
 

@@ -219,6 +219,76 @@ def test_a_captured_step_replays_while_caches_grow(fmt):
         assert torch.equal(eager[0], out) and torch.equal(eager[1], lse)
 
 
+FORMS = {"eight waves": 0, "four waves": 1, "tokens": 2}
+
+
+@pytest.mark.parametrize("num_cus", [1, 4096])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_row_counts_around_the_tiles(d, fmt, num_cus):
+    """One head per kv head, so rows are tokens: both sides of 16 and 32 (token items) and of 128 and 256 (tile items of
+    four and of eight waves); both workgroup sizes of heads of 128."""
+    rows = [1, 15, 16, 17, 31, 32, 33, 127, 128, 129, 255, 256, 257, 1024]
+    p, _, _ = run_and_check(rows, [n + 37 * (n % 3) for n in rows[:-1]] + [4024], 2, 2, d, fmt, num_cus=num_cus)
+    assert p.attn.info.form == FORMS["eight waves" if d == 128 and num_cus == 1 else "four waves"]
+
+
+@pytest.mark.parametrize("P", [1, 2, 4, 8])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_small_pages(d, fmt, P):
+    """Pages of fewer tokens than one load's rows, in items of both kinds."""
+    run_and_check([70, 1, 5], [200, 333, 64], 8, 2, d, fmt, "NHD" if P == 2 else "HND", P)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_large_pages_and_long_caches(fmt):
+    """Token tiles whose rows share pages wherever the window and the cache's end leave them whole."""
+    for window in (-1, 1000, 31):
+        run_and_check([1, 1, 4, 1], [4000, 4001, 2049, 30], 8, 2, 64, fmt, "HND", 64, window=window)
+        run_and_check([1, 1, 4, 1], [4000, 4001, 2049, 30], 8, 2, 128, fmt, "NHD", 256, window=window)
+
+
+def test_a_captured_run_holds_its_own_outputs_and_workspace():
+    """run() without outputs or workspace inside a capture; eager runs, allocations and synchronisations between the
+    replays."""
+    p = Problem([1, 60], [6000, 3000], 8, 2, 128, "mxfp8")
+    assert p.attn.info.num_merges > 0
+    graph = d2sd.HipGraph()
+    with graph.capture():
+        out, lse = p.run()
+    g = torch.Generator().manual_seed(12)
+    for _ in range(4):
+        p.qd.copy_(torch.randn(p.q.shape, generator=g).to(torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = p.run()
+        fill = [torch.full((1 << 20,), float("nan"), device=DEV) for _ in range(8)]
+        torch.cuda.synchronize()
+        assert torch.equal(eager[0], out) and torch.equal(eager[1], lse)
+        del fill
+    p.q = p.qd.cpu()
+    p.check(out, lse)
+
+
+def test_a_side_stream_orders_write_and_attention():
+    """All of a step on a stream that is not the default one."""
+    p = Problem([3, 40], [300, 700], 8, 2, 128, "mxfp4")
+    ref = p.run()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    x = torch.randn(43, 2, 128).to(torch.bfloat16).to(DEV)
+    with torch.cuda.stream(side):
+        p.cache.write(x, x, p.batch)
+        a = p.run()
+        k, v = p.cache.read(p.batch, new_only=True)
+    side.synchronize()
+    b = p.run()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and not torch.equal(a[0], ref[0])
+    want = po.values_ref(*po.quantise_ref(x.cpu(), "mxfp4"), "mxfp4").to(torch.bfloat16)
+    assert torch.equal(k.cpu(), want) and torch.equal(v.cpu(), want)
+
+
 def test_shared_pages_of_a_common_prefix():
     """Two requests whose tables begin with the same pages."""
     P, g = 16, torch.Generator().manual_seed(1)

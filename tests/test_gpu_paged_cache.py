@@ -235,6 +235,27 @@ def test_prompts_of_many_tokens(fmt, hkv, d, layout):
         assert bool((got[T:] == 9.0).all())
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_reads_of_more_than_the_caches_hold(fmt):
+    """0.14 GB of results, stored past the caches: every row is there."""
+    g = torch.Generator().manual_seed(6)
+    P, hkv, d = 64, 8, 128
+    kv = [16001, 3, 18500]
+    b, table, pi, pages = batch_of([0, 0, 0], kv, P, g)
+    c = make(fmt, "HND", pages, P, hkv, d, g)
+    fill = d2sd.PagedBatch(np.concatenate([[0], np.cumsum(kv)]), kv, pi, table.to(DEV), P)
+    x = torch.randn(500, hkv, d, generator=g).to(torch.bfloat16)  # token t holds row t % 500
+    rows = torch.arange(b.total_kv) % 500
+    xd = x.to(DEV)[rows.to(DEV)]
+    c.write(xd, -xd, fill)
+    k, v = c.read(b)
+    torch.cuda.synchronize()
+    for got, s, sc in ((k, 1, c.k_scale), (v, -1, c.v_scale)):
+        scale = sc.cpu() if fmt == "fp8" else None
+        want = po.values_ref(*po.quantise_ref(s * x, fmt, scale), fmt, scale).to(torch.bfloat16)
+        assert torch.equal(got, want.to(DEV)[rows.to(DEV)])
+
+
 def test_pools_serve_the_kv_commit_and_the_other_way_round():
     """fp8 and bf16 pools are PagedKVCommit's: the same bytes from either."""
     g = torch.Generator().manual_seed(4)

@@ -66,6 +66,25 @@ def test_fused_projection_views_and_unaligned_rows():
         assert torch.equal(heads[:, 10:].cpu(), x[:, 10:]) and torch.equal(dev[:, :pad].cpu(), base[:, :pad])
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_results_larger_than_the_caches(interleaved):
+    """Prompts whose results are stored past the caches: sampled tokens against the formula, in place and out of it."""
+    g = torch.Generator().manual_seed(21)
+    tokens, hq, hkv, d = 2500, 56, 8, 128
+    q = torch.randn(tokens, hq, d, generator=g).to(torch.bfloat16)
+    k = torch.randn(tokens, hkv, d, generator=g).to(torch.bfloat16)
+    pos = torch.randperm(1 << 20, generator=g)[:tokens]
+    f, s = d2sd.rotary_frequencies(96)
+    qd, kd = q.to(DEV), k.to(DEV)
+    out = d2sd.rotary_embedding(qd, kd, pos.to(DEV), f.to(DEV), interleaved=interleaved,
+                                out=(torch.empty_like(qd), torch.empty_like(kd)))
+    some = torch.cat([torch.randperm(tokens, generator=g)[:60], torch.tensor([0, tokens - 1])])
+    for name, got, x in (("q", out[0], q), ("k", out[1], k)):
+        _check(got[some.to(DEV)], x[some], pos[some], f, name, interleaved=interleaved)
+    q2, k2 = d2sd.rotary_embedding(qd, kd, pos.to(DEV), f.to(DEV), interleaved=interleaved)
+    assert q2.data_ptr() == qd.data_ptr() and torch.equal(q2, out[0]) and torch.equal(k2, out[1])
+
+
 def test_far_and_negative_positions():
     """Positions beyond 32 bits: the angle's error stays that of a near one (64-bit products: 2^-53 of the
     turns, under 2^-22 up to 2^31 turns)."""

@@ -42,7 +42,7 @@ def test_plan_covers_every_row_and_chunk_once(qo, kv, hq, hkv, d, cus, max_split
     for req, kvh, q0, nq, row0, nrows, pb, pe, chunk, nchunks, slot, kind in items[:, :12].tolist():
         assert q0 == starts[req] and nq == qo[req] and 0 <= chunk < nchunks
         assert (pe - pb) * 16 >= kv[req]
-        assert kind == (1 if qo[req] * g <= 32 else 0) and nrows <= (32 if kind else 256)
+        assert kind == (1 if qo[req] * g <= 32 else 0) and nrows <= (32 if kind else 256 if attn.info.form == 0 else 128)
         assert (req, kvh, row0, chunk) not in seen
         seen[(req, kvh, row0, chunk)] = (nrows, nchunks, slot)
         if nchunks > 1:
@@ -82,6 +82,15 @@ def test_plan_splits_a_lone_long_request_and_not_a_full_batch():
     assert len(items) > 64 and len(merges)
     _, items, merges = _plan([1] * 512, [500] * 512)
     assert len(items) == 512 * 8 and not len(merges)
+
+
+def test_plan_picks_the_workgroup_for_the_rows():
+    """Tokens alone, eight waves where rows fill the device, four where only shorter items do, four for heads of 64."""
+    form = lambda *a, **kw: _plan(*a, **kw)[0].info.form  # noqa: E731
+    assert form([1] * 4, [5000] * 4) == 2 and form([4], [900]) == 2
+    assert form([2048, 2048], [16384, 16384]) == 0
+    assert form([1000], [2100]) == 1
+    assert form([2048, 2048], [16384, 16384], 64, 8, 64) == 1
 
 
 def test_plan_deals_kv_heads_to_xcds_in_turn():
@@ -191,7 +200,7 @@ def test_cache_entries_refuse_bad_arguments(bad):
 @pytest.mark.parametrize("bad", [dict(q=None), dict(out=None), dict(lse=None), dict(plan=None), dict(kv_len=None),
                                  dict(page_table=None), dict(q=AT + 2), dict(q_stride_n=4), dict(o_stride_h=2),
                                  dict(sm_scale=0.0), dict(sm_scale=float("inf")), dict(workspace=None),
-                                 dict(workspace_bytes=8), dict(workspace=AT + 4), "format", "page_size", "heads", "dim"])
+                                 dict(workspace_bytes=8), dict(workspace=AT + 4), "format", "page_size", "heads", "dim", "form", "wide"])
 def test_chunk_run_refuses(bad):
     info = _plan([1], [32768])[0].info
     assert info.workspace_bytes > 0
@@ -204,6 +213,10 @@ def test_chunk_run_refuses(bad):
     if isinstance(bad, dict):
         for k, v in bad.items():
             setattr(a, k, v)
+    elif bad == "form":
+        info.form = 3
+    elif bad == "wide":
+        a.cache.stride_page = 1 << 32
     else:
         a.cache = _cache(AT, **{"format": dict(fmt=2), "page_size": dict(page_size=32), "heads": dict(num_kv_heads=4),
                                 "dim": dict(head_dim=64)}[bad])
