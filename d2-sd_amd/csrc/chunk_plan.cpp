@@ -74,10 +74,13 @@ struct Planner {
   // slow each other down on a CU; token items that read at the same time share
   // the HBM's rate.
   double span() const {
-    std::vector<double> times;
+    std::vector<std::pair<double, int>> times;  // of a workgroup, and how many are alike
+    times.reserve(groups.size());
+    long long items = 0;
     double partial = 0.0, readers = 0.0, work = 0.0, longest = 0.0;
     for (const Group& g : groups) {
       const int n = chunks(g);
+      items += (long long)n * in.num_kv_heads;
       work += g.work() * in.num_kv_heads;
       longest = std::max(longest, g.work() / n);
       if (g.kind == CHUNK_TOKEN) readers += (double)n * in.num_kv_heads;
@@ -89,22 +92,26 @@ struct Planner {
       const int n = chunks(g);
       if (n > 1) partial += (double)n * g.nrows * in.num_kv_heads * in.head_dim * 8.0;  // written and read
       const double us = g.kind == CHUNK_TOKEN ? std::max(g.work(), g.read_us() * slower_read) : g.work() * slower_tile;
-      times.insert(times.end(), (size_t)n * in.num_kv_heads, us / n + kItemUs);
+      times.push_back({us / n + kItemUs, n * in.num_kv_heads});
     }
     double last = 0.0;
-    if ((int)times.size() <= places) {
-      for (double t : times) last = std::max(last, t);
+    if (items <= places) {
+      for (const auto& x : times) last = std::max(last, x.first);
     } else {
-      std::sort(times.begin(), times.end(), std::greater<double>());
-      std::priority_queue<double, std::vector<double>, std::greater<double>> ends;
-      for (double t : times) {
-        double at = 0.0;
-        if ((int)ends.size() >= places) {
-          at = ends.top();
-          ends.pop();
+      std::sort(times.begin(), times.end(), std::greater<std::pair<double, int>>());
+      // places by the time they are free, those alike together
+      std::priority_queue<std::pair<double, int>, std::vector<std::pair<double, int>>, std::greater<std::pair<double, int>>> free;
+      free.push({0.0, places});
+      for (const auto& x : times) {
+        for (int left = x.second; left > 0;) {
+          const auto at = free.top();
+          free.pop();
+          const int k = std::min(left, at.second);
+          free.push({at.first + x.first, k});
+          if (k < at.second) free.push({at.first, at.second - k});
+          left -= k;
+          last = std::max(last, at.first + x.first);
         }
-        ends.push(at + t);
-        last = std::max(last, at + t);
       }
     }
     return last + (partial > 0.0 ? kMergeUs + partial / kMergeBytes : 0.0);
@@ -194,15 +201,33 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
     if (other.plan() < us) pl.take(std::move(other));
   }
   out.form = pl.form;
-  struct Timed {
-    double us;
-    ChunkItem item;
-  };
-  std::vector<Timed> items;
   const int merge_rows = 1024 / in.head_dim;  // rows of one merge workgroup: 256 threads, 4 head dims each
-  long long slot = 0;
-  for (const Group& g : pl.groups) {
+  struct Placed {
+    double us;   // of a chunk
+    int group, chunks;
+    long long slot;
+  };
+  std::vector<Placed> order;
+  order.reserve(pl.groups.size());
+  long long slot = 0, items = 0;
+  for (int i = 0; i < (int)pl.groups.size(); ++i) {
+    const Group& g = pl.groups[i];
     const int n = pl.chunks(g);
+    order.push_back({g.work() / n, i, n, slot});
+    items += (long long)n * in.num_kv_heads;
+    if (n == 1) continue;
+    const int q0 = in.qo_indptr[g.req];
+    for (int h = 0; h < in.num_kv_heads; ++h, slot += (long long)n * g.nrows)
+      for (int r = 0; r < g.nrows; r += merge_rows)
+        out.merges.push_back(ChunkMerge{q0, h, g.row0 + r, std::min(merge_rows, g.nrows - r), (int)slot + r, g.nrows, n, 0});
+  }
+  // Longest first; among equals the kv heads of one key chunk side by side, so
+  // that with 8 (or 16, ..) kv heads each XCD (workgroups are dealt to the 8 of
+  // them in turn) keeps a head's keys in its own L2 for all row tiles.
+  std::stable_sort(order.begin(), order.end(), [](const Placed& a, const Placed& b) { return a.us > b.us; });
+  out.items.reserve((size_t)items);
+  for (const Placed& x : order) {
+    const Group& g = pl.groups[x.group];
     ChunkItem it{};
     it.req = g.req;
     it.q0 = in.qo_indptr[g.req];
@@ -211,35 +236,14 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
     it.nrows = g.nrows;
     it.page_begin = in.page_indptr[g.req];
     it.page_end = in.page_indptr[g.req + 1];
-    it.nchunks = n;
+    it.nchunks = x.chunks;
     it.kind = g.kind;
-    for (int h = 0; h < in.num_kv_heads; ++h) {
-      it.kvh = h;
-      it.slot = n > 1 ? (int)slot : 0;
-      for (int c = 0; c < n; ++c) {
-        it.chunk = c;
-        items.push_back({g.work() / n, it});
+    for (it.chunk = 0; it.chunk < x.chunks; ++it.chunk)
+      for (it.kvh = 0; it.kvh < in.num_kv_heads; ++it.kvh) {
+        it.slot = x.chunks > 1 ? (int)(x.slot + (long long)it.kvh * x.chunks * g.nrows) : 0;
+        out.items.push_back(it);
       }
-      if (n > 1) {
-        for (int i = 0; i < g.nrows; i += merge_rows)
-          out.merges.push_back(ChunkMerge{it.q0, h, g.row0 + i, std::min(merge_rows, g.nrows - i), (int)slot + i, g.nrows,
-                                          n, 0});
-        slot += (long long)n * g.nrows;
-      }
-    }
   }
-  // Longest first; among equals the kv heads of one key chunk side by side, so
-  // that with 8 (or 16, ..) kv heads each XCD (workgroups are dealt to the 8 of
-  // them in turn) keeps a head's keys in its own L2 for all row tiles.
-  std::stable_sort(items.begin(), items.end(), [](const Timed& a, const Timed& b) {
-    if (a.us != b.us) return a.us > b.us;
-    if (a.item.req != b.item.req) return a.item.req < b.item.req;
-    if (a.item.row0 != b.item.row0) return a.item.row0 < b.item.row0;
-    if (a.item.chunk != b.item.chunk) return a.item.chunk < b.item.chunk;
-    return a.item.kvh < b.item.kvh;
-  });
-  out.items.reserve(items.size());
-  for (const Timed& t : items) out.items.push_back(t.item);
   out.partial_rows = slot;
 }
 

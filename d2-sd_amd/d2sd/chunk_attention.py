@@ -68,11 +68,11 @@ class PagedChunkAttention:
         desc.format, desc.page_size, desc.window_left = KV_FORMATS[kv_format], batch.page_size, window_left
         desc.num_cus, desc.max_splits = num_cus, max_splits
         info = _lib.ChunkPlanInfo()
-        host = np.zeros(1 << 14, dtype=np.int32)
+        host = np.empty(1 << 16, dtype=np.int32)
         with torch.cuda.device(batch.device) if batch.device.type == "cuda" else torch.no_grad():
             rc = lib.d2sd_chunk_plan(C.byref(desc), as_p(host), host.size, C.byref(info))
             if rc == _lib.D2SD_ERR_WORKSPACE and info.plan_ints > host.size:
-                host = np.zeros(info.plan_ints, dtype=np.int32)
+                host = np.empty(info.plan_ints, dtype=np.int32)
                 rc = lib.d2sd_chunk_plan(C.byref(desc), as_p(host), host.size, C.byref(info))
         check(rc, "chunk_plan")
         self.info, self.batch, self.sinks = info, batch, sinks
