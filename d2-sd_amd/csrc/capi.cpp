@@ -1355,7 +1355,7 @@ int d2sd_chunk_run(const d2sd_chunk_plan_info* info, const d2sd_chunk_run_args* 
   if (int rc = check_cache(a->cache, "chunk_run")) return rc;
   const d2sd_paged_cache& c = a->cache;
   if (c.format != info->format || c.page_size != info->page_size || c.num_kv_heads != info->num_kv_heads ||
-      c.head_dim != info->head_dim || info->form < 0 || info->form > d2sd::CHUNK_TOKENS)
+      c.head_dim != info->head_dim || info->form < 0 || info->form > d2sd::CHUNK_STREAM)
     return fail(D2SD_ERR_INVALID_ARG, "chunk_run: the cache is not the one planned for");
   if (!a->plan || !a->kv_len || !a->page_table || !a->q || !a->out || !a->lse)
     return fail(D2SD_ERR_INVALID_ARG, "chunk_run: null pointer");

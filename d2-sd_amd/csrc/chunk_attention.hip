@@ -198,6 +198,34 @@ __device__ __forceinline__ lds_char* lds_piece(lds_char* tile, int row, int chun
   return tile + row * D * 2 + 16 * (chunk ^ chunk_swizzle<D>(row));
 }
 
+// A lane that expands N chunks of a row writes them in the order i ^ turn: 16
+// lanes then write 16 different 16-byte columns of LDS at a time.  (In order,
+// rows beside each other meet in the same columns: half of the LDS cycles of
+// quantised batches were conflicts.)
+template <int D, int N>
+__device__ __forceinline__ unsigned write_turn(int row) {
+  if constexpr (D == 128) return row & (N - 1);
+  return (row >> 1 & 1) * (N / 2);
+}
+// chunk i of d becomes chunk i ^ turn
+template <int D, int N, int WORDS>
+__device__ __forceinline__ void turn_chunks(unsigned (&d)[N * WORDS], unsigned turn) {
+#pragma unroll
+  for (int bit = D == 128 ? 1 : N / 2; bit < N; bit *= 2) {
+    const bool swap = turn & bit;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i & bit) continue;
+#pragma unroll
+      for (int e = 0; e < WORDS; ++e) {
+        const unsigned a = d[i * WORDS + e], b = d[(i | bit) * WORDS + e];
+        d[i * WORDS + e] = swap ? b : a;
+        d[(i | bit) * WORDS + e] = swap ? a : b;
+      }
+    }
+  }
+}
+
 // Output of one row's state: normalised O and LSE to the output, or a partial.
 struct RowOut {
   int token, head;
@@ -310,15 +338,19 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
       vsc = ((const uint8_t*)p.vs.scale)[so];
     }
   };
+  constexpr int PN = EPT / 8, PW = FMT == CACHE_MXFP4 ? 1 : 2;  // chunks of a part, words of a chunk
+  const unsigned turn = write_turn<D, PN>(srow), pswz = chunk_swizzle<D>(srow) ^ turn;
   auto put = [&](lds_char* tile, const unsigned (&d)[WORDS], unsigned sc) {
     if constexpr (FMT != CACHE_BF16) {
       const float f = MX ? block_scale(sc) : 1.f;
+      unsigned x[PN * PW];
 #pragma unroll
-      for (int i = 0; i < EPT / 8; ++i) {
-        const bf16x8 v = FMT == CACHE_MXFP4 ? expand<FMT>(d[i % WORDS], 0u, f)
-                                            : expand<FMT>(d[2 * i % WORDS], d[(2 * i + 1) % WORDS], f);
-        *(__attribute__((address_space(3))) bf16x8*)lds_piece<D>(tile, srow, spart * (EPT / 8) + i) = v;
-      }
+      for (int i = 0; i < PN * PW; ++i) x[i] = d[i];
+      turn_chunks<D, PN, PW>(x, turn);
+#pragma unroll
+      for (int i = 0; i < PN; ++i)
+        *(__attribute__((address_space(3))) bf16x8*)(tile + srow * D * 2 + 16 * ((spart * PN + i) ^ pswz)) =
+            expand<FMT>(x[PW * i], x[PW * i + PW - 1], f);
     }
   };
 
@@ -446,13 +478,24 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
 // RB row blocks of 16 packed rows, shared by all waves; v_mfma_f32_16x16x32_bf16:
 // lane l holds row l % 16 of a block, and of a 16-key block the scores of keys
 // 4 (l / 16) .. + 3.  PF tiles of 32 keys are in flight per wave.
-template <int D, int FMT, int W, int RB, int PF>
+template <bool STREAM, typename T>
+__device__ __forceinline__ T load_kv(const T* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  return *p;
+}
+
+template <int D, int FMT, int W, int RB, int PF, bool STREAM>
 __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem& w, lds_char* lds, float* stats) {
   constexpr int MT = D / 16, KS = D / 32, ROW = Format<D, FMT>::ROW;
   constexpr bool MX = Format<D, FMT>::MX;
   constexpr int NK = ROW / 64;                  // 16-byte pieces of a lane's quarter of a key row
   constexpr int KW = NK > 0 ? 4 : ROW / 16;     // words of a piece (half pieces where a quarter row is 8 bytes)
   constexpr int NKP = NK > 0 ? NK : 1;
+  // Which pieces of a key row are a lane's: the four lanes of a row take
+  // neighbouring ones, so that a load reads whole 64-byte runs; with block scales
+  // a quarter of the row each, which one block covers at D = 128.
+  constexpr bool SPREAD = !MX && NK > 1;
+  constexpr int PE = 16 * D / ROW;              // elements of a piece
   constexpr int PPR = ROW / 16;                 // 16-byte pieces of a row
   constexpr int NV = PPR / 2;                   // value pieces per lane and tile
   constexpr int VB = 32 * D * 2;                // bytes of a wave's value tile
@@ -471,9 +514,10 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
     const RowOut at(p, w, row);
     pos[rb] = all.pos0 + (w.row0 + row) / p.group;
     row_lo[rb] = p.window_left >= 0 ? max(pos[rb] - p.window_left, 0) : 0;
-    const bf16_t* qp = (const bf16_t*)p.q + (long long)at.token * p.q_stride_n + (long long)at.head * p.q_stride_h + g4 * (D / 4);
+    const bf16_t* qp = (const bf16_t*)p.q + (long long)at.token * p.q_stride_n + (long long)at.head * p.q_stride_h;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[rb][ks] = *(const bf16x8*)(qp + 8 * ks);
+    for (int ks = 0; ks < KS; ++ks)
+      qf[rb][ks] = *(const bf16x8*)(qp + (SPREAD ? PE * (g4 + 4 * (8 * ks / PE)) + 8 * ks % PE : g4 * (D / 4) + 8 * ks));
   }
   float c = p.sm_scale * kLog2e, vscale = 1.f;
   if constexpr (FMT == CACHE_FP8) {
@@ -489,7 +533,8 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
   const char* vbase = (const char*)p.vs.codes + w.kvh * p.stride_head;
   const uint8_t* ksbase = (const uint8_t*)p.ks.scale + w.kvh * p.scale_stride_head;
   const uint8_t* vsbase = (const uint8_t*)p.vs.scale + w.kvh * p.scale_stride_head;
-  const unsigned kcol = g4 * (ROW / 4), vcol = 16 * (lane % PPR), kscol = g4 * (D / 4) / 32;
+  constexpr int PSTEP = SPREAD ? 64 : 16;  // bytes between a lane's pieces
+  const unsigned kcol = SPREAD ? 16 * g4 : g4 * (ROW / 4), vcol = 16 * (lane % PPR), kscol = g4 * (D / 4) / 32;
   const unsigned vscol = FMT == CACHE_MXFP4 ? lane % PPR : lane % PPR / 2;
   const int pmask = (1 << p.log2_page) - 1;
   const unsigned last_page = (unsigned)p.num_pages - 1u;  // (clamped where used, as above)
@@ -512,11 +557,11 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
 #pragma unroll
     for (int i = 0; i < NKP; ++i) {
       if constexpr (KW == 4) {
-        const u32x4 u = *(const u32x4*)(base + off + 16 * i);
+        const u32x4 u = load_kv<STREAM>((const u32x4*)(base + off + PSTEP * i));
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[i][e] = u[e];
       } else {
-        const u32x2 u = *(const u32x2*)(base + off);
+        const u32x2 u = load_kv<STREAM>((const u32x2*)(base + off));
         d[i][0] = u[0], d[i][1] = u[1];
       }
     }
@@ -533,7 +578,7 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const unsigned pg = __builtin_amdgcn_readlane(page, VR * i), slot = (32 * tile + VR * i) & pmask;
-        x.v[i] = *(const u32x4*)(vbase + row_offset(p, pg, slot) + vlane);
+        x.v[i] = load_kv<STREAM>((const u32x4*)(vbase + row_offset(p, pg, slot) + vlane));
         if constexpr (MX) x.vsc[i] = (vsbase + scale_offset(p, pg, slot))[vslane];
       }
       return;
@@ -548,7 +593,7 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
     for (int i = 0; i < NV; ++i) {
       const int kk = (64 * i + lane) / PPR;
       const unsigned pg = __shfl(page, kk), slot = key_at(tile, kk) & pmask;
-      x.v[i] = *(const u32x4*)(vbase + row_offset(p, pg, slot) + vcol);
+      x.v[i] = load_kv<STREAM>((const u32x4*)(vbase + row_offset(p, pg, slot) + vcol));
       if constexpr (MX) x.vsc[i] = (vsbase + scale_offset(p, pg, slot))[vscol];
     }
   };
@@ -609,14 +654,16 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
       if constexpr (FMT == CACHE_BF16) {
         *(__attribute__((address_space(3))) u32x4*)lds_piece<D>(vt, kk, col) = x.v[i];
       } else {
-        constexpr int CH = FMT == CACHE_MXFP4 ? 4 : 2;  // 8-element chunks of a piece
+        constexpr int CH = FMT == CACHE_MXFP4 ? 4 : 2, CW = 4 / CH;  // 8-element chunks of a piece, words of a chunk
         const float f = MX ? block_scale(x.vsc[i]) : 1.f;
+        const unsigned turn = write_turn<D, CH>(kk);
+        unsigned c[4] = {x.v[i][0], x.v[i][1], x.v[i][2], x.v[i][3]};
+        turn_chunks<D, CH, CW>(c, turn);
 #pragma unroll
-        for (int e = 0; e < CH; ++e) {
-          const bf16x8 v = FMT == CACHE_MXFP4 ? expand<FMT>(x.v[i][e], 0u, f)
-                                              : expand<FMT>(x.v[i][2 * e & 3], x.v[i][(2 * e + 1) & 3], f);
-          *(__attribute__((address_space(3))) bf16x8*)lds_piece<D>(vt, kk, CH * col + e) = v;
-        }
+        for (int e = 0; e < CH; ++e)
+          *(__attribute__((address_space(3))) bf16x8*)(vt + kk * D * 2 +
+                                                       16 * ((CH * col + e) ^ chunk_swizzle<D>(kk) ^ turn)) =
+              expand<FMT>(c[CW * e], c[CW * e + CW - 1], f);
       }
     }
     if (tn < te) {
@@ -760,26 +807,26 @@ constexpr int token_depth() {
 // Waves per SIMD: what the registers allow without spilling.
 template <int D, int FMT, int FORM>
 constexpr int chunk_occupancy() {
-  return FORM == CHUNK_TOKENS ? (FMT == CACHE_MXFP4 ? 3 : 2) : D == 64 ? 3 : 2;
+  return FORM >= CHUNK_TOKENS ? (FMT == CACHE_MXFP4 ? 3 : 2) : D == 64 ? 3 : 2;
 }
 
 template <int D, int FMT, int FORM>
 __global__ __launch_bounds__(64 * chunk_waves(FORM), (chunk_occupancy<D, FMT, FORM>())) void
 chunk_attn_kernel(const ChunkParams p) {
   constexpr int W = chunk_waves(FORM);
-  constexpr bool TOKENS = FORM == CHUNK_TOKENS;
+  constexpr bool TOKENS = FORM >= CHUNK_TOKENS;
   __shared__ __align__(16) char lds[TOKENS ? W * 32 * D * 2 : 4 * 64 * D * 2];
   __shared__ float stats[2 * W * kTokenRows];
   const ChunkItem w = p.items[blockIdx.x];
   if constexpr (TOKENS) {
-    token_item<D, FMT, W, 1, token_depth<FMT>()>(p, w, (lds_char*)lds, stats);
+    token_item<D, FMT, W, 1, token_depth<FMT>(), FORM == CHUNK_STREAM>(p, w, (lds_char*)lds, stats);
   } else {
     if (w.kind == CHUNK_TILE)
       tile_item<D, FMT, W>(p, w, (lds_char*)lds);
     else if (w.nrows <= 16)
-      token_item<D, FMT, W, 1, token_depth<FMT>()>(p, w, (lds_char*)lds, stats);
+      token_item<D, FMT, W, 1, token_depth<FMT>(), FORM == CHUNK_STREAM>(p, w, (lds_char*)lds, stats);
     else
-      token_item<D, FMT, W, 2, 1>(p, w, (lds_char*)lds, stats);
+      token_item<D, FMT, W, 2, 1, false>(p, w, (lds_char*)lds, stats);
   }
 }
 
@@ -817,6 +864,8 @@ hipError_t launch_f(const ChunkParams& p, int form, int nitems, int nmerges, hip
   const dim3 grid((unsigned)nitems), block(64 * chunk_waves(form));
   if (form == CHUNK_TOKENS) {
     hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, CHUNK_TOKENS>), grid, block, 0, s, p);
+  } else if (form == CHUNK_STREAM) {
+    hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, CHUNK_STREAM>), grid, block, 0, s, p);
   } else if (form == CHUNK_WAVES4) {
     hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, CHUNK_WAVES4>), grid, block, 0, s, p);
   } else {

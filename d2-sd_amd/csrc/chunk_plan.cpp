@@ -16,6 +16,7 @@ namespace {
 // bytes per us: what one CU reads at most, what all of them read together, what
 // a merge moves.
 constexpr double kItemUs = 5.0, kTokenTileUs = 1.2, kMergeUs = 5.0;
+constexpr double kStreamBytes = 128 << 20;
 constexpr double kCuBytes = 57e3, kHbmBytes = 5.4e6, kMergeBytes = 3.0e6;
 
 int row_bytes(int format, int d) {
@@ -201,6 +202,14 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
     if (other.plan() < us) pl.take(std::move(other));
   }
   out.form = pl.form;
+  // Token items alone that read more than half of the last-level cache (256 MB):
+  // what they read is not there when the next call reads it, and goes past the
+  // caches (32 requests of 8..32k tokens: bf16 452 -> 425 us, fp8 248 -> 224,
+  // mxfp4 149 -> 134).  Smaller reads may be found there (8 x 4000 tokens in bf16:
+  // 27 us, 30 past the caches).
+  double bytes = 0.0;
+  for (const Group& g : pl.groups) bytes += 64.0 * g.units * row_bytes(in.format, in.head_dim) * in.num_kv_heads;
+  if (tokens_only && bytes > kStreamBytes) out.form = CHUNK_STREAM;
   const int merge_rows = 1024 / in.head_dim;  // rows of one merge workgroup: 256 threads, 4 head dims each
   struct Placed {
     double us;   // of a chunk

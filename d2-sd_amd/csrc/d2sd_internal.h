@@ -291,8 +291,9 @@ struct CacheParams {
 // (chunk_attention.hip).
 // ---------------------------------------------------------------------------
 // Kernels that a plan may be for: workgroups of 8 or 4 waves, or those of plans
-// of token items of up to 16 rows alone (4 waves)
-enum ChunkForm : int { CHUNK_WAVES8 = 0, CHUNK_WAVES4 = 1, CHUNK_TOKENS = 2 };
+// of token items of up to 16 rows alone (4 waves), whose reads are larger than
+// the last-level cache holds (STREAM) or not
+enum ChunkForm : int { CHUNK_WAVES8 = 0, CHUNK_WAVES4 = 1, CHUNK_TOKENS = 2, CHUNK_STREAM = 3 };
 constexpr int chunk_waves(int form) { return form == CHUNK_WAVES8 ? 8 : 4; }
 constexpr int chunk_rows(int form) { return 32 * chunk_waves(form); }  // packed rows of a tile item (32 per wave)
 constexpr int kTokenRows = 32;      // packed rows a token item holds at most (all waves share them)

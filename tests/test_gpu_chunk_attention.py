@@ -289,6 +289,38 @@ def test_a_side_stream_orders_write_and_attention():
     assert torch.equal(k.cpu(), want) and torch.equal(v.cpu(), want)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (64, 8, 64)])
+def test_reads_larger_than_the_caches_give_the_same_bits(fmt, hq, hkv, d):
+    """Tokens over more than 128 MB of keys and values: read past the caches, and as smaller batches are read."""
+    g = torch.Generator().manual_seed(17)
+    row = {"bf16": 2 * d, "mxfp4": d // 2}.get(fmt, d)
+    P, R = 16, 12
+    L = [-(-150 * 2 ** 20 // (R * 2 * hkv * row)) + 61 * r for r in range(R)]
+    pi = np.concatenate([[0], np.cumsum([-(-n // P) for n in L])]).astype(int)
+    table = torch.randperm(int(pi[-1]), generator=g).to(torch.int32)
+    scale = dict(k_scale=torch.full((hkv,), 0.01, device=DEV), v_scale=torch.full((hkv,), 0.01, device=DEV)) if fmt == "fp8" else {}
+    c = d2sd.PagedKVCache.allocate(int(pi[-1]), P, hkv, d, fmt, device=DEV, **scale)
+    for t in (c.k_pool, c.v_pool):
+        if fmt == "bf16":
+            t.normal_()
+        else:  # any codes but NaN
+            t.view(torch.uint8).random_(0, 256).bitwise_and_(0xFF if fmt == "mxfp4" else 0xBF)
+    if fmt.startswith("mx"):
+        for t in (c.k_scale, c.v_scale):
+            t.random_(118, 124)
+    b = d2sd.PagedBatch(np.arange(R + 1), L, pi, table.to(DEV), P)
+    q = torch.randn(R, hq, d, generator=g).to(torch.bfloat16).to(DEV)
+    a = d2sd.PagedChunkAttention().plan(b, hq, hkv, d, kv_format=fmt)
+    assert a.info.form == 3
+    past = a.run(q, c)
+    a.info.form = 2
+    a._info = torch.frombuffer(bytearray(bytes(a.info)), dtype=torch.uint8)
+    kept = a.run(q, c)
+    torch.cuda.synchronize()
+    assert torch.isfinite(past[0]).all() and torch.equal(past[0], kept[0]) and torch.equal(past[1], kept[1])
+
+
 def test_shared_pages_of_a_common_prefix():
     """Two requests whose tables begin with the same pages."""
     P, g = 16, torch.Generator().manual_seed(1)

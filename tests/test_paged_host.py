@@ -88,6 +88,7 @@ def test_plan_picks_the_workgroup_for_the_rows():
     """Tokens alone, eight waves where rows fill the device, four where only shorter items do, four for heads of 64."""
     form = lambda *a, **kw: _plan(*a, **kw)[0].info.form  # noqa: E731
     assert form([1] * 4, [5000] * 4) == 2 and form([4], [900]) == 2
+    assert form([1] * 32, [20000] * 32) == 3 and form([1] * 32, [20000] * 32, window=127) == 2
     assert form([2048, 2048], [16384, 16384]) == 0
     assert form([1000], [2100]) == 1
     assert form([2048, 2048], [16384, 16384], 64, 8, 64) == 1
@@ -214,7 +215,7 @@ def test_chunk_run_refuses(bad):
         for k, v in bad.items():
             setattr(a, k, v)
     elif bad == "form":
-        info.form = 3
+        info.form = 4
     elif bad == "wide":
         a.cache.stride_page = 1 << 32
     else:

@@ -13,8 +13,8 @@ def test_no_scratch_in_loops():
     with open(d2sd.LIB_PATH, "rb") as f:
         kernels = [k for elf in _code_objects(f.read()) for k in _kernels(elf)]
     count = lambda name: [k for k in kernels if name in k[".name"]]  # noqa: E731
-    # formats x (heads of 64: four waves, tokens; heads of 128: eight waves too); merges by head dim
-    for name, n in (("chunk_attn_kernel", 20), ("chunk_merge_kernel", 2), ("cache_write_kernel", 8), ("cache_read_kernel", 8),
+    # formats x (heads of 64: four waves, tokens kept or streamed; heads of 128: eight waves too); merges by head dim
+    for name, n in (("chunk_attn_kernel", 28), ("chunk_merge_kernel", 2), ("cache_write_kernel", 8), ("cache_read_kernel", 8),
                     ("rotary_kernel", 6)):
         assert len(count(name)) == n, name
         for k in count(name):
