@@ -1,6 +1,7 @@
 // Work planner of the chunk attention (chunk_attention.hip): which workgroup
 // takes which rows and which share of their keys.
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <queue>
 #include <vector>
@@ -86,7 +87,10 @@ struct Planner {
       longest = std::max(longest, g.work() / n);
       if (g.kind == CHUNK_TOKEN) readers += (double)n * in.num_kv_heads;
     }
-    const double sharing = longest > 0.0 ? std::min<double>(per_cu, std::max(1.0, work / longest / in.num_cus)) : 1.0;
+    // Workgroups on a CU beside each other: those of the longest one's time, by CUs;
+    // with some more than CUs a few share theirs, and end last.
+    const double per = longest > 0.0 ? work / longest / in.num_cus : 0.0;
+    const double sharing = std::min<double>(per_cu, std::max(1.0, 0.6 * per + 0.4 * std::ceil(per - 0.02)));
     const double slower_tile = tile_us(form, in.head_dim, sharing) / tile_us(form, in.head_dim, 1.0);
     const double slower_read = std::max(1.0, std::min(readers, (double)places) * place_bytes / kHbmBytes);
     for (const Group& g : groups) {
@@ -162,7 +166,7 @@ struct Planner {
     const bool many = (double)groups.size() * in.num_kv_heads > 4.0 * places;
     double best = span(), best_limit = limit;
     const double even = total / places, shortest = many ? even * 0.5 : even / 16.0;
-    for (double x = longest * 0.7072; x > shortest && x > 1.0; x *= 0.7072) {
+    for (double x = longest * 0.8409; x > shortest && x > 1.0; x *= 0.8409) {
       if (many && x > 2.0 * even) continue;
       limit = x;
       const double t = span();
