@@ -198,20 +198,21 @@ __device__ __forceinline__ lds_char* lds_piece(lds_char* tile, int row, int chun
   return tile + row * D * 2 + 16 * (chunk ^ chunk_swizzle<D>(row));
 }
 
-// A lane that expands N chunks of a row writes them in the order i ^ turn: 16
-// lanes then write 16 different 16-byte columns of LDS at a time.  (In order,
-// rows beside each other meet in the same columns: half of the LDS cycles of
-// quantised batches were conflicts.)
+// A lane that expands N chunks of a row (part `col` of it) writes them in the
+// order i ^ turn, so that 8 lanes beside each other write 8 different 16-byte
+// columns of the 128 bytes that LDS takes at a time.  (In order they meet in 4 or
+// 2 of them: half of the LDS cycles of quantised batches were conflicts.)
 template <int D, int N>
-__device__ __forceinline__ unsigned write_turn(int row) {
-  if constexpr (D == 128) return row & (N - 1);
-  return (row >> 1 & 1) * (N / 2);
+__device__ __forceinline__ unsigned write_turn(int row, int col) {
+  if constexpr (D == 64) return row & (N - 1);
+  if constexpr (N == 2) return col >> 2 & 1;
+  return (col >> 1 & 1) | (row & 1) << 1;
 }
 // chunk i of d becomes chunk i ^ turn
-template <int D, int N, int WORDS>
+template <int N, int WORDS>
 __device__ __forceinline__ void turn_chunks(unsigned (&d)[N * WORDS], unsigned turn) {
 #pragma unroll
-  for (int bit = D == 128 ? 1 : N / 2; bit < N; bit *= 2) {
+  for (int bit = 1; bit < N; bit *= 2) {
     const bool swap = turn & bit;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -339,14 +340,14 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
     }
   };
   constexpr int PN = EPT / 8, PW = FMT == CACHE_MXFP4 ? 1 : 2;  // chunks of a part, words of a chunk
-  const unsigned turn = write_turn<D, PN>(srow), pswz = chunk_swizzle<D>(srow) ^ turn;
+  const unsigned turn = write_turn<D, PN>(srow, spart), pswz = chunk_swizzle<D>(srow) ^ turn;
   auto put = [&](lds_char* tile, const unsigned (&d)[WORDS], unsigned sc) {
     if constexpr (FMT != CACHE_BF16) {
       const float f = MX ? block_scale(sc) : 1.f;
       unsigned x[PN * PW];
 #pragma unroll
       for (int i = 0; i < PN * PW; ++i) x[i] = d[i];
-      turn_chunks<D, PN, PW>(x, turn);
+      turn_chunks<PN, PW>(x, turn);
 #pragma unroll
       for (int i = 0; i < PN; ++i)
         *(__attribute__((address_space(3))) bf16x8*)(tile + srow * D * 2 + 16 * ((spart * PN + i) ^ pswz)) =
@@ -656,9 +657,9 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
       } else {
         constexpr int CH = FMT == CACHE_MXFP4 ? 4 : 2, CW = 4 / CH;  // 8-element chunks of a piece, words of a chunk
         const float f = MX ? block_scale(x.vsc[i]) : 1.f;
-        const unsigned turn = write_turn<D, CH>(kk);
+        const unsigned turn = write_turn<D, CH>(kk, col);
         unsigned c[4] = {x.v[i][0], x.v[i][1], x.v[i][2], x.v[i][3]};
-        turn_chunks<D, CH, CW>(c, turn);
+        turn_chunks<CH, CW>(c, turn);
 #pragma unroll
         for (int e = 0; e < CH; ++e)
           *(__attribute__((address_space(3))) bf16x8*)(vt + kk * D * 2 +
