@@ -74,9 +74,9 @@ __device__ __forceinline__ void store_piece(const CacheSide& s, int fmt_head, lo
   if constexpr (FMT == CACHE_BF16) {
     *(u32x4*)((uint16_t*)s.codes + row + d) = val;
   } else {
-    float x[8];
-    expand8(val, x);
     if constexpr (FMT == CACHE_FP8) {
+      float x[8];
+      expand8(val, x);
       const float sc = ((const float*)s.scale)[fmt_head];
       u32x2 b;
 #pragma unroll
@@ -109,22 +109,51 @@ __device__ __forceinline__ void store_piece(const CacheSide& s, int fmt_head, lo
       constexpr unsigned FM = FP4 ? 0x00400000u : 0x00600000u;  // fraction bits of 1.5, 1.75
       constexpr int KM = FP4 ? 2 : 8, TOP = FP4 ? 125 : 119;
       int e = (int)(amax >> 23) - 127 - KM + ((amax & 0x007FFFFFu) > FM ? 1 : 0);
+      const bool over = finite && e > TOP;
       e = min(max(e, -117), TOP);
-      const float inv = __uint_as_float((unsigned)(127 - e) << 23);
-      constexpr float M = FP4 ? 6.f : 448.f;
+      u32x2 w = {0u, 0u};
+      if (!__any(over)) {
+        // the converters divide by 2^e, exactly, and round to nearest even
+        typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+        typedef short s16x2_t __attribute__((ext_vector_type(2)));
+        const float two_e = __uint_as_float((unsigned)(127 + e) << 23);
+        const unsigned u[4] = {val[0], val[1], val[2], val[3]};
+        auto pair = [&](int i) { return __builtin_bit_cast(bf16x2_t, u[i]); };
+        if constexpr (FP4) {
+          w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w[0], pair(0), two_e, 0);
+          w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w[0], pair(1), two_e, 1);
+          w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w[0], pair(2), two_e, 2);
+          w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w[0], pair(3), two_e, 3);
+        } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = finite ? fminf(fmaxf(x[i] * inv, -M), M) : 0.f;
-      if constexpr (FP4) {
-        unsigned w = 0;
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], 1.f, 0);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], 1.f, 1);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], 1.f, 2);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], 1.f, 3);
-        *(unsigned*)((uint8_t*)s.codes + row + d / 2) = w;
+          for (int i = 0; i < 2; ++i) {
+            s16x2_t x = {0, 0};
+            x = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(x, pair(2 * i), two_e, false);
+            x = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(x, pair(2 * i + 1), two_e, true);
+            w[i] = __builtin_bit_cast(unsigned, x);
+          }
+        }
       } else {
-        *(u32x2*)((uint8_t*)s.codes + row + d) =
-            (u32x2){fp8x4(x[0], x[1], x[2], x[3]), fp8x4(x[4], x[5], x[6], x[7])};
+        float x[8];
+        expand8(val, x);
+        const float inv = __uint_as_float((unsigned)(127 - e) << 23);
+        constexpr float M = FP4 ? 6.f : 448.f;  // (beyond the largest scale elements saturate)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i] * inv, -M), M);
+        if constexpr (FP4) {
+          w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], x[0], x[1], 1.f, 0);
+          w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], x[2], x[3], 1.f, 1);
+          w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], x[4], x[5], 1.f, 2);
+          w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[0], x[6], x[7], 1.f, 3);
+        } else {
+          w = (u32x2){fp8x4(x[0], x[1], x[2], x[3]), fp8x4(x[4], x[5], x[6], x[7])};
+        }
       }
+      if (!finite) w = (u32x2){0u, 0u};
+      if constexpr (FP4)
+        *(unsigned*)((uint8_t*)s.codes + row + d / 2) = w[0];
+      else
+        *(u32x2*)((uint8_t*)s.codes + row + d) = w;
       if ((d & 31) == 0) ((uint8_t*)s.scale)[srow + d / 32] = (uint8_t)(finite ? e + 127 : 255);
     }
   }
