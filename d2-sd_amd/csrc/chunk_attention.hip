@@ -27,17 +27,17 @@
 //    rows, the workgroup stages tiles of 64 keys into LDS (bf16 straight, codes
 //    through registers; two buffers, one barrier a tile).  Bound by MFMA and the
 //    softmax's vector instructions, which the lock-step of the waves lets overlap
-//    only in part: 2 x 2048 tokens at 16384 keys, 32 heads of 128, take 0.96 to
+//    only in part: 2 x 2048 tokens at 16384 keys, 32 heads of 128, take 0.93 to
 //    0.98 ms, 1.05 PFLOP/s, where a large library product reaches 1.36; a tile is
-//    2048 cycles of MFMA (of both waves of a SIMD) in 3800.
+//    2048 cycles of MFMA (of both waves of a SIMD) in 3700.
 //  * token items (up to 32 rows: decoding): v_mfma_f32_16x16x32_bf16; all waves
 //    share the rows, and wave w of W takes every W-th tile of 32 keys.  Keys go
 //    from the cache straight to the MFMA operand: the sum over head dims may run
-//    in any order, so lane l takes the contiguous quarter l / 16 of key l % 16's
-//    dims (through LDS instead: 168 -> 233 us on 32 x 8..32k mxfp4).  Values pass
-//    through the wave's own LDS to be read transposed.  No barrier until the
-//    waves' states are joined.  Bound by HBM: 32 requests of 8..32k tokens read
-//    5.8 TB/s in bf16, 5.2 in mxfp8, 4.5 in mxfp4 (1 KB of a page at a time).
+//    in any order, so lane l takes a quarter of key l % 16's dims (through LDS
+//    instead: 168 -> 233 us on 32 x 8..32k mxfp4).  Values pass through the
+//    wave's own LDS to be read transposed.  No barrier until the waves' states
+//    are joined.  Bound by HBM: 32 requests of 8..32k tokens read
+//    6.2 TB/s in bf16, 5.7 in mxfp8, 5.2 in mxfp4 (1 KB of a page at a time).
 //
 // Keys outside an item's visible range are never read: their addresses are
 // clamped to the range, so what lies behind a cache's end (or before its
@@ -527,9 +527,7 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
   }
   const float slack = c > 0.f ? kRescaleSlack / c : 0.f;
 
-  // keys go straight to the operand (the sum over head dims may run in any
-  // order: lane l takes quarter l / 16 of key l % 16's dims), values through
-  // the wave's LDS
+  // keys go straight to the operand, values through the wave's LDS
   const char* kbase = (const char*)p.ks.codes + w.kvh * p.stride_head;
   const char* vbase = (const char*)p.vs.codes + w.kvh * p.stride_head;
   const uint8_t* ksbase = (const uint8_t*)p.ks.scale + w.kvh * p.scale_stride_head;

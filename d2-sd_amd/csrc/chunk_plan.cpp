@@ -197,8 +197,11 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   for (int r = 0; r < in.num_reqs; ++r)
     if ((long long)(in.qo_indptr[r + 1] - in.qo_indptr[r]) * group > 16) tokens_only = false;
   // Heads of 128: workgroups of 8 waves share a tile's staging among more rows
-  // (2 x 2048 tokens at 16384: 1.03 against 1.13 ms), those of 4 fill the device
-  // with fewer rows (1000 tokens at 2100: 50 us against 65 unsplit).
+  // (2 x 2048 tokens at 16384 bf16 keys: 1060 us against 1155), those of 4 fill
+  // the device with fewer rows (1000 tokens at 2100: 49 us against 57 split in two
+  // and 65 unsplit).  Heads of 64: 4 waves, three workgroups on a CU (4 x 1024
+  // tokens, window 128: 39 us against 44; 8 x 300 at 1000: 66 against 74; 2 x 2048
+  // at 16384: 1340 against 1259 in bf16, 1201 against 1217 in mxfp4).
   Planner pl(in, tokens_only ? CHUNK_TOKENS : CHUNK_WAVES4);
   const double us = pl.plan();
   if (!tokens_only && in.head_dim == 128) {
