@@ -250,9 +250,10 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
   const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
 
   const Span all = item_span(p, w, w.row0 / p.group, (w.row0 + w.nrows - 1) / p.group);
-  const int tile0 = all.lo >> 6, ntiles_all = all.hi > all.lo ? ((all.hi + 63) >> 6) - tile0 : 0;
-  const int tb = tile0 + (int)((long long)ntiles_all * w.chunk / w.nchunks);
-  const int te = tile0 + (int)((long long)ntiles_all * (w.chunk + 1) / w.nchunks);
+  // tiles of 64 keys from the first visible one on
+  const int ntiles = max(all.hi - all.lo + 63, 0) >> 6;
+  const int tb = (int)((long long)ntiles * w.chunk / w.nchunks);
+  const int te = (int)((long long)ntiles * (w.chunk + 1) / w.nchunks);
 
   // this wave's rows
   const int wrow = 32 * wv, row = min(wrow + l32, w.nrows - 1);
@@ -281,7 +282,7 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
   // wait for it would be a wait for all the tile's loads before it)
   auto page_of = [&](int key) -> unsigned { return (unsigned)p.page_table[w.page_begin + (key >> p.log2_page)]; };
   const unsigned last_page = (unsigned)p.num_pages - 1u;
-  auto key_of = [&](int tile, int row_) -> int { return min(max(64 * tile + row_, all.lo), all.hi - 1); };
+  auto key_of = [&](int tile, int row_) -> int { return min(all.lo + 64 * tile + row_, all.hi - 1); };
   const int pmask = (1 << p.log2_page) - 1;
   // bf16: a wave copies 64 / W rows straight into LDS, 1 KB (1024 / ROW rows) at a time
   constexpr int RPC = 1024 / (2 * D), NC = 64 / W / RPC;  // rows per copy, copies per wave
@@ -394,7 +395,7 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
         pages_of(min(t + 2, te - 1));
       }
     }
-    const int kb = 64 * t;
+    const int kb = all.lo + 64 * t;
     const bool on = wave_on && kb < own.hi && kb + 64 > own.lo;
     f32x16 s[2];
     if (on) {

@@ -146,7 +146,9 @@ struct Planner {
         const long long first = pos0 + row0 / group, last = pos0 + (row0 + g.nrows - 1) / group;
         const long long hi = std::max(last + 1, 0ll);
         const long long lo = in.window_left >= 0 ? std::max(first - in.window_left, 0ll) : 0;
-        g.units = hi > lo ? (int)((hi + keys_per_unit - 1) / keys_per_unit - lo / keys_per_unit) : 0;
+        // (a tile item's tiles start at its first key, a token item's at multiples)
+        const long long from = kind == CHUNK_TOKEN ? lo / keys_per_unit * keys_per_unit : lo;
+        g.units = hi > lo ? (int)((hi - from + keys_per_unit - 1) / keys_per_unit) : 0;
         (kind == CHUNK_TOKEN ? tokens : tiles) = true;
         if (kind == CHUNK_TOKEN) {
           g.unit_read_us = unit_bytes / place_bytes;
