@@ -396,7 +396,9 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
       }
     }
     const int kb = all.lo + 64 * t;
-    const bool on = wave_on && kb < own.hi && kb + 64 > own.lo;
+    // which 32-key halves some row of the wave sees
+    const bool on0 = wave_on && kb < own.hi && kb + 32 > own.lo, on1 = wave_on && kb + 32 < own.hi && kb + 64 > own.lo;
+    const bool on = on0 && on1;
     f32x16 s[2];
     if (on) {
       // operands are read AHEAD steps before their product
@@ -439,6 +441,23 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
           o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vread(vt, mt, j), pb, o[mt], 0, 0, 0);
+      }
+    } else if (on0 || on1) {
+      const int half = on1 ? 32 : 0;
+      f32x16 s1[1];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const bf16x8 kf = *(const __attribute__((address_space(3))) bf16x8*)(kt + half * D * 2 + koff[ks]);
+        s1[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], ks ? s1[0] : f32x16{}, 0, 0, 0);
+      }
+      hide(s1[0], kb + half, row_lo, pos, hh);
+      softmax_step<1, MT>(s1, o, m, l, c, slack, hh);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const bf16x8 pb = p_operand(s1[0], j);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vread(vt + half * D * 2, mt, j), pb, o[mt], 0, 0, 0);
       }
     }
     if constexpr (FMT == CACHE_BF16) wait_vmcnt<0>();  // this wave's copies of the next tile have landed
