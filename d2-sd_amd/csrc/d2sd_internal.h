@@ -238,7 +238,6 @@ struct QkRopeParams {
 // Rotary embedding at positions (rotary.hip).
 // ---------------------------------------------------------------------------
 constexpr int kRotaryMaxPairs = 128;      // rotated pairs of a head
-constexpr int kRotaryManyTokens = 1024;   // from here on a wave takes all heads of its token
 struct RotaryParams {
   const void* q;             // bf16 [tokens, Hq, D], head_dim contiguous
   const void* k;             // bf16 [tokens, Hkv, D]

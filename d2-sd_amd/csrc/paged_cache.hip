@@ -33,7 +33,8 @@ namespace d2sd {
 namespace {
 
 constexpr int kWriteTokens = 8;         // of one block, where there are many
-constexpr int kWriteManyTokens = 8192;
+// (8 heads of 128 in mxfp4: 4096 tokens 7.1 and 7.2 us, 8000 tokens 13.3 one by one, 11.3 by eight)
+constexpr int kWriteManyTokens = 6144;
 // Results larger than half of the last-level cache are stored past it: nothing
 // of them would be found there by whoever reads them from their start (16
 // requests of 100..8000 tokens, 0.26 GB: 99 -> 94 us).
@@ -325,7 +326,6 @@ template <int FMT>
 static void launch_write(const CacheParams& p, hipStream_t s) {
   const int pieces = 2 * p.num_kv_heads * (p.head_dim / 8);
   const dim3 block((unsigned)std::min(256, (pieces + 63) / 64 * 64));
-  // (kWriteManyTokens: blocks of kWriteTokens still give every CU four)
   if (p.num_items >= kWriteManyTokens)
     hipLaunchKernelGGL((cache_write_kernel<FMT, kWriteTokens>), dim3((unsigned)((p.num_items + kWriteTokens - 1) / kWriteTokens)),
                        block, 0, s, p);

@@ -14,9 +14,11 @@
 // sine of pair i (and i + 64), through LDS all its heads share them.  A slot
 // (lane) holds VEC pairs of one head: two 16-byte loads and stores for rows on
 // 16-byte boundaries, else one element at a time.  Bound by HBM for prompts
-// (q and k once in, once out) and by latency for a step's few tokens, where
-// each wave takes only as many heads as one slot per lane covers: the sines
-// (about 100 instructions) cost less than a second round of loads.
+// (q and k once in, once out) and by latency for a step's few tokens.  A wave
+// takes only as many heads as one slot per lane covers: the sines (about 100
+// instructions) cost less than a second round of loads (8192 tokens of 72 heads
+// of 64, all heads in one wave: 29.5 us, this way 26.2; 1024 tokens of 40 heads
+// of 128: 7.2 and 5.6).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -31,8 +33,8 @@ namespace {
 
 constexpr int kRotaryWaves = 4;
 // Results larger than the L2s together are stored past the caches (8192 tokens of
-// 72 heads of 64: 36 -> 29 us, 5.2 TB/s; the kernels that read them next take as
-// long either way).
+// 72 heads of 64: 31.3 -> 26.3 us, 5.7 TB/s; the kernels that read them next take
+// as long either way).
 constexpr long long kRotaryStreamBytes = 32ll << 20;
 
 // bf16 of two floats, rounded to nearest even, as one word
@@ -145,9 +147,7 @@ hipError_t launch_rotary(RotaryParams p, bool interleaved, hipStream_t s) {
                        p.ko_stride_n | p.ko_stride_h;
   const bool vec = (at & 15) == 0 && (st & 7) == 0 && p.head_dim % 16 == 0 && p.pairs % 8 == 0;
   const int slots = p.head_dim / (vec ? 16 : 2);
-  // heads that one pass of a wave covers; prompts: all heads of a token in one wave
-  const int pass = slots >= 64 ? 1 : 64 / slots;
-  p.heads_per_run = p.num_tokens >= kRotaryManyTokens ? heads : pass;
+  p.heads_per_run = slots >= 64 ? 1 : 64 / slots;  // those that one pass of a wave covers
   p.runs = (heads + p.heads_per_run - 1) / p.heads_per_run;
   const long long grid = ((long long)p.num_tokens * p.runs + kRotaryWaves - 1) / kRotaryWaves;
   if (grid > 0x7FFFFFFFll) return hipErrorInvalidValue;
