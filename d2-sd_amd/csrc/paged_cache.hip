@@ -16,10 +16,10 @@
 // reads back as NaN.
 //
 // Both kernels move data once: bound by HBM (16 requests, 0.26 GB read back:
-// 94 us, 4.8 TB/s, where a large copy reaches 4.96) or, for a step's few tokens,
-// by the chain token -> cache length -> page id -> store (64 tokens: 3 us).  A thread carries 8
-// elements: a 16-byte bf16 load or store against 8 bytes (fp8, mxfp8) or 4
-// (mxfp4) of codes; the four threads of a block of 32 find its amax by DPP.
+// 90 us, 5.0 TB/s, the rate of a large copy) or, for a step's few tokens, by the
+// chain token -> cache length -> page id -> store (64 tokens: 3 us).  A thread
+// carries 8 elements: a 16-byte bf16 load or store against 8 bytes (fp8, mxfp8)
+// or 4 (mxfp4) of codes; the four threads of a block of 32 find its amax by DPP.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -32,12 +32,15 @@ namespace d2sd {
 
 namespace {
 
+// tokens of an item that one block reads (16 requests in mxfp8, 43k tokens: 1, 2, 4, 8, 16:
+// 102, 92, 90, 89, 95 us; 16.3k tokens in mxfp4 with their write: 47, 43.5, 43, 43.6, 46.7)
+constexpr int kReadShare = 4;
 constexpr int kWriteTokens = 8;         // of one block, where there are many
 // (8 heads of 128 in mxfp4: 4096 tokens 7.1 and 7.2 us, 8000 tokens 13.3 one by one, 11.3 by eight)
 constexpr int kWriteManyTokens = 6144;
 // Results larger than half of the last-level cache are stored past it: nothing
 // of them would be found there by whoever reads them from their start (16
-// requests of 100..8000 tokens, 0.26 GB: 99 -> 94 us).
+// requests of 100..8000 tokens, 0.26 GB: 99 -> 94 us with 16 tokens a block).
 constexpr long long kReadStreamBytes = 128ll << 20;
 
 // 2^(byte - 127); byte 255 stands for NaN, byte 0 for 2^-127
@@ -264,20 +267,22 @@ __device__ __forceinline__ u32x4 load_piece(const CacheSide& s, int h, long long
   }
 }
 
-// Block i: up to kReadTokens cached tokens of one request, all heads, keys then
-// values (items[i]: CacheReadItem).  A thread takes the same piece of every
+// Block (i, j): tokens kReadShare j .. of the up to kReadTokens cached tokens of one
+// request that items[i] names (CacheReadItem), all heads, keys then values.  A thread takes the same piece of every
 // token, or, where a token has at most 128 pieces, of every n-th one; the tokens'
 // pages are found once, by one lane each.  One load, then its store: with 8 loads
 // in flight a thread's stores scatter over 8 rows (99 -> 117 us).
 template <int FMT, bool STREAM>
 __global__ __launch_bounds__(256) void cache_read_kernel(const CacheParams p) {
   const CacheReadItem w = ((const CacheReadItem*)p.items)[blockIdx.x];
+  const int from = blockIdx.y * kReadShare, count = min(w.count - from, kReadShare);
+  if (count <= 0) return;
   const int len = p.kv_len[w.req];
-  const int pos0 = w.from_end ? len - w.first : w.first;  // cache position of the item's first token
+  const int pos0 = (w.from_end ? len - w.first : w.first) + from;  // cache position of the block's first token
   const int cpr = p.head_dim / 8, nch = p.num_kv_heads * cpr;
   const int lane = threadIdx.x & 63;
   int page = -1, slot = 0;
-  if (lane < w.count) {
+  if (lane < count) {
     const int pos = pos0 + lane, at = w.page_begin + (pos >> p.log2_page);
     slot = pos & ((1 << p.log2_page) - 1);
     if (pos >= 0 && pos < len && at < w.page_end) page = p.page_table[at];
@@ -287,27 +292,27 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheParams p) {
     const bool is_v = c >= nch;
     const int cc = is_v ? c - nch : c, h = cc / cpr, d = 8 * (cc - h * cpr);
     const long long row = h * p.stride_head, srow = h * p.scale_stride_head;
-    uint16_t* out = (uint16_t*)(is_v ? p.v : p.k) + (long long)w.row * p.stride_n + (long long)h * p.stride_h + d;
+    uint16_t* out = (uint16_t*)(is_v ? p.v : p.k) + (long long)(w.row + from) * p.stride_n + (long long)h * p.stride_h + d;
     tokens(is_v ? p.vs : p.ks, h, d, row, srow, out);
   };
   const int apart = 256 / (2 * nch);  // threads of a piece
   if (apart > 1) {
     const int first = threadIdx.x / (2 * nch);
     piece(threadIdx.x - first * 2 * nch, [&](const CacheSide& s, int h, int d, long long row, long long srow, uint16_t* out) {
-      for (int i0 = 0; i0 < kReadTokens; i0 += apart) {  // (every lane stays for the shuffles)
+      for (int i0 = 0; i0 < kReadShare; i0 += apart) {  // (every lane stays for the shuffles)
         const int i = i0 + first, pg = __shfl(page, i), sl = __shfl(slot, i);
-        if (first < apart && i < w.count && pg >= 0)
+        if (first < apart && i < count && pg >= 0)
           *(u32x4*)(out + i * p.stride_n) = load_piece<FMT>(s, h, row + pg * p.stride_page + sl * p.stride_tok,
                                                             srow + pg * p.scale_stride_page + sl * p.scale_stride_tok, d);
       }
     });
     return;
   }
-  const Places<kReadTokens> places(page, slot);
+  const Places<kReadShare> places(page, slot);
   for (int c = threadIdx.x; c < 2 * nch; c += 256) {
     piece(c, [&](const CacheSide& s, int h, int d, long long row, long long srow, uint16_t* out) {
 #pragma unroll
-      for (int i = 0; i < kReadTokens; ++i) {
+      for (int i = 0; i < kReadShare; ++i) {
         if (!places.on(i)) continue;
         const u32x4 val = load_piece<FMT>(s, h, row + places.row(p, i), srow + places.scale_row(p, i), d);
         u32x4* at = (u32x4*)(out + i * p.stride_n);
@@ -347,7 +352,7 @@ hipError_t launch_cache_write(const CacheParams& p, int format, hipStream_t s) {
 
 template <int FMT>
 static void launch_read(const CacheParams& p, hipStream_t s) {
-  const dim3 grid((unsigned)p.num_items), block(256);
+  const dim3 grid((unsigned)p.num_items, kReadTokens / kReadShare), block(256);
   if (4ll * p.num_kv_heads * p.head_dim * kReadTokens * p.num_items > kReadStreamBytes)
     hipLaunchKernelGGL((cache_read_kernel<FMT, true>), grid, block, 0, s, p);
   else
