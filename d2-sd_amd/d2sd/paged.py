@@ -9,7 +9,8 @@ block formats halve and quarter a cache's bytes without scales to calibrate.
 
     kv_format  pools                                scales
     "bf16"     bf16                                 none
-    "fp8"      float8_e4m3fn, value / scale[head]   fp32 [Hkv] each for K and V
+    "fp8"      float8_e4m3fn, value / scale[head]   fp32 [Hkv] each for K and V,
+                                                    positive
     "mxfp8"    float8_e4m3fn                        uint8, one per 32 head dims
     "mxfp4"    uint8, two e2m1 elements a byte      uint8, one per 32 head dims
                (the even one low)

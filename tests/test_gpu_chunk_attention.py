@@ -339,6 +339,31 @@ def test_shared_pages_of_a_common_prefix():
         assert ((out[rows].cpu().double() - o).abs() <= bound).all()
 
 
+def test_a_cache_of_a_quarter_million_tokens():
+    """Keys split as far as a plan goes, and not at all."""
+    for kw in (dict(), dict(max_splits=1)):
+        run_and_check([1, 9], [250001, 131072], 4, 2, 64, "bf16", P=64, **kw)
+
+
+def test_a_page_table_in_place_is_read_at_each_call():
+    """Pages moved by device writes to the table and the pools: the same batch and plan follow."""
+    p = Problem([2, 70], [100, 300], 8, 2, 64, "mxfp8")
+    ref = p.run()
+    torch.cuda.synchronize()
+    assert p.batch.page_table.data_ptr() == p.table.data_ptr()
+    n = p.cache.num_pages
+    perm = torch.randperm(n, generator=torch.Generator().manual_seed(2)).to(DEV)
+    for t in (p.cache.k_pool, p.cache.v_pool, p.cache.k_scale, p.cache.v_scale):
+        old = t.view(torch.uint8).clone()
+        t.view(torch.uint8)[perm] = old  # page i moves to perm[i]
+    p.table.copy_(perm[p.table.long()].to(torch.int32))
+    got = p.run()
+    k, v = p.cache.read(p.batch)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+    assert torch.equal(k.cpu().double(), p.kr) and torch.equal(v.cpu().double(), p.vr)
+
+
 def test_offsets_past_32_bits():
     """Pages beyond 4 GiB of a pool (token-major, so that rows of one head lie far apart as well)."""
     P, hkv, d, L = 16, 8, 128, 100
