@@ -850,24 +850,44 @@ chunk_attn_kernel(const ChunkParams p) {
 }
 
 // Row i of a merge item from its nchunks partial states: thread (i, d4) holds
-// head dims 4 d4 .. 4 d4 + 3.  Latency bound: all of a row's sums are read first,
-// then its states, in chunk order whatever the order they were written in.
+// head dims 4 d4 .. 4 d4 + 3.  Latency bound: the sums and states of eight chunks
+// are read at once (one token over 8 chunks: 3.8 -> 3.0 us against sums first),
+// joined in chunk order whatever the order they were written in.
 template <int D>
 __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkParams p) {
   const ChunkMerge w = p.merges[blockIdx.x];
   const int i = threadIdx.x / (D / 4), dd = 4 * (threadIdx.x % (D / 4));
   if (i >= w.nrows) return;
-  const float* ls = p.part_lse + w.slot + i;
-  float top = -INFINITY;
-  for (int c = 0; c < w.nchunks; ++c) top = fmaxf(top, ls[(long long)c * w.stride]);
+  constexpr int B = 8;
+  float top = -INFINITY, sum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
-  for (int c = 0; c < w.nchunks; ++c) {
-    const float s = ls[(long long)c * w.stride];
-    const float a = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - top);
-    const f32x4 v = *(const f32x4*)(p.part_o + (w.slot + (long long)c * w.stride + i) * D + dd);
-    sum += a;
-    acc += a * v;
+  for (int c0 = 0; c0 < w.nchunks; c0 += B) {
+    float s[B];
+    f32x4 v[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const long long pr = w.slot + i + (long long)min(c0 + u, w.nchunks - 1) * w.stride;
+      s[u] = c0 + u < w.nchunks ? p.part_lse[pr] : -INFINITY;
+      v[u] = *(const f32x4*)(p.part_o + pr * D + dd);
+    }
+    float mx = top;
+#pragma unroll
+    for (int u = 0; u < B; ++u) mx = fmaxf(mx, s[u]);
+    if (mx == -INFINITY) {  // no key in any of them (or NaN, which stays)
+#pragma unroll
+      for (int u = 0; u < B; ++u) sum = s[u] == s[u] ? sum : s[u];
+      continue;
+    }
+    const float a0 = __builtin_amdgcn_exp2f(top - mx);
+    top = mx;
+    sum *= a0;
+    acc *= a0;
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const float a = __builtin_amdgcn_exp2f(s[u] - top);
+      sum += a;
+      acc += s[u] == -INFINITY ? f32x4{0.f, 0.f, 0.f, 0.f} : a * v[u];
+    }
   }
   const float lse2 = sum > 0.f ? top + __builtin_amdgcn_logf(sum) : sum == 0.f ? -INFINITY : sum;
   const int r = w.row0 + i, token = w.q0 + r / p.group, head = w.kvh * p.group + r % p.group;
