@@ -342,17 +342,23 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
   };
   constexpr int PN = EPT / 8, PW = FMT == CACHE_MXFP4 ? 1 : 2;  // chunks of a part, words of a chunk
   const unsigned turn = write_turn<D, PN>(srow, spart), pswz = chunk_swizzle<D>(srow) ^ turn;
-  auto put = [&](lds_char* tile, const unsigned (&d)[WORDS], unsigned sc) {
+  // chunk i of the keys' part (the values' from PN on) to the tile (K, then V) at
+  // `tile`, in turn from 0 on
+  auto put = [&](lds_char* tile, int i) {
     if constexpr (FMT != CACHE_BF16) {
-      const float f = MX ? block_scale(sc) : 1.f;
-      unsigned x[PN * PW];
+      const bool is_v = i >= PN;
+      const int ch = i % PN;
+      unsigned(&x)[PN * PW] = is_v ? vw : kw;
+      if (ch == 0) turn_chunks<PN, PW>(x, turn);
+      const float f = MX ? block_scale(is_v ? vsc : ksc) : 1.f;
+      *(__attribute__((address_space(3))) bf16x8*)(tile + (is_v ? TB : 0) + srow * D * 2 + 16 * ((spart * PN + ch) ^ pswz)) =
+          expand<FMT>(x[PW * ch], x[PW * ch + PW - 1], f);
+    }
+  };
+  auto put_all = [&](lds_char* tile) {
+    if constexpr (FMT != CACHE_BF16) {
 #pragma unroll
-      for (int i = 0; i < PN * PW; ++i) x[i] = d[i];
-      turn_chunks<PN, PW>(x, turn);
-#pragma unroll
-      for (int i = 0; i < PN; ++i)
-        *(__attribute__((address_space(3))) bf16x8*)(tile + srow * D * 2 + 16 * ((spart * PN + i) ^ pswz)) =
-            expand<FMT>(x[PW * i], x[PW * i + PW - 1], f);
+      for (int i = 0; i < 2 * PN; ++i) put(tile, i);
     }
   };
 
@@ -366,7 +372,10 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
   const ValueRead<D> vread(lane);
 
   // Two buffers of (K, V).  bf16: tile t + 1 is on its way while tile t is
-  // worked on.  Quantised: tile t + 2 is, and t + 1 is expanded into LDS.
+  // worked on.  Quantised: tile t + 2 is, and t + 1 is expanded into LDS, beside
+  // the score products (24 requests with a chunk of 1000 in mxfp4 60 -> 55 us;
+  // but not where registers would spill: mxfp8 heads of 64, 1300 -> 1320).
+  constexpr bool BESIDE = FMT != CACHE_BF16 && !(D == 64 && FMT == CACHE_MXFP8);
   unsigned page = 0;
   if (tb < te) {
     if constexpr (FMT == CACHE_BF16) {
@@ -376,8 +385,7 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
       wait_vmcnt<0>();
     } else {
       fetch(tb, page_of(key_of(tb, srow)));
-      put(lds, kw, ksc);
-      put(lds + TB, vw, vsc);
+      put_all(lds);
       if (tb + 1 < te) {
         fetch(tb + 1, page_of(key_of(tb + 1, srow)));
         page = page_of(key_of(min(tb + 2, te - 1), srow));
@@ -417,16 +425,20 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
         s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks][0], qf[ks], ks ? s[0] : f32x16{}, 0, 0, 0);
         s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks][1], qf[ks], ks ? s[1] : f32x16{}, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (BESIDE) {
+          // tile t + 1 into LDS (behind the last tile nobody reads it)
+#pragma unroll
+          for (int i = 0; i < 2 * PN; ++i)
+            if (i * KS / (2 * PN) == ks) put(lds + nxt, i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
+    if (!BESIDE || !on) put_all(lds + nxt);
     if constexpr (FMT != CACHE_BF16) {
-      if (t + 1 < te) {
-        put(lds + nxt, kw, ksc);
-        put(lds + nxt + TB, vw, vsc);
-        if (t + 2 < te) {
-          fetch(t + 2, page);
-          page = page_of(key_of(min(t + 3, te - 1), srow));
-        }
+      if (t + 2 < te) {
+        fetch(t + 2, page);
+        page = page_of(key_of(min(t + 3, te - 1), srow));
       }
     }
     if (on) {
