@@ -1293,6 +1293,7 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t ho
     const int group = d->num_qo_heads / d->num_kv_heads;
     if (d->num_reqs > 0 && (d->qo_indptr[0] != 0 || d->page_indptr[0] < 0))
       return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: qo_indptr starts at 0, page_indptr at 0 or above");
+    int64_t room = 0, most_new = 0;  // tokens that a request's pages hold, that it brings: the largest
     for (int r = 0; r < d->num_reqs; ++r) {
       const int64_t n = (int64_t)d->qo_indptr[r + 1] - d->qo_indptr[r];
       const int64_t pages = (int64_t)d->page_indptr[r + 1] - d->page_indptr[r];
@@ -1302,7 +1303,15 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t ho
         return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: request " + std::to_string(r) + " has no pages for its cache");
       if ((pages << lg) > (int64_t)INT32_MAX - 64 || n * group > (int64_t)INT32_MAX)
         return fail(D2SD_ERR_UNSUPPORTED, "chunk_plan: request " + std::to_string(r) + " is too long");
+      room = std::max(room, pages << lg);
+      most_new = std::max(most_new, n);
     }
+    // A window as wide as all pages is none.  Narrower ones are subtracted from
+    // positions in 32 bits, and a cache cut back below its new tokens starts at a
+    // negative one.
+    const int window = d->window_left >= room ? -1 : d->window_left;
+    if (window >= 0 && most_new + window > (int64_t)INT32_MAX)
+      return fail(D2SD_ERR_UNSUPPORTED, "chunk_plan: window_left and new tokens exceed 2^31");
     d2sd::ChunkPlanInput in{};
     in.num_reqs = d->num_reqs;
     in.qo_indptr = d->qo_indptr;
@@ -1312,7 +1321,7 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t ho
     in.num_kv_heads = d->num_kv_heads;
     in.head_dim = d->head_dim;
     in.format = d->format;
-    in.window_left = d->window_left;
+    in.window_left = window;
     in.num_cus = d->num_cus > 0 ? d->num_cus : device_num_cus();
     in.max_splits = d->max_splits;
     d2sd::ChunkPlanOutput out;
@@ -1331,7 +1340,7 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t ho
     info->head_dim = d->head_dim;
     info->format = d->format;
     info->page_size = d->page_size;
-    info->window_left = d->window_left;
+    info->window_left = window;
     info->form = out.form;
     info->num_page_entries = d->num_reqs > 0 ? d->page_indptr[d->num_reqs] : 0;
     info->workspace_bytes = (size_t)out.partial_rows * (d->head_dim + 1) * sizeof(float);

@@ -658,7 +658,7 @@ typedef struct {
   int head_dim;
   int format;
   int page_size;
-  int window_left;
+  int window_left;       /* -1 too where the window covers all pages of every request */
   int num_page_entries;  /* page_table entries the plan may read */
   int form;              /* which of its kernels the plan is for */
   size_t workspace_bytes;
