@@ -39,8 +39,9 @@ class PagedChunkAttention:
     def plan(self, batch: PagedBatch, num_qo_heads: int, num_kv_heads: int, head_dim: int, *, kv_format: str = "bf16",
              sm_scale: Optional[float] = None, window_left: int = -1, sinks: Optional[torch.Tensor] = None,
              lse_base2: bool = False, max_splits: int = 0, num_cus: int = 0) -> "PagedChunkAttention":
-        """Plans the batch (its kv_len when it was made: the work is shared out
-        for those lengths, and right for any within the requests' pages).
+        """Plans the batch (its kv_len_host, of its making or the last
+        set_kv_len: the work is shared out for those lengths, and right for any
+        within the requests' pages).
 
         Query i of request r sits at position kv_len[r] - n_r + i and sees the
         cached keys up to it; window_left >= 0 keeps the window_left keys

@@ -80,8 +80,11 @@ class PagedBatch:
     `kv_len` (int32, on the device) holds the current lengths and is what the
     kernels read: update it in place (set_kv_len, or any device write) and the
     same batch, and graphs captured with it, serve the next step, as long as
-    the new tokens stay as many and the pages suffice.  A contiguous int32
-    device tensor given as page_table is used in place."""
+    the new tokens stay as many and the pages suffice.  kv_len_host,
+    kv_indptr_host and total_kv are the host's lengths, those of the last
+    set_kv_len (a device write does not move them): full reads cover them, and
+    plans made from now on share out work for them.  A contiguous int32 device
+    tensor given as page_table is used in place."""
 
     def __init__(self, qo_indptr: Sequence[int], kv_len: Sequence[int], page_indptr: Sequence[int],
                  page_table: Union[Sequence[int], torch.Tensor], page_size: int,
@@ -103,9 +106,9 @@ class PagedBatch:
             raise ValueError("page_table shorter than page_indptr[-1]")
         self.device = _device(device)
         self.page_size, self.num_reqs, self.total_q = P, R, int(qo[-1])
-        self.qo_indptr_host, self.kv_len_host, self.page_indptr_host = qo, kv, pi
-        self.kv_indptr_host = np.concatenate([[0], np.cumsum(kv, dtype=np.int64)])
-        self.total_kv = int(self.kv_indptr_host[-1])
+        self.qo_indptr_host, self.page_indptr_host = qo, pi
+        self._reads = {}
+        self._host_lengths(kv)
         if self.total_kv >= 2 ** 31:
             raise ValueError("the batch's caches hold 2^31 tokens or more")
         # one upload: a record per new token, then the lengths
@@ -120,19 +123,28 @@ class PagedBatch:
             self.page_table = page_table.reshape(-1)
         else:
             self.page_table = torch.from_numpy(_i32(page_table).reshape(-1)).to(self.device)
-        self._reads = {}
+
+    def _host_lengths(self, kv: np.ndarray) -> None:
+        self.kv_len_host = kv
+        self.kv_indptr_host = np.concatenate([[0], np.cumsum(kv, dtype=np.int64)])
+        self.total_kv = int(self.kv_indptr_host[-1])
+        self._reads.pop(False, None)  # (those of the new tokens count from a cache's end)
 
     def set_kv_len(self, kv_len: Sequence[int]) -> None:
-        """Current cache lengths (host write into `kv_len`)."""
+        """Current cache lengths (host write into `kv_len`).  The next full read
+        covers them; one captured before keeps the rows that it was captured
+        with."""
         v = _i32(kv_len)
         if v.shape != (self.num_reqs,) or (v < 0).any() or \
                 (v.astype(np.int64) > np.diff(self.page_indptr_host).astype(np.int64) * self.page_size).any():
             raise ValueError("one length per request, within its pages")
         self.kv_len.copy_(torch.from_numpy(v))
+        self._host_lengths(v)
 
     def prepare_read(self, new_only: bool = False) -> "PagedBatch":
         """Builds what PagedKVCache.read needs of this batch (done by the first
-        read; call it before a read that is captured into a graph)."""
+        read, and the first full one after set_kv_len; call it before a read
+        that is captured into a graph)."""
         if new_only not in self._reads:
             if self.device.type == "cuda" and capturing():
                 raise RuntimeError("PagedKVCache.read: call batch.prepare_read() before capturing a read")
@@ -141,6 +153,8 @@ class PagedBatch:
                 n = np.diff(self.qo_indptr_host)
                 spans = _spans(n, n, self.qo_indptr_host[:-1], req, True, self.page_indptr_host)
             else:
+                if self.total_kv >= 2 ** 31:
+                    raise ValueError("the batch's caches hold 2^31 tokens or more")
                 spans = _spans(np.zeros_like(self.kv_len_host), self.kv_len_host, self.kv_indptr_host[:-1], req, False,
                                self.page_indptr_host)
             self._reads[new_only] = torch.from_numpy(spans).to(self.device)
@@ -232,9 +246,9 @@ class PagedKVCache:
     def read(self, batch: PagedBatch, new_only: bool = False,
              out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """The batch's cached keys and values as contiguous bf16 [rows, Hkv, D]:
-        request r's tokens are rows kv_indptr_host[r] .. of the batch (its
-        lengths when it was made), or, with new_only, the batch's new tokens in
-        the rows of q.  Rows of tokens that the cache does not hold now (a
+        request r's tokens are rows kv_indptr_host[r] .. of the batch (the
+        host's lengths: set_kv_len's), or, with new_only, the batch's new tokens
+        in the rows of q.  Rows of tokens that the cache does not hold now (a
         shorter kv_len, a page id outside the pool) are not written.  out:
         (k, v) of any token and head strides, alike."""
         self._check_batch(batch)

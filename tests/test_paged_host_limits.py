@@ -23,3 +23,25 @@ def test_a_window_as_wide_as_the_pages_is_none():
     # and a narrower one that leaves them all the same is refused
     with pytest.raises(RuntimeError, match="window_left"):
         _plan([2 ** 21], [0], [2047], P=2 ** 20, window_left=2047 * 2 ** 20 - 1)
+
+
+def test_set_kv_len_moves_the_host_lengths():
+    """Full reads and plans made after it are for the lengths it gave."""
+    b = d2sd.PagedBatch([0, 1, 2], [1000, 20], [0, 4096, 4100], np.zeros(4100, np.int32), 16, device="cpu")
+    before = b.prepare_read()._reads[False]
+    new = b.prepare_read(new_only=True)._reads[True]
+    given = np.array([60000, 17])
+    b.set_kv_len(given)
+    given[:] = 0
+    assert b.kv_len_host.tolist() == [60000, 17] and b.kv_indptr_host.tolist() == [0, 60000, 60017] and b.total_kv == 60017
+    spans = b.prepare_read()._reads[False]
+    assert spans is not before and int(spans[:, 1].sum()) == 60017 and int(spans[:, 4].max()) == 60016
+    assert b.prepare_read(new_only=True)._reads[True] is new
+    grown = d2sd.PagedChunkAttention("cpu").plan(b, 8, 2, 128, num_cus=256)
+    fresh = _plan([1, 1], [60000, 17], [4096, 4])
+    assert np.array_equal(grown.plan_host, fresh.plan_host)
+    # batches over shared pages may hold more tokens than a read has rows
+    b = d2sd.PagedBatch(range(65), [1] * 64, range(0, 64 * 2048 + 1, 2048), np.zeros(64 * 2048, np.int32), 2 ** 14, device="cpu")
+    b.set_kv_len([2 ** 25] * 64)
+    with pytest.raises(ValueError, match="2\\^31"):
+        b.prepare_read()
