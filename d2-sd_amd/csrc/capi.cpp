@@ -1250,6 +1250,7 @@ int cache_params(const d2sd_cache_io_args* a, const char* who, d2sd::CacheParams
   p.head_dim = c.head_dim;
   p.log2_page = log2_of(c.page_size);
   p.num_pages = c.num_pages;
+  p.zero_missing = a->zero_missing ? 1 : 0;
   return D2SD_OK;
 }
 

@@ -283,6 +283,7 @@ struct CacheParams {
   long long stride_page, stride_head, stride_tok;                    // code elements (mxfp4: bytes)
   long long scale_stride_page, scale_stride_head, scale_stride_tok;  // bytes (mx formats)
   int num_items, num_kv_heads, head_dim, log2_page, num_pages;
+  int zero_missing;              // read: rows of tokens without a place become zero
 };
 
 // ---------------------------------------------------------------------------

@@ -351,7 +351,8 @@ d2sd_paged_cache cache_of(const at::Tensor& k_pool, const at::Tensor& v_pool, co
 
 void cache_io(bool write, const at::Tensor& k, const at::Tensor& v, int64_t rows, const at::Tensor& items, int64_t num_items,
               const at::Tensor& kv_len, const at::Tensor& page_table, const at::Tensor& k_pool, const at::Tensor& v_pool,
-              const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale, int64_t format, bool nhd) {
+              const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale, int64_t format, bool nhd,
+              bool zero_missing = false) {
   d2sd_cache_io_args a;
   std::memset(&a, 0, sizeof(a));
   a.cache = cache_of(k_pool, v_pool, k_scale, v_scale, format, nhd);
@@ -377,6 +378,7 @@ void cache_io(bool write, const at::Tensor& k, const at::Tensor& v, int64_t rows
   a.stride_n = k.stride(0);
   a.stride_h = k.stride(1);
   a.num_items = (int)num_items;
+  a.zero_missing = zero_missing;
   const c10::DeviceGuard guard(dev);
   check(write ? d2sd_cache_write(&a, current_stream()) : d2sd_cache_read(&a, current_stream()),
         write ? "d2sd.cache_write" : "d2sd.cache_read");
@@ -399,7 +401,7 @@ std::tuple<at::Tensor, at::Tensor> cache_read(int64_t rows, const at::Tensor& it
   const auto opt = k_pool.options().dtype(at::kBFloat16);
   const int64_t hkv = k_pool.size(nhd ? 2 : 1), d = k_pool.size(3) * (format == D2SD_CACHE_MXFP4 ? 2 : 1);
   at::Tensor k = at::empty({rows, hkv, d}, opt), v = at::empty({rows, hkv, d}, opt);
-  cache_io(false, k, v, rows, items, num_items, CACHE_PASS);
+  cache_io(false, k, v, rows, items, num_items, CACHE_PASS, true);
   return {k, v};
 }
 

@@ -311,6 +311,7 @@ class CacheIoArgs(C.Structure):
         ("stride_n", C.c_int64),
         ("stride_h", C.c_int64),
         ("num_items", C.c_int),
+        ("zero_missing", C.c_int),
     ]
 
 

@@ -249,8 +249,8 @@ class PagedKVCache:
         request r's tokens are rows kv_indptr_host[r] .. of the batch (the
         host's lengths: set_kv_len's), or, with new_only, the batch's new tokens
         in the rows of q.  Rows of tokens that the cache does not hold now (a
-        shorter kv_len, a page id outside the pool) are not written.  out:
-        (k, v) of any token and head strides, alike."""
+        shorter kv_len, a page id outside the pool) are zero; in a given `out`
+        they are left alone.  out: (k, v) of any token and head strides, alike."""
         self._check_batch(batch)
         rows = batch.total_q if new_only else batch.total_kv
         if new_only not in batch._reads:

@@ -610,6 +610,7 @@ typedef struct {
   void* v;
   int64_t stride_n, stride_h; /* elements, of k and v */
   int num_items;
+  int zero_missing;          /* read: rows of tokens the cache does not hold are set to zero */
 } d2sd_cache_io_args;
 
 /* Writes new keys and values into their pages.  A slot that two tokens of one
@@ -617,7 +618,8 @@ typedef struct {
  * are skipped. */
 int d2sd_cache_write(const d2sd_cache_io_args* args, d2sd_stream_t stream);
 /* Reads cached tokens as bf16 (fp8: code * scale, rounded once; the other
- * formats exactly).  Rows of tokens the cache does not hold stay as they are. */
+ * formats exactly).  Rows of tokens the cache does not hold stay as they are, or,
+ * with zero_missing, become zero. */
 int d2sd_cache_read(const d2sd_cache_io_args* args, d2sd_stream_t stream);
 
 /* Attention of each request's newest tokens over its cache, which already

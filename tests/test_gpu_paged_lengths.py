@@ -62,3 +62,37 @@ def test_captured_reads_keep_their_rows_and_later_ones_follow():
         torch.cuda.synchronize()
         for x, y, want in zip(out, now, vals):
             assert torch.equal(x.cpu(), want[rows([20, 50])]) and torch.equal(y.cpu(), want[rows(lens)])
+
+
+@pytest.mark.parametrize("hkv,d", [(2, 64), (8, 128)])
+@pytest.mark.parametrize("fmt", ["bf16", "fp8", "mxfp8", "mxfp4"])
+def test_rows_that_the_cache_does_not_hold_are_zero(fmt, hkv, d):
+    """Tensors that a read allocates (in memory that held something else): zeros for tokens past a length that a device
+    write shortened, before a cache's start, and in pages outside the pool; the others as they are."""
+    room = [40, 100, 33]
+    c, pi, table, vals, rows = _caches(fmt, 16, hkv, d, room, 5)
+    b = d2sd.PagedBatch([0, 5, 5, 25], room, pi, table, 16)
+    b.prepare_read().prepare_read(new_only=True)
+    lens = [38, 61, 12]
+    b.kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+    b.page_table[1] = 2 ** 31 - 1       # tokens 16 .. 31 of request 0
+    b.page_table[int(pi[1])] = -1       # 0 .. 15 of request 1
+    held = [torch.arange(n) < m for n, m in zip(room, lens)]
+    held[0][16:32] = False
+    held[1][:16] = False
+    full = torch.cat(held)
+    # new tokens of requests 0 and 2: 33 .. 37, and -8 .. 11 (of which 8 have no place)
+    new = torch.cat([torch.arange(33, 38), torch.full((8,), -1), 140 + torch.arange(12)])
+    for new_only in (False, True):
+        n = b.total_q if new_only else b.total_kv
+        for _ in range(3):
+            stale = [torch.full((n, hkv, d), 7.0, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+            torch.cuda.synchronize()
+            del stale
+            got = c.read(b, new_only=new_only)
+            torch.cuda.synchronize()
+            for x, want in zip(got, vals):
+                want = torch.where((new >= 0)[:, None, None], want[new], 0) if new_only else \
+                    torch.where(full[:, None, None], want, 0)
+                assert torch.equal(x.cpu(), want.to(torch.bfloat16))
+            del got, x
