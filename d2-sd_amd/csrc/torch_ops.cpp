@@ -22,11 +22,14 @@
 // dispatch key named CUDA is where torch registers its GPU (here HIP) device.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/library.h>
 
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 
 #include "d2sd.h"
 
@@ -246,6 +249,23 @@ void need_type(const at::Tensor& t, at::ScalarType dt, const char* name) {
   TORCH_CHECK_TYPE(t.scalar_type() == dt, "d2sd: ", name, " must be ", dt, " (got ", t.scalar_type(), ")");
 }
 
+const at::Tensor* or_null(const c10::optional<at::Tensor>& t) { return t.has_value() ? &*t : nullptr; }
+
+// Tensors that a batch, plan or cache holds for its caller: made on one stream and
+// read by a call on another, they may be let go of while the call is under way, and
+// their memory waits for it then.  home: the stream all of them were made on
+// (nothing to do for calls on it), -1 for any.  Captured calls have them held by the
+// graph.
+void in_use(int64_t home, std::initializer_list<const at::Tensor*> held) {
+  const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream();
+  if (home == (int64_t)(intptr_t)stream.stream()) return;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) (void)hipGetLastError();
+  if (status != hipStreamCaptureStatusNone) return;
+  for (const at::Tensor* t : held)
+    if (t) c10::hip::HIPCachingAllocator::recordStream(t->storage().data_ptr(), stream);
+}
+
 void rotary_embedding(const c10::optional<at::Tensor>& q, const c10::optional<at::Tensor>& k, const at::Tensor& positions,
                       const at::Tensor& inv_freq, const c10::optional<at::Tensor>& q_out,
                       const c10::optional<at::Tensor>& k_out, bool interleaved, double scale, bool inverse) {
@@ -352,7 +372,7 @@ d2sd_paged_cache cache_of(const at::Tensor& k_pool, const at::Tensor& v_pool, co
 void cache_io(bool write, const at::Tensor& k, const at::Tensor& v, int64_t rows, const at::Tensor& items, int64_t num_items,
               const at::Tensor& kv_len, const at::Tensor& page_table, const at::Tensor& k_pool, const at::Tensor& v_pool,
               const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale, int64_t format, bool nhd,
-              bool zero_missing = false) {
+              int64_t home, bool zero_missing = false) {
   d2sd_cache_io_args a;
   std::memset(&a, 0, sizeof(a));
   a.cache = cache_of(k_pool, v_pool, k_scale, v_scale, format, nhd);
@@ -382,6 +402,7 @@ void cache_io(bool write, const at::Tensor& k, const at::Tensor& v, int64_t rows
   const c10::DeviceGuard guard(dev);
   check(write ? d2sd_cache_write(&a, current_stream()) : d2sd_cache_read(&a, current_stream()),
         write ? "d2sd.cache_write" : "d2sd.cache_read");
+  in_use(home, {&items, &kv_len, &page_table, &k_pool, &v_pool, or_null(k_scale), or_null(v_scale)});
 }
 
 #define CACHE_ARGS                                                                                             \
@@ -389,25 +410,28 @@ void cache_io(bool write, const at::Tensor& k, const at::Tensor& v, int64_t rows
       const c10::optional<at::Tensor>&k_scale, const c10::optional<at::Tensor>&v_scale, int64_t format, bool nhd
 #define CACHE_PASS kv_len, page_table, k_pool, v_pool, k_scale, v_scale, format, nhd
 
-void cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& items, int64_t num_items, CACHE_ARGS) {
-  cache_io(true, k, v, num_items, items, num_items, CACHE_PASS);
+void cache_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& items, int64_t num_items, CACHE_ARGS,
+                 int64_t home) {
+  cache_io(true, k, v, num_items, items, num_items, CACHE_PASS, home);
 }
 
-void cache_read_out(at::Tensor& k, at::Tensor& v, int64_t rows, const at::Tensor& items, int64_t num_items, CACHE_ARGS) {
-  cache_io(false, k, v, rows, items, num_items, CACHE_PASS);
+void cache_read_out(at::Tensor& k, at::Tensor& v, int64_t rows, const at::Tensor& items, int64_t num_items, CACHE_ARGS,
+                    int64_t home) {
+  cache_io(false, k, v, rows, items, num_items, CACHE_PASS, home);
 }
 
-std::tuple<at::Tensor, at::Tensor> cache_read(int64_t rows, const at::Tensor& items, int64_t num_items, CACHE_ARGS) {
+std::tuple<at::Tensor, at::Tensor> cache_read(int64_t rows, const at::Tensor& items, int64_t num_items, CACHE_ARGS,
+                                              int64_t home) {
   const auto opt = k_pool.options().dtype(at::kBFloat16);
   const int64_t hkv = k_pool.size(nhd ? 2 : 1), d = k_pool.size(3) * (format == D2SD_CACHE_MXFP4 ? 2 : 1);
   at::Tensor k = at::empty({rows, hkv, d}, opt), v = at::empty({rows, hkv, d}, opt);
-  cache_io(false, k, v, rows, items, num_items, CACHE_PASS, true);
+  cache_io(false, k, v, rows, items, num_items, CACHE_PASS, home, true);
   return {k, v};
 }
 
-void cache_write_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, CACHE_ARGS) {}
-void cache_read_out_meta(at::Tensor&, at::Tensor&, int64_t, const at::Tensor&, int64_t, CACHE_ARGS) {}
-std::tuple<at::Tensor, at::Tensor> cache_read_meta(int64_t rows, const at::Tensor&, int64_t, CACHE_ARGS) {
+void cache_write_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, CACHE_ARGS, int64_t) {}
+void cache_read_out_meta(at::Tensor&, at::Tensor&, int64_t, const at::Tensor&, int64_t, CACHE_ARGS, int64_t) {}
+std::tuple<at::Tensor, at::Tensor> cache_read_meta(int64_t rows, const at::Tensor&, int64_t, CACHE_ARGS, int64_t) {
   const auto opt = k_pool.options().dtype(at::kBFloat16);
   const int64_t hkv = k_pool.size(nhd ? 2 : 1), d = k_pool.size(3) * (format == D2SD_CACHE_MXFP4 ? 2 : 1);
   return {at::empty({rows, hkv, d}, opt), at::empty({rows, hkv, d}, opt)};
@@ -417,7 +441,7 @@ std::tuple<at::Tensor, at::Tensor> cache_read_meta(int64_t rows, const at::Tenso
 // info: the d2sd_chunk_plan_info bytes plan() produced (CPU uint8 tensor).
 void chunk_attention_out(const at::Tensor& q, at::Tensor& out, at::Tensor& lse, const c10::optional<at::Tensor>& workspace,
                          const at::Tensor& info, const at::Tensor& plan, CACHE_ARGS, const c10::optional<at::Tensor>& sinks,
-                         double sm_scale, bool lse_base2) {
+                         double sm_scale, bool lse_base2, int64_t home) {
   TORCH_CHECK(info.device().is_cpu() && info.scalar_type() == at::kByte && info.is_contiguous() &&
                   (size_t)info.numel() == sizeof(d2sd_chunk_plan_info),
               "d2sd: info must hold the bytes of a d2sd_chunk_plan_info");
@@ -480,16 +504,17 @@ void chunk_attention_out(const at::Tensor& q, at::Tensor& out, at::Tensor& lse, 
   a.sm_scale = (float)sm_scale;
   a.lse_base2 = lse_base2;
   check(d2sd_chunk_run(&pi, &a, current_stream()), "d2sd.chunk_attention");
+  in_use(home, {&plan, &kv_len, &page_table, or_null(sinks), &k_pool, &v_pool, or_null(k_scale), or_null(v_scale)});
 }
 
 std::tuple<at::Tensor, at::Tensor> chunk_attention(const at::Tensor& q, const c10::optional<at::Tensor>& workspace,
                                                    const at::Tensor& info, const at::Tensor& plan, CACHE_ARGS,
                                                    const c10::optional<at::Tensor>& sinks, double sm_scale,
-                                                   bool lse_base2) {
+                                                   bool lse_base2, int64_t home) {
   TORCH_CHECK_VALUE(q.dim() == 3, "d2sd: q must be [tokens, Hq, D]");
   at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   at::Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
-  chunk_attention_out(q, out, lse, workspace, info, plan, CACHE_PASS, sinks, sm_scale, lse_base2);
+  chunk_attention_out(q, out, lse, workspace, info, plan, CACHE_PASS, sinks, sm_scale, lse_base2, home);
   d2sd_chunk_plan_info pi;
   std::memcpy(&pi, info.data_ptr(), sizeof(pi));
   if (q.size(0) > pi.total_q) {  // rows behind the last request: empty ones
@@ -500,10 +525,11 @@ std::tuple<at::Tensor, at::Tensor> chunk_attention(const at::Tensor& q, const c1
 }
 
 void chunk_attention_out_meta(const at::Tensor&, at::Tensor&, at::Tensor&, const c10::optional<at::Tensor>&, const at::Tensor&,
-                              const at::Tensor&, CACHE_ARGS, const c10::optional<at::Tensor>&, double, bool) {}
+                              const at::Tensor&, CACHE_ARGS, const c10::optional<at::Tensor>&, double, bool, int64_t) {}
 std::tuple<at::Tensor, at::Tensor> chunk_attention_meta(const at::Tensor& q, const c10::optional<at::Tensor>&,
                                                         const at::Tensor&, const at::Tensor&, CACHE_ARGS,
-                                                        const c10::optional<at::Tensor>&, double, bool) {
+                                                        const c10::optional<at::Tensor>&, double, bool,
+                                                        int64_t) {
   return {at::empty(q.sizes(), q.options()), at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat))};
 }
 
@@ -528,11 +554,12 @@ TORCH_LIBRARY(d2sd, m) {
   const std::string read = "Tensor kv_len, Tensor page_table, Tensor k_pool, Tensor v_pool, Tensor? k_scale, Tensor? v_scale, "
                            "int format, bool nhd";
   m.def("cache_write(Tensor k, Tensor v, Tensor items, int num_items, Tensor kv_len, Tensor page_table, "
-        "Tensor(a!) k_pool, Tensor(b!) v_pool, Tensor(c!)? k_scale, Tensor(d!)? v_scale, int format, bool nhd) -> ()");
-  m.def(("cache_read_out(Tensor(a!) k, Tensor(b!) v, int rows, Tensor items, int num_items, " + read + ") -> ()").c_str());
-  m.def(("cache_read(int rows, Tensor items, int num_items, " + read + ") -> (Tensor, Tensor)").c_str());
+        "Tensor(a!) k_pool, Tensor(b!) v_pool, Tensor(c!)? k_scale, Tensor(d!)? v_scale, int format, bool nhd, "
+        "int home=-1) -> ()");
+  m.def(("cache_read_out(Tensor(a!) k, Tensor(b!) v, int rows, Tensor items, int num_items, " + read + ", int home=-1) -> ()").c_str());
+  m.def(("cache_read(int rows, Tensor items, int num_items, " + read + ", int home=-1) -> (Tensor, Tensor)").c_str());
   const std::string attn = "Tensor? workspace, Tensor info, Tensor plan, " + read +
-                           ", Tensor? sinks, float sm_scale, bool lse_base2";
+                           ", Tensor? sinks, float sm_scale, bool lse_base2, int home=-1";
   m.def(("chunk_attention_out(Tensor q, Tensor(a!) out, Tensor(b!) lse, " + attn + ") -> ()").c_str());
   m.def(("chunk_attention(Tensor q, " + attn + ") -> (Tensor, Tensor)").c_str());
 }

@@ -25,7 +25,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .graph import _CAPTURING, keep_alive
+from .graph import _CAPTURING, home_stream, keep_alive
 from .paged import KV_FORMATS, PagedBatch, PagedKVCache, _device
 
 _attention, _attention_out = (torch.ops.d2sd.chunk_attention.default, torch.ops.d2sd.chunk_attention_out.default)
@@ -79,6 +79,7 @@ class PagedChunkAttention:
         self.info, self.batch, self.sinks = info, batch, sinks
         self.plan_host = host[:info.plan_ints]
         self.plan_dev = torch.from_numpy(self.plan_host).to(batch.device)
+        self._home = home_stream(batch.device)
         self.kv_format, self.sm_scale, self.lse_base2 = kv_format, scale, bool(lse_base2)
         self.num_qo_heads, self.num_kv_heads, self.head_dim = num_qo_heads, num_kv_heads, head_dim
         self._info = torch.frombuffer(bytearray(bytes(info)), dtype=torch.uint8)
@@ -105,7 +106,7 @@ class PagedChunkAttention:
         if cache.kv_format != self.kv_format:
             raise ValueError(f"the plan is for a {self.kv_format} cache, not {cache.kv_format}")
         rest = (self._info, self.plan_dev, batch.kv_len, batch.page_table, *cache._pools, self.sinks, self.sm_scale,
-                self.lse_base2)
+                self.lse_base2, self._home if self._home == batch._home == cache._home else -1)
         if workspace is None and self.info.workspace_bytes and _CAPTURING:
             workspace = self.workspace()  # the graph holds it
         if out is None and lse is None:

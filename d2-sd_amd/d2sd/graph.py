@@ -24,6 +24,12 @@ def capturing() -> bool:
     return bool(_CAPTURING) or torch.cuda.is_current_stream_capturing()
 
 
+def home_stream(device: torch.device) -> int:
+    """Handle of the device's current stream, which tensors made now belong to: calls on other streams have the
+    allocator keep their memory until they have run."""
+    return torch.cuda.current_stream(device).cuda_stream if device.type == "cuda" else 0
+
+
 def keep_alive(*objs) -> None:
     """Called by d2sd ops with the device buffers a launch reads or writes:
     while a HipGraph is capturing, it holds references to them for as long as

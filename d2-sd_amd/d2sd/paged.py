@@ -31,7 +31,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .graph import capturing, keep_alive
+from .graph import capturing, home_stream, keep_alive
 
 _write, _read, _read_out = (getattr(torch.ops.d2sd, n).default for n in ("cache_write", "cache_read", "cache_read_out"))
 KV_FORMATS = {"bf16": _lib.D2SD_CACHE_BF16, "fp8": _lib.D2SD_CACHE_FP8, "mxfp8": _lib.D2SD_CACHE_MXFP8,
@@ -105,6 +105,7 @@ class PagedBatch:
         if n < pi[-1]:
             raise ValueError("page_table shorter than page_indptr[-1]")
         self.device = _device(device)
+        self._home = home_stream(self.device)  # of the batch's tensors (-1: of several)
         self.page_size, self.num_reqs, self.total_q = P, R, int(qo[-1])
         self.qo_indptr_host, self.page_indptr_host = qo, pi
         self._reads = {}
@@ -158,6 +159,8 @@ class PagedBatch:
                 spans = _spans(np.zeros_like(self.kv_len_host), self.kv_len_host, self.kv_indptr_host[:-1], req, False,
                                self.page_indptr_host)
             self._reads[new_only] = torch.from_numpy(spans).to(self.device)
+            if home_stream(self.device) != self._home:
+                self._home = -1
         return self
 
 
@@ -207,6 +210,7 @@ class PagedKVCache:
         self._pools = (k_pool, v_pool, k_scale, v_scale, KV_FORMATS[kv_format], kv_layout == "NHD")
         self.k_pool, self.v_pool, self.k_scale, self.v_scale = k_pool, v_pool, k_scale, v_scale
         self.kv_format, self.kv_layout, self.device = kv_format, kv_layout, k_pool.device
+        self._home = home_stream(self.device)
         self.num_pages, self.page_size, self.num_kv_heads, self.head_dim = k_pool.shape[0], P, hkv, d
 
     @classmethod
@@ -240,7 +244,8 @@ class PagedKVCache:
         outside the pool are skipped.  Two tokens of one call must not share a
         slot."""
         self._check_batch(batch)
-        _write(k, v, batch._tokens, batch.total_q, batch.kv_len, batch.page_table, *self._pools)
+        home = self._home if self._home == batch._home else -1
+        _write(k, v, batch._tokens, batch.total_q, batch.kv_len, batch.page_table, *self._pools, home)
         keep_alive(k, v, batch._tokens, batch.kv_len, batch.page_table, *self._pools[:4])
 
     def read(self, batch: PagedBatch, new_only: bool = False,
@@ -256,10 +261,11 @@ class PagedKVCache:
         if new_only not in batch._reads:
             batch.prepare_read(new_only)
         items = batch._reads[new_only]
+        home = self._home if self._home == batch._home else -1
         if out is None:
-            out = _read(rows, items, items.shape[0], batch.kv_len, batch.page_table, *self._pools)
+            out = _read(rows, items, items.shape[0], batch.kv_len, batch.page_table, *self._pools, home)
         else:
             k, v = out
-            _read_out(k, v, rows, items, items.shape[0], batch.kv_len, batch.page_table, *self._pools)
+            _read_out(k, v, rows, items, items.shape[0], batch.kv_len, batch.page_table, *self._pools, home)
         keep_alive(*out, items, batch.kv_len, batch.page_table, *self._pools[:4])
         return out
