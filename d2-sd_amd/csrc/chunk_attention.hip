@@ -237,8 +237,9 @@ struct RowOut {
   }
 };
 
+// (A row without a key has output 0 whatever its sink: -inf less -inf is no number.)
 __device__ __forceinline__ float sink_factor(const ChunkParams& p, int head, float lse2) {
-  if (!p.sinks) return 1.f;
+  if (!p.sinks || lse2 == -INFINITY) return 1.f;
   return 1.f / (1.f + __builtin_amdgcn_exp2f((p.sinks[head] - lse2 * kLn2) * kLog2e));
 }
 

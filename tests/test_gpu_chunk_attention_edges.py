@@ -1,5 +1,7 @@
 """PagedChunkAttention at the edges of what it accepts, against the 64-bit form
 with the tolerances that test_gpu_chunk_attention.py derives."""
+import math
+
 import pytest
 import torch
 
@@ -23,3 +25,23 @@ def test_the_widest_windows_over_caches_cut_back(window, fmt, d):
         torch.cuda.synchronize()
         wide.check(*got[0], kv=lens)
         assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+@pytest.mark.parametrize("num_cus", [1, 256, 4096])
+@pytest.mark.parametrize("fmt,d", [("bf16", 128), ("mxfp8", 64)])
+def test_a_sink_of_minus_infinity_is_no_sink(fmt, d, num_cus):
+    """Heads without a sink beside heads with one, plans with and without split keys: rows without a key get output 0
+    and lse -inf from them too, the others the output of a plan without sinks."""
+    qo, kv = [40, 3, 1, 6], [900, 2500, 2100, 2200]
+    p, plain = (Problem(qo, kv, 8, 2, d, fmt, sinks=s, num_cus=num_cus) for s in (True, False))
+    p.attn.sinks[::3] = -math.inf
+    p.sinks[::3] = -1e30  # in the 64-bit form: the same, but for rows without a key, where -inf - -inf is no number
+    assert (num_cus == 1) == (p.attn.info.num_merges == 0)
+    for lens in (kv, [25, 1, 0, 3]):
+        got = []
+        for x in (p, plain):
+            x.batch.set_kv_len(lens)
+            got.append(x.run())
+        torch.cuda.synchronize()
+        p.check(*got[0], kv=lens)
+        assert torch.equal(got[0][0][:, ::3], got[1][0][:, ::3]) and torch.equal(got[0][1], got[1][1])
