@@ -1372,8 +1372,9 @@ int d2sd_chunk_run(const d2sd_chunk_plan_info* info, const d2sd_chunk_run_args* 
   if (!aligned16(a->q) || !aligned16(a->out) || !stride_ok(a->q_stride_n) || !stride_ok(a->q_stride_h) ||
       !stride_ok(a->o_stride_n) || !stride_ok(a->o_stride_h))
     return fail(D2SD_ERR_INVALID_ARG, "chunk_run: q and out need 16-byte rows");
-  if (!(a->sm_scale > 0.f) || !std::isfinite(a->sm_scale))
-    return fail(D2SD_ERR_INVALID_ARG, "chunk_run: sm_scale must be positive and finite");
+  // (the softmax's slack, 8 / (sm_scale log2 e) in score units, has to be a number)
+  if (!(a->sm_scale >= 2e-38f) || !std::isfinite(a->sm_scale))
+    return fail(D2SD_ERR_INVALID_ARG, "chunk_run: sm_scale must be at least 2e-38 and finite");
   if (info->workspace_bytes > 0 && (!a->workspace || !aligned16(a->workspace)))
     return fail(D2SD_ERR_INVALID_ARG, "chunk_run: a 16-byte aligned workspace is required");
   if (a->workspace_bytes < info->workspace_bytes)

@@ -46,7 +46,7 @@ class PagedChunkAttention:
         Query i of request r sits at position kv_len[r] - n_r + i and sees the
         cached keys up to it; window_left >= 0 keeps the window_left keys
         before it and its own.  sm_scale defaults to head_dim ** -0.5 and must
-        be positive.  sinks [Hq] fp32 applies O *= sigmoid(lse - sink).  Rows
+        be at least 2e-38 (over fp8 caches, times each k_scale too).  sinks [Hq] fp32 applies O *= sigmoid(lse - sink).  Rows
         that see no key (a request whose kv_len is below its new tokens) get
         output 0 and lse -inf."""
         if kv_format not in KV_FORMATS:
@@ -58,8 +58,8 @@ class PagedChunkAttention:
                     or sinks.device != batch.device:
                 raise ValueError("sinks must be a contiguous float32 [num_qo_heads] tensor on the batch's device")
         scale = head_dim ** -0.5 if sm_scale is None else float(sm_scale)
-        if not (scale > 0.0 and scale < float("inf")):
-            raise ValueError("sm_scale must be positive and finite")
+        if not (scale >= 2e-38 and scale <= torch.finfo(torch.float32).max):
+            raise ValueError("sm_scale must be at least 2e-38 and finite")
         as_p = lambda x: x.ctypes.data_as(C.POINTER(C.c_int32))  # noqa: E731
         desc = _lib.ChunkPlanDesc()
         desc.num_reqs = batch.num_reqs

@@ -681,7 +681,7 @@ typedef struct {
   float* lse;                /* [total_q, Hq] */
   int64_t lse_stride_n;
   const float* sinks;        /* nullable, [Hq] */
-  float sm_scale;            /* > 0 */
+  float sm_scale;            /* >= 2e-38 (fp8 caches: times each k_scale too) */
   int lse_base2;
   void* workspace;           /* >= info.workspace_bytes, 16-byte aligned */
   size_t workspace_bytes;

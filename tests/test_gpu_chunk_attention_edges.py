@@ -45,3 +45,15 @@ def test_a_sink_of_minus_infinity_is_no_sink(fmt, d, num_cus):
         torch.cuda.synchronize()
         p.check(*got[0], kv=lens)
         assert torch.equal(got[0][0][:, ::3], got[1][0][:, ::3]) and torch.equal(got[0][1], got[1][1])
+
+
+@pytest.mark.parametrize("num_cus", [1, 4096])
+@pytest.mark.parametrize("sm_scale", [2.1e-38, 1e-36, 1e-30])
+@pytest.mark.parametrize("fmt,d", [("bf16", 128), ("mxfp4", 64)])
+def test_scales_near_the_smallest_float(fmt, d, sm_scale, num_cus):
+    """Every visible key weighs the same; the rescaling's slack, about 8 / sm_scale, is near the largest float."""
+    p = Problem([40, 3, 1], [900, 1500, 2100], 8, 2, d, fmt, sm_scale=sm_scale, num_cus=num_cus)
+    assert (num_cus == 1) == (p.attn.info.num_merges == 0)
+    out, lse = p.run()
+    torch.cuda.synchronize()
+    p.check(out, lse)

@@ -1,8 +1,11 @@
 """Host side of the paged-cache operators at the limits of their arguments.  CPU."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import d2sd
+from d2sd import _lib
 
 
 def _plan(qo, kv, pages, P=16, **kw):
@@ -45,3 +48,21 @@ def test_set_kv_len_moves_the_host_lengths():
     b.set_kv_len([2 ** 25] * 64)
     with pytest.raises(ValueError, match="2\\^31"):
         b.prepare_read()
+
+
+@pytest.mark.parametrize("sm_scale", [1.9e-38, 1e-44, 1e-60, 3.5e38, float("inf")])
+def test_scales_that_32_bits_do_not_hold_are_refused(sm_scale):
+    """Below 2e-38 the rescaling's slack is infinite: rows whose keys were split got output 0 and lse -inf."""
+    with pytest.raises(ValueError, match="sm_scale"):
+        _plan([1], [3], [1], sm_scale=sm_scale)
+    info, a = _plan([1], [3], [1]).info, _lib.ChunkRunArgs()
+    a.cache.format, a.cache.num_pages, a.cache.page_size, a.cache.num_kv_heads, a.cache.head_dim = 0, 4, 16, 2, 128
+    a.cache.stride_page, a.cache.stride_head, a.cache.stride_tok = 4096, 2048, 128
+    a.cache.k = a.cache.v = a.plan = a.kv_len = a.page_table = a.q = a.out = a.lse = 4096  # (refused before any is used)
+    a.sm_scale = sm_scale
+    assert _lib.lib.d2sd_chunk_run(C.byref(info), C.byref(a), None) != 0
+    assert b"sm_scale" in _lib.lib.d2sd_last_error()
+
+
+def test_the_smallest_scale_is_planned():
+    assert _plan([1], [3], [1], sm_scale=2e-38).sm_scale == 2e-38
