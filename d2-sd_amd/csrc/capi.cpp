@@ -1291,6 +1291,7 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t ho
     if (lg < 0) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: page_size must be a power of two");
     if (d->window_left < -1) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: window_left must be >= -1");
     if (d->max_splits < 0 || d->num_cus < 0) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: negative count");
+    if (d->num_cus > 1 << 20) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: num_cus above 2^20");
     const int group = d->num_qo_heads / d->num_kv_heads;
     if (d->num_reqs > 0 && (d->qo_indptr[0] != 0 || d->page_indptr[0] < 0))
       return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: qo_indptr starts at 0, page_indptr at 0 or above");

@@ -645,7 +645,7 @@ typedef struct {
   int format;                 /* D2SD_CACHE_* */
   int page_size;
   int window_left;            /* -1: all keys up to the position */
-  int num_cus;                /* 0: query the device */
+  int num_cus;                /* 0: query the device; at most 2^20 */
   int max_splits;             /* 0: default cap */
 } d2sd_chunk_plan_desc;
 

@@ -66,3 +66,11 @@ def test_scales_that_32_bits_do_not_hold_are_refused(sm_scale):
 
 def test_the_smallest_scale_is_planned():
     assert _plan([1], [3], [1], sm_scale=2e-38).sm_scale == 2e-38
+
+
+def test_more_cus_than_the_planner_counts_are_refused():
+    """Twice 2^30 workgroups wrapped to a negative number of places, which the schedule never filled."""
+    for n in (2 ** 20 + 1, 2 ** 30, 2 ** 31 - 1):
+        with pytest.raises(RuntimeError, match="num_cus"):
+            _plan([1, 1], [1000, 2000], [63, 125], num_cus=n)
+    assert _plan([1, 1], [1000, 2000], [63, 125], num_cus=2 ** 20).info.num_items > 0
