@@ -119,5 +119,6 @@ class PagedChunkAttention:
                 lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
                 lse[batch.total_q:].fill_(-float("inf"))
             _attention_out(q, out, lse, workspace, *rest)
-        keep_alive(self.plan_dev, batch.kv_len, batch.page_table, self.sinks, q, out, lse, workspace, *cache._pools[:4])
+        if _CAPTURING:
+            keep_alive(self.plan_dev, batch.kv_len, batch.page_table, self.sinks, q, out, lse, workspace, *cache._pools[:4])
         return out, lse

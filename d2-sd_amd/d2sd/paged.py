@@ -31,7 +31,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .graph import capturing, home_stream, keep_alive
+from .graph import _CAPTURING, capturing, home_stream, keep_alive
 
 _write, _read, _read_out = (getattr(torch.ops.d2sd, n).default for n in ("cache_write", "cache_read", "cache_read_out"))
 KV_FORMATS = {"bf16": _lib.D2SD_CACHE_BF16, "fp8": _lib.D2SD_CACHE_FP8, "mxfp8": _lib.D2SD_CACHE_MXFP8,
@@ -246,7 +246,8 @@ class PagedKVCache:
         self._check_batch(batch)
         home = self._home if self._home == batch._home else -1
         _write(k, v, batch._tokens, batch.total_q, batch.kv_len, batch.page_table, *self._pools, home)
-        keep_alive(k, v, batch._tokens, batch.kv_len, batch.page_table, *self._pools[:4])
+        if _CAPTURING:
+            keep_alive(k, v, batch._tokens, batch.kv_len, batch.page_table, *self._pools[:4])
 
     def read(self, batch: PagedBatch, new_only: bool = False,
              out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -267,5 +268,6 @@ class PagedKVCache:
         else:
             k, v = out
             _read_out(k, v, rows, items, items.shape[0], batch.kv_len, batch.page_table, *self._pools, home)
-        keep_alive(*out, items, batch.kv_len, batch.page_table, *self._pools[:4])
+        if _CAPTURING:
+            keep_alive(*out, items, batch.kv_len, batch.page_table, *self._pools[:4])
         return out
