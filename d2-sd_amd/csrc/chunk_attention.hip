@@ -41,10 +41,13 @@
 //
 // Keys outside an item's visible range are never read: their addresses are
 // clamped to the range, so what lies behind a cache's end (or before its
-// window) may hold anything.
+// window) may hold anything.  What lies inside and is not finite reaches the rows
+// that see it alone ("values that are not finite" below).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "d2sd_internal.h"
 #include "kernel_common.h"
@@ -184,6 +187,15 @@ struct ValueRead {
   }
 };
 
+// Bits of an operand's words that belong to element e of the lanes that are `on`.
+__device__ __forceinline__ u32x4 one_element(int e, bool on) {
+  const unsigned bits = on ? 0xFFFFu << 16 * (e & 1) : 0u;
+  u32x4 x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = i == e >> 1 ? bits : 0u;
+  return x;
+}
+
 // Byte offset of a cache row / its block scales (head 0) in page `page`: strides
 // below 2^32, one 32 x 32 -> 64-bit multiply each.
 __device__ __forceinline__ unsigned long long row_offset(const ChunkParams& p, unsigned page, unsigned slot) {
@@ -241,6 +253,102 @@ struct RowOut {
 __device__ __forceinline__ float sink_factor(const ChunkParams& p, int head, float lse2) {
   if (!p.sinks || lse2 == -INFINITY) return 1.f;
   return 1.f / (1.f + __builtin_amdgcn_exp2f((p.sinks[head] - lse2 * kLn2) * kLog2e));
+}
+
+// ---- values that are not finite ----
+// A hidden key has probability 0, but 0 times an infinite or NaN value is NaN: the
+// second product would carry it into the rows of its tile that do not see the key.
+// Where a row does not see all of a wave's keys and a sum came out not finite, the
+// wave takes its keys again, and those that some row does not see one at a time, each
+// for the rows that see it.  The check, one instruction an output once an item, is all
+// that other items pay (24 requests with a chunk of 1000 in mxfp4 55.2 -> 55.7 us, 4 x
+// 1024 tokens of 64 heads of 64 with a window 27.8 -> 28.3); items that meet one take
+// about three times as long (2 x 2048 at 16384 keys, a NaN in each request's newest
+// token: bf16 1.1 -> 3.3 ms).
+// Tile items: a wave's 32 rows over their part of the item's chunk of keys, straight
+// from the cache, values through 32 rows of its own LDS.  o, m, l: from the start.
+template <int D, int FMT>
+__device__ __forceinline__ void tile_rows_by_key(lds_char* lds, f32x16 (&o)[D / 32], float& m, float& l) {
+  constexpr int MT = D / 32, KS = D / 16;
+  constexpr bool MX = Format<D, FMT>::MX;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
+  // (arguments and item are read again: nothing need be kept for here over the tile loop)
+  auto at = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
+  __asm__ volatile("" : "+s"(at));
+  const ChunkParams& p = *(const ChunkParams*)at;
+  const ChunkItem w = p.items[blockIdx.x];
+  const Span all = item_span(p, w, w.row0 / p.group, (w.row0 + w.nrows - 1) / p.group);
+  const Span own = item_span(p, w, (w.row0 + 32 * wv) / p.group, (w.row0 + min(32 * wv + 31, w.nrows - 1)) / p.group);
+  if (own.lo == own.all_lo && own.hi == own.all_hi) return;
+  const int ntiles = max(all.hi - all.lo + 63, 0) >> 6;
+  const int from = max(all.lo + 64 * (int)((long long)ntiles * w.chunk / w.nchunks), own.lo);
+  const int to = min(all.lo + 64 * (int)((long long)ntiles * (w.chunk + 1) / w.nchunks), own.hi);
+  lds_char* vt = lds + wv * 32 * D * 2;
+  const int row = min(32 * wv + l32, w.nrows - 1), pos = all.pos0 + (w.row0 + row) / p.group, hi = min(pos, to - 1);
+  const RowOut qat(p, w, row);
+  const bf16_t* qp = (const bf16_t*)p.q + (long long)qat.token * p.q_stride_n + (long long)qat.head * p.q_stride_h + 8 * hh;
+  const int row_lo = p.window_left >= 0 ? max(pos - p.window_left, 0) : 0;
+  float c = p.sm_scale * kLog2e;
+  if constexpr (FMT == CACHE_FP8) c *= ((const float*)p.ks.scale)[w.kvh];
+  const float slack = c > 0.f ? kRescaleSlack / c : 0.f;
+  const unsigned last_page = (unsigned)p.num_pages - 1u;
+  const int pmask = (1 << p.log2_page) - 1;
+  // 8 elements of a key's row from `d` on
+  auto piece = [&](const CacheSide& s, int key, int d) -> bf16x8 {
+    const unsigned page = min((unsigned)p.page_table[w.page_begin + (key >> p.log2_page)], last_page), slot = key & pmask;
+    const char* row = (const char*)s.codes + w.kvh * p.stride_head + row_offset(p, page, slot);
+    if constexpr (FMT == CACHE_BF16) return *(const bf16x8*)(row + 2 * d);
+    float f = 1.f;
+    if constexpr (MX) f = block_scale(((const uint8_t*)s.scale + w.kvh * p.scale_stride_head)[scale_offset(p, page, slot) + d / 32]);
+    if constexpr (FMT == CACHE_MXFP4) return expand<FMT>(*(const unsigned*)(row + d / 2), 0u, f);
+    const u32x2 x = *(const u32x2*)(row + (FMT == CACHE_MXFP4 ? 0 : d));
+    return expand<FMT>(x[0], x[1], f);
+  };
+  const ValueRead<D> vread(lane);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) o[mt] = f32x16{};
+  m = -INFINITY, l = 0.f;
+  for (int kb = from; kb < to; kb += 32) {
+    f32x16 s[1];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(piece(p.ks, min(kb + l32, to - 1), 16 * ks + 8 * hh), *(const bf16x8*)(qp + 16 * ks),
+                                                     ks ? s[0] : f32x16{}, 0, 0, 0);
+    hide(s[0], kb, row_lo, hi, hh);
+    softmax_step<1, MT>(s, o, m, l, c, slack, hh);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+    for (int i = lane; i < 32 * (D / 8); i += 64)
+      *(__attribute__((address_space(3))) bf16x8*)lds_piece<D>(vt, i / (D / 8), i % (D / 8)) =
+          piece(p.vs, min(kb + i / (D / 8), to - 1), 8 * (i % (D / 8)));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (kb >= own.all_lo && kb + 32 <= min(own.all_hi, to)) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vread(vt, mt, j), p_operand(s[0], j), o[mt], 0, 0, 0);
+      continue;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const u32x4 pb = __builtin_bit_cast(u32x4, p_operand(s[0], j));
+#pragma unroll 1
+      for (int k = 0; k < 16; ++k) {
+        const u32x4 keep = one_element(4 * (k >> 3) + (k & 3), hh == (k >> 2 & 1));
+        const int key = kb + 16 * j + k;
+        const bool sees = key >= row_lo && key <= hi;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const f32x16 x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, vread(vt, mt, j)) & keep),
+              __builtin_bit_cast(bf16x8, pb & keep), f32x16{}, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[mt][i] = sees ? o[mt][i] + x[i] : o[mt][i];
+        }
+      }
+    }
+  }
 }
 
 // ---- tile items ----
@@ -478,6 +586,13 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
   }
 
   if (!wave_on) return;
+  float zero = 0.f;  // (NaN once a sum is not finite)
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) zero = fmaf(o[mt][i], 0.f, zero);
+  // (no wave reads the tiles any more: the last step's barrier)
+  if (__any(zero != 0.f)) tile_rows_by_key<D, FMT>(lds, o, m, l);
   l += xor32(l, hh);
   const float lse2 = l > 0.f ? m * c + __builtin_amdgcn_logf(l) : l == 0.f ? -INFINITY : l;
   float inv = l != 0.f ? vscale / l : 0.f;
@@ -655,12 +770,16 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
     return f(x, __shfl_xor(x, 32));
   };
 
-  auto step = [&](Raw& x, int t) {
+  auto step = [&](Raw& x, int t, auto by_key) {
+    constexpr bool BY_KEY = decltype(by_key)::value;
     const int tn = t + PF * W;  // the tile that takes these registers next
     // (page ids are loaded a round before the rows they lead to: the wait for
     // one is a wait for every load before it)
-    const unsigned pg = min(x.next, last_page);
-    x.next = page_at(key_at(tn + PF * W, lane & 31));
+    unsigned pg = 0;
+    if constexpr (!BY_KEY) {
+      pg = min(x.next, last_page);
+      x.next = page_at(key_at(tn + PF * W, lane & 31));
+    }
     f32x4 s[RB][2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -698,7 +817,7 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
               expand<FMT>(c[CW * e], c[CW * e + CW - 1], f);
       }
     }
-    if (tn < te) {
+    if (!BY_KEY && tn < te) {
       fetch(x, tn, pg);
     }
     const int kb = 32 * t;
@@ -738,12 +857,32 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
     }
     // (LDS serves a wave's accesses in order; the fences keep the compiler's order)
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (BY_KEY && edge) {
+#pragma unroll 1
+      for (int k = 0; k < 32; ++k) {
+        const u32x4 keep = one_element(4 * (k >> 4) + (k & 3), g4 == (k >> 2 & 3));
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const bf16x8 a = vread(mt);
+        for (int mt = 0; mt < MT; ++mt) {
+          const u32x4 a = __builtin_bit_cast(u32x4, vread(mt)) & keep;
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-        o[rb][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[rb], o[rb][mt], 0, 0, 0);
+          for (int rb = 0; rb < RB; ++rb) {
+            const f32x4 y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, pb[rb]) & keep), f32x4{}, 0,
+                0, 0);
+            const bool sees = kb + k >= row_lo[rb] && kb + k <= pos[rb];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[rb][mt][i] = sees ? o[rb][mt][i] + y[i] : o[rb][mt][i];
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const bf16x8 a = vread(mt);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          o[rb][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb[rb], o[rb][mt], 0, 0, 0);
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
@@ -769,7 +908,30 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
   for (int t = t0; t < te; t += PF * W) {
 #pragma unroll
     for (int i = 0; i < PF; ++i)
-      if (t + i * W < te) step(raw[i], t + i * W);
+      if (t + i * W < te) step(raw[i], t + i * W, std::false_type{});
+  }
+  if (all.lo < all.all_lo || all.hi > all.all_hi) {
+    float zero = 0.f;  // (NaN once a sum is not finite)
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) zero = fmaf(o[rb][mt][i], 0.f, zero);
+    if (__any(zero != 0.f)) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) o[rb][mt] = f32x4{};
+        m[rb] = -INFINITY, l[rb] = 0.f;
+      }
+#pragma unroll 1
+      for (int t = t0; t < te; t += W) {
+        const unsigned pg = min(page_at(key_at(t, lane & 31)), last_page);
+        fetch(raw[0], t, pg);
+        step(raw[0], t, std::true_type{});
+      }
+    }
   }
 
   // join the waves' states through LDS

@@ -48,7 +48,8 @@ class PagedChunkAttention:
         before it and its own.  sm_scale defaults to head_dim ** -0.5 and must
         be at least 2e-38 (over fp8 caches, times each k_scale too).  sinks [Hq] fp32 applies O *= sigmoid(lse - sink).  Rows
         that see no key (a request whose kv_len is below its new tokens) get
-        output 0 and lse -inf."""
+        output 0 and lse -inf.  A NaN or infinity in K or V reaches the rows
+        that see its token and no others."""
         if kv_format not in KV_FORMATS:
             raise ValueError(f"kv_format must be one of {sorted(KV_FORMATS)}")
         if self._want_device is not None and _device(self._want_device) != batch.device:

@@ -632,8 +632,8 @@ int d2sd_cache_read(const d2sd_cache_io_args* args, d2sd_stream_t stream);
  * the caller uploads; run() is one launch, and a second that joins partial
  * states where keys were split (info.num_merges > 0).  run() allocates nothing
  * and does not synchronise; calls that may overlap need workspaces of their
- * own.  K and V of the tokens a request sees must be finite (a NaN or infinity
- * reaches every row whose 64-key tile holds it); anything may lie elsewhere. */
+ * own.  A NaN or infinity in K or V reaches the rows that see its token, no
+ * others, whatever it lies beside; anything may lie behind the lengths. */
 typedef struct {
   int num_reqs;
   const int32_t* qo_indptr;   /* host [num_reqs + 1], from 0 */
