@@ -52,7 +52,8 @@ struct Planner {
   double token_share = 1.0;  // of that, a token item's longest
 
   Planner(const ChunkPlanInput& input, int f) : in(input), form(f) {
-    // (register bound: chunk_attn_kernel)
+    // (by registers: chunk_attn_kernel; the token kernels of heads of 64 would fit four
+    // but for mxfp8, the schedule counts three)
     per_cu = form == CHUNK_WAVES8 ? 1 : in.head_dim == 64 ? 3 : form == CHUNK_TOKENS && in.format == CACHE_MXFP4 ? 3 : 2;
     places = in.num_cus * per_cu;
     place_bytes = kCuBytes / per_cu;
@@ -199,11 +200,12 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   for (int r = 0; r < in.num_reqs; ++r)
     if ((long long)(in.qo_indptr[r + 1] - in.qo_indptr[r]) * group > 16) tokens_only = false;
   // Heads of 128: workgroups of 8 waves share a tile's staging among more rows
-  // (2 x 2048 tokens at 16384 bf16 keys: 1060 us against 1155), those of 4 fill
-  // the device with fewer rows (1000 tokens at 2100: 49 us against 57 split in two
-  // and 65 unsplit).  Heads of 64: 4 waves, three workgroups on a CU (4 x 1024
-  // tokens, window 128: 39 us against 44; 8 x 300 at 1000: 66 against 74; 2 x 2048
-  // at 16384: 1340 against 1259 in bf16, 1201 against 1217 in mxfp4).
+  // (2 x 2048 tokens at 16384 bf16 keys: 953 us against 1045), those of 4 fill
+  // the device with fewer rows (1000 tokens at 2100: 47 us against 50 split in two
+  // and 60 unsplit).  Heads of 64: 4 waves, three workgroups on a CU (before tiles
+  // were kept in L2, 4 x 1024 tokens, window 128: 39 us against 44; 8 x 300 at 1000:
+  // 66 against 74; but 2 x 2048 at 16384: 1340 against 1259 in bf16, 1201 against
+  // 1217 in mxfp4; now 28, 55, 1200 and 1145 of 4 waves, 8 were not measured again).
   Planner pl(in, tokens_only ? CHUNK_TOKENS : CHUNK_WAVES4);
   const double us = pl.plan();
   if (!tokens_only && in.head_dim == 128) {

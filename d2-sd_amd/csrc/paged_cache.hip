@@ -15,8 +15,8 @@
 // is exact.  A block that holds an infinity or NaN gets the scale byte 255 and
 // reads back as NaN.
 //
-// Both kernels move data once: bound by HBM (16 requests, 0.26 GB read back:
-// 90 us, 5.0 TB/s, the rate of a large copy) or, for a step's few tokens, by the
+// Both kernels move data once: bound by HBM (16 requests, 72.6k tokens in mxfp8 read
+// back, 0.45 GB moved: 90 us, 5.0 TB/s, the rate of a large copy) or, for a step's few tokens, by the
 // chain token -> cache length -> page id -> store (64 tokens: 3 us).  A thread
 // carries 8 elements: a 16-byte bf16 load or store against 8 bytes (fp8, mxfp8)
 // or 4 (mxfp4) of codes; the four threads of a block of 32 find its amax by DPP.
@@ -32,15 +32,16 @@ namespace d2sd {
 
 namespace {
 
-// tokens of an item that one block reads (16 requests in mxfp8, 43k tokens: 1, 2, 4, 8, 16:
-// 102, 92, 90, 89, 95 us; 16.3k tokens in mxfp4 with their write: 47, 43.5, 43, 43.6, 46.7)
+// tokens of an item that one block reads (16 requests in mxfp8, 72.6k tokens: 1, 2, 4, 8, 16:
+// 127, 93, 91, 89, 95.5 us; 18.2k tokens in mxfp4 with their write, three states in turn:
+// 48.5, 43.7, 43.2, 44.1, 47)
 constexpr int kReadShare = 4;
 constexpr int kWriteTokens = 8;         // of one block, where there are many
 // (8 heads of 128 in mxfp4: 4096 tokens 7.1 and 7.2 us, 8000 tokens 13.3 one by one, 11.3 by eight)
 constexpr int kWriteManyTokens = 6144;
 // Results larger than half of the last-level cache are stored past it: nothing
 // of them would be found there by whoever reads them from their start (16
-// requests of 100..8000 tokens, 0.26 GB: 99 -> 94 us with 16 tokens a block).
+// requests of 100..8000 tokens, 0.30 GB of results: 99 -> 94 us with 16 tokens a block).
 constexpr long long kReadStreamBytes = 128ll << 20;
 
 // 2^(byte - 127); byte 255 stands for NaN, byte 0 for 2^-127
@@ -187,7 +188,7 @@ struct Places {
 // Block b: new tokens TOK b .., all heads, keys then values.  tokens[t] =
 // (request, tokens from it to its request's end, first page table entry, page
 // table end).  A thread takes the same piece of every token: TOK = 8 keeps as
-// many loads in flight and starts fewer blocks (16.3k tokens of 8 heads of 128 in mxfp4: 35 -> 22 us, 84 MB at 3.8 TB/s),
+// many loads in flight and starts fewer blocks (one request of 16.3k tokens, 8 heads of 128 in mxfp4: 35 -> 22 us, 84 MB at 3.8 TB/s),
 // TOK = 1 spreads a step's few tokens.
 template <int FMT, int TOK>
 __global__ __launch_bounds__(256) void cache_write_kernel(const CacheParams p) {
