@@ -128,3 +128,20 @@ def test_rows_without_a_key_beside_values_that_are_not_finite(fmt):
     assert bool((out[empty] == 0).all()) and bool((lse[empty] == -math.inf).all())
     rest = torch.cat([15 + torch.arange(25), 42 + torch.arange(2)])
     assert not torch.isfinite(out[rest]).any() and torch.isfinite(lse[rest]).all()
+
+
+@pytest.mark.parametrize("num_cus", [1, 4096])
+@pytest.mark.parametrize("fmt,d", [("bf16", 128), ("mxfp8", 64)])
+def test_a_query_that_is_no_number_stays_in_its_row(fmt, d, num_cus):
+    """Beside it: rows of the same wave, the same token's other heads, other tokens; output over the queries."""
+    p = Problem([100, 3, 1], [1500, 300, 2000], 8, 2, d, fmt, num_cus=num_cus, window=400)
+    o, most, s, lse_most = _expected(p)
+    bad = torch.zeros(p.q.shape[:2], dtype=torch.bool)
+    for row, head, what in ((0, 0, math.nan), (17, 5, math.inf), (99, 7, math.nan), (101, 2, -math.inf), (103, 6, math.nan)):
+        p.qd[row, head, 3] = what
+        bad[row, head] = True
+    lse = torch.empty(p.q.shape[:2], device=DEV)
+    out, lse = (t.cpu().double() for t in p.attn.run(p.qd, p.cache, out=p.qd, lse=lse))
+    torch.cuda.synchronize()
+    assert not torch.isfinite(out[bad]).any()
+    assert bool(((out - o).abs() <= most)[~bad].all()) and bool(((lse - s).abs() <= lse_most)[~bad].all())

@@ -1,7 +1,5 @@
 """What a batch, a plan and a cache hold for their caller, used on another stream
 than the one that they were made on and let go of while that is under way."""
-import gc
-
 import numpy as np
 import pytest
 import torch
@@ -50,10 +48,9 @@ def test_buffers_outlive_their_last_use_on_another_stream(fmt):
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
-        torch.cuda._sleep(int(4e8))  # some 0.2 s
+        torch.cuda._sleep(int(1e9))  # some 0.5 s
         got = _step(c, b, a, q, x)
     del held, c, b, a
-    gc.collect()
     # as many tensors of each size as the pool may hand out (none is written to)
     taken = [torch.empty(n, dtype=torch.uint8, device=DEV) for n in places.values() for _ in range(8)]
     assert not side.query(), "the side stream ended before its buffers were let go of"
@@ -80,7 +77,7 @@ def test_a_re_planned_attention_and_moved_lengths_let_go_safely():
     torch.cuda.synchronize()
     side, lens = torch.cuda.Stream(), b.kv_len_host.copy()
     with torch.cuda.stream(side):
-        torch.cuda._sleep(int(4e8))
+        torch.cuda._sleep(int(1e9))
         got = _step(c, b, a, q, x)
         done = side.record_event()
     a.plan(b, 8, 2, 64, kv_format="mxfp8", sinks=a.sinks)
@@ -109,7 +106,7 @@ def test_read_lists_made_on_another_stream_than_their_batch():
         b.prepare_read()
     at, n = b._reads[False].data_ptr(), b._reads[False].untyped_storage().nbytes()
     side.synchronize()
-    torch.cuda._sleep(int(4e8))
+    torch.cuda._sleep(int(1e9))
     got = c.read(b)
     done = torch.cuda.current_stream().record_event()
     b._host_lengths(lens)
