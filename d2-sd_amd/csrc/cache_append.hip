@@ -1,0 +1,216 @@
+// gfx950 kernel: the new tokens of a ragged batch from their projection to the
+// attention in one launch.  Query and key heads are normed (with weights given)
+// and rotated at their positions, queries stored, keys and values quantised into
+// their pages.
+//
+//   y = x / sqrt(mean(x^2) + eps) * w
+//   (a, b) -> s (a cos t - b sin t, b cos t + a sin t),  t = position * f
+//
+// with the pairs, angles and codes of rotary.hip and paged_cache.hip.  Everything
+// between the loads and the stores is 32-bit (angles: 64-bit turns); queries and
+// keys are rounded once, keys straight to the cache's elements.  (Calls of
+// rotary_embedding and cache_write round a key to bf16 between them.)
+//
+// A wave owns one token and a run of its heads, queries, keys and values in this
+// order; a lane holds eight neighbouring head dims of a head and reads the eight
+// that they are paired with too (from the vector cache: the same lines), so that
+// a block of 32 dims is four lanes side by side, as the quantiser wants it.  The
+// run's cosines and sines are computed once, lane i those of pair i, and shared
+// through LDS.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "d2sd_internal.h"
+#include "kernel_common.h"
+#include "paged_store.h"
+#include "plan.h"
+
+namespace d2sd {
+
+namespace {
+
+constexpr int kAppendWaves = 4;
+constexpr int kAppendRows = 2;  // heads of a lane
+// Queries of more than this are stored past the caches, as rotary_embedding's.
+constexpr long long kAppendStreamBytes = 32ll << 20;
+
+__device__ __forceinline__ float bf16_at(const uint16_t* p) { return __uint_as_float((unsigned)*p << 16); }
+
+template <int FMT, bool STREAM>
+__global__ __launch_bounds__(64 * kAppendWaves) void cache_append_kernel(const AppendParams p) {
+  __shared__ float2 turns[kAppendWaves][kRotaryMaxPairs];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long unit = (long long)blockIdx.x * kAppendWaves + wv;
+  const int num_tokens = p.c.num_items, hq = p.num_qo_heads, hkv = p.c.num_kv_heads, D = p.c.head_dim;
+  if (unit >= (long long)num_tokens * p.runs) return;  // (no barrier below: waves are on their own)
+  const int t = (int)(unit / p.runs);
+  const int h0 = (int)(unit - (long long)t * p.runs) * p.heads_per_run, h1 = min(h0 + p.heads_per_run, hq + 2 * hkv);
+  const int lph = 1 << p.log2_lanes;  // lanes of a head
+  const int d = 8 * (lane & (lph - 1));
+  const int pairs = p.pairs, turning = 2 * pairs;
+  // eight pairs whose other elements are eight neighbours too
+  const bool wide = !p.interleaved && pairs % 8 == 0;
+  const int mate = d < pairs ? d + pairs : d - pairs;
+
+  // the rows' loads first: they do not wait for the place they go to
+  u32x4 own[kAppendRows], other[kAppendRows];
+  const uint16_t* row[kAppendRows];
+  int head[kAppendRows];  // of q, of k plus hq, of v plus hq + hkv; -1: none
+#pragma unroll
+  for (int u = 0; u < kAppendRows; ++u) {
+    const int h = h0 + (u << (6 - p.log2_lanes)) + (lane >> p.log2_lanes);
+    head[u] = h < h1 && d < D ? h : -1;
+    own[u] = other[u] = u32x4{0u, 0u, 0u, 0u};
+    row[u] = nullptr;
+    if (head[u] < 0) continue;
+    row[u] = h < hq         ? (const uint16_t*)p.q + (long long)t * p.q_stride_n + (long long)h * p.q_stride_h
+             : h < hq + hkv ? (const uint16_t*)p.c.k + (long long)t * p.c.stride_n + (long long)(h - hq) * p.c.stride_h
+                            : (const uint16_t*)p.c.v + (long long)t * p.v_stride_n + (long long)(h - hq - hkv) * p.v_stride_h;
+    own[u] = *(const u32x4*)(row[u] + d);
+    if (wide && d < turning && h < hq + hkv) other[u] = *(const u32x4*)(row[u] + mate);
+  }
+
+  const int4 tok = ((const int4*)p.c.items)[t];
+  const int place = p.c.kv_len[tok.x] - tok.y;  // the token's position in its cache
+  int page = -1;
+  if (h1 > hq) {
+    const int at = tok.z + (place >> p.c.log2_page);
+    // (before the cache's start, or no page is reserved for it: nothing to write)
+    if (place >= 0 && at < tok.w) page = p.c.page_table[at];
+    if (page >= p.c.num_pages) page = -1;
+  }
+  const int slot = place & ((1 << p.c.log2_page) - 1);
+  float2* turn = turns[wv];
+  if (h0 < hq + hkv) {
+    const long long pos = !p.positions ? (long long)place
+                          : p.pos64    ? ((const long long*)p.positions)[t]
+                                       : (long long)((const int*)p.positions)[t];
+    for (int i = lane; i < pairs; i += 64) turn[i] = rotary_turn(pos, p.inv_freq[i], p.scale);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+
+#pragma unroll
+  for (int u = 0; u < kAppendRows; ++u) {
+    const int h = head[u];
+    const bool is_q = h >= 0 && h < hq, is_k = h >= hq && h < hq + hkv;
+    float x[8], y[8];
+    expand8(own[u], x);
+    expand8(other[u], y);
+    float pre = 1.f, inv = 1.f;
+    const uint16_t* weight = (const uint16_t*)(is_q ? p.q_norm : is_k ? p.k_norm : nullptr);
+    if (p.q_norm || p.k_norm) {
+      // (every lane takes part; heads without a norm drop the result)
+      auto squares = [&](float f) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(x[i] * f, x[i] * f, ss);
+        for (int m = lph >> 1; m > 0; m >>= 1) ss += __shfl_xor(ss, m);
+        return ss;
+      };
+      float ss = squares(1.f);
+      if (__any(isinf(ss))) {  // values above 2^59: squares of values 2^64 smaller
+        const float small = squares(0x1p-64f);
+        if (isinf(ss)) pre = 0x1p-64f, ss = small;
+      }
+      if (weight) inv = rsqrtf(ss / (float)D + p.eps * pre * pre);
+      else pre = 1.f;
+    }
+    if (h < 0) continue;
+    if (h >= hq + hkv) {
+      if (page >= 0) {
+        const int hv = h - hq - hkv;
+        store_piece<FMT>(p.c.vs, hv, page * p.c.stride_page + hv * p.c.stride_head + slot * p.c.stride_tok,
+                         page * p.c.scale_stride_page + hv * p.c.scale_stride_head + slot * p.c.scale_stride_tok, d, own[u]);
+      }
+      continue;
+    }
+    if (weight) {
+      float w[8];
+      expand8(*(const u32x4*)(weight + d), w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = x[i] * pre * inv * w[i];
+      if (wide && d < turning) {
+        expand8(*(const u32x4*)(weight + mate), w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * pre * inv * w[i];
+      }
+    }
+    if (d < turning) {
+      if (wide) {
+        const float2* cs = turn + (d < pairs ? d : mate);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 c = cs[i];
+          x[i] = x[i] * c.x + (d < pairs ? -y[i] : y[i]) * c.y;
+        }
+      } else if (p.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (d + 2 * i >= turning) continue;
+          const float2 c = turn[d / 2 + i];
+          const float a = x[2 * i], b = x[2 * i + 1];
+          x[2 * i] = a * c.x - b * c.y;
+          x[2 * i + 1] = b * c.x + a * c.y;
+        }
+      } else {
+        // (pairs that come in no eights: one element at a time)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int e = d + i;
+          if (e >= turning) continue;
+          const int m = e < pairs ? e + pairs : e - pairs;
+          const float2 c = turn[e < pairs ? e : m];
+          float b = bf16_at(row[u] + m);
+          if (weight) b = b * pre * inv * bf16_at(weight + m);
+          x[i] = x[i] * c.x + (e < pairs ? -b : b) * c.y;
+        }
+      }
+    }
+    if (is_q) {
+      u32x4* at = (u32x4*)((uint16_t*)p.q_out + (long long)t * p.qo_stride_n + (long long)h * p.qo_stride_h + d);
+      const u32x4 out = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+      if constexpr (STREAM)
+        __builtin_nontemporal_store(out, at);
+      else
+        *at = out;
+    } else {
+      const int hk = h - hq;
+      store_values<FMT>(p.c.ks, hk, page * p.c.stride_page + hk * p.c.stride_head + slot * p.c.stride_tok,
+                        page * p.c.scale_stride_page + hk * p.c.scale_stride_head + slot * p.c.scale_stride_tok, d, x,
+                        page >= 0);
+    }
+  }
+}
+
+template <int FMT>
+void launch_t(const AppendParams& p, bool stream, unsigned grid, hipStream_t s) {
+  if (stream)
+    hipLaunchKernelGGL((cache_append_kernel<FMT, true>), dim3(grid), dim3(64 * kAppendWaves), 0, s, p);
+  else
+    hipLaunchKernelGGL((cache_append_kernel<FMT, false>), dim3(grid), dim3(64 * kAppendWaves), 0, s, p);
+}
+
+}  // namespace
+
+hipError_t launch_cache_append(AppendParams p, int format, hipStream_t s) {
+  if (p.c.num_items <= 0) return hipSuccess;
+  p.log2_lanes = 2;  // head dims come in thirty-twos
+  while ((8 << p.log2_lanes) < p.c.head_dim) ++p.log2_lanes;
+  p.heads_per_run = kAppendRows * (64 >> p.log2_lanes);
+  p.runs = (p.num_qo_heads + 2 * p.c.num_kv_heads + p.heads_per_run - 1) / p.heads_per_run;
+  const long long grid = ((long long)p.c.num_items * p.runs + kAppendWaves - 1) / kAppendWaves;
+  if (grid > 0x7FFFFFFFll) return hipErrorInvalidValue;
+  const bool stream = 2ll * p.c.num_items * p.num_qo_heads * p.c.head_dim > kAppendStreamBytes;
+  switch (format) {
+    case CACHE_BF16: launch_t<CACHE_BF16>(p, stream, (unsigned)grid, s); break;
+    case CACHE_FP8: launch_t<CACHE_FP8>(p, stream, (unsigned)grid, s); break;
+    case CACHE_MXFP8: launch_t<CACHE_MXFP8>(p, stream, (unsigned)grid, s); break;
+    case CACHE_MXFP4: launch_t<CACHE_MXFP4>(p, stream, (unsigned)grid, s); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace d2sd

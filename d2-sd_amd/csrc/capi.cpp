@@ -1272,6 +1272,58 @@ int d2sd_cache_read(const d2sd_cache_io_args* a, d2sd_stream_t stream) {
   return e == hipSuccess ? D2SD_OK : fail_hip(e, "cache_read launch");
 }
 
+int d2sd_cache_append(const d2sd_cache_append_args* a, d2sd_stream_t stream) {
+  g_last_error.clear();
+  if (!a) return fail(D2SD_ERR_INVALID_ARG, "cache_append: null args");
+  d2sd_cache_io_args io{};
+  io.cache = a->cache;
+  io.items = a->items;
+  io.kv_len = a->kv_len;
+  io.page_table = a->page_table;
+  io.k = const_cast<void*>(a->k);
+  io.v = const_cast<void*>(a->v);
+  io.stride_n = a->k_stride_n;
+  io.stride_h = a->k_stride_h;
+  io.num_items = a->num_tokens;
+  d2sd::AppendParams p{};
+  if (int rc = cache_params(&io, "cache_append", p.c)) return rc;
+  if (a->num_qo_heads < 0) return fail(D2SD_ERR_INVALID_ARG, "cache_append: negative count");
+  if (a->num_pairs < 1 || 2 * (int64_t)a->num_pairs > a->cache.head_dim)
+    return fail(D2SD_ERR_INVALID_ARG, "cache_append: 2 * num_pairs must be in [2, head_dim]");
+  if (!std::isfinite(a->scale)) return fail(D2SD_ERR_INVALID_ARG, "cache_append: scale must be finite");
+  if ((a->q_norm || a->k_norm) && !(a->eps >= 1e-30f && std::isfinite(a->eps)))
+    return fail(D2SD_ERR_INVALID_ARG, "cache_append: eps must be at least 1e-30 and finite");
+  if (a->num_tokens == 0) return D2SD_OK;
+  if (!a->inv_freq || (a->num_qo_heads > 0 && (!a->q || !a->q_out)))
+    return fail(D2SD_ERR_INVALID_ARG, "cache_append: null pointer");
+  if (!aligned16(a->q) || !aligned16(a->q_out) || !aligned16(a->q_norm) || !aligned16(a->k_norm))
+    return fail(D2SD_ERR_INVALID_ARG, "cache_append: q, q_out and the norms' weights must be 16-byte aligned");
+  for (int64_t st : {a->v_stride_n, a->v_stride_h, a->q_stride_n, a->q_stride_h, a->qo_stride_n, a->qo_stride_h})
+    if (!stride_ok(st) || st < 0) return fail(D2SD_ERR_INVALID_ARG, "cache_append: strides must be multiples of 8 elements");
+  if (a->num_qo_heads > 0 && a->q == a->q_out && (a->q_stride_n != a->qo_stride_n || a->q_stride_h != a->qo_stride_h))
+    return fail(D2SD_ERR_INVALID_ARG, "cache_append: in place needs the same strides");
+  p.v_stride_n = a->v_stride_n;
+  p.v_stride_h = a->v_stride_h;
+  p.q = a->q;
+  p.q_out = a->q_out;
+  p.q_stride_n = a->q_stride_n;
+  p.q_stride_h = a->q_stride_h;
+  p.qo_stride_n = a->qo_stride_n;
+  p.qo_stride_h = a->qo_stride_h;
+  p.positions = a->positions;
+  p.inv_freq = a->inv_freq;
+  p.q_norm = a->q_norm;
+  p.k_norm = a->k_norm;
+  p.eps = a->eps;
+  p.scale = a->scale;
+  p.num_qo_heads = a->num_qo_heads;
+  p.pairs = a->num_pairs;
+  p.pos64 = a->positions_64 ? 1 : 0;
+  p.interleaved = a->interleaved ? 1 : 0;
+  hipError_t e = d2sd::launch_cache_append(p, a->cache.format, (hipStream_t)stream);
+  return e == hipSuccess ? D2SD_OK : fail_hip(e, "cache_append launch");
+}
+
 int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t host_plan_ints,
                     d2sd_chunk_plan_info* info) {
   g_last_error.clear();

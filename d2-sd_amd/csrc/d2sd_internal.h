@@ -287,6 +287,24 @@ struct CacheParams {
 };
 
 // ---------------------------------------------------------------------------
+// New tokens normed, rotated and written (cache_append.hip).
+// ---------------------------------------------------------------------------
+struct AppendParams {
+  CacheParams c;             // items: int4 per token; k and v: the new rows, strides of k
+  long long v_stride_n, v_stride_h;  // elements
+  const void* q;             // bf16 [tokens, Hq, D], head_dim contiguous
+  void* q_out;               // may be q
+  long long q_stride_n, q_stride_h, qo_stride_n, qo_stride_h;
+  const void* positions;     // [tokens] int32, or int64 (pos64); null: the cache positions
+  const double* inv_freq;    // [pairs] radians per position
+  const void* q_norm;        // bf16 [D], null: not normed
+  const void* k_norm;
+  float eps, scale;          // of the norm; factor on cos and sin
+  int num_qo_heads, pairs, pos64, interleaved;
+  int runs, heads_per_run, log2_lanes;  // launcher: waves of a token, heads of a wave, lanes of a head
+};
+
+// ---------------------------------------------------------------------------
 // Attention of each request's newest tokens over its paged cache
 // (chunk_attention.hip).
 // ---------------------------------------------------------------------------

@@ -94,6 +94,9 @@ hipError_t launch_rotary(RotaryParams p, bool interleaved, hipStream_t s);
 hipError_t launch_cache_write(const CacheParams& p, int format, hipStream_t s);
 hipError_t launch_cache_read(const CacheParams& p, int format, hipStream_t s);
 
+// ---- new tokens normed, rotated and written (cache_append.hip); format: CACHE_* ----
+hipError_t launch_cache_append(AppendParams p, int format, hipStream_t s);
+
 // ---- attention of new tokens over the paged cache (chunk_attention.hip, chunk_plan.cpp) ----
 struct ChunkPlanInput {
   int num_reqs;

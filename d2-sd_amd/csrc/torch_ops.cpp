@@ -12,9 +12,9 @@
 //   cascade_run / cascade_run_no_alloc
 //                                 one cascade verify call of a d2sd_cascade_plan
 //                                 (generation/verification.py:127-176 over a token tree)
-//   rotary_embedding, cache_write, cache_read(_out), chunk_attention(_out)
+//   rotary_embedding, cache_write, cache_append, cache_read(_out), chunk_attention(_out)
 //                                 the paged-cache operators: d2sd_rotary_embedding,
-//                                 d2sd_cache_write / _read, d2sd_chunk_run
+//                                 d2sd_cache_write / _append / _read, d2sd_chunk_run
 //
 // Each operator checks its tensors, then calls the C entry point on the
 // current HIP stream of the tensors' device; there is no other code path.
@@ -429,6 +429,91 @@ std::tuple<at::Tensor, at::Tensor> cache_read(int64_t rows, const at::Tensor& it
   return {k, v};
 }
 
+// ---- cache_append ----
+void cache_append(const c10::optional<at::Tensor>& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& items,
+                  int64_t num_items, CACHE_ARGS, const at::Tensor& inv_freq, const c10::optional<at::Tensor>& positions,
+                  const c10::optional<at::Tensor>& q_norm, const c10::optional<at::Tensor>& k_norm, double eps, double scale,
+                  bool interleaved, const c10::optional<at::Tensor>& q_out, int64_t home) {
+  d2sd_cache_append_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.cache = cache_of(k_pool, v_pool, k_scale, v_scale, format, nhd);
+  const at::Device dev = k_pool.device();
+  const int64_t d = a.cache.head_dim;
+  for (const at::Tensor* t : {&k, &v}) {
+    need_type(*t, at::kBFloat16, "k / v");
+    TORCH_CHECK_VALUE(t->dim() == 3 && t->size(0) >= num_items && t->size(1) == a.cache.num_kv_heads && t->size(2) == d &&
+                          t->stride(2) == 1,
+                      "d2sd: k and v must be [>= ", num_items, ", ", a.cache.num_kv_heads, ", ", d,
+                      "] with a contiguous head_dim");
+    same_device(*t, dev, "k / v");
+  }
+  TORCH_CHECK_VALUE(q.has_value() == q_out.has_value(), "d2sd: q and its output go together");
+  if (q.has_value()) {
+    for (const at::Tensor* t : {&*q, &*q_out}) {
+      need_type(*t, at::kBFloat16, "q / q_out");
+      TORCH_CHECK_VALUE(t->dim() == 3 && t->size(0) >= num_items && t->size(1) == q->size(1) && t->size(2) == d &&
+                            t->size(0) == q->size(0) && t->stride(2) == 1,
+                        "d2sd: q and q_out must be [>= ", num_items, ", Hq, ", d, "] alike with a contiguous head_dim");
+      same_device(*t, dev, "q / q_out");
+    }
+    TORCH_CHECK_VALUE((q_out->size(0) < 2 || q_out->stride(0) >= d) && (q_out->size(1) < 2 || q_out->stride(1) >= d),
+                      "d2sd: the rows of q_out must lie apart");
+    TORCH_CHECK_VALUE(q->size(1) <= INT32_MAX, "d2sd: too many heads");
+    a.q = q->data_ptr();
+    a.q_out = q_out->data_ptr();
+    a.q_stride_n = q->stride(0), a.q_stride_h = q->stride(1);
+    a.qo_stride_n = q_out->stride(0), a.qo_stride_h = q_out->stride(1);
+    a.num_qo_heads = (int)q->size(1);
+  }
+  for (const at::Tensor* t : {&items, &kv_len, &page_table}) {
+    TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->is_contiguous(), "d2sd: a batch's tensors are contiguous int32");
+    same_device(*t, dev, "the batch");
+  }
+  TORCH_CHECK_VALUE(items.numel() >= num_items * 4, "d2sd: too few items");
+  need_type(inv_freq, at::kDouble, "inv_freq");
+  TORCH_CHECK_VALUE(inv_freq.dim() == 1 && inv_freq.is_contiguous() && inv_freq.size(0) <= d / 2,
+                    "d2sd: inv_freq must be contiguous and 1-D, at most head_dim / 2 entries");
+  same_device(inv_freq, dev, "inv_freq");
+  if (positions.has_value()) {
+    TORCH_CHECK_TYPE(positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong,
+                     "d2sd: positions must be int32 or int64");
+    TORCH_CHECK_VALUE(positions->dim() == 1 && positions->size(0) >= num_items && positions->is_contiguous(),
+                      "d2sd: positions must be a contiguous [>= ", num_items, "] tensor");
+    same_device(*positions, dev, "positions");
+    a.positions = positions->data_ptr();
+    a.positions_64 = positions->scalar_type() == at::kLong;
+  }
+  auto weight = [&](const c10::optional<at::Tensor>& t, const char* name) -> const void* {
+    if (!t.has_value()) return nullptr;
+    need_type(*t, at::kBFloat16, name);
+    TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == d && t->is_contiguous(), "d2sd: ", name, " must be a contiguous [", d,
+                      "] tensor");
+    same_device(*t, dev, name);
+    return t->data_ptr();
+  };
+  a.q_norm = weight(q_norm, "q_norm");
+  a.k_norm = weight(k_norm, "k_norm");
+  a.items = (const d2sd_cache_token*)items.data_ptr();
+  a.kv_len = kv_len.data_ptr<int32_t>();
+  a.page_table = page_table.data_ptr<int32_t>();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.k_stride_n = k.stride(0), a.k_stride_h = k.stride(1);
+  a.v_stride_n = v.stride(0), a.v_stride_h = v.stride(1);
+  a.inv_freq = inv_freq.data_ptr<double>();
+  a.eps = (float)eps;
+  a.scale = (float)scale;
+  a.num_tokens = (int)num_items;
+  a.num_pairs = (int)inv_freq.size(0);
+  a.interleaved = interleaved;
+  const c10::DeviceGuard guard(dev);
+  check(d2sd_cache_append(&a, current_stream()), "d2sd.cache_append");
+  in_use(home, {&items, &kv_len, &page_table, &k_pool, &v_pool, or_null(k_scale), or_null(v_scale)});
+}
+
+void cache_append_meta(const c10::optional<at::Tensor>&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t,
+                       CACHE_ARGS, const at::Tensor&, const c10::optional<at::Tensor>&, const c10::optional<at::Tensor>&,
+                       const c10::optional<at::Tensor>&, double, double, bool, const c10::optional<at::Tensor>&, int64_t) {}
 void cache_write_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, CACHE_ARGS, int64_t) {}
 void cache_read_out_meta(at::Tensor&, at::Tensor&, int64_t, const at::Tensor&, int64_t, CACHE_ARGS, int64_t) {}
 std::tuple<at::Tensor, at::Tensor> cache_read_meta(int64_t rows, const at::Tensor&, int64_t, CACHE_ARGS, int64_t) {
@@ -556,6 +641,10 @@ TORCH_LIBRARY(d2sd, m) {
   m.def("cache_write(Tensor k, Tensor v, Tensor items, int num_items, Tensor kv_len, Tensor page_table, "
         "Tensor(a!) k_pool, Tensor(b!) v_pool, Tensor(c!)? k_scale, Tensor(d!)? v_scale, int format, bool nhd, "
         "int home=-1) -> ()");
+  m.def("cache_append(Tensor? q, Tensor k, Tensor v, Tensor items, int num_items, Tensor kv_len, Tensor page_table, "
+        "Tensor(a!) k_pool, Tensor(b!) v_pool, Tensor(c!)? k_scale, Tensor(d!)? v_scale, int format, bool nhd, "
+        "Tensor inv_freq, Tensor? positions, Tensor? q_norm, Tensor? k_norm, float eps, float scale, bool interleaved, "
+        "Tensor(e!)? q_out, int home=-1) -> ()");
   m.def(("cache_read_out(Tensor(a!) k, Tensor(b!) v, int rows, Tensor items, int num_items, " + read + ", int home=-1) -> ()").c_str());
   m.def(("cache_read(int rows, Tensor items, int num_items, " + read + ", int home=-1) -> (Tensor, Tensor)").c_str());
   const std::string attn = "Tensor? workspace, Tensor info, Tensor plan, " + read +
@@ -572,6 +661,7 @@ TORCH_LIBRARY_IMPL(d2sd, CUDA, m) {
   m.impl("cascade_run_no_alloc", &cascade_run_no_alloc);
   m.impl("rotary_embedding", &rotary_embedding);
   m.impl("cache_write", &cache_write);
+  m.impl("cache_append", &cache_append);
   m.impl("cache_read_out", &cache_read_out);
   m.impl("cache_read", &cache_read);
   m.impl("chunk_attention_out", &chunk_attention_out);
@@ -582,6 +672,7 @@ TORCH_LIBRARY_IMPL(d2sd, CUDA, m) {
 TORCH_LIBRARY_IMPL(d2sd, CPU, m) {
   m.impl("rotary_embedding", &rotary_embedding);
   m.impl("cache_write", &cache_write);
+  m.impl("cache_append", &cache_append);
   m.impl("cache_read_out", &cache_read_out);
   m.impl("chunk_attention_out", &chunk_attention_out);
 }
@@ -594,6 +685,7 @@ TORCH_LIBRARY_IMPL(d2sd, Meta, m) {
   m.impl("cascade_run_no_alloc", &cascade_meta);
   m.impl("rotary_embedding", &rotary_meta);
   m.impl("cache_write", &cache_write_meta);
+  m.impl("cache_append", &cache_append_meta);
   m.impl("cache_read_out", &cache_read_out_meta);
   m.impl("cache_read", &cache_read_meta);
   m.impl("chunk_attention_out", &chunk_attention_out_meta);

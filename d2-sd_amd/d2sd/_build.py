@@ -28,7 +28,7 @@ ARCH = "gfx950"
 # waves per workgroup, and once without for the rest), so that the parts
 # build in parallel.
 SOURCES = ["attention.hip", "verify_attention.hip", "kv_append.hip", "accept.hip", "qk_rope.hip", "tree_build.hip",
-           "rotary.hip", "paged_cache.hip", "chunk_attention.hip", "plan.cpp", "chunk_plan.cpp", "capi.cpp"]
+           "rotary.hip", "paged_cache.hip", "cache_append.hip", "chunk_attention.hip", "plan.cpp", "chunk_plan.cpp", "capi.cpp"]
 PARTS = {"verify_attention.hip": [{"D2SD_VERIFY_D": d, "D2SD_VERIFY_WAVES": w} for d in (128, 64) for w in (4, 2, 8, 1)]
          + [{}]}
 

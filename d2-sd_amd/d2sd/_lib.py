@@ -315,6 +315,38 @@ class CacheIoArgs(C.Structure):
     ]
 
 
+class CacheAppendArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("items", C.c_void_p),
+        ("kv_len", C.c_void_p),
+        ("page_table", C.c_void_p),
+        ("q", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("q_stride_n", C.c_int64),
+        ("q_stride_h", C.c_int64),
+        ("qo_stride_n", C.c_int64),
+        ("qo_stride_h", C.c_int64),
+        ("k_stride_n", C.c_int64),
+        ("k_stride_h", C.c_int64),
+        ("v_stride_n", C.c_int64),
+        ("v_stride_h", C.c_int64),
+        ("positions", C.c_void_p),
+        ("inv_freq", C.c_void_p),
+        ("q_norm", C.c_void_p),
+        ("k_norm", C.c_void_p),
+        ("eps", C.c_float),
+        ("scale", C.c_float),
+        ("num_tokens", C.c_int),
+        ("num_qo_heads", C.c_int),
+        ("num_pairs", C.c_int),
+        ("positions_64", C.c_int),
+        ("interleaved", C.c_int),
+    ]
+
+
 class ChunkPlanDesc(C.Structure):
     _fields_ = [
         ("num_reqs", C.c_int),
@@ -440,6 +472,8 @@ def _load() -> C.CDLL:
         fn = getattr(lib, name)
         fn.restype = i32
         fn.argtypes = [C.POINTER(CacheIoArgs), vp]
+    lib.d2sd_cache_append.restype = i32
+    lib.d2sd_cache_append.argtypes = [C.POINTER(CacheAppendArgs), vp]
     lib.d2sd_chunk_plan.restype = i32
     lib.d2sd_chunk_plan.argtypes = [C.POINTER(ChunkPlanDesc), C.POINTER(C.c_int32), sz, C.POINTER(ChunkPlanInfo)]
     lib.d2sd_chunk_run.restype = i32

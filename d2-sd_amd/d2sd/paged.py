@@ -22,6 +22,9 @@ Writing takes the smallest power of two that keeps the block's largest
 magnitude within the elements' range, from 2^-117 on, and rounds to nearest
 even, so that reading back gives exact bf16 values and a block holding a NaN
 or infinity reads back as NaN.
+
+append() takes queries, keys and values from their projection: norm, rotation
+and write in one launch.
 """
 from __future__ import annotations
 
@@ -33,7 +36,8 @@ import torch
 from . import _lib
 from .graph import _CAPTURING, capturing, home_stream, keep_alive
 
-_write, _read, _read_out = (getattr(torch.ops.d2sd, n).default for n in ("cache_write", "cache_read", "cache_read_out"))
+_write, _append, _read, _read_out = (getattr(torch.ops.d2sd, n).default
+                                     for n in ("cache_write", "cache_append", "cache_read", "cache_read_out"))
 KV_FORMATS = {"bf16": _lib.D2SD_CACHE_BF16, "fp8": _lib.D2SD_CACHE_FP8, "mxfp8": _lib.D2SD_CACHE_MXFP8,
               "mxfp4": _lib.D2SD_CACHE_MXFP4}
 _BLOCK = 32
@@ -248,6 +252,34 @@ class PagedKVCache:
         _write(k, v, batch._tokens, batch.total_q, batch.kv_len, batch.page_table, *self._pools, home)
         if _CAPTURING:
             keep_alive(k, v, batch._tokens, batch.kv_len, batch.page_table, *self._pools[:4])
+
+    def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, batch: PagedBatch,
+               inv_freq: torch.Tensor, positions: Optional[torch.Tensor] = None, *, scale: float = 1.0,
+               interleaved: bool = False, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
+               eps: float = 1e-6, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """The batch's new tokens from their projection to the attention, in one
+        launch: the heads of q [total_q, Hq, D] (None: no queries) and k
+        [total_q, Hkv, D] rotated as rotary_embedding does (inv_freq, scale,
+        interleaved; positions: int32 or int64, one per token, by default each
+        token's place in its cache), k and v written as write() does.  With
+        weights (bf16 [D]) q_norm / k_norm, each head of q / k is first divided
+        by sqrt(mean(x^2) + eps) and multiplied by them.
+
+        Everything is computed in 32 bits and rounded once, keys straight to the
+        cache's elements (rotary_embedding and write() round them to bf16 in
+        between).  The rotated queries go to q_out (as large as q, its rows
+        apart), or back into q; k and v stay as they are.  Returns q_out.  Rows
+        behind the last request's are left alone."""
+        self._check_batch(batch)
+        if q_out is None:
+            q_out = q
+        home = self._home if self._home == batch._home else -1
+        _append(q, k, v, batch._tokens, batch.total_q, batch.kv_len, batch.page_table, *self._pools, inv_freq, positions,
+                q_norm, k_norm, eps, scale, interleaved, q_out, home)
+        if _CAPTURING:
+            keep_alive(q, k, v, batch._tokens, batch.kv_len, batch.page_table, *self._pools[:4], inv_freq, positions,
+                       q_norm, k_norm, q_out)
+        return q_out
 
     def read(self, batch: PagedBatch, new_only: bool = False,
              out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -622,6 +622,40 @@ int d2sd_cache_write(const d2sd_cache_io_args* args, d2sd_stream_t stream);
  * with zero_missing, become zero. */
 int d2sd_cache_read(const d2sd_cache_io_args* args, d2sd_stream_t stream);
 
+/* New tokens from their projection to the attention in one launch: query and
+ * key heads normed (where weights are given) and rotated, queries stored, keys
+ * and values written as d2sd_cache_write does.
+ *   x -> x / sqrt(mean(x^2) + eps) * weight          (over a head's dims)
+ *   pairs, angles and scale as d2sd_rotary_embedding
+ * in 32 bits, rounded once: queries to bf16, keys to the cache's elements.
+ * Without positions a token's position is its place in its cache.  Rows: 16-byte
+ * boundaries.  q_out may be q with the same strides, or lie apart. */
+typedef struct {
+  d2sd_paged_cache cache;
+  const d2sd_cache_token* items; /* device [num_tokens]; token i is row i of q, k and v */
+  const int32_t* kv_len;         /* device [requests] */
+  const int32_t* page_table;     /* device */
+  const void* q;                 /* bf16 [tokens, Hq, D]; may be NULL with num_qo_heads 0 */
+  void* q_out;
+  const void* k;                 /* bf16 [tokens, Hkv, D] */
+  const void* v;
+  int64_t q_stride_n, q_stride_h, qo_stride_n, qo_stride_h; /* elements; head_dim contiguous */
+  int64_t k_stride_n, k_stride_h, v_stride_n, v_stride_h;
+  const void* positions;         /* nullable; device [tokens] int32, or int64 (positions_64) */
+  const double* inv_freq;        /* device [num_pairs], radians per position */
+  const void* q_norm;            /* nullable; bf16 [D] */
+  const void* k_norm;            /* nullable; bf16 [D] */
+  float eps;                     /* with a norm: from 1e-30 on, finite */
+  float scale;                   /* factor on cos and sin */
+  int num_tokens;
+  int num_qo_heads;
+  int num_pairs;                 /* 2 * num_pairs <= head_dim */
+  int positions_64;
+  int interleaved;
+} d2sd_cache_append_args;
+
+int d2sd_cache_append(const d2sd_cache_append_args* args, d2sd_stream_t stream);
+
 /* Attention of each request's newest tokens over its cache, which already
  * holds them.  Query i of request r (row qo_indptr[r] + i of q) sits at
  * position kv_len[r] - n_r + i and sees keys j <= its position, with
