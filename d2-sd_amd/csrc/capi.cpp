@@ -1326,6 +1326,12 @@ int d2sd_cache_append(const d2sd_cache_append_args* a, d2sd_stream_t stream) {
 
 int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t host_plan_ints,
                     d2sd_chunk_plan_info* info) {
+  return d2sd_chunk_plan_shared(d, 0, nullptr, nullptr, host_plan, host_plan_ints, info);
+}
+
+int d2sd_chunk_plan_shared(const d2sd_chunk_plan_desc* d, int num_groups, const int32_t* shared_indptr,
+                           const int32_t* shared_len, int32_t* host_plan, size_t host_plan_ints,
+                           d2sd_chunk_plan_info* info) {
   g_last_error.clear();
   try {
     if (!d || !info) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: null argument");
@@ -1360,6 +1366,24 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t ho
       room = std::max(room, pages << lg);
       most_new = std::max(most_new, n);
     }
+    if (num_groups < 0) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: negative num_groups");
+    if (num_groups > 0) {
+      if (!shared_indptr || !shared_len) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: null pointer");
+      if (shared_indptr[0] != 0 || shared_indptr[num_groups] != d->num_reqs)
+        return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: the groups of shared keys must hold every request");
+      for (int i = 0; i < num_groups; ++i)
+        if (shared_indptr[i + 1] < shared_indptr[i] || shared_indptr[i + 1] > d->num_reqs)
+          return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: shared_indptr must not decrease");
+      for (int i = 0; i < num_groups; ++i) {
+        const int a = shared_indptr[i], b = shared_indptr[i + 1];
+        if (shared_len[i] < 0) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: lengths must not be negative");
+        if (b == a) continue;
+        if (shared_len[i] > ((int64_t)(d->page_indptr[a + 1] - d->page_indptr[a]) << lg))
+          return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: request " + std::to_string(a) + " has no pages for what it shares");
+        if (((int64_t)d->qo_indptr[b] - d->qo_indptr[a]) * group > (int64_t)INT32_MAX)
+          return fail(D2SD_ERR_UNSUPPORTED, "chunk_plan: a group of shared keys has too many rows");
+      }
+    }
     // A window as wide as all pages is none.  Narrower ones are subtracted from
     // positions in 32 bits, and a cache cut back below its new tokens starts at a
     // negative one.
@@ -1378,14 +1402,27 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t ho
     in.window_left = window;
     in.num_cus = d->num_cus > 0 ? d->num_cus : device_num_cus();
     in.max_splits = d->max_splits;
+    in.page_size = d->page_size;
+    in.num_groups = num_groups;
+    in.shared_indptr = shared_indptr;
+    in.shared_len = shared_len;
     d2sd::ChunkPlanOutput out;
     d2sd::plan_chunk(in, out);
-    constexpr size_t item_ints = sizeof(d2sd::ChunkItem) / 4, merge_ints = sizeof(d2sd::ChunkMerge) / 4;
-    const size_t ints = out.items.size() * item_ints + out.merges.size() * merge_ints;
+    const bool shared = (out.form & d2sd::CHUNK_SHARED) != 0;
+    struct Part {
+      const void* data;
+      size_t bytes;
+    };
+    const Part parts[] = {{out.items.data(), out.items.size() * sizeof(d2sd::ChunkItem)},
+                          {out.merges.data(), out.merges.size() * sizeof(d2sd::ChunkMerge)},
+                          {out.shared_merges.data(), out.shared_merges.size() * sizeof(d2sd::SharedMerge)},
+                          {out.tokens.data(), out.tokens.size() * sizeof(d2sd::SharedToken)}};
+    size_t ints = 0;
+    for (const Part& x : parts) ints += x.bytes / 4;
     if (ints > (size_t)INT32_MAX || out.partial_rows > (long long)INT32_MAX)
       return fail(D2SD_ERR_UNSUPPORTED, "chunk_plan: the batch is too large for one plan");
     info->num_items = (int)out.items.size();
-    info->num_merges = (int)out.merges.size();
+    info->num_merges = (int)(shared ? out.shared_merges.size() : out.merges.size());
     info->plan_ints = (int)ints;
     info->total_q = d->num_reqs > 0 ? d->qo_indptr[d->num_reqs] : 0;
     info->num_reqs = d->num_reqs;
@@ -1401,10 +1438,10 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t ho
     if (!host_plan) return D2SD_OK;
     if (host_plan_ints < ints)
       return fail(D2SD_ERR_WORKSPACE, "chunk_plan: host_plan too small (need " + std::to_string(ints) + " ints)");
-    if (!out.items.empty()) std::memcpy(host_plan, out.items.data(), out.items.size() * sizeof(d2sd::ChunkItem));
-    if (!out.merges.empty())
-      std::memcpy(host_plan + out.items.size() * item_ints, out.merges.data(),
-                  out.merges.size() * sizeof(d2sd::ChunkMerge));
+    for (const Part& x : parts) {
+      if (x.bytes) std::memcpy(host_plan, x.data, x.bytes);
+      host_plan += x.bytes / 4;
+    }
     return D2SD_OK;
   } catch (const std::exception& e) {
     return fail(D2SD_ERR_INVALID_ARG, std::string("chunk_plan: ") + e.what());
@@ -1418,7 +1455,7 @@ int d2sd_chunk_run(const d2sd_chunk_plan_info* info, const d2sd_chunk_run_args* 
   if (int rc = check_cache(a->cache, "chunk_run")) return rc;
   const d2sd_paged_cache& c = a->cache;
   if (c.format != info->format || c.page_size != info->page_size || c.num_kv_heads != info->num_kv_heads ||
-      c.head_dim != info->head_dim || info->form < 0 || info->form > d2sd::CHUNK_STREAM)
+      c.head_dim != info->head_dim || info->form < 0 || (info->form & ~d2sd::CHUNK_SHARED) > d2sd::CHUNK_STREAM)
     return fail(D2SD_ERR_INVALID_ARG, "chunk_run: the cache is not the one planned for");
   if (!a->plan || !a->kv_len || !a->page_table || !a->q || !a->out || !a->lse)
     return fail(D2SD_ERR_INVALID_ARG, "chunk_run: null pointer");
@@ -1444,7 +1481,10 @@ int d2sd_chunk_run(const d2sd_chunk_plan_info* info, const d2sd_chunk_run_args* 
   p.lse = a->lse;
   p.lse_stride_n = a->lse_stride_n;
   p.items = (const d2sd::ChunkItem*)a->plan;
-  p.merges = (const d2sd::ChunkMerge*)(a->plan + (size_t)info->num_items * (sizeof(d2sd::ChunkItem) / 4));
+  const bool shared = (info->form & d2sd::CHUNK_SHARED) != 0;
+  const int32_t* merges = a->plan + (size_t)info->num_items * (sizeof(d2sd::ChunkItem) / 4);
+  p.merges = (const d2sd::ChunkMerge*)merges;
+  p.tokens = (const d2sd::SharedToken*)(shared ? merges + (size_t)info->num_merges * (sizeof(d2sd::SharedMerge) / 4) : nullptr);
   p.kv_len = a->kv_len;
   p.page_table = a->page_table;
   p.ks = {c.k, c.k_scale};
@@ -1469,8 +1509,9 @@ int d2sd_chunk_run(const d2sd_chunk_plan_info* info, const d2sd_chunk_run_args* 
   p.log2_page = log2_of(c.page_size);
   p.num_pages = c.num_pages;
   p.lse_base2 = a->lse_base2 ? 1 : 0;
-  hipError_t e = d2sd::launch_chunk_attention(p, info->head_dim, info->format, info->form, info->num_items, info->num_merges,
-                                              (hipStream_t)stream);
+  const int form = info->form & ~d2sd::CHUNK_SHARED;
+  hipError_t e = (shared ? d2sd::launch_shared_attention : d2sd::launch_chunk_attention)(
+      p, info->head_dim, info->format, form, info->num_items, info->num_merges, (hipStream_t)stream);
   return e == hipSuccess ? D2SD_OK : fail_hip(e, "chunk_run launch");
 }
 

@@ -95,7 +95,7 @@ __device__ __forceinline__ float block_scale(unsigned byte) {
 
 // What an item's rows see: query i of the request sits at pos0 + i.
 struct Span {
-  int pos0;       // position of the request's query 0 (negative: it has no key yet)
+  int pos0;       // position of the request's query 0 (negative: it has no key yet; items of shared keys: unused)
   int lo, hi;     // keys [lo, hi) are visible to some row of the item
   int all_lo, all_hi;  // keys [all_lo, all_hi) are visible to every row
 };
@@ -110,6 +110,79 @@ __device__ __forceinline__ Span item_span(const ChunkParams& p, const ChunkItem&
   s.all_hi = first + 1;
   s.all_lo = p.window_left >= 0 ? max(last - p.window_left, 0) : 0;
   return s;
+}
+
+// ---- shared keys ----
+// Plans whose requests share their first keys (SHARED) have three parts of work:
+// the rows of a whole group of requests over the keys that they share
+// (PART_SHARED: keys [0, bound) of the group's first request), each request's rows
+// over its keys from `bound` on (PART_OWN), and requests that share nothing.  Rows
+// of a group lie one after the other, so that an item's rows are packed as ever;
+// but they sit at positions of their own.
+__device__ __forceinline__ int shared_pos(const ChunkParams& p, const ChunkItem& w, int row) {
+  const int4 t = ((const int4*)p.tokens)[w.q0 + (w.row0 + row) / p.group];  // request, tokens to its end, tokens its pages hold
+  return min(p.kv_len[t.x], t.z) - t.y;
+}
+
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) x = min(x, __shfl_xor(x, m));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+// The span of packed rows row_a .. row_b of the item.  edges: all_lo and all_hi are
+// wanted too.  (Without a window an item of shared keys takes lo and hi as they are
+// planned, so that its first keys wait for no length.)
+template <bool SHARED>
+__device__ __forceinline__ Span rows_span(const ChunkParams& p, const ChunkItem& w, int row_a, int row_b, bool edges = true) {
+  if constexpr (!SHARED) return item_span(p, w, (w.row0 + row_a) / p.group, (w.row0 + row_b) / p.group);
+  if (w.part != PART_SHARED) {
+    Span s = item_span(p, w, (w.row0 + row_a) / p.group, (w.row0 + row_b) / p.group);
+    s.lo = max(s.lo, w.bound);
+    s.all_lo = max(s.all_lo, w.bound);
+    return s;
+  }
+  Span s{0, 0, w.bound, w.bound, 0};
+  if (!edges && p.window_left < 0) return s;
+  int first = 0x7FFFFFFF, past = 0x7FFFFFFF;  // lowest position; 0 - highest
+  for (int row = row_a + (threadIdx.x & 63); row <= row_b; row += 64) {
+    const int pos = shared_pos(p, w, row);
+    first = min(first, pos);
+    past = min(past, -pos);
+  }
+  first = wave_min(first);
+  const int last = -wave_min(past);
+  s.all_hi = min(w.bound, first + 1);
+  if (p.window_left >= 0) {
+    s.hi = min(w.bound, max(last + 1, 0));
+    s.lo = max(first - p.window_left, 0);
+    s.all_lo = max(last - p.window_left, 0);
+  }
+  return s;
+}
+
+// Keys that a row at `pos` sees: first and last of the item's.
+template <bool SHARED>
+__device__ __forceinline__ int row_first(const ChunkParams& p, const ChunkItem& w, int pos) {
+  const int lo = p.window_left >= 0 ? max(pos - p.window_left, 0) : 0;
+  if constexpr (SHARED) return w.part == PART_SHARED ? lo : max(lo, w.bound);
+  return lo;
+}
+template <bool SHARED>
+__device__ __forceinline__ int row_last(const ChunkItem& w, int pos) {
+  if constexpr (SHARED) return w.part == PART_SHARED ? min(pos, w.bound - 1) : pos;
+  return pos;
+}
+template <bool SHARED>
+__device__ __forceinline__ int row_pos(const ChunkParams& p, const ChunkItem& w, int pos0, int row) {
+  if constexpr (SHARED)
+    if (w.part == PART_SHARED) return shared_pos(p, w, row);
+  return pos0 + (w.row0 + row) / p.group;
+}
+// Whether the item's state is one of several of its rows.
+template <bool SHARED>
+__device__ __forceinline__ bool is_partial(const ChunkItem& w) {
+  return w.nchunks > 1 || (SHARED && w.part != PART_ALONE);
 }
 
 // Online softmax of 16 * N scores of this lane's row: the running maximum m (raw
@@ -267,7 +340,7 @@ __device__ __forceinline__ float sink_factor(const ChunkParams& p, int head, flo
 // token: bf16 1.1 -> 3.3 ms).
 // Tile items: a wave's 32 rows over their part of the item's chunk of keys, straight
 // from the cache, values through 32 rows of its own LDS.  o, m, l: from the start.
-template <int D, int FMT>
+template <int D, int FMT, bool SHARED>
 __device__ __forceinline__ void tile_rows_by_key(lds_char* lds, f32x16 (&o)[D / 32], float& m, float& l) {
   constexpr int MT = D / 32, KS = D / 16;
   constexpr bool MX = Format<D, FMT>::MX;
@@ -277,17 +350,18 @@ __device__ __forceinline__ void tile_rows_by_key(lds_char* lds, f32x16 (&o)[D / 
   __asm__ volatile("" : "+s"(at));
   const ChunkParams& p = *(const ChunkParams*)at;
   const ChunkItem w = p.items[blockIdx.x];
-  const Span all = item_span(p, w, w.row0 / p.group, (w.row0 + w.nrows - 1) / p.group);
-  const Span own = item_span(p, w, (w.row0 + 32 * wv) / p.group, (w.row0 + min(32 * wv + 31, w.nrows - 1)) / p.group);
+  const Span all = rows_span<SHARED>(p, w, 0, w.nrows - 1, false);
+  const Span own = rows_span<SHARED>(p, w, 32 * wv, min(32 * wv + 31, w.nrows - 1));
   if (own.lo == own.all_lo && own.hi == own.all_hi) return;
   const int ntiles = max(all.hi - all.lo + 63, 0) >> 6;
   const int from = max(all.lo + 64 * (int)((long long)ntiles * w.chunk / w.nchunks), own.lo);
   const int to = min(all.lo + 64 * (int)((long long)ntiles * (w.chunk + 1) / w.nchunks), own.hi);
   lds_char* vt = lds + wv * 32 * D * 2;
-  const int row = min(32 * wv + l32, w.nrows - 1), pos = all.pos0 + (w.row0 + row) / p.group, hi = min(pos, to - 1);
+  const int row = min(32 * wv + l32, w.nrows - 1), pos = row_pos<SHARED>(p, w, all.pos0, row),
+            hi = min(row_last<SHARED>(w, pos), to - 1);
   const RowOut qat(p, w, row);
   const bf16_t* qp = (const bf16_t*)p.q + (long long)qat.token * p.q_stride_n + (long long)qat.head * p.q_stride_h + 8 * hh;
-  const int row_lo = p.window_left >= 0 ? max(pos - p.window_left, 0) : 0;
+  const int row_lo = row_first<SHARED>(p, w, pos);
   float c = p.sm_scale * kLog2e;
   if constexpr (FMT == CACHE_FP8) c *= ((const float*)p.ks.scale)[w.kvh];
   const float slack = c > 0.f ? kRescaleSlack / c : 0.f;
@@ -352,13 +426,13 @@ __device__ __forceinline__ void tile_rows_by_key(lds_char* lds, f32x16 (&o)[D / 
 }
 
 // ---- tile items ----
-template <int D, int FMT, int W>
+template <int D, int FMT, int W, bool SHARED>
 __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem& w, lds_char* lds) {
   constexpr int MT = D / 32, KS = D / 16, ROW = Format<D, FMT>::ROW, TB = 64 * D * 2;
   constexpr bool MX = Format<D, FMT>::MX;
   const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
 
-  const Span all = item_span(p, w, w.row0 / p.group, (w.row0 + w.nrows - 1) / p.group);
+  const Span all = rows_span<SHARED>(p, w, 0, w.nrows - 1, false);
   // tiles of 64 keys from the first visible one on
   const int ntiles = max(all.hi - all.lo + 63, 0) >> 6;
   const int tb = (int)((long long)ntiles * w.chunk / w.nchunks);
@@ -367,11 +441,9 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
   // this wave's rows
   const int wrow = 32 * wv, row = min(wrow + l32, w.nrows - 1);
   const bool wave_on = wrow < w.nrows;
-  const int t_row = (w.row0 + row) / p.group;
-  const int pos = all.pos0 + t_row;
-  const int row_lo = p.window_left >= 0 ? max(pos - p.window_left, 0) : 0;
-  const Span own = item_span(p, w, (w.row0 + min(wrow, w.nrows - 1)) / p.group,
-                             (w.row0 + min(wrow + 31, w.nrows - 1)) / p.group);
+  const int pos = row_pos<SHARED>(p, w, all.pos0, row);
+  const int row_lo = row_first<SHARED>(p, w, pos), row_hi = row_last<SHARED>(w, pos);
+  const Span own = rows_span<SHARED>(p, w, min(wrow, w.nrows - 1), min(wrow + 31, w.nrows - 1));
   const RowOut at(p, w, row);
   bf16x8 qf[KS];
   {
@@ -552,8 +624,8 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
     }
     if (on) {
       if (kb < own.all_lo || kb + 64 > own.all_hi) {
-        hide(s[0], kb, row_lo, pos, hh);
-        hide(s[1], kb + 32, row_lo, pos, hh);
+        hide(s[0], kb, row_lo, row_hi, hh);
+        hide(s[1], kb + 32, row_lo, row_hi, hh);
       }
       softmax_step<2, MT>(s, o, m, l, c, slack, hh);
 #pragma unroll
@@ -571,7 +643,7 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
         const bf16x8 kf = *(const __attribute__((address_space(3))) bf16x8*)(kt + half * D * 2 + koff[ks]);
         s1[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], ks ? s1[0] : f32x16{}, 0, 0, 0);
       }
-      hide(s1[0], kb + half, row_lo, pos, hh);
+      hide(s1[0], kb + half, row_lo, row_hi, hh);
       softmax_step<1, MT>(s1, o, m, l, c, slack, hh);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -592,12 +664,12 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
 #pragma unroll
     for (int i = 0; i < 16; ++i) zero = fmaf(o[mt][i], 0.f, zero);
   // (no wave reads the tiles any more: the last step's barrier)
-  if (__any(zero != 0.f)) tile_rows_by_key<D, FMT>(lds, o, m, l);
+  if (__any(zero != 0.f)) tile_rows_by_key<D, FMT, SHARED>(lds, o, m, l);
   l += xor32(l, hh);
   const float lse2 = l > 0.f ? m * c + __builtin_amdgcn_logf(l) : l == 0.f ? -INFINITY : l;
   float inv = l != 0.f ? vscale / l : 0.f;
   const bool mine = wrow + l32 < w.nrows;
-  if (w.nchunks > 1) {
+  if (is_partial<SHARED>(w)) {
     if (!mine) return;
     const long long pr = w.slot + (long long)w.chunk * w.nrows + row;
     float* po = p.part_o + pr * D + 4 * hh;
@@ -633,7 +705,7 @@ __device__ __forceinline__ T load_kv(const T* p) {
   return *p;
 }
 
-template <int D, int FMT, int W, int RB, int PF, bool STREAM>
+template <int D, int FMT, int W, int RB, int PF, bool STREAM, bool SHARED>
 __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem& w, lds_char* lds, float* stats) {
   constexpr int MT = D / 16, KS = D / 32, ROW = Format<D, FMT>::ROW;
   constexpr bool MX = Format<D, FMT>::MX;
@@ -650,19 +722,20 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
   constexpr int VB = 32 * D * 2;                // bytes of a wave's value tile
   const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
 
-  const Span all = item_span(p, w, w.row0 / p.group, (w.row0 + w.nrows - 1) / p.group);
+  const Span all = rows_span<SHARED>(p, w, 0, w.nrows - 1);
   const int tile0 = all.lo >> 5, ntiles_all = all.hi > all.lo ? ((all.hi + 31) >> 5) - tile0 : 0;
   const int tb = tile0 + (int)((long long)ntiles_all * w.chunk / w.nchunks);
   const int te = tile0 + (int)((long long)ntiles_all * (w.chunk + 1) / w.nchunks);
 
-  int pos[RB], row_lo[RB];
+  int pos[RB], row_lo[RB];  // last and first key of a row
   bf16x8 qf[RB][KS];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const int row = min(16 * rb + l16, w.nrows - 1);
     const RowOut at(p, w, row);
-    pos[rb] = all.pos0 + (w.row0 + row) / p.group;
-    row_lo[rb] = p.window_left >= 0 ? max(pos[rb] - p.window_left, 0) : 0;
+    pos[rb] = row_pos<SHARED>(p, w, all.pos0, row);
+    row_lo[rb] = row_first<SHARED>(p, w, pos[rb]);
+    pos[rb] = row_last<SHARED>(w, pos[rb]);
     const bf16_t* qp = (const bf16_t*)p.q + (long long)at.token * p.q_stride_n + (long long)at.head * p.q_stride_h;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
@@ -976,7 +1049,7 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
       }
       const float lse2 = sum > 0.f ? top * c + __builtin_amdgcn_logf(sum) : sum == 0.f ? -INFINITY : sum;
       float inv = sum != 0.f ? vscale / sum : 0.f;
-      if (w.nchunks > 1) {
+      if (is_partial<SHARED>(w)) {
         const long long pr = w.slot + (long long)w.chunk * nr + r;
         *(f32x4*)(p.part_o + pr * D + dd) = acc * inv;
         if (dd == 0) p.part_lse[pr] = lse2;
@@ -1004,45 +1077,70 @@ constexpr int chunk_occupancy() {
   return FORM >= CHUNK_TOKENS ? (FMT == CACHE_MXFP4 ? 3 : 2) : D == 64 ? 3 : 2;
 }
 
-template <int D, int FMT, int FORM>
-__global__ __launch_bounds__(64 * chunk_waves(FORM), (chunk_occupancy<D, FMT, FORM>())) void
-chunk_attn_kernel(const ChunkParams p) {
+template <int D, int FMT, int FORM, bool SHARED>
+__device__ __forceinline__ void chunk_work(const ChunkParams& p) {
   constexpr int W = chunk_waves(FORM);
   constexpr bool TOKENS = FORM >= CHUNK_TOKENS;
   __shared__ __align__(16) char lds[TOKENS ? W * 32 * D * 2 : 4 * 64 * D * 2];
   __shared__ float stats[2 * W * kTokenRows];
   const ChunkItem w = p.items[blockIdx.x];
   if constexpr (TOKENS) {
-    token_item<D, FMT, W, 1, token_depth<FMT>(), FORM == CHUNK_STREAM>(p, w, (lds_char*)lds, stats);
+    token_item<D, FMT, W, 1, token_depth<FMT>(), FORM == CHUNK_STREAM, SHARED>(p, w, (lds_char*)lds, stats);
   } else {
     if (w.kind == CHUNK_TILE)
-      tile_item<D, FMT, W>(p, w, (lds_char*)lds);
+      tile_item<D, FMT, W, SHARED>(p, w, (lds_char*)lds);
     else if (w.nrows <= 16)
-      token_item<D, FMT, W, 1, token_depth<FMT>(), FORM == CHUNK_STREAM>(p, w, (lds_char*)lds, stats);
+      token_item<D, FMT, W, 1, token_depth<FMT>(), FORM == CHUNK_STREAM, SHARED>(p, w, (lds_char*)lds, stats);
     else
-      token_item<D, FMT, W, 2, 1, false>(p, w, (lds_char*)lds, stats);
+      token_item<D, FMT, W, 2, 1, false, SHARED>(p, w, (lds_char*)lds, stats);
   }
 }
 
-// Row i of a merge item from its nchunks partial states: thread (i, d4) holds
-// head dims 4 d4 .. 4 d4 + 3.  Latency bound: the sums and states of eight chunks
-// are read at once (one token over 8 chunks: 3.8 -> 3.0 us against sums first),
-// joined in chunk order whatever the order they were written in.
-template <int D>
-__global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkParams p) {
-  const ChunkMerge w = p.merges[blockIdx.x];
+// (This file is compiled twice: its kernels for plans without and with shared keys.)
+#ifndef D2SD_CHUNK_SHARED
+#define ATTN_KERNEL chunk_attn_kernel
+#define MERGE_KERNEL chunk_merge_kernel
+#define LAUNCH launch_chunk_attention
+template <int D, int FMT, int FORM>
+__global__ __launch_bounds__(64 * chunk_waves(FORM), (chunk_occupancy<D, FMT, FORM>())) void
+chunk_attn_kernel(const ChunkParams p) {
+  chunk_work<D, FMT, FORM, false>(p);
+}
+#else
+#define ATTN_KERNEL shared_attn_kernel
+#define MERGE_KERNEL shared_merge_kernel
+#define LAUNCH launch_shared_attention
+template <int D, int FMT, int FORM>
+__global__ __launch_bounds__(64 * chunk_waves(FORM), (chunk_occupancy<D, FMT, FORM>())) void
+shared_attn_kernel(const ChunkParams p) {
+  chunk_work<D, FMT, FORM, true>(p);
+}
+#endif
+
+// Row i of a merge item from its partial states, nchunks of them, then (SHARED)
+// those over the keys that it shares: thread (i, d4) holds head dims 4 d4 .. 4 d4 +
+// 3.  Latency bound: the sums and states of eight chunks are read at once (one
+// token over 8 chunks: 3.8 -> 3.0 us against sums first), joined in chunk order
+// whatever the order they were written in.
+template <int D, bool SHARED, typename Merge>
+__device__ __forceinline__ void merge_rows(const ChunkParams& p, const Merge& w) {
   const int i = threadIdx.x / (D / 4), dd = 4 * (threadIdx.x % (D / 4));
   if (i >= w.nrows) return;
   constexpr int B = 8;
   float top = -INFINITY, sum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int c0 = 0; c0 < w.nchunks; c0 += B) {
+  int nchunks = w.nchunks;
+  if constexpr (SHARED) nchunks += w.shared_chunks;
+  for (int c0 = 0; c0 < nchunks; c0 += B) {
     float s[B];
     f32x4 v[B];
 #pragma unroll
     for (int u = 0; u < B; ++u) {
-      const long long pr = w.slot + i + (long long)min(c0 + u, w.nchunks - 1) * w.stride;
-      s[u] = c0 + u < w.nchunks ? p.part_lse[pr] : -INFINITY;
+      const int c = min(c0 + u, nchunks - 1);
+      long long pr = w.slot + i + (long long)c * w.stride;
+      if constexpr (SHARED)
+        if (c >= w.nchunks) pr = w.shared_slot + i + (long long)(c - w.nchunks) * w.shared_stride;
+      s[u] = c0 + u < nchunks ? p.part_lse[pr] : -INFINITY;
       v[u] = *(const f32x4*)(p.part_o + pr * D + dd);
     }
     float mx = top;
@@ -1073,22 +1171,34 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkParams p) {
   if (dd == 0) p.lse[token * p.lse_stride_n + head] = p.lse_base2 ? lse2 : lse2 * kLn2;
 }
 
+#ifndef D2SD_CHUNK_SHARED
+template <int D>
+__global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkParams p) {
+  merge_rows<D, false>(p, p.merges[blockIdx.x]);
+}
+#else
+template <int D>
+__global__ __launch_bounds__(256) void shared_merge_kernel(const ChunkParams p) {
+  merge_rows<D, true>(p, ((const SharedMerge*)p.merges)[blockIdx.x]);
+}
+#endif
+
 template <int D, int FMT>
 hipError_t launch_f(const ChunkParams& p, int form, int nitems, int nmerges, hipStream_t s) {
   const dim3 grid((unsigned)nitems), block(64 * chunk_waves(form));
   if (form == CHUNK_TOKENS) {
-    hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, CHUNK_TOKENS>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((ATTN_KERNEL<D, FMT, CHUNK_TOKENS>), grid, block, 0, s, p);
   } else if (form == CHUNK_STREAM) {
-    hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, CHUNK_STREAM>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((ATTN_KERNEL<D, FMT, CHUNK_STREAM>), grid, block, 0, s, p);
   } else if (form == CHUNK_WAVES4) {
-    hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, CHUNK_WAVES4>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((ATTN_KERNEL<D, FMT, CHUNK_WAVES4>), grid, block, 0, s, p);
   } else {
     if constexpr (D == 64) return hipErrorInvalidValue;  // (the planner gives heads of 64 four waves)
-    else hipLaunchKernelGGL((chunk_attn_kernel<D, FMT, CHUNK_WAVES8>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((ATTN_KERNEL<D, FMT, CHUNK_WAVES8>), grid, block, 0, s, p);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (nmerges > 0) hipLaunchKernelGGL(chunk_merge_kernel<D>, dim3((unsigned)nmerges), dim3(256), 0, s, p);
+  if (nmerges > 0) hipLaunchKernelGGL(MERGE_KERNEL<D>, dim3((unsigned)nmerges), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 
@@ -1105,8 +1215,7 @@ hipError_t launch_d(const ChunkParams& p, int format, int form, int nitems, int 
 
 }  // namespace
 
-hipError_t launch_chunk_attention(const ChunkParams& p, int head_dim, int format, int form, int nitems, int nmerges,
-                                  hipStream_t s) {
+hipError_t LAUNCH(const ChunkParams& p, int head_dim, int format, int form, int nitems, int nmerges, hipStream_t s) {
   if (nitems <= 0) return hipSuccess;
   return head_dim == 64    ? launch_d<64>(p, format, form, nitems, nmerges, s)
          : head_dim == 128 ? launch_d<128>(p, format, form, nitems, nmerges, s)

@@ -32,17 +32,29 @@ double tile_us(int form, int head_dim, double n) {
   return form == CHUNK_WAVES8 ? 2.0 : 0.35 + n;
 }
 
+// Rows that are packed together: a request's, or, over the keys that they share,
+// those of all requests of a group.
+struct Rows {
+  int part, req;        // PART_*; the (first) request
+  int q0, nq;           // first row of q, their number
+  int last_req;         // behind the last of its requests
+  int bound;            // keys [0, bound) are shared
+};
+
 struct Group {         // one row tile of a request, for every kv head
-  int req, row0, nrows, kind;
+  int rows;            // index of its Rows
+  int row0, nrows, kind;
   int units, least;    // key tiles, and those of the shortest chunk
   double unit_us;      // of a tile, alone
   double unit_read_us; // of that, its bytes at a workgroup's highest rate
+  bool partial;        // its state is joined with another's whatever its chunks
   double work() const { return units * unit_us; }
   double read_us() const { return units * unit_read_us; }
 };
 
 struct Planner {
   const ChunkPlanInput& in;
+  const std::vector<Rows>& rows_list;
   int form;
   std::vector<Group> groups;
   int per_cu, places;   // workgroups resident on a CU, on the device
@@ -51,7 +63,7 @@ struct Planner {
   double limit = 0.0;   // the longest chunk, in us of one workgroup alone on its CU
   double token_share = 1.0;  // of that, a token item's longest
 
-  Planner(const ChunkPlanInput& input, int f) : in(input), form(f) {
+  Planner(const ChunkPlanInput& input, const std::vector<Rows>& rows, int f) : in(input), rows_list(rows), form(f) {
     // (by registers: chunk_attn_kernel; the token kernels of heads of 64 would fit four
     // but for mxfp8, the schedule counts three)
     per_cu = form == CHUNK_WAVES8 ? 1 : in.head_dim == 64 ? 3 : form == CHUNK_TOKENS && in.format == CACHE_MXFP4 ? 3 : 2;
@@ -96,7 +108,7 @@ struct Planner {
     const double slower_read = std::max(1.0, std::min(readers, (double)places) * place_bytes / kHbmBytes);
     for (const Group& g : groups) {
       const int n = chunks(g);
-      if (n > 1) partial += (double)n * g.nrows * in.num_kv_heads * in.head_dim * 8.0;  // written and read
+      if (n > 1 || g.partial) partial += (double)n * g.nrows * in.num_kv_heads * in.head_dim * 8.0;  // written and read
       const double us = g.kind == CHUNK_TOKEN ? std::max(g.work(), g.read_us() * slower_read) : g.work() * slower_tile;
       times.push_back({us / n + kItemUs, n * in.num_kv_heads});
     }
@@ -131,22 +143,43 @@ struct Planner {
     const double token_us = kTokenTileUs * (in.head_dim == 64 ? 0.5 : 1.0) / waves;
     double longest = 0.0, total = 0.0;
     bool tiles = false, tokens = false;
-    for (int r = 0; r < in.num_reqs; ++r) {
-      const int nq = in.qo_indptr[r + 1] - in.qo_indptr[r];
-      const long long rows = (long long)nq * group;
+    for (int at = 0; at < (int)rows_list.size(); ++at) {
+      const Rows& set = rows_list[at];
+      const long long rows = (long long)set.nq * group;
       const int kind = rows <= kTokenRows ? CHUNK_TOKEN : CHUNK_TILE;
       const int step = kind == CHUNK_TOKEN ? kTokenRows : chunk_rows(form), keys_per_unit = kind == CHUNK_TOKEN ? 32 : 64;
       const double unit_bytes = 2.0 * keys_per_unit * row_bytes(in.format, in.head_dim);
+      int req = set.req;  // (of shared keys: that of the row tile's first token)
       for (long long row0 = 0; row0 < rows; row0 += step) {
         Group g{};
-        g.req = r;
+        g.rows = at;
         g.row0 = (int)row0;
         g.nrows = (int)std::min<long long>(step, rows - row0);
         g.kind = kind;
-        const long long pos0 = (long long)in.kv_len[r] - nq;
-        const long long first = pos0 + row0 / group, last = pos0 + (row0 + g.nrows - 1) / group;
-        const long long hi = std::max(last + 1, 0ll);
-        const long long lo = in.window_left >= 0 ? std::max(first - in.window_left, 0ll) : 0;
+        g.partial = set.part != PART_ALONE;
+        long long lo, hi;
+        if (set.part == PART_SHARED) {
+          lo = 0, hi = set.bound;
+          if (in.window_left >= 0) {
+            // the first and last key that some token of the tile sees
+            const int t0 = set.q0 + (int)(row0 / group), t1 = set.q0 + (int)((row0 + g.nrows - 1) / group);
+            while (in.qo_indptr[req + 1] <= t0) ++req;
+            long long first = 1ll << 40, last = -1;
+            for (int r = req; r < set.last_req && in.qo_indptr[r] <= t1; ++r) {
+              if (in.qo_indptr[r + 1] <= std::max(in.qo_indptr[r], t0)) continue;
+              const long long end = (long long)in.kv_len[r] - in.qo_indptr[r + 1];
+              first = std::min(first, end + std::max(in.qo_indptr[r], t0));
+              last = std::max(last, end + std::min(in.qo_indptr[r + 1] - 1, t1));
+            }
+            lo = std::max(first - in.window_left, 0ll);
+            hi = std::min<long long>(set.bound, std::max(last + 1, 0ll));
+          }
+        } else {
+          const long long pos0 = (long long)in.kv_len[set.req] - set.nq;
+          const long long first = pos0 + row0 / group, last = pos0 + (row0 + g.nrows - 1) / group;
+          hi = std::max(last + 1, 0ll);
+          lo = std::max<long long>(in.window_left >= 0 ? std::max(first - in.window_left, 0ll) : 0, set.bound);
+        }
         // (a tile item's tiles start at its first key, a token item's at multiples)
         const long long from = kind == CHUNK_TOKEN ? lo / keys_per_unit * keys_per_unit : lo;
         g.units = hi > lo ? (int)((hi - from + keys_per_unit - 1) / keys_per_unit) : 0;
@@ -196,9 +229,24 @@ struct Planner {
 void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   out = ChunkPlanOutput{};
   const int group = in.num_qo_heads / in.num_kv_heads;
+  std::vector<Rows> rows;
+  bool shared = false;
+  std::vector<int> shared_rows(in.num_reqs, -1);  // of a request: the Rows of what it shares
+  for (int i = 0; i < in.num_groups; ++i) {
+    const int a = in.shared_indptr[i], b = in.shared_indptr[i + 1];
+    const int q0 = in.qo_indptr[a], nq = in.qo_indptr[b] - q0;
+    if (b - a < 2 || in.shared_len[i] == 0 || nq == 0) continue;
+    for (int r = a; r < b; ++r) shared_rows[r] = (int)rows.size();
+    rows.push_back({PART_SHARED, a, q0, nq, b, in.shared_len[i]});
+    shared = true;
+  }
+  for (int r = 0; r < in.num_reqs; ++r) {
+    const int q0 = in.qo_indptr[r], nq = in.qo_indptr[r + 1] - q0, s = shared_rows[r];
+    rows.push_back({s < 0 ? PART_ALONE : PART_OWN, r, q0, nq, r + 1, s < 0 ? 0 : rows[s].bound});
+  }
   bool tokens_only = true;
-  for (int r = 0; r < in.num_reqs; ++r)
-    if ((long long)(in.qo_indptr[r + 1] - in.qo_indptr[r]) * group > 16) tokens_only = false;
+  for (const Rows& x : rows)
+    if ((long long)x.nq * group > 16) tokens_only = false;
   // Heads of 128: workgroups of 8 waves share a tile's staging among more rows
   // (2 x 2048 tokens at 16384 bf16 keys: 953 us against 1045), those of 4 fill
   // the device with fewer rows (1000 tokens at 2100: 47 us against 50 split in two
@@ -206,10 +254,10 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   // were kept in L2, 4 x 1024 tokens, window 128: 39 us against 44; 8 x 300 at 1000:
   // 66 against 74; but 2 x 2048 at 16384: 1340 against 1259 in bf16, 1201 against
   // 1217 in mxfp4; now 28, 55, 1200 and 1145 of 4 waves, 8 were not measured again).
-  Planner pl(in, tokens_only ? CHUNK_TOKENS : CHUNK_WAVES4);
+  Planner pl(in, rows, tokens_only ? CHUNK_TOKENS : CHUNK_WAVES4);
   const double us = pl.plan();
   if (!tokens_only && in.head_dim == 128) {
-    Planner other(in, CHUNK_WAVES8);
+    Planner other(in, rows, CHUNK_WAVES8);
     if (other.plan() < us) pl.take(std::move(other));
   }
   out.form = pl.form;
@@ -230,16 +278,44 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   std::vector<Placed> order;
   order.reserve(pl.groups.size());
   long long slot = 0, items = 0;
+  std::vector<long long> slots(pl.groups.size());  // of head 0
+  std::vector<int> first_group(rows.size(), -1);   // of a Rows' row tiles, which follow each other
   for (int i = 0; i < (int)pl.groups.size(); ++i) {
     const Group& g = pl.groups[i];
     const int n = pl.chunks(g);
     order.push_back({g.work() / n, i, n, slot});
     items += (long long)n * in.num_kv_heads;
-    if (n == 1) continue;
-    const int q0 = in.qo_indptr[g.req];
-    for (int h = 0; h < in.num_kv_heads; ++h, slot += (long long)n * g.nrows)
-      for (int r = 0; r < g.nrows; r += merge_rows)
-        out.merges.push_back(ChunkMerge{q0, h, g.row0 + r, std::min(merge_rows, g.nrows - r), (int)slot + r, g.nrows, n, 0});
+    if (first_group[g.rows] < 0) first_group[g.rows] = i;
+    if (n == 1 && !g.partial) continue;
+    slots[i] = slot;
+    slot += (long long)n * g.nrows * in.num_kv_heads;
+    const Rows& set = rows[g.rows];
+    if (set.part == PART_SHARED) continue;
+    for (int h = 0; h < in.num_kv_heads; ++h) {
+      const long long at = slots[i] + (long long)h * n * g.nrows;
+      if (!shared) {
+        for (int r = 0; r < g.nrows; r += merge_rows)
+          out.merges.push_back(ChunkMerge{set.q0, h, g.row0 + r, std::min(merge_rows, g.nrows - r), (int)at + r, g.nrows, n, 0});
+        continue;
+      }
+      for (int r = 0, take; r < g.nrows; r += take) {
+        take = std::min(merge_rows, g.nrows - r);
+        SharedMerge m{set.q0, h, g.row0 + r, take, (int)at + r, g.nrows, n, 0, 0, 0, {0, 0}};
+        if (set.part == PART_OWN) {
+          // its rows among those of the group, within one of their row tiles
+          const int sh = shared_rows[set.req], from = (set.q0 - rows[sh].q0) * group + g.row0 + r;
+          int k = first_group[sh];
+          while (from >= pl.groups[k].row0 + pl.groups[k].nrows) ++k;
+          const Group& sg = pl.groups[k];
+          const int sn = pl.chunks(sg);
+          take = m.nrows = std::min(take, sg.row0 + sg.nrows - from);
+          m.shared_slot = (int)(slots[k] + (long long)h * sn * sg.nrows) + from - sg.row0;
+          m.shared_stride = sg.nrows;
+          m.shared_chunks = sn;
+        }
+        out.shared_merges.push_back(m);
+      }
+    }
   }
   // Longest first; among equals the kv heads of one key chunk side by side, so
   // that with 8 (or 16, ..) kv heads each XCD (workgroups are dealt to the 8 of
@@ -249,22 +325,30 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   for (const Placed& x : order) {
     const Group& g = pl.groups[x.group];
     ChunkItem it{};
-    it.req = g.req;
-    it.q0 = in.qo_indptr[g.req];
-    it.nq = in.qo_indptr[g.req + 1] - it.q0;
+    const Rows& set = rows[g.rows];
+    it.req = set.req;
+    it.q0 = set.q0;
+    it.nq = set.nq;
     it.row0 = g.row0;
     it.nrows = g.nrows;
-    it.page_begin = in.page_indptr[g.req];
-    it.page_end = in.page_indptr[g.req + 1];
+    it.page_begin = in.page_indptr[set.req];
+    it.page_end = in.page_indptr[set.req + 1];
     it.nchunks = x.chunks;
     it.kind = g.kind;
+    it.part = set.part;
+    it.bound = set.bound;
     for (it.chunk = 0; it.chunk < x.chunks; ++it.chunk)
       for (it.kvh = 0; it.kvh < in.num_kv_heads; ++it.kvh) {
-        it.slot = x.chunks > 1 ? (int)(x.slot + (long long)it.kvh * x.chunks * g.nrows) : 0;
+        it.slot = x.chunks > 1 || g.partial ? (int)(x.slot + (long long)it.kvh * x.chunks * g.nrows) : 0;
         out.items.push_back(it);
       }
   }
   out.partial_rows = slot;
+  if (!shared) return;
+  out.form |= CHUNK_SHARED;
+  for (int r = 0; r < in.num_reqs; ++r)
+    for (int t = in.qo_indptr[r]; t < in.qo_indptr[r + 1]; ++t)
+      out.tokens.push_back({r, in.qo_indptr[r + 1] - t, (in.page_indptr[r + 1] - in.page_indptr[r]) * in.page_size, 0});
 }
 
 }  // namespace d2sd

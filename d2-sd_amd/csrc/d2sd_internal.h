@@ -314,6 +314,8 @@ struct AppendParams {
 enum ChunkForm : int { CHUNK_WAVES8 = 0, CHUNK_WAVES4 = 1, CHUNK_TOKENS = 2, CHUNK_STREAM = 3 };
 constexpr int chunk_waves(int form) { return form == CHUNK_WAVES8 ? 8 : 4; }
 constexpr int chunk_rows(int form) { return 32 * chunk_waves(form); }  // packed rows of a tile item (32 per wave)
+constexpr int CHUNK_SHARED = 8;     // added to the form of plans with shared keys
+enum : int { PART_ALONE = 0, PART_SHARED = 1, PART_OWN = 2 };
 constexpr int kTokenRows = 32;      // packed rows a token item holds at most (all waves share them)
 constexpr int kChunkMaxSplits = 64;
 enum : int { CHUNK_TILE = 0, CHUNK_TOKEN = 1 };
@@ -325,12 +327,25 @@ struct ChunkItem {                  // one workgroup (64 bytes)
   int chunk, nchunks;               // key chunk of its rows' visible keys
   int slot;                         // first partial row (nchunks > 1)
   int kind;                         // CHUNK_TILE / CHUNK_TOKEN
-  int pad[4];
+  // plans with shared keys (CHUNK_SHARED): req, q0, nq and the pages of PART_SHARED
+  // items are the group's first request's, first row, rows and pages
+  int part;                         // PART_*
+  int bound;                        // keys [0, bound) are shared
+  int pad[2];
 };
 struct ChunkMerge {                 // 32 bytes: rows merged by one workgroup
   int q0, kvh, row0, nrows;
   int slot, stride, nchunks;        // chunk c's partial of row i: slot + c * stride + i
   int pad;
+};
+struct SharedMerge {                // 48 bytes: the same in plans with shared keys
+  int q0, kvh, row0, nrows;
+  int slot, stride, nchunks;        // over the rows' own keys (all of them where none are shared)
+  int shared_slot, shared_stride, shared_chunks;  // over the shared ones (0 chunks: none)
+  int pad[2];
+};
+struct SharedToken {                // a row of q: its request, tokens from it to the request's end, tokens that the
+  int req, back, room, pad;         // request's pages hold
 };
 struct ChunkParams {
   const void* q;
@@ -340,7 +355,8 @@ struct ChunkParams {
   float* lse;                        // [rows, Hq]
   long long lse_stride_n;
   const ChunkItem* items;
-  const ChunkMerge* merges;
+  const ChunkMerge* merges;          // CHUNK_SHARED: SharedMerge
+  const SharedToken* tokens;         // CHUNK_SHARED: [rows]
   const int* kv_len;
   const int* page_table;
   CacheSide ks, vs;

@@ -105,19 +105,29 @@ struct ChunkPlanInput {
   const int* page_indptr;  // host [num_reqs + 1]
   int num_qo_heads, num_kv_heads, head_dim;
   int format;              // CACHE_*
+  int page_size;
   int window_left;
   int num_cus;
   int max_splits;          // 0: up to kChunkMaxSplits
+  // Groups of requests that share their first keys (0: none): group i is requests
+  // [shared_indptr[i], shared_indptr[i + 1]), all of them in one, and shares shared_len[i].
+  int num_groups;
+  const int* shared_indptr;
+  const int* shared_len;
 };
 struct ChunkPlanOutput {
   std::vector<ChunkItem> items;
   std::vector<ChunkMerge> merges;
+  std::vector<SharedMerge> shared_merges;  // CHUNK_SHARED: in the place of merges
+  std::vector<SharedToken> tokens;         // CHUNK_SHARED
   long long partial_rows;
-  int form;                // ChunkForm: the kernel that the items are for
+  int form;                // ChunkForm: the kernel that the items are for, and CHUNK_SHARED
 };
 void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out);
 hipError_t launch_chunk_attention(const ChunkParams& p, int head_dim, int format, int form, int nitems, int nmerges,
                                   hipStream_t s);
+hipError_t launch_shared_attention(const ChunkParams& p, int head_dim, int format, int form, int nitems, int nmerges,
+                                   hipStream_t s);
 
 // ---- greedy acceptance walk (accept.hip) ----
 hipError_t launch_greedy_accept(const AcceptParams& p, bool bf16, hipStream_t s);

@@ -25,12 +25,14 @@ INCLUDE = ROOT.parent / "include"
 ARCH = "gfx950"
 # One object each; a source with parts is compiled once per part with the
 # part's definitions (verify_attention.hip: its kernels by head size and
-# waves per workgroup, and once without for the rest), so that the parts
-# build in parallel.
+# waves per workgroup, and once without for the rest; chunk_attention.hip: the
+# kernels of plans without and with shared keys), so that the parts build in
+# parallel.
 SOURCES = ["attention.hip", "verify_attention.hip", "kv_append.hip", "accept.hip", "qk_rope.hip", "tree_build.hip",
            "rotary.hip", "paged_cache.hip", "cache_append.hip", "chunk_attention.hip", "plan.cpp", "chunk_plan.cpp", "capi.cpp"]
 PARTS = {"verify_attention.hip": [{"D2SD_VERIFY_D": d, "D2SD_VERIFY_WAVES": w} for d in (128, 64) for w in (4, 2, 8, 1)]
-         + [{}]}
+         + [{}],
+         "chunk_attention.hip": [{}, {"D2SD_CHUNK_SHARED": 1}]}
 
 COMMON = ["-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", f"-I{INCLUDE}", f"-I{CSRC}"]
 # Device code: never let the compiler emit packed-fp32 VALU forms.

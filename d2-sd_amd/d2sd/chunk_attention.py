@@ -6,7 +6,9 @@ verify step under its tree mask.  A prompt's chunks and plain decoding steps
 are causal and write their keys first (PagedKVCache.write, quantised if the
 cache is): this operator reads keys and values from the cache only, for
 batches that mix chunks and single tokens, in every cache format, with a
-window that follows each token and attention sinks.
+window that follows each token and attention sinks.  Where groups of requests
+begin with the same tokens, plan() takes them and their keys are read and
+multiplied once for all rows of the group.
 
 plan() does the host work once for a batch's shape; run() launches one kernel,
 and a second that joins partial states where a request's keys were split.
@@ -18,7 +20,7 @@ may overlap on different streams.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -26,7 +28,7 @@ import torch
 from . import _lib
 from ._lib import check, lib
 from .graph import _CAPTURING, home_stream, keep_alive
-from .paged import KV_FORMATS, PagedBatch, PagedKVCache, _device
+from .paged import KV_FORMATS, PagedBatch, PagedKVCache, _device, _i32
 
 _attention, _attention_out = (torch.ops.d2sd.chunk_attention.default, torch.ops.d2sd.chunk_attention_out.default)
 
@@ -38,7 +40,9 @@ class PagedChunkAttention:
 
     def plan(self, batch: PagedBatch, num_qo_heads: int, num_kv_heads: int, head_dim: int, *, kv_format: str = "bf16",
              sm_scale: Optional[float] = None, window_left: int = -1, sinks: Optional[torch.Tensor] = None,
-             lse_base2: bool = False, max_splits: int = 0, num_cus: int = 0) -> "PagedChunkAttention":
+             lse_base2: bool = False, max_splits: int = 0, num_cus: int = 0,
+             shared_indptr: Optional[Sequence[int]] = None, shared_len: Optional[Sequence[int]] = None
+             ) -> "PagedChunkAttention":
         """Plans the batch (its kv_len_host, of its making or the last
         set_kv_len: the work is shared out for those lengths, and right for any
         within the requests' pages).
@@ -49,7 +53,16 @@ class PagedChunkAttention:
         be at least 2e-38 (over fp8 caches, times each k_scale too).  sinks [Hq] fp32 applies O *= sigmoid(lse - sink).  Rows
         that see no key (a request whose kv_len is below its new tokens) get
         output 0 and lse -inf.  A NaN or infinity in K or V reaches the rows
-        that see its token and no others."""
+        that see its token and no others.
+
+        Requests whose caches begin alike (a system prompt, a document):
+        requests shared_indptr[i] .. shared_indptr[i + 1] - 1 hold the same
+        tokens in their first shared_len[i] positions (0: none).  Those keys
+        are read once for all of them, through the first one's pages; the
+        others' pages of that range are not looked at.  shared_indptr starts at
+        0 and ends at the number of requests; a group's shared_len is any
+        number that its first request's pages hold.  The result is that of a
+        plan without groups, whatever lengths the caches have later."""
         if kv_format not in KV_FORMATS:
             raise ValueError(f"kv_format must be one of {sorted(KV_FORMATS)}")
         if self._want_device is not None and _device(self._want_device) != batch.device:
@@ -69,13 +82,25 @@ class PagedChunkAttention:
         desc.num_qo_heads, desc.num_kv_heads, desc.head_dim = num_qo_heads, num_kv_heads, head_dim
         desc.format, desc.page_size, desc.window_left = KV_FORMATS[kv_format], batch.page_size, window_left
         desc.num_cus, desc.max_splits = num_cus, max_splits
+        if (shared_indptr is None) != (shared_len is None):
+            raise ValueError("shared_indptr and shared_len go together")
+        groups, indptr, shared = 0, None, None
+        if shared_len is not None:
+            ip, n = _i32(shared_indptr), _i32(shared_len)
+            if ip.ndim != 1 or n.ndim != 1 or ip.size != n.size + 1:
+                raise ValueError("shared_indptr must have len(shared_len) + 1 entries")
+            groups, indptr, shared = n.size, as_p(ip), as_p(n)
+            if not groups and batch.num_reqs:
+                raise ValueError("shared_indptr must hold every request")
         info = _lib.ChunkPlanInfo()
         host = np.empty(1 << 16, dtype=np.int32)
+        plan = lambda: lib.d2sd_chunk_plan_shared(C.byref(desc), groups, indptr, shared, as_p(host), host.size,  # noqa: E731
+                                                  C.byref(info))
         with torch.cuda.device(batch.device) if batch.device.type == "cuda" else torch.no_grad():
-            rc = lib.d2sd_chunk_plan(C.byref(desc), as_p(host), host.size, C.byref(info))
+            rc = plan()
             if rc == _lib.D2SD_ERR_WORKSPACE and info.plan_ints > host.size:
                 host = np.empty(info.plan_ints, dtype=np.int32)
-                rc = lib.d2sd_chunk_plan(C.byref(desc), as_p(host), host.size, C.byref(info))
+                rc = plan()
         check(rc, "chunk_plan")
         self.info, self.batch, self.sinks = info, batch, sinks
         self.plan_host = host[:info.plan_ints]

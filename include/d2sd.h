@@ -702,6 +702,17 @@ typedef struct {
 
 int d2sd_chunk_plan(const d2sd_chunk_plan_desc* desc, int32_t* host_plan, size_t host_plan_ints,
                     d2sd_chunk_plan_info* info);
+/* The same for requests whose caches begin alike: group i, requests
+ * shared_indptr[i] .. shared_indptr[i + 1] - 1 (host [num_groups + 1], from 0 to
+ * num_reqs), holds the same tokens in its first shared_len[i] positions (host
+ * [num_groups]; any number that the first request's pages hold).  Keys and values
+ * of these are read through the first request's pages alone, once for the rows of
+ * the whole group; what a row sees, and the result, are those of d2sd_chunk_plan
+ * where the tokens are indeed the same.  Lengths stay free: a request may be cut
+ * back below what it shares. */
+int d2sd_chunk_plan_shared(const d2sd_chunk_plan_desc* desc, int num_groups, const int32_t* shared_indptr,
+                           const int32_t* shared_len, int32_t* host_plan, size_t host_plan_ints,
+                           d2sd_chunk_plan_info* info);
 
 typedef struct {
   d2sd_paged_cache cache;

@@ -1,0 +1,199 @@
+"""Host side of plans with shared keys: their work list, read as the kernels read
+it, gives every row each of its keys once, through the right pages, and every
+partial state to one merge; what a plan does not take is refused."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import d2sd
+from d2sd import _lib
+
+ITEM, MERGE, TOKEN = 16, 12, 4
+ALONE, SHARED, OWN = 0, 1, 2
+
+
+def plan(qo, kv, groups, prefix, hq=8, hkv=2, d=128, P=16, cus=256, splits=0, window=-1, fmt="bf16", extra=0):
+    """groups: requests of each; prefix: what each group shares."""
+    pi = np.concatenate([[0], np.cumsum([-(-(n + extra) // P) for n in kv])])
+    starts = np.concatenate([[0], np.cumsum(qo)])
+    b = d2sd.PagedBatch(starts, kv, pi, np.arange(max(int(pi[-1]), 1)), P, device="cpu")
+    a = d2sd.PagedChunkAttention("cpu").plan(b, hq, hkv, d, kv_format=fmt, num_cus=cus, max_splits=splits, window_left=window,
+                                             shared_indptr=np.concatenate([[0], np.cumsum(groups)]), shared_len=prefix)
+    return a, b
+
+
+def parts(a):
+    i, n, m = a.info, a.info.num_items * ITEM, a.info.num_merges * MERGE
+    h = a.plan_host
+    return (h[:n].reshape(-1, ITEM), h[n:n + m].reshape(-1, MERGE),
+            h[n + m:n + m + i.total_q * TOKEN].reshape(-1, TOKEN))
+
+
+def keys_of(item, tokens, kv, P, group, window, wave):
+    """Keys [from, to) that the item reads, as the kernels find them: (position of a row, first and last key)."""
+    req, kvh, q0, nq, row0, nrows, pb, pe, chunk, nchunks, slot, kind, part, bound = (int(x) for x in item[:14])
+    if part == SHARED:
+        pos = [min(kv[tokens[q0 + (row0 + i) // group][0]], tokens[q0 + (row0 + i) // group][2])
+               - tokens[q0 + (row0 + i) // group][1] for i in range(nrows)]
+        lo, hi = 0, bound
+        if window >= 0:
+            lo, hi = max(min(pos) - window, 0), min(bound, max(max(pos) + 1, 0))
+        see = [(max(p - window, 0) if window >= 0 else 0, min(p, bound - 1)) for p in pos]
+    else:
+        L = min(kv[req], (pe - pb) * P)
+        pos = [L - nq + (row0 + i) // group for i in range(nrows)]
+        lo = max(max(pos[0] - window, 0) if window >= 0 else 0, bound)
+        hi = max(pos[-1] + 1, 0)
+        see = [(max(max(p - window, 0) if window >= 0 else 0, bound), p) for p in pos]
+    if kind == 0:
+        n = max(hi - lo + 63, 0) >> 6
+        a, b = lo + 64 * (n * chunk // nchunks), min(lo + 64 * (n * (chunk + 1) // nchunks), hi)
+    else:
+        t0 = lo >> 5
+        n = ((hi + 31) >> 5) - t0 if hi > lo else 0
+        a, b = max(32 * (t0 + n * chunk // nchunks), lo), min(32 * (t0 + n * (chunk + 1) // nchunks), hi)
+    return a, b, see
+
+
+def check(a, b, qo, kv, groups, prefix, hkv, group, P, window, now=None):
+    items, merges, tokens = parts(a)
+    now = list(kv) if now is None else now
+    first = np.concatenate([[0], np.cumsum(groups)])
+    leader = {r: int(first[g]) for g in range(len(groups)) for r in range(first[g], first[g + 1])}
+    # (those of one request, or with nothing to share, read their own pages)
+    alone = {r: groups[g] < 2 or prefix[g] == 0 for g in range(len(groups)) for r in range(first[g], first[g + 1])}
+    starts = b.qo_indptr_host
+    seen = {}                # (row of q, head) -> keys and the request whose pages they come through
+    slots, written = {}, 0   # partial row -> (row of q, head)
+    direct = set()
+    for it in items:
+        req, kvh, q0, nq, row0, nrows, pb, pe, chunk, nchunks, slot, kind, part, bound = (int(x) for x in it[:14])
+        assert (pb, pe) == (b.page_indptr_host[req], b.page_indptr_host[req + 1]) and nrows > 0
+        lo, hi, see = keys_of(it, tokens, now, P, group, window, kind)
+        for i in range(nrows):
+            row = (q0 + (row0 + i) // group, kvh * group + (row0 + i) % group)
+            mine = seen.setdefault(row, [])
+            mine += [(k, req if part == SHARED else req) for k in range(max(lo, see[i][0]), min(hi, see[i][1] + 1))]
+            if part != ALONE or nchunks > 1:
+                at = slot + chunk * nrows + i
+                assert at not in slots
+                slots[at] = row
+            else:
+                assert row not in direct
+                direct.add(row)
+    assert not slots or (min(slots) == 0 and max(slots) == len(slots) - 1)
+    assert len(slots) * (a.head_dim + 1) * 4 == a.info.workspace_bytes
+    assert a.info.plan_ints == items.size + merges.size + (tokens.size if a.info.form & 8 else 0)
+    for r in range(len(qo)):
+        for t in range(qo[r]):
+            pos = min(now[r], int(b.page_indptr_host[r + 1] - b.page_indptr_host[r]) * P) - qo[r] + t
+            bound = 0 if alone[r] else prefix[int(np.searchsorted(first, r, side="right")) - 1]
+            want = [(k, leader[r] if k < bound else r) for k in range(max(pos - window, 0) if window >= 0 else 0, pos + 1)]
+            for h in range(hkv * group):
+                assert sorted(seen.get((int(starts[r]) + t, h), [])) == want, (r, t, h)
+    if not a.info.form & 8:
+        return
+    left = set(slots)
+    for q0, kvh, row0, nrows, slot, stride, n, s2, stride2, n2, _, _ in merges.tolist():
+        assert 0 < nrows <= 1024 // a.head_dim
+        for i in range(nrows):
+            row = (q0 + (row0 + i) // group, kvh * group + (row0 + i) % group)
+            for c in range(n):
+                assert slots[slot + i + c * stride] == row
+                left.remove(slot + i + c * stride)
+            for c in range(n2):
+                assert slots[s2 + i + c * stride2] == row
+                left.remove(s2 + i + c * stride2)
+            assert row not in direct
+            direct.add(row)
+    assert not left and len(direct) == sum(qo) * hkv * group
+
+
+CASES = [
+    # requests' new tokens, lengths, groups, what they share
+    ([1, 1, 1, 1], [70, 90, 65, 200], [4], [64]),
+    ([1] * 9, [300 + 7 * i for i in range(9)], [9], [290]),
+    ([1, 5, 0, 2, 40, 1], [40, 60, 30, 33, 90, 17], [4, 1, 1], [30, 50, 0]),
+    ([3, 40, 9, 1, 2], [100, 140, 109, 101, 33], [2, 2, 1], [97, 16, 20]),
+    ([2, 2, 2], [50, 60, 70], [0, 3, 0], [5, 50, 0]),
+    ([100, 60, 1], [164, 124, 65], [3], [64]),
+    ([0, 0], [50, 50], [2], [50]),
+    ([1, 1], [20, 20], [2], [20]),       # the new tokens among what is shared
+    ([2, 2], [20, 8], [2], [20]),        # one cut back below it
+]
+
+
+@pytest.mark.parametrize("case", CASES)
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (8, 1, 64), (3, 3, 64), (20, 1, 128)])
+@pytest.mark.parametrize("cus,splits", [(256, 0), (4096, 0), (256, 1), (8, 5)])
+@pytest.mark.parametrize("window", [-1, 0, 30, 77])
+def test_every_row_gets_its_keys_once(case, hq, hkv, d, cus, splits, window):
+    qo, kv, groups, prefix = case
+    a, b = plan(qo, kv, groups, prefix, hq, hkv, d, cus=cus, splits=splits, window=window)
+    check(a, b, qo, kv, groups, prefix, hkv, hq // hkv, 16, a.info.window_left)
+    # other lengths later, with the same plan
+    for now in ([max(n - 25, 0) for n in kv], [0] * len(kv), [-(-n // 16) * 16 for n in kv]):
+        check(a, b, qo, kv, groups, prefix, hkv, hq // hkv, 16, a.info.window_left, now)
+
+
+def test_random_plans():
+    rng = np.random.default_rng(0)
+    for _ in range(60):
+        n = int(rng.integers(1, 9))
+        cuts = np.sort(rng.integers(0, n + 1, int(rng.integers(0, 3))))
+        groups = np.diff(np.concatenate([[0], cuts, [n]])).tolist()
+        kv = rng.integers(1, 300, n).tolist()
+        qo = [int(min(k, rng.choice([0, 1, 1, 3, 50]))) for k in kv]
+        first = np.concatenate([[0], np.cumsum(groups)])
+        prefix = [int(rng.integers(0, kv[first[i]] + 1)) if g else 3 for i, g in enumerate(groups)]
+        hq, hkv = [(8, 2), (4, 4), (7, 1)][int(rng.integers(3))]
+        P = int(rng.choice([1, 16, 64]))
+        window = int(rng.choice([-1, -1, 50]))
+        a, b = plan(qo, kv, groups, prefix, hq, hkv, int(rng.choice([64, 128])), P, int(rng.choice([8, 256])), window=window)
+        check(a, b, qo, kv, groups, prefix, hkv, hq // hkv, P, a.info.window_left)
+
+
+def test_groups_without_a_shared_key_change_nothing():
+    qo, kv = [1, 30, 2], [500, 700, 90]
+    for groups, prefix in (([1, 1, 1], [5, 5, 5]), ([3], [0]), ([0, 3], [7, 0])):
+        a, _ = plan(qo, kv, groups, prefix)
+        b = d2sd.PagedChunkAttention("cpu").plan(a.batch, 8, 2, 128, num_cus=256)
+        assert np.array_equal(a.plan_host, b.plan_host) and bytes(a.info) == bytes(b.info)
+
+
+@pytest.mark.parametrize("groups,prefix,error", [
+    ([3, 1], [10, 10], RuntimeError), ([1], [10], RuntimeError), ([2, -1, 1], [1, 1, 1], RuntimeError),
+    ([3, -1], [1, 1], RuntimeError), ([2], [-1], RuntimeError), ([2], [49], RuntimeError), ([], [], ValueError),
+    ([2], [1, 1], ValueError), ([2], [2 ** 40], ValueError)])
+def test_refusals(groups, prefix, error):
+    with pytest.raises(error):
+        plan([1, 1], [40, 200], groups, prefix)
+
+
+def test_groups_and_lengths_go_together():
+    b = d2sd.PagedBatch([0, 1], [3], [0, 1], [0], 16, device="cpu")
+    for kw in (dict(shared_indptr=[0, 1]), dict(shared_len=[3])):
+        with pytest.raises(ValueError):
+            d2sd.PagedChunkAttention("cpu").plan(b, 8, 2, 128, **kw)
+    e = d2sd.PagedBatch([0], [], [0], [0], 16, device="cpu")
+    a = d2sd.PagedChunkAttention("cpu").plan(e, 8, 2, 128, num_cus=8, shared_indptr=[0], shared_len=[])
+    assert a.info.num_items == 0
+
+
+def test_c_entry_refuses_null_groups():
+    b = d2sd.PagedBatch([0, 1, 2], [3, 3], [0, 1, 2], [0, 1], 16, device="cpu")
+    as_p = lambda x: x.ctypes.data_as(C.POINTER(C.c_int32))  # noqa: E731
+    desc = _lib.ChunkPlanDesc()
+    desc.num_reqs, desc.num_qo_heads, desc.num_kv_heads, desc.head_dim, desc.page_size = 2, 8, 2, 128, 16
+    desc.qo_indptr, desc.kv_len, desc.page_indptr = as_p(b.qo_indptr_host), as_p(b.kv_len_host), as_p(b.page_indptr_host)
+    desc.window_left, desc.num_cus = -1, 8
+    info = _lib.ChunkPlanInfo()
+    ip, n = np.array([0, 2], dtype=np.int32), np.array([3], dtype=np.int32)
+    fn = _lib.lib.d2sd_chunk_plan_shared
+    assert fn(C.byref(desc), 1, as_p(ip), as_p(n), None, 0, C.byref(info)) == 0 and info.form & 8
+    for args in ((1, None, as_p(n)), (1, as_p(ip), None), (-1, as_p(ip), as_p(n))):
+        assert fn(C.byref(desc), *args, None, 0, C.byref(info)) != 0
+        assert b"chunk_plan" in _lib.lib.d2sd_last_error()
+    host = np.empty(8, dtype=np.int32)  # too small: refused before anything is written
+    assert fn(C.byref(desc), 1, as_p(ip), as_p(n), as_p(host), 8, C.byref(info)) == _lib.D2SD_ERR_WORKSPACE
