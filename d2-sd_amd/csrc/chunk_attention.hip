@@ -152,7 +152,7 @@ __device__ __forceinline__ Span rows_span(const ChunkParams& p, const ChunkItem&
   }
   first = wave_min(first);
   const int last = -wave_min(past);
-  s.all_hi = min(w.bound, first + 1);
+  s.all_lo = 0, s.all_hi = min(w.bound, first + 1);
   if (p.window_left >= 0) {
     s.hi = min(w.bound, max(last + 1, 0));
     s.lo = max(first - p.window_left, 0);
@@ -183,6 +183,28 @@ __device__ __forceinline__ int row_pos(const ChunkParams& p, const ChunkItem& w,
 template <bool SHARED>
 __device__ __forceinline__ bool is_partial(const ChunkItem& w) {
   return w.nchunks > 1 || (SHARED && w.part != PART_ALONE);
+}
+
+// Partial states of a wave's 32 rows over shared keys are stored as the registers
+// hold them (lane hh * 32 + row has dims 32 mt + 8 q + 4 hh .. + 3 of its row), 1 KB
+// a store: by rows a store would touch 32 lines.  Blocks of 32 rows follow each
+// other, then chunks.
+template <int D>
+__device__ __forceinline__ long long image_at(long long row0, int d4, int row) {
+  return row0 * D + (((d4 >> 1) * 64 + (d4 & 1) * 32 + row) << 2);  // row0: the block's first
+}
+template <int D>
+__device__ __forceinline__ void store_image(const ChunkParams& p, const ChunkItem& w, const f32x16 (&o)[D / 32], float inv,
+                                            float lse2, int wrow, int l32, int hh) {
+  if (wrow + l32 >= w.nrows) return;
+  const long long row0 = w.slot + (long long)w.chunk * ((w.nrows + 31) & ~31) + wrow;
+#pragma unroll
+  for (int mt = 0; mt < D / 32; ++mt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *(f32x4*)(p.part_o + image_at<D>(row0, 8 * mt + 2 * q + hh, l32)) =
+          (f32x4){o[mt][4 * q] * inv, o[mt][4 * q + 1] * inv, o[mt][4 * q + 2] * inv, o[mt][4 * q + 3] * inv};
+  if (hh == 0) p.part_lse[row0 + l32] = lse2;
 }
 
 // Online softmax of 16 * N scores of this lane's row: the running maximum m (raw
@@ -669,6 +691,12 @@ __device__ __forceinline__ void tile_item(const ChunkParams& p, const ChunkItem&
   const float lse2 = l > 0.f ? m * c + __builtin_amdgcn_logf(l) : l == 0.f ? -INFINITY : l;
   float inv = l != 0.f ? vscale / l : 0.f;
   const bool mine = wrow + l32 < w.nrows;
+  if constexpr (SHARED) {
+    if (w.part == PART_SHARED) {
+      store_image<D>(p, w, o, inv, lse2, wrow, l32, hh);
+      return;
+    }
+  }
   if (is_partial<SHARED>(w)) {
     if (!mine) return;
     const long long pr = w.slot + (long long)w.chunk * w.nrows + row;
@@ -705,8 +733,11 @@ __device__ __forceinline__ T load_kv(const T* p) {
   return *p;
 }
 
-template <int D, int FMT, int W, int RB, int PF, bool STREAM, bool SHARED>
+// SOLO (plans with shared keys): each wave of the workgroup has rows or keys of its
+// own, w is the wave's, and its state goes out as it is.
+template <int D, int FMT, int W, int RB, int PF, bool STREAM, bool SHARED, bool SOLO = false>
 __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem& w, lds_char* lds, float* stats) {
+  constexpr int TW = SOLO ? 1 : W;  // waves that share the item's tiles
   constexpr int MT = D / 16, KS = D / 32, ROW = Format<D, FMT>::ROW;
   constexpr bool MX = Format<D, FMT>::MX;
   constexpr int NK = ROW / 64;                  // 16-byte pieces of a lane's quarter of a key row
@@ -845,13 +876,13 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
 
   auto step = [&](Raw& x, int t, auto by_key) {
     constexpr bool BY_KEY = decltype(by_key)::value;
-    const int tn = t + PF * W;  // the tile that takes these registers next
+    const int tn = t + PF * TW;  // the tile that takes these registers next
     // (page ids are loaded a round before the rows they lead to: the wait for
     // one is a wait for every load before it)
     unsigned pg = 0;
     if constexpr (!BY_KEY) {
       pg = min(x.next, last_page);
-      x.next = page_at(key_at(tn + PF * W, lane & 31));
+      x.next = page_at(key_at(tn + PF * TW, lane & 31));
     }
     f32x4 s[RB][2];
 #pragma unroll
@@ -960,28 +991,28 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
 
-  const int t0 = tb + __builtin_amdgcn_readfirstlane(wv);
+  const int t0 = tb + (SOLO ? 0 : __builtin_amdgcn_readfirstlane(wv));
   unsigned pages[PF];
 #pragma unroll
   for (int i = 0; i < PF; ++i) {
     // (keys past the range are clamped to its last one; an item without keys loads nothing)
     if (te > tb) {
-      raw[i].next = page_at(key_at(t0 + (PF + i) * W, lane & 31));
-      pages[i] = page_at(key_at(t0 + i * W, lane & 31));
+      raw[i].next = page_at(key_at(t0 + (PF + i) * TW, lane & 31));
+      pages[i] = page_at(key_at(t0 + i * TW, lane & 31));
     }
   }
 #pragma unroll
   for (int i = 0; i < PF; ++i) {
-    const int t = t0 + i * W;
+    const int t = t0 + i * TW;
     if (t < te) {
       const unsigned pg = min(pages[i], last_page);
       fetch(raw[i], t, pg);
     }
   }
-  for (int t = t0; t < te; t += PF * W) {
+  for (int t = t0; t < te; t += PF * TW) {
 #pragma unroll
     for (int i = 0; i < PF; ++i)
-      if (t + i * W < te) step(raw[i], t + i * W, std::false_type{});
+      if (t + i * TW < te) step(raw[i], t + i * TW, std::false_type{});
   }
   if (all.lo < all.all_lo || all.hi > all.all_hi) {
     float zero = 0.f;  // (NaN once a sum is not finite)
@@ -999,12 +1030,39 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
         m[rb] = -INFINITY, l[rb] = 0.f;
       }
 #pragma unroll 1
-      for (int t = t0; t < te; t += W) {
+      for (int t = t0; t < te; t += TW) {
         const unsigned pg = min(page_at(key_at(t, lane & 31)), last_page);
         fetch(raw[0], t, pg);
         step(raw[0], t, std::true_type{});
       }
     }
+  }
+
+  if constexpr (SOLO) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const int row = 16 * rb + l16;
+      const float sum = over_row(l[rb], [](float u, float v) { return u + v; });
+      const float lse2 = sum > 0.f ? m[rb] * c + __builtin_amdgcn_logf(sum) : sum == 0.f ? -INFINITY : sum;
+      float inv = sum != 0.f ? vscale / sum : 0.f;
+      if (row >= w.nrows) continue;
+      if (is_partial<SHARED>(w)) {
+        const long long pr = w.slot + (long long)w.chunk * w.nrows + row;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) *(f32x4*)(p.part_o + pr * D + 16 * mt + 4 * g4) = o[rb][mt] * inv;
+        if (g4 == 0) p.part_lse[pr] = lse2;
+      } else {
+        const RowOut at(p, w, row);
+        inv *= sink_factor(p, at.head, lse2);
+        bf16_t* op = (bf16_t*)p.o + (long long)at.token * p.o_stride_n + (long long)at.head * p.o_stride_h + 4 * g4;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          *(u32x2*)(op + 16 * mt) = (u32x2){pack_bf16x2(o[rb][mt][0] * inv, o[rb][mt][1] * inv),
+                                            pack_bf16x2(o[rb][mt][2] * inv, o[rb][mt][3] * inv)};
+        if (g4 == 0) p.lse[at.token * p.lse_stride_n + at.head] = p.lse_base2 ? lse2 : lse2 * kLn2;
+      }
+    }
+    return;
   }
 
   // join the waves' states through LDS
@@ -1064,6 +1122,10 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
   }
 }
 
+#ifdef D2SD_CHUNK_SHARED
+#include "shared_tile.h"
+#endif
+
 // Tiles of 32 keys a wave of a token item has in flight (more than one does
 // not help bf16, whose tiles are 16 KB)
 template <int FMT>
@@ -1081,25 +1143,75 @@ template <int D, int FMT, int FORM, bool SHARED>
 __device__ __forceinline__ void chunk_work(const ChunkParams& p) {
   constexpr int W = chunk_waves(FORM);
   constexpr bool TOKENS = FORM >= CHUNK_TOKENS;
-  __shared__ __align__(16) char lds[TOKENS ? W * 32 * D * 2 : 4 * 64 * D * 2];
-  __shared__ float stats[2 * W * kTokenRows];
+  constexpr int VALUES = W * 32 * D * 2, STATS = 2 * W * kTokenRows * 4;  // of token items
+#ifdef D2SD_CHUNK_SHARED
+  constexpr int TILES = SharedRing<D, FMT, W>::bytes;
+#else
+  constexpr int TILES = 4 * 64 * D * 2;
+#endif
+  __shared__ __align__(16) char lds[TOKENS || VALUES + STATS > TILES ? VALUES + STATS : TILES];
+  float* const stats = (float*)(lds + VALUES);
   const ChunkItem w = p.items[blockIdx.x];
   if constexpr (TOKENS) {
     token_item<D, FMT, W, 1, token_depth<FMT>(), FORM == CHUNK_STREAM, SHARED>(p, w, (lds_char*)lds, stats);
   } else {
-    if (w.kind == CHUNK_TILE)
+    if (w.kind == CHUNK_TILE) {
+#ifdef D2SD_CHUNK_SHARED
+      if (w.part == PART_SHARED) {
+        auto chunk_of = [&](int lo, int hi, int& from, int& to) {
+          const int ntiles = max(hi - lo + 63, 0) >> 6;
+          from = lo + 64 * (int)((long long)ntiles * w.chunk / w.nchunks);
+          to = min(lo + 64 * (int)((long long)ntiles * (w.chunk + 1) / w.nchunks), hi);
+        };
+        int from, to;
+        if (p.window_left < 0 && w.heads > 0 && shared_tile_takes<D, FMT, W>(p, 0)) {
+          // The usual case, taken for granted: every row sees all shared keys, that is
+          // no cache of the rows' requests is cut back to less than bound + back - 1.
+          // The lengths are looked at last, so that the first keys do not wait for them.
+          const int lane = threadIdx.x & 63;
+          const int len = lane < w.heads ? p.kv_len[w.nq + lane] : 0x7FFFFFFF;
+          chunk_of(0, w.bound, from, to);
+          if (from < to) {
+            shared_tile<D, FMT, W>(p, w, (lds_char*)lds, from, to);
+            if (!__any(len < to + w.back - 1)) return;
+            __syncthreads();  // (the tiles: all waves are done with them)
+          }
+        } else {
+          const Span all = rows_span<true>(p, w, 0, w.nrows - 1);
+          chunk_of(all.lo, all.hi, from, to);
+          if (from < to && from >= all.all_lo && to <= all.all_hi && shared_tile_takes<D, FMT, W>(p, from)) {
+            shared_tile<D, FMT, W>(p, w, (lds_char*)lds, from, to);
+            return;
+          }
+        }
+      }
+#endif
       tile_item<D, FMT, W, SHARED>(p, w, (lds_char*)lds);
-    else if (w.nrows <= 16)
-      token_item<D, FMT, W, 1, token_depth<FMT>(), FORM == CHUNK_STREAM, SHARED>(p, w, (lds_char*)lds, stats);
-    else
-      token_item<D, FMT, W, 2, 1, false, SHARED>(p, w, (lds_char*)lds, stats);
+      return;
+    }
+    if constexpr (SHARED) {
+      // wave wv takes unit kvh + wv of the request's chunks x heads
+      ChunkItem u = w;
+      const int unit = __builtin_amdgcn_readfirstlane(w.kvh + (threadIdx.x >> 6));
+      if (unit >= w.heads * w.nchunks) return;
+      u.chunk = unit / w.heads;
+      u.kvh = unit - u.chunk * w.heads;
+      u.slot = w.slot + u.kvh * w.nchunks * w.nrows;
+      if (w.nrows <= 16)
+        token_item<D, FMT, W, 1, token_depth<FMT>(), false, true, true>(p, u, (lds_char*)lds, stats);
+      else
+        token_item<D, FMT, W, 2, 1, false, true, true>(p, u, (lds_char*)lds, stats);
+    } else if (w.nrows <= 16) {
+      token_item<D, FMT, W, 1, token_depth<FMT>(), FORM == CHUNK_STREAM, false>(p, w, (lds_char*)lds, stats);
+    } else {
+      token_item<D, FMT, W, 2, 1, false, false>(p, w, (lds_char*)lds, stats);
+    }
   }
 }
 
 // (This file is compiled twice: its kernels for plans without and with shared keys.)
 #ifndef D2SD_CHUNK_SHARED
 #define ATTN_KERNEL chunk_attn_kernel
-#define MERGE_KERNEL chunk_merge_kernel
 #define LAUNCH launch_chunk_attention
 template <int D, int FMT, int FORM>
 __global__ __launch_bounds__(64 * chunk_waves(FORM), (chunk_occupancy<D, FMT, FORM>())) void
@@ -1108,23 +1220,24 @@ chunk_attn_kernel(const ChunkParams p) {
 }
 #else
 #define ATTN_KERNEL shared_attn_kernel
-#define MERGE_KERNEL shared_merge_kernel
 #define LAUNCH launch_shared_attention
 template <int D, int FMT, int FORM>
-__global__ __launch_bounds__(64 * chunk_waves(FORM), (chunk_occupancy<D, FMT, FORM>())) void
+__global__ __launch_bounds__(64 * chunk_waves(FORM), (FORM < CHUNK_TOKENS ? 2 : chunk_occupancy<D, FMT, FORM>())) void
 shared_attn_kernel(const ChunkParams p) {
   chunk_work<D, FMT, FORM, true>(p);
 }
 #endif
 
 // Row i of a merge item from its partial states, nchunks of them, then (SHARED)
-// those over the keys that it shares: thread (i, d4) holds head dims 4 d4 .. 4 d4 +
-// 3.  Latency bound: the sums and states of eight chunks are read at once (one
+// those over the keys that it shares (IMAGE: as store_image left them): thread (i,
+// d4) holds head dims 4 d4 .. 4 d4 + 3; of the images eight rows lie side by side.  Latency bound: the sums and states of eight chunks are read at once (one
 // token over 8 chunks: 3.8 -> 3.0 us against sums first), joined in chunk order
 // whatever the order they were written in.
-template <int D, bool SHARED, typename Merge>
+template <int D, bool SHARED, bool IMAGE, typename Merge>
 __device__ __forceinline__ void merge_rows(const ChunkParams& p, const Merge& w) {
-  const int i = threadIdx.x / (D / 4), dd = 4 * (threadIdx.x % (D / 4));
+  constexpr int ROWS = 1024 / D;
+  const int i = SHARED ? threadIdx.x % ROWS : threadIdx.x / (D / 4);
+  const int dd = 4 * (SHARED ? threadIdx.x / ROWS : threadIdx.x % (D / 4));
   if (i >= w.nrows) return;
   constexpr int B = 8;
   float top = -INFINITY, sum = 0.f;
@@ -1138,10 +1251,15 @@ __device__ __forceinline__ void merge_rows(const ChunkParams& p, const Merge& w)
     for (int u = 0; u < B; ++u) {
       const int c = min(c0 + u, nchunks - 1);
       long long pr = w.slot + i + (long long)c * w.stride;
+      long long at = pr * D + dd;
       if constexpr (SHARED)
-        if (c >= w.nchunks) pr = w.shared_slot + i + (long long)(c - w.nchunks) * w.shared_stride;
+        if (c >= w.nchunks) {
+          const int row = w.shared_row + i;
+          pr = w.shared_slot + row + (long long)(c - w.nchunks) * w.shared_stride;
+          at = IMAGE ? image_at<D>(pr - (row & 31), dd / 4, row & 31) : pr * D + dd;
+        }
       s[u] = c0 + u < nchunks ? p.part_lse[pr] : -INFINITY;
-      v[u] = *(const f32x4*)(p.part_o + pr * D + dd);
+      v[u] = *(const f32x4*)(p.part_o + at);
     }
     float mx = top;
 #pragma unroll
@@ -1174,12 +1292,12 @@ __device__ __forceinline__ void merge_rows(const ChunkParams& p, const Merge& w)
 #ifndef D2SD_CHUNK_SHARED
 template <int D>
 __global__ __launch_bounds__(256) void chunk_merge_kernel(const ChunkParams p) {
-  merge_rows<D, false>(p, p.merges[blockIdx.x]);
+  merge_rows<D, false, false>(p, p.merges[blockIdx.x]);
 }
 #else
-template <int D>
+template <int D, bool IMAGE>
 __global__ __launch_bounds__(256) void shared_merge_kernel(const ChunkParams p) {
-  merge_rows<D, true>(p, ((const SharedMerge*)p.merges)[blockIdx.x]);
+  merge_rows<D, true, IMAGE>(p, ((const SharedMerge*)p.merges)[blockIdx.x]);
 }
 #endif
 
@@ -1191,6 +1309,10 @@ hipError_t launch_f(const ChunkParams& p, int form, int nitems, int nmerges, hip
   } else if (form == CHUNK_STREAM) {
     hipLaunchKernelGGL((ATTN_KERNEL<D, FMT, CHUNK_STREAM>), grid, block, 0, s, p);
   } else if (form == CHUNK_WAVES4) {
+#ifdef D2SD_CHUNK_SHARED
+    if constexpr (!shared_waves4(D, FMT)) return hipErrorInvalidValue;
+    else
+#endif
     hipLaunchKernelGGL((ATTN_KERNEL<D, FMT, CHUNK_WAVES4>), grid, block, 0, s, p);
   } else {
     if constexpr (D == 64) return hipErrorInvalidValue;  // (the planner gives heads of 64 four waves)
@@ -1198,7 +1320,15 @@ hipError_t launch_f(const ChunkParams& p, int form, int nitems, int nmerges, hip
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (nmerges > 0) hipLaunchKernelGGL(MERGE_KERNEL<D>, dim3((unsigned)nmerges), dim3(256), 0, s, p);
+  if (nmerges <= 0) return hipSuccess;
+#ifdef D2SD_CHUNK_SHARED
+  if (form >= CHUNK_TOKENS)
+    hipLaunchKernelGGL((shared_merge_kernel<D, false>), dim3((unsigned)nmerges), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((shared_merge_kernel<D, true>), dim3((unsigned)nmerges), dim3(256), 0, s, p);
+#else
+  hipLaunchKernelGGL(chunk_merge_kernel<D>, dim3((unsigned)nmerges), dim3(256), 0, s, p);
+#endif
   return hipGetLastError();
 }
 

@@ -41,6 +41,32 @@ struct Rows {
   int bound;            // keys [0, bound) are shared
 };
 
+// Keys [lo, hi) that packed rows [row0, row0 + nrows) of a set see.  req: of shared
+// keys, a request at or before that of the first row (moved on to it).
+void seen_keys(const ChunkPlanInput& in, const Rows& set, int group, long long row0, int nrows, int& req, long long& lo,
+               long long& hi) {
+  if (set.part == PART_SHARED) {
+    lo = 0, hi = set.bound;
+    if (in.window_left < 0) return;
+    const int t0 = set.q0 + (int)(row0 / group), t1 = set.q0 + (int)((row0 + nrows - 1) / group);
+    while (in.qo_indptr[req + 1] <= t0) ++req;
+    long long first = 1ll << 40, last = -1;
+    for (int r = req; r < set.last_req && in.qo_indptr[r] <= t1; ++r) {
+      if (in.qo_indptr[r + 1] <= std::max(in.qo_indptr[r], t0)) continue;
+      const long long end = (long long)in.kv_len[r] - in.qo_indptr[r + 1];
+      first = std::min(first, end + std::max(in.qo_indptr[r], t0));
+      last = std::max(last, end + std::min(in.qo_indptr[r + 1] - 1, t1));
+    }
+    lo = std::max(first - in.window_left, 0ll);
+    hi = std::min<long long>(set.bound, std::max(last + 1, 0ll));
+    return;
+  }
+  const long long pos0 = (long long)in.kv_len[set.req] - set.nq;
+  const long long first = pos0 + row0 / group, last = pos0 + (row0 + nrows - 1) / group;
+  hi = std::max(last + 1, 0ll);
+  lo = std::max<long long>(in.window_left >= 0 ? std::max(first - in.window_left, 0ll) : 0, set.bound);
+}
+
 struct Group {         // one row tile of a request, for every kv head
   int rows;            // index of its Rows
   int row0, nrows, kind;
@@ -158,28 +184,7 @@ struct Planner {
         g.kind = kind;
         g.partial = set.part != PART_ALONE;
         long long lo, hi;
-        if (set.part == PART_SHARED) {
-          lo = 0, hi = set.bound;
-          if (in.window_left >= 0) {
-            // the first and last key that some token of the tile sees
-            const int t0 = set.q0 + (int)(row0 / group), t1 = set.q0 + (int)((row0 + g.nrows - 1) / group);
-            while (in.qo_indptr[req + 1] <= t0) ++req;
-            long long first = 1ll << 40, last = -1;
-            for (int r = req; r < set.last_req && in.qo_indptr[r] <= t1; ++r) {
-              if (in.qo_indptr[r + 1] <= std::max(in.qo_indptr[r], t0)) continue;
-              const long long end = (long long)in.kv_len[r] - in.qo_indptr[r + 1];
-              first = std::min(first, end + std::max(in.qo_indptr[r], t0));
-              last = std::max(last, end + std::min(in.qo_indptr[r + 1] - 1, t1));
-            }
-            lo = std::max(first - in.window_left, 0ll);
-            hi = std::min<long long>(set.bound, std::max(last + 1, 0ll));
-          }
-        } else {
-          const long long pos0 = (long long)in.kv_len[set.req] - set.nq;
-          const long long first = pos0 + row0 / group, last = pos0 + (row0 + g.nrows - 1) / group;
-          hi = std::max(last + 1, 0ll);
-          lo = std::max<long long>(in.window_left >= 0 ? std::max(first - in.window_left, 0ll) : 0, set.bound);
-        }
+        seen_keys(in, set, group, row0, g.nrows, req, lo, hi);
         // (a tile item's tiles start at its first key, a token item's at multiples)
         const long long from = kind == CHUNK_TOKEN ? lo / keys_per_unit * keys_per_unit : lo;
         g.units = hi > lo ? (int)((hi - from + keys_per_unit - 1) / keys_per_unit) : 0;
@@ -224,6 +229,260 @@ struct Planner {
   }
 };
 
+// Workgroup items and merges of plans with shared keys for workgroups of `form`'s
+// waves: group i in chunks[i] chunks of keys.
+struct SharedGroup {
+  int rows, row0, nrows, kind;
+  int units;    // 64-key tiles (CHUNK_TILE) or 32-key tiles
+  int chunks;
+};
+
+// ---- plans with shared keys (but for those of a few rows, which stay above) ----
+// Row tiles of a group's rows over the shared keys (tile items, whatever their rows),
+// and each request's own keys: tile items where it brings more than 32 rows, else
+// units of one wave (a request, kv head and chunk of keys each), which fill
+// workgroups of as many waves.
+constexpr double kSharedItemUs = 6.0, kWaveItemUs = 6.0, kWaveTileUs = 1.3;  // a workgroup's start and end; a 32-key tile of a wave
+constexpr double kPartialBytes = 1.8e6;  // partial states written and read, per us
+
+struct SharedPlanner {
+  const ChunkPlanInput& in;
+  const std::vector<Rows>& rows_list;
+  int form, waves, per_cu;
+  std::vector<SharedGroup> groups;
+  double tile_limit, wave_limit;  // longest chunks, in tiles
+  double own_bytes, shared_bytes; // of the keys and values
+  int most_units, most_own;       // tiles of the longest tile item, of the longest wave's
+
+  SharedPlanner(const ChunkPlanInput& input, const std::vector<Rows>& rows, int f) : in(input), rows_list(rows), form(f) {
+    waves = chunk_waves(form);
+    per_cu = form == CHUNK_WAVES8 ? 1 : 2;
+    const int group = in.num_qo_heads / in.num_kv_heads;
+    for (int at = 0; at < (int)rows_list.size(); ++at) {
+      const Rows& set = rows_list[at];
+      const long long rows = (long long)set.nq * group;
+      const int kind = set.part == PART_SHARED || rows > kTokenRows ? CHUNK_TILE : CHUNK_TOKEN;
+      const int step = kind == CHUNK_TOKEN ? kTokenRows : chunk_rows(form), keys = kind == CHUNK_TOKEN ? 32 : 64;
+      int req = set.req;
+      for (long long row0 = 0; row0 < rows; row0 += step) {
+        SharedGroup g{at, (int)row0, (int)std::min<long long>(step, rows - row0), kind, 0, 1};
+        long long lo, hi;
+        seen_keys(in, set, group, row0, g.nrows, req, lo, hi);
+        const long long from = kind == CHUNK_TOKEN ? lo / keys * keys : lo;
+        g.units = hi > lo ? (int)((hi - from + keys - 1) / keys) : 0;
+        groups.push_back(g);
+      }
+    }
+    own_bytes = shared_bytes = 0.0;
+    most_units = most_own = 0;
+    for (const SharedGroup& g : groups) {
+      const bool over_shared = rows_list[g.rows].part == PART_SHARED;
+      // (row tiles of a set read the same keys, from L2 but for the first)
+      if (g.row0 == 0 || !over_shared)
+        (over_shared ? shared_bytes : own_bytes) +=
+            2.0 * (g.kind == CHUNK_TILE ? 64 : 32) * g.units * row_bytes(in.format, in.head_dim) * in.num_kv_heads;
+      if (g.kind == CHUNK_TILE) most_units = std::max(most_units, g.units);
+      else most_own = std::max(most_own, g.units);
+    }
+  }
+
+  void take(SharedPlanner&& other) {
+    form = other.form;
+    waves = other.waves;
+    groups = std::move(other.groups);
+  }
+
+  int chunks_of(const SharedGroup& g, double tiles, double own) const {
+    const int most = in.max_splits > 0 ? std::min(in.max_splits, kChunkMaxSplits) : kChunkMaxSplits;
+    return std::max(1, std::min(most, (int)std::ceil(g.units / (g.kind == CHUNK_TILE ? tiles : own) - 1e-6)));
+  }
+
+  // Time until the last workgroup ends, those of tile items first, the longest before
+  // the others, and the merge of the partial states.
+  double span(double tile_limit, double own_limit) const {
+    std::vector<std::pair<double, int>> tiles, solo;
+    double partial = 0.0;
+    long long count = 0;
+    for (const SharedGroup& g : groups)
+      if (g.kind == CHUNK_TILE) count += (long long)chunks_of(g, tile_limit, own_limit) * in.num_kv_heads;
+    const bool alone = per_cu == 1 || count <= in.num_cus;
+    const int own_rows = chunk_rows(form);
+    for (const SharedGroup& g : groups) {
+      const int n = chunks_of(g, tile_limit, own_limit);
+      const bool over_shared = rows_list[g.rows].part == PART_SHARED;
+      if (n > 1 || rows_list[g.rows].part != PART_ALONE) partial += (double)n * g.nrows * in.num_kv_heads * in.head_dim * 4.0;
+      if (g.kind == CHUNK_TILE)
+        tiles.push_back({kSharedItemUs + (double)g.units / n * step_us(over_shared, alone, g.nrows * 2 > own_rows), n * in.num_kv_heads});
+      else
+        solo.push_back({kWaveItemUs + (double)g.units / n * kWaveTileUs * (in.head_dim == 64 ? 0.7 : 1.0),
+                        (n * in.num_kv_heads + waves - 1) / waves});
+    }
+    auto longest = [](const std::pair<double, int>& x, const std::pair<double, int>& y) { return x.first > y.first; };
+    std::sort(tiles.begin(), tiles.end(), longest);
+    std::sort(solo.begin(), solo.end(), longest);
+    tiles.insert(tiles.end(), solo.begin(), solo.end());
+    double last = 0.0;
+    std::priority_queue<std::pair<double, int>, std::vector<std::pair<double, int>>, std::greater<std::pair<double, int>>> free;
+    free.push({0.0, in.num_cus * per_cu});
+    for (const auto& x : tiles) {
+      for (int left = x.second; left > 0;) {
+        const auto at = free.top();
+        free.pop();
+        const int k = std::min(left, at.second);
+        free.push({at.first + x.first, k});
+        if (k < at.second) free.push({at.first, at.second - k});
+        left -= k;
+        last = std::max(last, at.first + x.first);
+      }
+    }
+    last = std::max(last, kSharedItemUs + (own_bytes + shared_bytes) / kHbmBytes);
+    return last + partial / kPartialBytes;
+  }
+
+  double plan() {
+    double best = 1e30;
+    tile_limit = wave_limit = 1.0;
+    for (double t = std::max(1, most_units); t >= 2.0 || t == std::max(1, most_units); t *= 0.87) {
+      for (double o = std::max(4, most_own);; o = std::max(4.0, o * 0.62)) {
+        const double us = span(t, o);
+        if (us < best * 0.995) best = us, tile_limit = t, wave_limit = o;
+        if (o <= 4.0) break;
+      }
+      if (most_units <= 2) break;
+    }
+    for (SharedGroup& g : groups) g.chunks = chunks_of(g, tile_limit, wave_limit);
+    return best;
+  }
+
+  // A 64-key tile of a tile item, alone on its CU or beside another.  Over shared keys
+  // the inner loop of shared_tile, else that of tile_item.
+  double step_us(bool over_shared, bool alone, bool full) const {
+    if (in.head_dim == 64) return over_shared ? (alone ? 0.8 : 1.4) : (alone ? 1.0 : 1.5);
+    if (form == CHUNK_WAVES8) return over_shared ? (full ? 1.9 : 1.4) : 2.0;
+    return over_shared ? (alone ? 1.1 : 1.8) : (alone ? 1.35 : 2.35);
+  }
+};
+
+// Rows of one chunk's partial states: those over shared keys in blocks of 32.
+int partial_rows(const Rows& set, const SharedGroup& g) {
+  return set.part == PART_SHARED ? (g.nrows + 31) & ~31 : g.nrows;
+}
+
+void shared_tokens(const ChunkPlanInput& in, ChunkPlanOutput& out) {
+  for (int r = 0; r < in.num_reqs; ++r)
+    for (int t = in.qo_indptr[r]; t < in.qo_indptr[r + 1]; ++t)
+      out.tokens.push_back({r, in.qo_indptr[r + 1] - t, (in.page_indptr[r + 1] - in.page_indptr[r]) * in.page_size, 0});
+}
+
+// Items and merges of the groups.  shared_rows: of a request, the Rows of what it shares.
+void plan_shared(const ChunkPlanInput& in, const std::vector<Rows>& rows, const std::vector<int>& shared_rows,
+                 ChunkPlanOutput& out) {
+  const int group = in.num_qo_heads / in.num_kv_heads, heads = in.num_kv_heads;
+  SharedPlanner pl(in, rows, shared_waves4(in.head_dim, in.format) ? CHUNK_WAVES4 : CHUNK_WAVES8);
+  const double us = pl.plan();
+  if (in.head_dim == 128 && pl.form == CHUNK_WAVES4) {
+    SharedPlanner other(in, rows, CHUNK_WAVES8);
+    const double o = other.plan();
+    if (o < us) pl.take(std::move(other));
+  }
+  out.form = pl.form | CHUNK_SHARED;
+  const int merge_rows = 1024 / in.head_dim;
+  long long slot = 0;
+  std::vector<long long> slots(pl.groups.size());
+  std::vector<int> first_group(rows.size(), -1);
+  for (int i = 0; i < (int)pl.groups.size(); ++i) {
+    const SharedGroup& g = pl.groups[i];
+    const Rows& set = rows[g.rows];
+    if (first_group[g.rows] < 0) first_group[g.rows] = i;
+    if (g.chunks == 1 && set.part == PART_ALONE) continue;
+    slots[i] = slot;
+    slot += (long long)g.chunks * partial_rows(set, g) * heads;
+    if (set.part == PART_SHARED) continue;
+    // (kv heads side by side: a merge on the XCD whose L2 has the head's partial states)
+    for (int r = 0, take; r < g.nrows; r += take) {
+      for (int h = 0; h < heads; ++h) {
+        const long long at = slots[i] + (long long)h * g.chunks * g.nrows;
+        take = std::min(merge_rows, g.nrows - r);
+        SharedMerge m{set.q0, h, g.row0 + r, take, (int)at + r, g.nrows, g.chunks, 0, 0, 0, 0, 0};
+        if (set.part == PART_OWN) {
+          // its rows among those of the group, within one of their row tiles
+          const int sh = shared_rows[set.req], from = (set.q0 - rows[sh].q0) * group + g.row0 + r;
+          int k = first_group[sh];
+          while (from >= pl.groups[k].row0 + pl.groups[k].nrows) ++k;
+          const SharedGroup& sg = pl.groups[k];
+          take = m.nrows = std::min(take, sg.row0 + sg.nrows - from);
+          const int stride = partial_rows(rows[sh], sg);
+          m.shared_slot = (int)(slots[k] + (long long)h * sg.chunks * stride);
+          m.shared_row = from - sg.row0;
+          m.shared_stride = stride;
+          m.shared_chunks = sg.chunks;
+        }
+        out.shared_merges.push_back(m);
+      }
+    }
+  }
+  auto item_of = [&](int i) {
+    const SharedGroup& g = pl.groups[i];
+    const Rows& set = rows[g.rows];
+    ChunkItem it{};
+    it.req = set.req;
+    it.q0 = set.q0;
+    it.nq = set.nq;
+    it.row0 = g.row0;
+    it.nrows = g.nrows;
+    it.page_begin = in.page_indptr[set.req];
+    it.page_end = in.page_indptr[set.req + 1];
+    it.nchunks = g.chunks;
+    it.kind = g.kind;
+    it.part = set.part;
+    it.bound = set.bound;
+    it.heads = heads;
+    it.slot = (int)slots[i];
+    if (set.part == PART_SHARED) {
+      // The row tile's requests, where a wave's lanes can hold their lengths and their
+      // pages hold all that is shared and the tokens behind it.
+      const int t0 = set.q0 + g.row0 / group, t1 = set.q0 + (g.row0 + g.nrows - 1) / group;
+      int first = set.req;
+      while (in.qo_indptr[first + 1] <= t0) ++first;
+      int last = first;
+      long long room = 1ll << 40;
+      for (; last < set.last_req && in.qo_indptr[last] <= t1; ++last) {
+        if (in.qo_indptr[last + 1] == in.qo_indptr[last]) continue;
+        it.back = std::max(it.back, in.qo_indptr[last + 1] - std::max(in.qo_indptr[last], t0));
+        room = std::min(room, (long long)(in.page_indptr[last + 1] - in.page_indptr[last]) * in.page_size);
+      }
+      it.nq = first;
+      it.heads = last - first <= 64 && room >= (long long)set.bound + it.back ? last - first : 0;
+    }
+    return it;
+  };
+  std::vector<ChunkItem> tiles, solo;
+  std::vector<int> order(pl.groups.size());
+  for (int i = 0; i < (int)order.size(); ++i) order[i] = i;
+  std::stable_sort(order.begin(), order.end(), [&](int a, int b) {
+    return (double)pl.groups[a].units / pl.groups[a].chunks > (double)pl.groups[b].units / pl.groups[b].chunks;
+  });
+  for (int i : order) {
+    const SharedGroup& g = pl.groups[i];
+    const Rows& set = rows[g.rows];
+    ChunkItem it = item_of(i);
+    if (g.kind == CHUNK_TILE) {
+      for (it.chunk = 0; it.chunk < g.chunks; ++it.chunk)
+        for (it.kvh = 0; it.kvh < heads; ++it.kvh) {
+          it.slot = (int)(slots[i] + (long long)it.kvh * g.chunks * partial_rows(set, g));
+          tiles.push_back(it);
+        }
+    } else {
+      for (it.kvh = 0; it.kvh < g.chunks * heads; it.kvh += pl.waves) solo.push_back(it);
+    }
+  }
+  // Tile items first, the longest before the others: what they leave free takes the waves' units.
+  out.items = std::move(tiles);
+  out.items.insert(out.items.end(), solo.begin(), solo.end());
+  out.partial_rows = slot;
+  shared_tokens(in, out);
+}
+
 }  // namespace
 
 void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
@@ -247,6 +506,10 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   bool tokens_only = true;
   for (const Rows& x : rows)
     if ((long long)x.nq * group > 16) tokens_only = false;
+  if (shared && !tokens_only) {
+    plan_shared(in, rows, shared_rows, out);
+    return;
+  }
   // Heads of 128: workgroups of 8 waves share a tile's staging among more rows
   // (2 x 2048 tokens at 16384 bf16 keys: 953 us against 1045), those of 4 fill
   // the device with fewer rows (1000 tokens at 2100: 47 us against 50 split in two
@@ -300,7 +563,7 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
       }
       for (int r = 0, take; r < g.nrows; r += take) {
         take = std::min(merge_rows, g.nrows - r);
-        SharedMerge m{set.q0, h, g.row0 + r, take, (int)at + r, g.nrows, n, 0, 0, 0, {0, 0}};
+        SharedMerge m{set.q0, h, g.row0 + r, take, (int)at + r, g.nrows, n, 0, 0, 0, 0, 0};
         if (set.part == PART_OWN) {
           // its rows among those of the group, within one of their row tiles
           const int sh = shared_rows[set.req], from = (set.q0 - rows[sh].q0) * group + g.row0 + r;
@@ -309,7 +572,8 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
           const Group& sg = pl.groups[k];
           const int sn = pl.chunks(sg);
           take = m.nrows = std::min(take, sg.row0 + sg.nrows - from);
-          m.shared_slot = (int)(slots[k] + (long long)h * sn * sg.nrows) + from - sg.row0;
+          m.shared_slot = (int)(slots[k] + (long long)h * sn * sg.nrows);
+          m.shared_row = from - sg.row0;
           m.shared_stride = sg.nrows;
           m.shared_chunks = sn;
         }
@@ -346,9 +610,7 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   out.partial_rows = slot;
   if (!shared) return;
   out.form |= CHUNK_SHARED;
-  for (int r = 0; r < in.num_reqs; ++r)
-    for (int t = in.qo_indptr[r]; t < in.qo_indptr[r + 1]; ++t)
-      out.tokens.push_back({r, in.qo_indptr[r + 1] - t, (in.page_indptr[r + 1] - in.page_indptr[r]) * in.page_size, 0});
+  shared_tokens(in, out);
 }
 
 }  // namespace d2sd

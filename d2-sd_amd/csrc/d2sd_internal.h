@@ -316,6 +316,8 @@ constexpr int chunk_waves(int form) { return form == CHUNK_WAVES8 ? 8 : 4; }
 constexpr int chunk_rows(int form) { return 32 * chunk_waves(form); }  // packed rows of a tile item (32 per wave)
 constexpr int CHUNK_SHARED = 8;     // added to the form of plans with shared keys
 enum : int { PART_ALONE = 0, PART_SHARED = 1, PART_OWN = 2 };
+// Plans with shared keys: quantised heads of 128 take workgroups of eight waves alone.
+constexpr bool shared_waves4(int head_dim, int format) { return head_dim == 64 || format == CACHE_BF16; }
 constexpr int kTokenRows = 32;      // packed rows a token item holds at most (all waves share them)
 constexpr int kChunkMaxSplits = 64;
 enum : int { CHUNK_TILE = 0, CHUNK_TOKEN = 1 };
@@ -327,11 +329,16 @@ struct ChunkItem {                  // one workgroup (64 bytes)
   int chunk, nchunks;               // key chunk of its rows' visible keys
   int slot;                         // first partial row (nchunks > 1)
   int kind;                         // CHUNK_TILE / CHUNK_TOKEN
-  // plans with shared keys (CHUNK_SHARED): req, q0, nq and the pages of PART_SHARED
-  // items are the group's first request's, first row, rows and pages
+  // plans with shared keys (CHUNK_SHARED): req, q0 and the pages of PART_SHARED items
+  // are the group's first request's, first row and pages
   int part;                         // PART_*
   int bound;                        // keys [0, bound) are shared
-  int pad[2];
+  // token items of CHUNK_WAVES8 and CHUNK_WAVES4: a unit for each wave, from unit
+  // `kvh` of the nchunks x heads ones on (unit = chunk * heads + kv head).
+  // PART_SHARED tile items: the rows' requests are nq .. nq + heads - 1 and the rows sit
+  // at most `back` tokens before their requests' ends (heads 0: no such promise).
+  int heads;
+  int back;
 };
 struct ChunkMerge {                 // 32 bytes: rows merged by one workgroup
   int q0, kvh, row0, nrows;
@@ -342,7 +349,8 @@ struct SharedMerge {                // 48 bytes: the same in plans with shared k
   int q0, kvh, row0, nrows;
   int slot, stride, nchunks;        // over the rows' own keys (all of them where none are shared)
   int shared_slot, shared_stride, shared_chunks;  // over the shared ones (0 chunks: none)
-  int pad[2];
+  int shared_row;                   // of their partial rows, the merge's first
+  int pad;
 };
 struct SharedToken {                // a row of q: its request, tokens from it to the request's end, tokens that the
   int req, back, room, pad;         // request's pages hold

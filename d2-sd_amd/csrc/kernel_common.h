@@ -168,6 +168,48 @@ __device__ __forceinline__ void dma16s(const void* sbase, unsigned voff, unsigne
       : "memory", "m0");
 }
 
+// dma16s of tiles that other workgroups read too (dma16_kept).
+__device__ __forceinline__ void dma16s_kept(const void* sbase, unsigned voff, unsigned lds_addr) {
+  const unsigned long long b = (unsigned long long)sbase;
+  const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(b >> 32));
+  const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((unsigned)b);
+  const unsigned long long sb = ((unsigned long long)hi << 32) | (unsigned long long)lo;
+  __asm__ volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2"
+      :
+      : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(voff), "s"((const void*)sb)
+      : "memory", "m0");
+}
+
+// 4 or 2 bytes a lane to LDS byte address lds_addr + 4 * lane (2: zero-extended); lanes
+// that are off write nothing.
+template <int BYTES>
+__device__ __forceinline__ void dma_scale(const void* sbase, unsigned voff, unsigned lds_addr) {
+  const unsigned long long b = (unsigned long long)sbase;
+  const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(b >> 32));
+  const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((unsigned)b);
+  const unsigned long long sb = ((unsigned long long)hi << 32) | (unsigned long long)lo;
+  static_assert(BYTES == 4 || BYTES == 2, "a row's block scales");
+  if constexpr (BYTES == 4)
+    __asm__ volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dword %1, %2"
+        :
+        : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(voff), "s"((const void*)sb)
+        : "memory", "m0");
+  else
+    __asm__ volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_ushort %1, %2"
+        :
+        : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(voff), "s"((const void*)sb)
+        : "memory", "m0");
+}
+
 // dma16s to LDS byte address lds_base + OFF (lds_base already in a scalar
 // register): one scalar instruction per copy besides the load.
 template <int OFF>

@@ -48,7 +48,9 @@ DEVICE = [f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-p
 # launch, so a workgroup's first loads (its item, request 0's prefix length)
 # depend on nothing.
 EXTRA = {"verify_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-fno-honor-nans",
-                                  "-mllvm", "-amdgpu-kernarg-preload-count=4"]}
+                                  "-mllvm", "-amdgpu-kernarg-preload-count=4"],
+         # (accumulators in VGPRs, as there)
+         "chunk_attention_1": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def hipcc() -> str:
@@ -63,7 +65,7 @@ def _compile(src: str, defs: dict) -> Path:
     obj = OBJ_DIR / ("_".join([path.stem, *map(str, defs.values())]) + ".o")
     cmd = [hipcc(), *COMMON, *[f"-D{k}={v}" for k, v in defs.items()]]
     if path.suffix == ".hip":
-        cmd += DEVICE + EXTRA.get(src, [])
+        cmd += DEVICE + EXTRA.get(src, []) + EXTRA.get(obj.stem, [])
     else:
         cmd += ["-x", "c++", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include"]
     cmd += ["-c", str(path), "-o", str(obj)]

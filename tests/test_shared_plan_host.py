@@ -56,6 +56,22 @@ def keys_of(item, tokens, kv, P, group, window, wave):
     return a, b, see
 
 
+def units(items, hkv, waves):
+    """Token items whose waves have units of their own, one item for each."""
+    out = []
+    for it in items:
+        if it[11] == 0:
+            out.append(it)
+            continue
+        assert it[14] == hkv and it[15] == 0
+        for u in range(int(it[1]), min(int(it[1]) + waves, int(it[9]) * hkv)):
+            one = it.copy()
+            one[8], one[1] = u // hkv, u % hkv
+            one[10] = it[10] + one[1] * it[9] * it[5]
+            out.append(one)
+    return out
+
+
 def check(a, b, qo, kv, groups, prefix, hkv, group, P, window, now=None):
     items, merges, tokens = parts(a)
     now = list(kv) if now is None else now
@@ -67,24 +83,35 @@ def check(a, b, qo, kv, groups, prefix, hkv, group, P, window, now=None):
     seen = {}                # (row of q, head) -> keys and the request whose pages they come through
     slots, written = {}, 0   # partial row -> (row of q, head)
     direct = set()
+    assert a.info.plan_ints == items.size + merges.size + (tokens.size if a.info.form & 8 else 0)
+    if a.info.form & 8 and a.info.form & 7 < 2:
+        items = units(items, hkv, 8 if a.info.form & 7 == 0 else 4)
     for it in items:
         req, kvh, q0, nq, row0, nrows, pb, pe, chunk, nchunks, slot, kind, part, bound = (int(x) for x in it[:14])
         assert (pb, pe) == (b.page_indptr_host[req], b.page_indptr_host[req + 1]) and nrows > 0
         lo, hi, see = keys_of(it, tokens, now, P, group, window, kind)
+        if part == SHARED and kind == 0 and int(it[14]):
+            # the promise that lets the lengths be looked at last
+            r0, rn, back = nq, int(it[14]), int(it[15])
+            assert rn <= 64 and first[0] <= r0 and r0 + rn <= len(qo)
+            for i in range(nrows):
+                tok = tokens[q0 + (row0 + i) // group]
+                assert r0 <= tok[0] < r0 + rn and tok[1] <= back and tok[2] >= bound + back
         for i in range(nrows):
             row = (q0 + (row0 + i) // group, kvh * group + (row0 + i) % group)
             mine = seen.setdefault(row, [])
             mine += [(k, req if part == SHARED else req) for k in range(max(lo, see[i][0]), min(hi, see[i][1] + 1))]
             if part != ALONE or nchunks > 1:
-                at = slot + chunk * nrows + i
+                # (over shared keys, tile items store blocks of 32 rows)
+                at = slot + chunk * (-(-nrows // 32) * 32 if part == SHARED and kind == 0 else nrows) + i
                 assert at not in slots
                 slots[at] = row
             else:
                 assert row not in direct
                 direct.add(row)
-    assert not slots or (min(slots) == 0 and max(slots) == len(slots) - 1)
-    assert len(slots) * (a.head_dim + 1) * 4 == a.info.workspace_bytes
-    assert a.info.plan_ints == items.size + merges.size + (tokens.size if a.info.form & 8 else 0)
+    room = a.info.workspace_bytes // ((a.head_dim + 1) * 4)
+    assert not slots or (min(slots) == 0 and max(slots) < room <= len(slots) + 31 * len(items))
+    assert a.info.workspace_bytes == room * (a.head_dim + 1) * 4
     for r in range(len(qo)):
         for t in range(qo[r]):
             pos = min(now[r], int(b.page_indptr_host[r + 1] - b.page_indptr_host[r]) * P) - qo[r] + t
@@ -95,7 +122,7 @@ def check(a, b, qo, kv, groups, prefix, hkv, group, P, window, now=None):
     if not a.info.form & 8:
         return
     left = set(slots)
-    for q0, kvh, row0, nrows, slot, stride, n, s2, stride2, n2, _, _ in merges.tolist():
+    for q0, kvh, row0, nrows, slot, stride, n, s2, stride2, n2, r2, _ in merges.tolist():
         assert 0 < nrows <= 1024 // a.head_dim
         for i in range(nrows):
             row = (q0 + (row0 + i) // group, kvh * group + (row0 + i) % group)
@@ -103,8 +130,8 @@ def check(a, b, qo, kv, groups, prefix, hkv, group, P, window, now=None):
                 assert slots[slot + i + c * stride] == row
                 left.remove(slot + i + c * stride)
             for c in range(n2):
-                assert slots[s2 + i + c * stride2] == row
-                left.remove(s2 + i + c * stride2)
+                assert slots[s2 + r2 + i + c * stride2] == row
+                left.remove(s2 + r2 + i + c * stride2)
             assert row not in direct
             direct.add(row)
     assert not left and len(direct) == sum(qo) * hkv * group
