@@ -753,12 +753,13 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
   constexpr int VB = 32 * D * 2;                // bytes of a wave's value tile
   const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
 
-  const Span all = rows_span<SHARED>(p, w, 0, w.nrows - 1);
+  Span all = rows_span<SHARED>(p, w, 0, w.nrows - 1, false);
   const int tile0 = all.lo >> 5, ntiles_all = all.hi > all.lo ? ((all.hi + 31) >> 5) - tile0 : 0;
   const int tb = tile0 + (int)((long long)ntiles_all * w.chunk / w.nchunks);
   const int te = tile0 + (int)((long long)ntiles_all * (w.chunk + 1) / w.nchunks);
 
   int pos[RB], row_lo[RB];  // last and first key of a row
+  int least = 0x7FFFFFFF;   // lowest position of the lane's rows
   bf16x8 qf[RB][KS];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
@@ -766,6 +767,7 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
     const RowOut at(p, w, row);
     pos[rb] = row_pos<SHARED>(p, w, all.pos0, row);
     row_lo[rb] = row_first<SHARED>(p, w, pos[rb]);
+    if constexpr (SHARED) least = min(least, pos[rb]);
     pos[rb] = row_last<SHARED>(w, pos[rb]);
     const bf16_t* qp = (const bf16_t*)p.q + (long long)at.token * p.q_stride_n + (long long)at.head * p.q_stride_h;
 #pragma unroll
@@ -1009,6 +1011,8 @@ __device__ __forceinline__ void token_item(const ChunkParams& p, const ChunkItem
       fetch(raw[i], t, pg);
     }
   }
+  if constexpr (SHARED)  // (not before the first keys are on their way)
+    if (w.part == PART_SHARED && p.window_left < 0) all.all_lo = 0, all.all_hi = min(w.bound, wave_min(least) + 1);
   for (int t = t0; t < te; t += PF * TW) {
 #pragma unroll
     for (int i = 0; i < PF; ++i)
