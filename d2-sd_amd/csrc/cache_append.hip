@@ -17,6 +17,11 @@
 // a block of 32 dims is four lanes side by side, as the quantiser wants it.  The
 // run's cosines and sines are computed once, lane i those of pair i, and shared
 // through LDS.
+//
+// Bound by HBM: 8192 tokens of 64 + 16 heads of 128 into a bf16 cache, 336 MB, take
+// 83 us, 4.0 TB/s, where a large copy reaches 5.0; 11 x 512 tokens of 64 + 16 heads
+// of 64 into mxfp4, 247 MB with the read back, 54 us.  A decoding step is one
+// launch's latency: a token 5.5 us, 48 tokens of 32 + 16 heads into mxfp8 7 us.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -31,7 +36,12 @@ namespace d2sd {
 namespace {
 
 constexpr int kAppendWaves = 4;
-constexpr int kAppendRows = 2;  // heads of a lane
+// Heads of a lane: two.  With one there are more waves than cosines repay (8192 tokens
+// 105 us, 48 tokens 12.6 with their read back), with four too few loads are on their
+// way (87.6 and 12.6; two: 83 and 11.8).  The paired eight through ds_bpermute instead
+// of a second load of the same lines, 83 us too, took 20 us where the loads take 16.4 (2000
+// tokens into fp8), and waves that go on from token to token 191.
+constexpr int kAppendRows = 2;
 // Queries of more than this are stored past the caches, as rotary_embedding's.
 constexpr long long kAppendStreamBytes = 32ll << 20;
 
@@ -75,9 +85,9 @@ __global__ __launch_bounds__(64 * kAppendWaves) void cache_append_kernel(const A
   const int place = p.c.kv_len[tok.x] - tok.y;  // the token's position in its cache
   int page = -1;
   if (h1 > hq) {
-    const int at = tok.z + (place >> p.c.log2_page);
+    const int behind = place >> p.c.log2_page;
     // (before the cache's start, or no page is reserved for it: nothing to write)
-    if (place >= 0 && at < tok.w) page = p.c.page_table[at];
+    if (place >= 0 && behind < tok.w - tok.z) page = p.c.page_table[tok.z + behind];
     if (page >= p.c.num_pages) page = -1;
   }
   const int slot = place & ((1 << p.c.log2_page) - 1);

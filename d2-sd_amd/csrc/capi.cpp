@@ -1326,11 +1326,11 @@ int d2sd_cache_append(const d2sd_cache_append_args* a, d2sd_stream_t stream) {
 
 int d2sd_chunk_plan(const d2sd_chunk_plan_desc* d, int32_t* host_plan, size_t host_plan_ints,
                     d2sd_chunk_plan_info* info) {
-  return d2sd_chunk_plan_shared(d, 0, nullptr, nullptr, host_plan, host_plan_ints, info);
+  return d2sd_chunk_plan_shared(d, 0, nullptr, nullptr, 0, host_plan, host_plan_ints, info);
 }
 
 int d2sd_chunk_plan_shared(const d2sd_chunk_plan_desc* d, int num_groups, const int32_t* shared_indptr,
-                           const int32_t* shared_len, int32_t* host_plan, size_t host_plan_ints,
+                           const int32_t* shared_len, int keep_shared, int32_t* host_plan, size_t host_plan_ints,
                            d2sd_chunk_plan_info* info) {
   g_last_error.clear();
   try {
@@ -1406,6 +1406,7 @@ int d2sd_chunk_plan_shared(const d2sd_chunk_plan_desc* d, int num_groups, const 
     in.num_groups = num_groups;
     in.shared_indptr = shared_indptr;
     in.shared_len = shared_len;
+    in.keep_shared = keep_shared != 0;
     d2sd::ChunkPlanOutput out;
     d2sd::plan_chunk(in, out);
     const bool shared = (out.form & d2sd::CHUNK_SHARED) != 0;

@@ -3,7 +3,11 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <functional>
+#include <map>
 #include <queue>
+#include <tuple>
+#include <utility>
 #include <vector>
 
 #include "plan.h"
@@ -88,6 +92,9 @@ struct Planner {
   int most;             // chunks of a group
   double limit = 0.0;   // the longest chunk, in us of one workgroup alone on its CU
   double token_share = 1.0;  // of that, a token item's longest
+  // Beside a plan with shared keys: what is read again comes from L2, and rows of token
+  // items beyond 16 are waited for (their loads no longer are).
+  double read_rate = kHbmBytes, wide_tokens = 1.0;
 
   Planner(const ChunkPlanInput& input, const std::vector<Rows>& rows, int f) : in(input), rows_list(rows), form(f) {
     // (by registers: chunk_attn_kernel; the token kernels of heads of 64 would fit four
@@ -131,7 +138,7 @@ struct Planner {
     const double per = longest > 0.0 ? work / longest / in.num_cus : 0.0;
     const double sharing = std::min<double>(per_cu, std::max(1.0, 0.6 * per + 0.4 * std::ceil(per - 0.02)));
     const double slower_tile = tile_us(form, in.head_dim, sharing) / tile_us(form, in.head_dim, 1.0);
-    const double slower_read = std::max(1.0, std::min(readers, (double)places) * place_bytes / kHbmBytes);
+    const double slower_read = std::max(1.0, std::min(readers, (double)places) * place_bytes / read_rate);
     for (const Group& g : groups) {
       const int n = chunks(g);
       if (n > 1 || g.partial) partial += (double)n * g.nrows * in.num_kv_heads * in.head_dim * 8.0;  // written and read
@@ -191,7 +198,7 @@ struct Planner {
         (kind == CHUNK_TOKEN ? tokens : tiles) = true;
         if (kind == CHUNK_TOKEN) {
           g.unit_read_us = unit_bytes / place_bytes;
-          g.unit_us = std::max(token_us, g.unit_read_us);
+          g.unit_us = std::max(rows > 16 ? token_us * wide_tokens : token_us, g.unit_read_us);
           g.least = waves;
         } else {
           g.unit_us = tile_us(form, in.head_dim, 1.0);
@@ -241,9 +248,12 @@ struct SharedGroup {
 // Row tiles of a group's rows over the shared keys (tile items, whatever their rows),
 // and each request's own keys: tile items where it brings more than 32 rows, else
 // units of one wave (a request, kv head and chunk of keys each), which fill
-// workgroups of as many waves.
+// workgroups of as many waves.  Chunk lengths are those that end soonest by the times
+// below, all measured: plans for decoding 64 requests behind 16K keys, swept over both
+// lengths, are within 3% of the best.
 constexpr double kSharedItemUs = 6.0, kWaveItemUs = 6.0, kWaveTileUs = 1.3;  // a workgroup's start and end; a 32-key tile of a wave
-constexpr double kPartialBytes = 1.8e6;  // partial states written and read, per us
+constexpr double kSharedMergeUs = 3.0, kPartialBytes = 2.6e6;  // the merge's launch; partial states written and read, per us
+constexpr double kAgainBytes = 13e6, kWideTokens = 1.5;  // keys that other requests read too, per us; 17 to 32 rows to 16
 
 struct SharedPlanner {
   const ChunkPlanInput& in;
@@ -253,6 +263,19 @@ struct SharedPlanner {
   double tile_limit, wave_limit;  // longest chunks, in tiles
   double own_bytes, shared_bytes; // of the keys and values
   int most_units, most_own;       // tiles of the longest tile item, of the longest wave's
+  struct Alike {                  // groups that a schedule need not tell apart
+    int kind, units;              // units: of three bits, rounded up
+    bool shared, full, partial;
+    bool operator<(const Alike& x) const {
+      return std::tie(kind, units, shared, full, partial) < std::tie(x.kind, x.units, x.shared, x.full, x.partial);
+    }
+  };
+  struct Many {
+    long long count, rows;
+  };
+  std::map<Alike, Many> alike;
+  mutable std::vector<std::pair<double, long long>> tiles, solo;  // items: time of each, how many
+  mutable std::vector<std::pair<double, long long>> free;         // places: when they are free, how many
 
   SharedPlanner(const ChunkPlanInput& input, const std::vector<Rows>& rows, int f) : in(input), rows_list(rows), form(f) {
     waves = chunk_waves(form);
@@ -283,6 +306,12 @@ struct SharedPlanner {
             2.0 * (g.kind == CHUNK_TILE ? 64 : 32) * g.units * row_bytes(in.format, in.head_dim) * in.num_kv_heads;
       if (g.kind == CHUNK_TILE) most_units = std::max(most_units, g.units);
       else most_own = std::max(most_own, g.units);
+      int fine = 0;
+      while (g.units >> fine >= 16) ++fine;
+      Many& m = alike[{g.kind, (g.units + (1 << fine) - 1) >> fine << fine, over_shared, g.nrows * 2 > chunk_rows(form),
+                       rows_list[g.rows].part != PART_ALONE}];
+      ++m.count;
+      m.rows += g.nrows;
     }
   }
 
@@ -292,76 +321,109 @@ struct SharedPlanner {
     groups = std::move(other.groups);
   }
 
-  int chunks_of(const SharedGroup& g, double tiles, double own) const {
+  int chunks_of(int kind, int units, double tiles, double own) const {
     const int most = in.max_splits > 0 ? std::min(in.max_splits, kChunkMaxSplits) : kChunkMaxSplits;
-    return std::max(1, std::min(most, (int)std::ceil(g.units / (g.kind == CHUNK_TILE ? tiles : own) - 1e-6)));
+    return std::max(1, std::min(most, (int)std::ceil(units / (kind == CHUNK_TILE ? tiles : own) - 1e-6)));
   }
 
   // Time until the last workgroup ends, those of tile items first, the longest before
-  // the others, and the merge of the partial states.
-  double span(double tile_limit, double own_limit) const {
-    std::vector<std::pair<double, int>> tiles, solo;
-    double partial = 0.0;
+  // the others, and the merge of the partial states.  At `enough` or more: some bound
+  // below it, not less than that.
+  double span(double tile_limit, double own_limit, double enough) const {
+    tiles.clear(), solo.clear(), free.clear();
+    double partial = 0.0, work = 0.0, last = kSharedItemUs + (own_bytes + shared_bytes) / kHbmBytes;
+    const long long heads = in.num_kv_heads, places = (long long)in.num_cus * per_cu;
     long long count = 0;
-    for (const SharedGroup& g : groups)
-      if (g.kind == CHUNK_TILE) count += (long long)chunks_of(g, tile_limit, own_limit) * in.num_kv_heads;
+    for (const auto& x : alike)
+      if (x.first.kind == CHUNK_TILE) count += x.second.count * chunks_of(CHUNK_TILE, x.first.units, tile_limit, own_limit) * heads;
     const bool alone = per_cu == 1 || count <= in.num_cus;
-    const int own_rows = chunk_rows(form);
-    for (const SharedGroup& g : groups) {
-      const int n = chunks_of(g, tile_limit, own_limit);
-      const bool over_shared = rows_list[g.rows].part == PART_SHARED;
-      if (n > 1 || rows_list[g.rows].part != PART_ALONE) partial += (double)n * g.nrows * in.num_kv_heads * in.head_dim * 4.0;
-      if (g.kind == CHUNK_TILE)
-        tiles.push_back({kSharedItemUs + (double)g.units / n * step_us(over_shared, alone, g.nrows * 2 > own_rows), n * in.num_kv_heads});
-      else
-        solo.push_back({kWaveItemUs + (double)g.units / n * kWaveTileUs * (in.head_dim == 64 ? 0.7 : 1.0),
-                        (n * in.num_kv_heads + waves - 1) / waves});
+    for (const auto& x : alike) {
+      const Alike& g = x.first;
+      const int n = chunks_of(g.kind, g.units, tile_limit, own_limit);
+      if (n > 1 || g.partial) partial += (double)n * x.second.rows * heads * in.head_dim * 4.0;
+      const double us = g.kind == CHUNK_TILE ? kSharedItemUs + (double)g.units / n * step_us(g.shared, alone, g.full)
+                                             : kWaveItemUs + (double)g.units / n * kWaveTileUs * (in.head_dim == 64 ? 0.7 : 1.0);
+      const long long items = x.second.count * (g.kind == CHUNK_TILE ? n * heads : (n * heads + waves - 1) / waves);
+      (g.kind == CHUNK_TILE ? tiles : solo).push_back({us, items});
+      work += us * items;
+      last = std::max(last, us);
     }
-    auto longest = [](const std::pair<double, int>& x, const std::pair<double, int>& y) { return x.first > y.first; };
-    std::sort(tiles.begin(), tiles.end(), longest);
-    std::sort(solo.begin(), solo.end(), longest);
-    tiles.insert(tiles.end(), solo.begin(), solo.end());
-    double last = 0.0;
-    std::priority_queue<std::pair<double, int>, std::vector<std::pair<double, int>>, std::greater<std::pair<double, int>>> free;
-    free.push({0.0, in.num_cus * per_cu});
-    for (const auto& x : tiles) {
-      for (int left = x.second; left > 0;) {
-        const auto at = free.top();
-        free.pop();
-        const int k = std::min(left, at.second);
-        free.push({at.first + x.first, k});
-        if (k < at.second) free.push({at.first, at.second - k});
-        left -= k;
-        last = std::max(last, at.first + x.first);
-      }
-    }
-    last = std::max(last, kSharedItemUs + (own_bytes + shared_bytes) / kHbmBytes);
-    return last + partial / kPartialBytes;
+    if (partial > 0.0) partial = kSharedMergeUs + partial / kPartialBytes;
+    const double bound = std::max(last, work / places) + partial;
+    if (bound >= enough) return bound;
+    std::sort(tiles.begin(), tiles.end(), std::greater<>());
+    std::sort(solo.begin(), solo.end(), std::greater<>());
+    const auto later = std::greater<std::pair<double, long long>>();
+    free.push_back({0.0, places});
+    for (const auto* list : {&tiles, &solo})
+      for (const auto& x : *list)
+        for (long long left = x.second; left > 0;) {
+          std::pop_heap(free.begin(), free.end(), later);
+          const auto at = free.back();
+          free.pop_back();
+          // (rounds in which the same places take items of the same length again and again)
+          const long long rounds = free.empty() ? std::max(1ll, left / at.second) : 1, k = rounds > 1 ? at.second : std::min(left, at.second);
+          const double end = at.first + rounds * x.first;
+          free.push_back({end, k});
+          std::push_heap(free.begin(), free.end(), later);
+          if (k < at.second) {
+            free.push_back({at.first, at.second - k});
+            std::push_heap(free.begin(), free.end(), later);
+          }
+          left -= rounds * k;
+          last = std::max(last, end);
+        }
+    return last + partial;
   }
 
   double plan() {
     double best = 1e30;
     tile_limit = wave_limit = 1.0;
-    for (double t = std::max(1, most_units); t >= 2.0 || t == std::max(1, most_units); t *= 0.87) {
-      for (double o = std::max(4, most_own);; o = std::max(4.0, o * 0.62)) {
-        const double us = span(t, o);
-        if (us < best * 0.995) best = us, tile_limit = t, wave_limit = o;
-        if (o <= 4.0) break;
-      }
-      if (most_units <= 2) break;
-    }
-    for (SharedGroup& g : groups) g.chunks = chunks_of(g, tile_limit, wave_limit);
+    const double longest = std::max(1, most_units);
+    // (a coarse search first: the fine one then knows what need not be looked at)
+    for (const auto& step : {std::pair<double, double>{0.6, 0.4}, {0.87, 0.62}})
+      for (double t = longest; t >= 2.0 || t == longest; t *= step.first)
+        for (double o = std::max(4, most_own);; o = std::max(4.0, o * step.second)) {
+          const double us = span(t, o, best * 0.995);
+          if (us < best * 0.995) best = us, tile_limit = t, wave_limit = o;
+          if (o <= 4.0) break;
+        }
+    for (SharedGroup& g : groups) g.chunks = chunks_of(g.kind, g.units, tile_limit, wave_limit);
     return best;
   }
 
   // A 64-key tile of a tile item, alone on its CU or beside another.  Over shared keys
   // the inner loop of shared_tile, else that of tile_item.
   double step_us(bool over_shared, bool alone, bool full) const {
-    if (in.head_dim == 64) return over_shared ? (alone ? 0.8 : 1.4) : (alone ? 1.0 : 1.5);
-    if (form == CHUNK_WAVES8) return over_shared ? (full ? 1.9 : 1.4) : 2.0;
-    return over_shared ? (alone ? 1.1 : 1.8) : (alone ? 1.35 : 2.35);
+    if (in.head_dim == 64) return over_shared ? (alone ? 0.7 : 1.15) : (alone ? 1.0 : 1.5);
+    if (form == CHUNK_WAVES8) return over_shared ? (!full ? 1.4 : in.format == CACHE_BF16 ? 1.75 : 1.9) : 2.0;
+    return over_shared ? (alone ? 1.1 : 1.75) : (alone ? 1.35 : 2.35);
   }
 };
+
+// Plans of the waves that end soonest by their schedule, and that time.
+double plan_waves(Planner& pl) {
+  double us = pl.plan();
+  if (pl.form == CHUNK_WAVES4 && pl.in.head_dim == 128) {
+    Planner other(pl.in, pl.rows_list, CHUNK_WAVES8);
+    other.read_rate = pl.read_rate, other.wide_tokens = pl.wide_tokens;
+    const double o = other.plan();
+    if (o < us) pl.take(std::move(other)), us = o;
+  }
+  return us;
+}
+double plan_waves(SharedPlanner& pl) {
+  double us = pl.plan();
+  if (pl.form == CHUNK_WAVES4 && pl.in.head_dim == 128) {
+    SharedPlanner other(pl.in, pl.rows_list, CHUNK_WAVES8);
+    const double o = other.plan();
+    if (o < us) pl.take(std::move(other)), us = o;
+  }
+  return us;
+}
+
+// Waves to begin with: two workgroups on a CU where their rings fit.
+int shared_form(const ChunkPlanInput& in) { return shared_waves4(in.head_dim, in.format) ? CHUNK_WAVES4 : CHUNK_WAVES8; }
 
 // Rows of one chunk's partial states: those over shared keys in blocks of 32.
 int partial_rows(const Rows& set, const SharedGroup& g) {
@@ -378,13 +440,8 @@ void shared_tokens(const ChunkPlanInput& in, ChunkPlanOutput& out) {
 void plan_shared(const ChunkPlanInput& in, const std::vector<Rows>& rows, const std::vector<int>& shared_rows,
                  ChunkPlanOutput& out) {
   const int group = in.num_qo_heads / in.num_kv_heads, heads = in.num_kv_heads;
-  SharedPlanner pl(in, rows, shared_waves4(in.head_dim, in.format) ? CHUNK_WAVES4 : CHUNK_WAVES8);
-  const double us = pl.plan();
-  if (in.head_dim == 128 && pl.form == CHUNK_WAVES4) {
-    SharedPlanner other(in, rows, CHUNK_WAVES8);
-    const double o = other.plan();
-    if (o < us) pl.take(std::move(other));
-  }
+  SharedPlanner pl(in, rows, shared_form(in));
+  plan_waves(pl);
   out.form = pl.form | CHUNK_SHARED;
   const int merge_rows = 1024 / in.head_dim;
   long long slot = 0;
@@ -407,8 +464,7 @@ void plan_shared(const ChunkPlanInput& in, const std::vector<Rows>& rows, const 
         if (set.part == PART_OWN) {
           // its rows among those of the group, within one of their row tiles
           const int sh = shared_rows[set.req], from = (set.q0 - rows[sh].q0) * group + g.row0 + r;
-          int k = first_group[sh];
-          while (from >= pl.groups[k].row0 + pl.groups[k].nrows) ++k;
+          const int k = first_group[sh] + from / chunk_rows(pl.form);
           const SharedGroup& sg = pl.groups[k];
           take = m.nrows = std::min(take, sg.row0 + sg.nrows - from);
           const int stride = partial_rows(rows[sh], sg);
@@ -483,30 +539,98 @@ void plan_shared(const ChunkPlanInput& in, const std::vector<Rows>& rows, const 
   shared_tokens(in, out);
 }
 
+// The rows of requests [r0, r1).  use: groups whose keys are shared.  shared_rows: of a
+// request, the Rows of what it shares (-1: nothing).  Returns whether any shares.
+bool batch_rows(const ChunkPlanInput& in, const std::vector<char>& use, int r0, int r1, std::vector<Rows>& rows,
+                std::vector<int>& shared_rows) {
+  rows.clear();
+  shared_rows.assign(in.num_reqs, -1);
+  for (int i = 0; i < in.num_groups; ++i) {
+    const int a = in.shared_indptr[i], b = in.shared_indptr[i + 1];
+    if (!use[i] || a < r0 || b > r1) continue;
+    for (int r = a; r < b; ++r) shared_rows[r] = (int)rows.size();
+    rows.push_back({PART_SHARED, a, in.qo_indptr[a], in.qo_indptr[b] - in.qo_indptr[a], b, in.shared_len[i]});
+  }
+  const bool shared = !rows.empty();
+  for (int r = r0; r < r1; ++r) {
+    const int q0 = in.qo_indptr[r], nq = in.qo_indptr[r + 1] - q0, s = shared_rows[r];
+    rows.push_back({s < 0 ? PART_ALONE : PART_OWN, r, q0, nq, r + 1, s < 0 ? 0 : rows[s].bound});
+  }
+  return shared;
+}
+
+bool tokens_only(const ChunkPlanInput& in, const std::vector<Rows>& rows) {
+  const int group = in.num_qo_heads / in.num_kv_heads;
+  for (const Rows& x : rows)
+    if ((long long)x.nq * group > 16) return false;
+  return true;
+}
+
+// Time of requests [r0, r1) with the keys of these groups shared.
+double batch_us(const ChunkPlanInput& in, const std::vector<char>& use, int r0, int r1) {
+  std::vector<Rows> rows;
+  std::vector<int> shared_rows;
+  const bool shared = batch_rows(in, use, r0, r1, rows, shared_rows), few = tokens_only(in, rows);
+  if (shared && !few) {
+    SharedPlanner pl(in, rows, shared_form(in));
+    return plan_waves(pl);
+  }
+  Planner pl(in, rows, few ? CHUNK_TOKENS : CHUNK_WAVES4);
+  if (!shared) {
+    double keys = 1.0, again = 0.0;  // of those that are read, those that another request read before
+    for (int i = 0; i < in.num_groups; ++i)
+      for (int r = in.shared_indptr[i]; r < in.shared_indptr[i + 1]; ++r) {
+        if (r < r0 || r >= r1) continue;
+        const int nq = in.qo_indptr[r + 1] - in.qo_indptr[r];
+        const long long lo = in.window_left >= 0 ? std::max(0ll, (long long)in.kv_len[r] - nq - in.window_left) : 0;
+        keys += std::max(0ll, in.kv_len[r] - lo);
+        if (r > in.shared_indptr[i]) again += std::max(0ll, std::min(in.kv_len[r], in.shared_len[i]) - lo);
+      }
+    pl.read_rate = 1.0 / (again / keys / kAgainBytes + (1.0 - again / keys) / kHbmBytes);
+    pl.wide_tokens = kWideTokens;
+  }
+  return plan_waves(pl);
+}
+
+// Groups whose keys are read once for all of their rows.  Sharing costs partial states
+// and a launch that joins them, so that it is not worth a few keys, nor many rows that
+// are bound by their products either way: all of the groups share, or those that gain
+// by themselves, or none, whichever ends soonest by the schedules' times.  (Of 135
+// batches of 2 to 64 requests of 1 to 200 tokens behind 64 to 4096 keys, shared they
+// took 0.26 to 2.4 times what they take apart.)
+std::vector<char> sharing(const ChunkPlanInput& in) {
+  std::vector<char> use(in.num_groups, 0);
+  int groups = 0;
+  for (int i = 0; i < in.num_groups; ++i) {
+    const int a = in.shared_indptr[i], b = in.shared_indptr[i + 1];
+    use[i] = b - a > 1 && in.shared_len[i] > 0 && in.qo_indptr[b] > in.qo_indptr[a];
+    groups += use[i];
+  }
+  if (groups == 0 || in.keep_shared) return use;
+  const std::vector<char> none(in.num_groups, 0);
+  double best = batch_us(in, none, 0, in.num_reqs);
+  const double all = batch_us(in, use, 0, in.num_reqs);
+  std::vector<char> kept = none;
+  if (all < best) best = all, kept = use;
+  if (groups == 1) return kept;
+  std::vector<char> gain = use;
+  for (int i = 0; i < in.num_groups; ++i)
+    if (use[i])
+      gain[i] = batch_us(in, use, in.shared_indptr[i], in.shared_indptr[i + 1]) <
+                batch_us(in, none, in.shared_indptr[i], in.shared_indptr[i + 1]);
+  if (gain != use && gain != none && batch_us(in, gain, 0, in.num_reqs) < best) kept = gain;
+  return kept;
+}
+
 }  // namespace
 
 void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   out = ChunkPlanOutput{};
   const int group = in.num_qo_heads / in.num_kv_heads;
   std::vector<Rows> rows;
-  bool shared = false;
-  std::vector<int> shared_rows(in.num_reqs, -1);  // of a request: the Rows of what it shares
-  for (int i = 0; i < in.num_groups; ++i) {
-    const int a = in.shared_indptr[i], b = in.shared_indptr[i + 1];
-    const int q0 = in.qo_indptr[a], nq = in.qo_indptr[b] - q0;
-    if (b - a < 2 || in.shared_len[i] == 0 || nq == 0) continue;
-    for (int r = a; r < b; ++r) shared_rows[r] = (int)rows.size();
-    rows.push_back({PART_SHARED, a, q0, nq, b, in.shared_len[i]});
-    shared = true;
-  }
-  for (int r = 0; r < in.num_reqs; ++r) {
-    const int q0 = in.qo_indptr[r], nq = in.qo_indptr[r + 1] - q0, s = shared_rows[r];
-    rows.push_back({s < 0 ? PART_ALONE : PART_OWN, r, q0, nq, r + 1, s < 0 ? 0 : rows[s].bound});
-  }
-  bool tokens_only = true;
-  for (const Rows& x : rows)
-    if ((long long)x.nq * group > 16) tokens_only = false;
-  if (shared && !tokens_only) {
+  std::vector<int> shared_rows;  // of a request: the Rows of what it shares
+  const bool shared = batch_rows(in, sharing(in), 0, in.num_reqs, rows, shared_rows), few = tokens_only(in, rows);
+  if (shared && !few) {
     plan_shared(in, rows, shared_rows, out);
     return;
   }
@@ -517,12 +641,8 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   // were kept in L2, 4 x 1024 tokens, window 128: 39 us against 44; 8 x 300 at 1000:
   // 66 against 74; but 2 x 2048 at 16384: 1340 against 1259 in bf16, 1201 against
   // 1217 in mxfp4; now 28, 55, 1200 and 1145 of 4 waves, 8 were not measured again).
-  Planner pl(in, rows, tokens_only ? CHUNK_TOKENS : CHUNK_WAVES4);
-  const double us = pl.plan();
-  if (!tokens_only && in.head_dim == 128) {
-    Planner other(in, rows, CHUNK_WAVES8);
-    if (other.plan() < us) pl.take(std::move(other));
-  }
+  Planner pl(in, rows, few ? CHUNK_TOKENS : CHUNK_WAVES4);
+  plan_waves(pl);
   out.form = pl.form;
   // Token items alone that read more than half of the last-level cache (256 MB):
   // what they read is not there when the next call reads it, and goes past the
@@ -531,7 +651,7 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
   // 27 us, 30 past the caches).
   double bytes = 0.0;
   for (const Group& g : pl.groups) bytes += 64.0 * g.units * row_bytes(in.format, in.head_dim) * in.num_kv_heads;
-  if (tokens_only && bytes > kStreamBytes) out.form = CHUNK_STREAM;
+  if (few && bytes > kStreamBytes) out.form = CHUNK_STREAM;
   const int merge_rows = 1024 / in.head_dim;  // rows of one merge workgroup: 256 threads, 4 head dims each
   struct Placed {
     double us;   // of a chunk
@@ -567,8 +687,7 @@ void plan_chunk(const ChunkPlanInput& in, ChunkPlanOutput& out) {
         if (set.part == PART_OWN) {
           // its rows among those of the group, within one of their row tiles
           const int sh = shared_rows[set.req], from = (set.q0 - rows[sh].q0) * group + g.row0 + r;
-          int k = first_group[sh];
-          while (from >= pl.groups[k].row0 + pl.groups[k].nrows) ++k;
+          const int k = first_group[sh] + from / chunk_rows(pl.form);
           const Group& sg = pl.groups[k];
           const int sn = pl.chunks(sg);
           take = m.nrows = std::min(take, sg.row0 + sg.nrows - from);

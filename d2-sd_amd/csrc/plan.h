@@ -114,6 +114,7 @@ struct ChunkPlanInput {
   int num_groups;
   const int* shared_indptr;
   const int* shared_len;
+  bool keep_shared;        // also where that is slower
 };
 struct ChunkPlanOutput {
   std::vector<ChunkItem> items;

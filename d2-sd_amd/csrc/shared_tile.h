@@ -20,6 +20,11 @@
 // K and one of V a tile into two slots each: loaded through registers instead, a tile
 // and a half ahead, tiles took 2.7 us in mxfp8 where memory was busy, and registers
 // spilled.  One barrier a tile.
+//
+// Bound by MFMA and, with all CUs at work, by the clock that power leaves: 256 rows x
+// 64 keys of 128 dims take a CU 1.4 to 1.6 us while half of the others idle, 1.7 in
+// bf16 and 1.9 quantised with all of them, 1.25 PFLOP/s, 92% of a large library
+// product; tile_item's loop took 2.0 to 3.3.
 #pragma once
 
 // LDS of the tiles.  bf16: KST slots of K, VST of V, the LDS share of a workgroup (two

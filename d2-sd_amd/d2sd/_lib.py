@@ -477,7 +477,7 @@ def _load() -> C.CDLL:
     lib.d2sd_chunk_plan.restype = i32
     lib.d2sd_chunk_plan.argtypes = [C.POINTER(ChunkPlanDesc), C.POINTER(C.c_int32), sz, C.POINTER(ChunkPlanInfo)]
     lib.d2sd_chunk_plan_shared.restype = i32
-    lib.d2sd_chunk_plan_shared.argtypes = [C.POINTER(ChunkPlanDesc), i32, C.POINTER(C.c_int32), C.POINTER(C.c_int32),
+    lib.d2sd_chunk_plan_shared.argtypes = [C.POINTER(ChunkPlanDesc), i32, C.POINTER(C.c_int32), C.POINTER(C.c_int32), i32,
                                            C.POINTER(C.c_int32), sz, C.POINTER(ChunkPlanInfo)]
     lib.d2sd_chunk_run.restype = i32
     lib.d2sd_chunk_run.argtypes = [C.POINTER(ChunkPlanInfo), C.POINTER(ChunkRunArgs), vp]

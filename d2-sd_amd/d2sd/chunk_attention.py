@@ -41,8 +41,8 @@ class PagedChunkAttention:
     def plan(self, batch: PagedBatch, num_qo_heads: int, num_kv_heads: int, head_dim: int, *, kv_format: str = "bf16",
              sm_scale: Optional[float] = None, window_left: int = -1, sinks: Optional[torch.Tensor] = None,
              lse_base2: bool = False, max_splits: int = 0, num_cus: int = 0,
-             shared_indptr: Optional[Sequence[int]] = None, shared_len: Optional[Sequence[int]] = None
-             ) -> "PagedChunkAttention":
+             shared_indptr: Optional[Sequence[int]] = None, shared_len: Optional[Sequence[int]] = None,
+             keep_shared: bool = False) -> "PagedChunkAttention":
         """Plans the batch (its kv_len_host, of its making or the last
         set_kv_len: the work is shared out for those lengths, and right for any
         within the requests' pages).
@@ -58,11 +58,15 @@ class PagedChunkAttention:
         Requests whose caches begin alike (a system prompt, a document):
         requests shared_indptr[i] .. shared_indptr[i + 1] - 1 hold the same
         tokens in their first shared_len[i] positions (0: none).  Those keys
-        are read once for all of them, through the first one's pages; the
-        others' pages of that range are not looked at.  shared_indptr starts at
-        0 and ends at the number of requests; a group's shared_len is any
-        number that its first request's pages hold.  The result is that of a
-        plan without groups, whatever lengths the caches have later."""
+        are read once for all of them, through the first one's pages, where
+        that is faster by the plan's estimate (joining partial states costs
+        time; few shared keys, or many new tokens, do not repay it), else by
+        each request through its own.  keep_shared=True shares them in any
+        case; the others' pages of that range are then never looked at.
+        shared_indptr starts at 0 and ends at the number of requests; a
+        group's shared_len is any number that its first request's pages hold.
+        The result is that of a plan without groups, whatever lengths the
+        caches have later."""
         if kv_format not in KV_FORMATS:
             raise ValueError(f"kv_format must be one of {sorted(KV_FORMATS)}")
         if self._want_device is not None and _device(self._want_device) != batch.device:
@@ -94,8 +98,8 @@ class PagedChunkAttention:
                 raise ValueError("shared_indptr must hold every request")
         info = _lib.ChunkPlanInfo()
         host = np.empty(1 << 16, dtype=np.int32)
-        plan = lambda: lib.d2sd_chunk_plan_shared(C.byref(desc), groups, indptr, shared, as_p(host), host.size,  # noqa: E731
-                                                  C.byref(info))
+        plan = lambda: lib.d2sd_chunk_plan_shared(C.byref(desc), groups, indptr, shared, bool(keep_shared), as_p(host),  # noqa: E731
+                                                  host.size, C.byref(info))
         with torch.cuda.device(batch.device) if batch.device.type == "cuda" else torch.no_grad():
             rc = plan()
             if rc == _lib.D2SD_ERR_WORKSPACE and info.plan_ints > host.size:

@@ -24,7 +24,7 @@ class Problem:
     """Groups of requests: request r's cache is its group's shared tokens, then its own (own[r] of them)."""
 
     def __init__(self, groups, prefix, own, new, hq, hkv, d, fmt="bf16", layout="HND", P=16, window=-1, sinks=False, seed=0,
-                 extra=0, pad=0, spread=1.0, **plan):
+                 extra=0, pad=0, spread=1.0, keep_shared=True, **plan):
         g = torch.Generator().manual_seed(seed + sum(own) + sum(prefix) + hq + d)
         first = np.concatenate([[0], np.cumsum(groups)]).astype(int)
         share = [prefix[i] for i, n in enumerate(groups) for _ in range(n)]
@@ -71,7 +71,7 @@ class Problem:
         self.sinks = torch.randn(hq, generator=g) if sinks else None
         self.attn = d2sd.PagedChunkAttention().plan(
             self.batch, hq, hkv, d, kv_format=fmt, window_left=window, sinks=None if self.sinks is None else self.sinks.to(DEV),
-            shared_indptr=first, shared_len=prefix, **plan)
+            shared_indptr=first, shared_len=prefix, keep_shared=keep_shared, **plan)
         self.scale = plan.get("sm_scale") or d ** -0.5
         self.kr, self.vr = (po.values_ref(*po.quantise_ref(t, fmt, s), fmt, s) for t, s in zip(x, scale))
 
@@ -375,7 +375,8 @@ def test_offsets_past_32_bits():
     for n in (1, 25):
         q = torch.randn(2 * n, 16, d, generator=g).to(torch.bfloat16)
         b = d2sd.PagedBatch([0, n, 2 * n], kv, pi, table, P, device=DEV)
-        out, _ = d2sd.PagedChunkAttention().plan(b, 16, hkv, d, shared_indptr=[0, 2], shared_len=[S]).run(q.to(DEV), c)
+        out, _ = d2sd.PagedChunkAttention().plan(b, 16, hkv, d, shared_indptr=[0, 2], shared_len=[S],
+                                                   keep_shared=True).run(q.to(DEV), c)
         torch.cuda.synchronize()
         for r, rows in ((0, torch.arange(130)), (1, torch.cat([torch.arange(S), torch.arange(130, 160)]))):
             o, s, A, size = po.attention_ref(q[r * n:r * n + n], k[rows], v[rows], 130 - n, 2, d ** -0.5)
@@ -389,7 +390,8 @@ def test_page_ids_outside_the_pool_stay_in_bounds():
         t.view(torch.uint8).fill_(0x38)
     R = 20
     b = d2sd.PagedBatch(np.arange(R + 1), [64] * R, 4 * np.arange(R + 1), [0, 2 ** 31 - 1, -5, 4] * R, 16, device=DEV)
-    out, lse = d2sd.PagedChunkAttention().plan(b, 4, 2, 64, kv_format="mxfp8", shared_indptr=[0, R], shared_len=[40]).run(
+    out, lse = d2sd.PagedChunkAttention().plan(b, 4, 2, 64, kv_format="mxfp8", shared_indptr=[0, R], shared_len=[40],
+                                                 keep_shared=True).run(
         torch.zeros(R, 4, 64, dtype=torch.bfloat16, device=DEV), c)
     torch.cuda.synchronize()
     assert torch.isfinite(out).all() and (lse - math.log(64)).abs().max() < 1e-5

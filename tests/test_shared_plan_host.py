@@ -13,13 +13,15 @@ ITEM, MERGE, TOKEN = 16, 12, 4
 ALONE, SHARED, OWN = 0, 1, 2
 
 
-def plan(qo, kv, groups, prefix, hq=8, hkv=2, d=128, P=16, cus=256, splits=0, window=-1, fmt="bf16", extra=0):
+def plan(qo, kv, groups, prefix, hq=8, hkv=2, d=128, P=16, cus=256, splits=0, window=-1, fmt="bf16", extra=0,
+         keep=True):
     """groups: requests of each; prefix: what each group shares."""
     pi = np.concatenate([[0], np.cumsum([-(-(n + extra) // P) for n in kv])])
     starts = np.concatenate([[0], np.cumsum(qo)])
     b = d2sd.PagedBatch(starts, kv, pi, np.arange(max(int(pi[-1]), 1)), P, device="cpu")
     a = d2sd.PagedChunkAttention("cpu").plan(b, hq, hkv, d, kv_format=fmt, num_cus=cus, max_splits=splits, window_left=window,
-                                             shared_indptr=np.concatenate([[0], np.cumsum(groups)]), shared_len=prefix)
+                                             shared_indptr=np.concatenate([[0], np.cumsum(groups)]), shared_len=prefix,
+                                             keep_shared=keep)
     return a, b
 
 
@@ -218,9 +220,45 @@ def test_c_entry_refuses_null_groups():
     info = _lib.ChunkPlanInfo()
     ip, n = np.array([0, 2], dtype=np.int32), np.array([3], dtype=np.int32)
     fn = _lib.lib.d2sd_chunk_plan_shared
-    assert fn(C.byref(desc), 1, as_p(ip), as_p(n), None, 0, C.byref(info)) == 0 and info.form & 8
+    assert fn(C.byref(desc), 1, as_p(ip), as_p(n), 1, None, 0, C.byref(info)) == 0 and info.form & 8
     for args in ((1, None, as_p(n)), (1, as_p(ip), None), (-1, as_p(ip), as_p(n))):
-        assert fn(C.byref(desc), *args, None, 0, C.byref(info)) != 0
+        assert fn(C.byref(desc), *args, 1, None, 0, C.byref(info)) != 0
         assert b"chunk_plan" in _lib.lib.d2sd_last_error()
     host = np.empty(8, dtype=np.int32)  # too small: refused before anything is written
-    assert fn(C.byref(desc), 1, as_p(ip), as_p(n), as_p(host), 8, C.byref(info)) == _lib.D2SD_ERR_WORKSPACE
+    assert fn(C.byref(desc), 1, as_p(ip), as_p(n), 1, as_p(host), 8, C.byref(info)) == _lib.D2SD_ERR_WORKSPACE
+
+
+def test_sharing_that_does_not_pay_is_left():
+    """Few shared keys, or many rows: the plan is that of the requests apart, unless it is to be kept."""
+    for qo, prefix, fmt in (([1] * 16, 64, "mxfp8"), ([200] * 16, 512, "bf16"), ([5] * 16, 64, "mxfp4")):
+        kv = [prefix + n + 50 + 9 * i for i, n in enumerate(qo)]
+        kept, b = plan(qo, kv, [16], [prefix], hq=32, hkv=8, fmt=fmt)
+        left, _ = plan(qo, kv, [16], [prefix], hq=32, hkv=8, fmt=fmt, keep=False)
+        apart = d2sd.PagedChunkAttention("cpu").plan(b, 32, 8, 128, kv_format=fmt, num_cus=256)
+        assert kept.info.form & 8 and not left.info.form & 8
+        assert np.array_equal(left.plan_host, apart.plan_host) and left.info.workspace_bytes == apart.info.workspace_bytes
+    for keep in (True, False):  # many conversations behind a document
+        a, b = plan([1] * 32, [8300] * 32, [32], [8192], hq=32, hkv=8, keep=keep)
+        assert a.info.form & 8
+
+
+def test_only_groups_that_gain_share():
+    qo, groups, prefix = [1] * 32 + [200] * 8, [32, 8], [8192, 64]
+    kv = [8192 + 60 + i for i in range(32)] + [64 + 200 + 30 * i for i in range(8)]
+    a, b = plan(qo, kv, groups, prefix, hq=32, hkv=8, keep=False)
+    items = parts(a)[0]
+    assert a.info.form & 8 and (items[items[:, 12] == SHARED][:, 13] == 8192).all()
+    assert set(items[items[:, 0] >= 32][:, 12]) == {ALONE} and set(items[items[:, 0] < 32][:, 12]) == {SHARED, OWN}
+
+
+@pytest.mark.parametrize("qo,kv,groups,prefix", CASES)
+@pytest.mark.parametrize("cus", [8, 256])
+def test_every_row_sees_each_key_once_where_sharing_is_free(qo, kv, groups, prefix, cus):
+    """Whatever is shared in the end: every position once, of the request's own pages or the group's first."""
+    a, b = plan(qo, kv, groups, prefix, cus=cus, keep=False)
+    if a.info.form & 8:
+        shared = {int(i[13]) for i in parts(a)[0] if i[12] == SHARED}
+        check(a, b, qo, kv, groups, [p if p in shared else 0 for p in prefix], 2, 4, 16, -1)
+    else:
+        apart = d2sd.PagedChunkAttention("cpu").plan(b, 8, 2, 128, num_cus=cus)
+        assert np.array_equal(a.plan_host, apart.plan_host)
