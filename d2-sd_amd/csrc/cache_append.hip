@@ -19,7 +19,7 @@
 // through LDS.
 //
 // Bound by HBM: 8192 tokens of 64 + 16 heads of 128 into a bf16 cache, 336 MB, take
-// 83 us, 4.0 TB/s, where a large copy reaches 5.0; 11 x 512 tokens of 64 + 16 heads
+// 81 us, 4.2 TB/s, where a large copy reaches 5.0; 11 x 512 tokens of 64 + 16 heads
 // of 64 into mxfp4, 247 MB with the read back, 54 us.  A decoding step is one
 // launch's latency: a token 5.5 us, 48 tokens of 32 + 16 heads into mxfp8 7 us.
 #include <hip/hip_runtime.h>
@@ -47,8 +47,10 @@ constexpr long long kAppendStreamBytes = 32ll << 20;
 
 __device__ __forceinline__ float bf16_at(const uint16_t* p) { return __uint_as_float((unsigned)*p << 16); }
 
+// bf16 fits eight waves on a SIMD if asked to (8192 tokens 83 -> 80.6 us);
+// the quantising ones would set registers aside (2000 tokens into fp8 16.4 -> 18.4).
 template <int FMT, bool STREAM>
-__global__ __launch_bounds__(64 * kAppendWaves) void cache_append_kernel(const AppendParams p) {
+__global__ __launch_bounds__(64 * kAppendWaves, FMT == CACHE_BF16 ? 8 : 1) void cache_append_kernel(const AppendParams p) {
   __shared__ float2 turns[kAppendWaves][kRotaryMaxPairs];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long long unit = (long long)blockIdx.x * kAppendWaves + wv;
