@@ -249,11 +249,14 @@ struct SharedGroup {
 // and each request's own keys: tile items where it brings more than 32 rows, else
 // units of one wave (a request, kv head and chunk of keys each), which fill
 // workgroups of as many waves.  Chunk lengths are those that end soonest by the times
-// below, all measured: plans for decoding 64 requests behind 16K keys, swept over both
-// lengths, are within 3% of the best.
-constexpr double kSharedItemUs = 6.0, kWaveItemUs = 6.0, kWaveTileUs = 1.3;  // a workgroup's start and end; a 32-key tile of a wave
+// below, all measured.  (A wave's 32-key tile takes 1.3 alone; beside tile items that
+// wait for memory too, 1.7: 96 requests behind 32K mxfp8 keys 186 us planned by 1.3,
+// 160 by 1.7, 168 by 2.  Without what reads and work cost beside each other, chunks
+// come out long where reads bound them: 48 behind 8K in bf16, heads of 64, 43 -> 35.)
+constexpr double kSharedItemUs = 6.0, kWaveItemUs = 6.0, kWaveTileUs = 1.7;  // a workgroup's start and end; a 32-key tile of a wave
+constexpr double kReadBeside = 0.2;      // of reads and work, how much of the shorter is not hidden
 constexpr double kSharedMergeUs = 3.0, kPartialBytes = 2.6e6;  // the merge's launch; partial states written and read, per us
-constexpr double kAgainBytes = 13e6, kWideTokens = 1.5;  // keys that other requests read too, per us; 17 to 32 rows to 16
+constexpr double kAgainBytes = 13e6, kWideTokens = 2.0;  // keys that other requests read too, per us; 17 to 32 rows to 16
 
 struct SharedPlanner {
   const ChunkPlanInput& in;
@@ -264,7 +267,7 @@ struct SharedPlanner {
   double own_bytes, shared_bytes; // of the keys and values
   int most_units, most_own;       // tiles of the longest tile item, of the longest wave's
   struct Alike {                  // groups that a schedule need not tell apart
-    int kind, units;              // units: of three bits, rounded up
+    int kind, units;              // units: of four bits, rounded up
     bool shared, full, partial;
     bool operator<(const Alike& x) const {
       return std::tie(kind, units, shared, full, partial) < std::tie(x.kind, x.units, x.shared, x.full, x.partial);
@@ -304,11 +307,12 @@ struct SharedPlanner {
       if (g.row0 == 0 || !over_shared)
         (over_shared ? shared_bytes : own_bytes) +=
             2.0 * (g.kind == CHUNK_TILE ? 64 : 32) * g.units * row_bytes(in.format, in.head_dim) * in.num_kv_heads;
-      if (g.kind == CHUNK_TILE) most_units = std::max(most_units, g.units);
-      else most_own = std::max(most_own, g.units);
       int fine = 0;
       while (g.units >> fine >= 16) ++fine;
-      Many& m = alike[{g.kind, (g.units + (1 << fine) - 1) >> fine << fine, over_shared, g.nrows * 2 > chunk_rows(form),
+      const int units = (g.units + (1 << fine) - 1) >> fine << fine;
+      int& most = g.kind == CHUNK_TILE ? most_units : most_own;
+      most = std::max(most, units);
+      Many& m = alike[{g.kind, units, over_shared, g.nrows * 2 > chunk_rows(form),
                        rows_list[g.rows].part != PART_ALONE}];
       ++m.count;
       m.rows += g.nrows;
@@ -331,7 +335,7 @@ struct SharedPlanner {
   // below it, not less than that.
   double span(double tile_limit, double own_limit, double enough) const {
     tiles.clear(), solo.clear(), free.clear();
-    double partial = 0.0, work = 0.0, last = kSharedItemUs + (own_bytes + shared_bytes) / kHbmBytes;
+    double partial = 0.0, work = 0.0, last = 0.0;
     const long long heads = in.num_kv_heads, places = (long long)in.num_cus * per_cu;
     long long count = 0;
     for (const auto& x : alike)
@@ -349,7 +353,12 @@ struct SharedPlanner {
       last = std::max(last, us);
     }
     if (partial > 0.0) partial = kSharedMergeUs + partial / kPartialBytes;
-    const double bound = std::max(last, work / places) + partial;
+    const double read = (own_bytes + shared_bytes) / kHbmBytes;
+    auto total = [&](double us) {
+      us -= kSharedItemUs;
+      return kSharedItemUs + std::max(us, read) + kReadBeside * std::min(us, read) + partial;
+    };
+    const double bound = total(std::max(last, work / places));
     if (bound >= enough) return bound;
     std::sort(tiles.begin(), tiles.end(), std::greater<>());
     std::sort(solo.begin(), solo.end(), std::greater<>());
@@ -373,7 +382,7 @@ struct SharedPlanner {
           left -= rounds * k;
           last = std::max(last, end);
         }
-    return last + partial;
+    return total(last);
   }
 
   double plan() {
@@ -381,9 +390,9 @@ struct SharedPlanner {
     tile_limit = wave_limit = 1.0;
     const double longest = std::max(1, most_units);
     // (a coarse search first: the fine one then knows what need not be looked at)
-    for (const auto& step : {std::pair<double, double>{0.6, 0.4}, {0.87, 0.62}})
-      for (double t = longest; t >= 2.0 || t == longest; t *= step.first)
-        for (double o = std::max(4, most_own);; o = std::max(4.0, o * step.second)) {
+    for (const auto& step : {std::pair<double, double>{1.6, 0.4}, {1.08, 0.62}})
+      for (double n = 1.0; n == 1.0 || longest / n >= 2.0; n = std::max(n + 1.0, std::floor(n * step.first)))
+        for (double t = longest / n, o = std::max(4, most_own);; o = std::max(4.0, o * step.second)) {
           const double us = span(t, o, best * 0.995);
           if (us < best * 0.995) best = us, tile_limit = t, wave_limit = o;
           if (o <= 4.0) break;
