@@ -47,16 +47,16 @@
 //  * keys of a request's own, up to 32 rows: a wave each, without a partner or a
 //    barrier, so that a workgroup holds as many requests and heads as waves (token
 //    items, one a workgroup, spent most of their time on their start and joins: 64
-//    requests behind 16K bf16 keys took 65 us, now 42);
+//    requests behind 16K bf16 keys took 65 us, now 43);
 //  * a request's own rows beyond 32: tile items.
 // A plan of so few rows that no tile fills takes the kernels above over all of its
 // parts.  Partial states over shared keys lie as the registers hold them; 20 MB of
 // partial states otherwise cost as many lines a store as rows.  Measured, one token
 // a request, heads of 128: 4 requests behind 2K bf16 keys 12 us, most of it two
-// launches; 32 behind 8K in mxfp8 27; 64 behind 16K in bf16 42.  96 behind 32K in
-// mxfp8 with 64 query heads 183: their products take 79 at a library's rate and
+// launches; 32 behind 8K in mxfp8 26; 64 behind 16K in bf16 43.  96 behind 32K in
+// mxfp8 with 64 query heads 158: their products take 79 at a library's rate and
 // their own keys, 0.32 GB, 65 beside them, but the two share power and memory.  Six
-// chunks of 100..700 tokens behind 8K in mxfp4 253, products 185.
+// chunks of 100..700 tokens behind 8K in mxfp4 257, products 185.
 //
 // Keys outside an item's visible range are never read: their addresses are
 // clamped to the range, so what lies behind a cache's end (or before its

@@ -249,11 +249,13 @@ struct SharedGroup {
 // and each request's own keys: tile items where it brings more than 32 rows, else
 // units of one wave (a request, kv head and chunk of keys each), which fill
 // workgroups of as many waves.  Chunk lengths are those that end soonest by the times
-// below, all measured.  (A wave's 32-key tile takes 1.3 alone; beside tile items that
-// wait for memory too, 1.7: 96 requests behind 32K mxfp8 keys 186 us planned by 1.3,
-// 160 by 1.7, 168 by 2.  Without what reads and work cost beside each other, chunks
+// below, all measured.  (A wave's 32-key tile takes 1.3; one of eight on a CU, which
+// wait for memory beside tile items, 1.7: 96 requests behind 32K mxfp8 keys 186 us
+// planned by 1.3, 158 by 1.7, 168 by 2; 64 behind 16K in bf16, of four waves, 42.8 by
+// 1.3, 44.1 by 1.7.  Without what reads and work cost beside each other, chunks
 // come out long where reads bound them: 48 behind 8K in bf16, heads of 64, 43 -> 35.)
-constexpr double kSharedItemUs = 6.0, kWaveItemUs = 6.0, kWaveTileUs = 1.7;  // a workgroup's start and end; a 32-key tile of a wave
+constexpr double kSharedItemUs = 6.0, kWaveItemUs = 6.0;  // a workgroup's start and end
+constexpr double kWaveTileUs = 1.3, kWaveTile8Us = 1.7;  // a 32-key tile of one of 4 waves, of 8
 constexpr double kReadBeside = 0.2;      // of reads and work, how much of the shorter is not hidden
 constexpr double kSharedMergeUs = 3.0, kPartialBytes = 2.6e6;  // the merge's launch; partial states written and read, per us
 constexpr double kAgainBytes = 13e6, kWideTokens = 2.0;  // keys that other requests read too, per us; 17 to 32 rows to 16
@@ -346,7 +348,7 @@ struct SharedPlanner {
       const int n = chunks_of(g.kind, g.units, tile_limit, own_limit);
       if (n > 1 || g.partial) partial += (double)n * x.second.rows * heads * in.head_dim * 4.0;
       const double us = g.kind == CHUNK_TILE ? kSharedItemUs + (double)g.units / n * step_us(g.shared, alone, g.full)
-                                             : kWaveItemUs + (double)g.units / n * kWaveTileUs * (in.head_dim == 64 ? 0.7 : 1.0);
+                                             : kWaveItemUs + (double)g.units / n * (waves == 8 ? kWaveTile8Us : kWaveTileUs) * (in.head_dim == 64 ? 0.7 : 1.0);
       const long long items = x.second.count * (g.kind == CHUNK_TILE ? n * heads : (n * heads + waves - 1) / waves);
       (g.kind == CHUNK_TILE ? tiles : solo).push_back({us, items});
       work += us * items;
