@@ -6,10 +6,10 @@
 //   y = x / sqrt(mean(x^2) + eps) * w
 //   (a, b) -> s (a cos t - b sin t, b cos t + a sin t),  t = position * f
 //
-// with the pairs, angles and codes of rotary.hip and paged_cache.hip.  Everything
-// between the loads and the stores is 32-bit (angles: 64-bit turns); queries and
-// keys are rounded once, keys straight to the cache's elements.  (Calls of
-// rotary_embedding and cache_write round a key to bf16 between them.)
+// with the pairs and codes of rotary.hip and paged_cache.hip.  Everything between the
+// loads and the stores is 32-bit (angles: 64-bit turns); queries and keys are rounded
+// once, keys straight to the cache's elements.  (Calls of rotary_embedding and
+// cache_write round a key to bf16 between them.)
 //
 // A wave owns one token and a run of its heads, queries, keys and values in this
 // order; a lane holds eight neighbouring head dims of a head and reads the eight
@@ -44,6 +44,20 @@ constexpr int kAppendWaves = 4;
 constexpr int kAppendRows = 2;
 // Queries of more than this are stored past the caches, as rotary_embedding's.
 constexpr long long kAppendStreamBytes = 32ll << 20;
+
+// Scaled cosine and sine of position * frequency.  32 bits hold what is left of the
+// angle behind quarter turns, within 2^-28 of a turn, below what the products round.
+// (Behind whole turns, 2^-26: 1.6 to 1.8 times as many keys round to another value
+// than those of exact angles.)
+__device__ __forceinline__ float2 fine_turn(long long pos, double f, float scale) {
+  const double quarters = (double)pos * f * 0.63661977236758134307553505349;
+  const double n = rint(quarters);
+  float s, c;
+  sincospif(0.5f * (float)(quarters - n), &s, &c);
+  const int k = (int)(n - 4.0 * floor(0.25 * n));
+  const float x = k & 1 ? -s : c, y = k & 1 ? c : s;
+  return k & 2 ? float2{-x * scale, -y * scale} : float2{x * scale, y * scale};
+}
 
 __device__ __forceinline__ float bf16_at(const uint16_t* p) { return __uint_as_float((unsigned)*p << 16); }
 
@@ -98,7 +112,7 @@ __global__ __launch_bounds__(64 * kAppendWaves, FMT == CACHE_BF16 ? 8 : 1) void 
     const long long pos = !p.positions ? (long long)place
                           : p.pos64    ? ((const long long*)p.positions)[t]
                                        : (long long)((const int*)p.positions)[t];
-    for (int i = lane; i < pairs; i += 64) turn[i] = rotary_turn(pos, p.inv_freq[i], p.scale);
+    for (int i = lane; i < pairs; i += 64) turn[i] = fine_turn(pos, p.inv_freq[i], p.scale);
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();

@@ -54,17 +54,6 @@ __device__ __forceinline__ unsigned pack_bf16x2(float a, float b) {
 __device__ __forceinline__ float bf16_lo(unsigned w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
 
-// Cosine and sine of pos * f radians, times scale.  The angle is taken in turns:
-// pos * (f / 2 pi) in 64 bits (off by 2^-53 of the turns made, 1e-9 turns at a
-// million turns), its fraction of a turn in 32.
-__device__ __forceinline__ float2 rotary_turn(long long pos, double f, float scale) {
-  const double turns = (double)pos * f * 0.15915494309189533576888376337251;
-  const float part = (float)(turns - rint(turns));  // [-0.5, 0.5] of a turn
-  float s, c;
-  sincospif(2.f * part, &s, &c);
-  return float2{c * scale, s * scale};
-}
-
 // Element offset, inside one partial slot, of the 8 values (q4 = 2pr and
 // 2pr + 1 of block mt) that lane `lane` of 32-row block `blk` holds: the
 // accumulator register image in 16-byte lane pieces, so that every partial

@@ -51,8 +51,11 @@ __global__ __launch_bounds__(64 * kRotaryWaves) void rotary_kernel(const RotaryP
   const int h0 = run * p.heads_per_run, h1 = min(h0 + p.heads_per_run, p.num_qo_heads + p.num_kv_heads);
   const long long pos = p.pos64 ? ((const long long*)p.positions)[t] : (long long)((const int*)p.positions)[t];
   for (int i = lane; i < p.pairs; i += 64) {
-    const float2 c = rotary_turn(pos, p.inv_freq[i], p.scale);
-    turn[wv][i] = float2{c.x, p.inverse ? -c.y : c.y};
+    const double turns = (double)pos * p.inv_freq[i] * 0.15915494309189533576888376337251;
+    const float f = (float)(turns - rint(turns));  // [-0.5, 0.5] of a turn
+    float s, c;
+    sincospif(2.f * f, &s, &c);
+    turn[wv][i] = float2{c * p.scale, (p.inverse ? -s : s) * p.scale};
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
