@@ -422,3 +422,50 @@ def test_refusals_on_the_device():
         p.attn.run(p.qd[:2], p.cache)
     with pytest.raises(RuntimeError, match="chunk_plan"):
         d2sd.PagedChunkAttention().plan(p.batch, 8, 2, 64, shared_indptr=[0, 2], shared_len=[113])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [-1, 300])
+def test_more_requests_in_a_row_tile_than_lanes(d, fmt, window):
+    """One query head a kv head: a row tile of 128 or 256 rows has more requests than a wave has lanes."""
+    n = 200
+    run_and_check([n], [400], [1 + 2 * (i % 9) for i in range(n)], [1] * n, 2, 2, d, fmt, window=window, num_cus=64)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_scales_off_the_boundaries_of_their_copies(d, fmt):
+    """Block scales whose rows start at odd bytes: shared keys take another way through LDS, to the same result."""
+    p = Problem([3, 40], [500, 300], [70, 5, 2] + [1 + i % 40 for i in range(40)], [60, 5, 2] + [1] * 40, 8, 2, d, fmt)
+    assert p.attn.info.form & 8
+    out, lse = p.run()
+    c = p.cache
+
+    def odd(t):
+        wide = torch.full((*t.shape[:-1], t.shape[-1] + 1), 0xFF, dtype=torch.uint8, device=DEV)
+        wide[..., :-1] = t.view(torch.uint8)
+        return wide[..., :-1]
+
+    moved = d2sd.PagedKVCache(c.k_pool, c.v_pool, fmt, k_scale=odd(c.k_scale), v_scale=odd(c.v_scale), kv_layout=p.layout)
+    got, glse = p.attn.run(p.qd, moved)
+    torch.cuda.synchronize()
+    p.check(out, lse)
+    p.check(got, glse)
+
+
+def test_sharing_that_does_not_pay_gives_the_same_result():
+    """Planned apart, requests read the shared tokens through pages of their own."""
+    new, own = [60] * 8, [60 + 9 * i for i in range(8)]
+    p = Problem([8], [48], own, new, 8, 2, 128, "mxfp8", num_cus=256)
+    pi = p.batch.page_indptr_host
+    for r in range(1, 8):
+        p.batch.page_table[pi[r]:pi[r] + 3] = p.batch.page_table[:3]
+    assert p.attn.info.form & 8
+    a = p.run()
+    p.attn.plan(p.batch, 8, 2, 128, kv_format="mxfp8", shared_indptr=[0, 8], shared_len=[48], num_cus=256)
+    assert not p.attn.info.form & 8
+    b = p.run()
+    torch.cuda.synchronize()
+    p.check(*a)
+    p.check(*b)
