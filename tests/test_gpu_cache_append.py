@@ -169,6 +169,17 @@ def test_append_matches_the_formulas(fmt, layout, P, hq, hkv, d, r, interleaved)
     assert torch.equal(p.dev, before)  # the projection stays as it was
 
 
+@pytest.mark.parametrize("d,r", [(32, 16), (32, 32), (64, 16), (64, 32), (64, 48), (96, 64), (128, 16), (128, 32), (128, 64),
+                                 (128, 80), (160, 128), (256, 128), (256, 48), (256, 256)])
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("norm", ["qk", ""])
+def test_partners_in_any_lane(d, r, fmt, norm):
+    """Dims that are paired 1 to 16 lanes apart, and distances that are no power of two."""
+    p = Problem([2, 33], [9, 61], 5, 3, d, r, fmt, norm=norm)
+    p.check_queries(p.run(q_out=torch.empty(p.T, 5, d, dtype=torch.bfloat16, device=DEV)))
+    p.check_cache()
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
 @pytest.mark.parametrize("norm", ["qk", ""])
 def test_given_positions_and_long_batches(fmt, norm):
