@@ -6,9 +6,10 @@ Drop-in surface of the reference's verify path:
 and the tree-level API
   CascadeVerifyAttention.plan() / .run()
   PagedKVCommit.commit()        (accepted-branch KV append, d3_generator.py:227-232)
-  rotary_embedding(), PagedKVCache.write() / .read(), PagedChunkAttention.plan() / .run()
+  rotary_embedding(), PagedKVCache.write() / .append() / .read(), PagedChunkAttention.plan() / .run()
                                 (a prompt's chunks and decoding steps over a paged,
-                                 optionally quantised cache)
+                                 optionally quantised cache, whose requests may
+                                 share their first keys)
   GreedyAccept() / TreeAccept() (acceptance walk, greedy or sampled, d3_generator.py:204-225)
 All device work runs hand-written HIP kernels in libd2sd.so (C ABI:
 include/d2sd.h); importing raises if the library has not been built.
