@@ -1288,6 +1288,8 @@ int d2sd_cache_append(const d2sd_cache_append_args* a, d2sd_stream_t stream) {
   d2sd::AppendParams p{};
   if (int rc = cache_params(&io, "cache_append", p.c)) return rc;
   if (a->num_qo_heads < 0) return fail(D2SD_ERR_INVALID_ARG, "cache_append: negative count");
+  if ((int64_t)a->num_qo_heads + 2 * (int64_t)a->cache.num_kv_heads > (int64_t)INT32_MAX - 64)
+    return fail(D2SD_ERR_UNSUPPORTED, "cache_append: too many heads");
   if (a->num_pairs < 1 || 2 * (int64_t)a->num_pairs > a->cache.head_dim)
     return fail(D2SD_ERR_INVALID_ARG, "cache_append: 2 * num_pairs must be in [2, head_dim]");
   if (!std::isfinite(a->scale)) return fail(D2SD_ERR_INVALID_ARG, "cache_append: scale must be finite");

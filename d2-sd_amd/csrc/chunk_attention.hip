@@ -1253,9 +1253,10 @@ shared_attn_kernel(const ChunkParams p) {
 
 // Row i of a merge item from its partial states, nchunks of them, then (SHARED)
 // those over the keys that it shares (IMAGE: as store_image left them): thread (i,
-// d4) holds head dims 4 d4 .. 4 d4 + 3; of the images eight rows lie side by side.  Latency bound: the sums and states of eight chunks are read at once (one
-// token over 8 chunks: 3.8 -> 3.0 us against sums first), joined in chunk order
-// whatever the order they were written in.
+// d4) holds head dims 4 d4 .. 4 d4 + 3; of the images eight rows lie side by side.
+// Latency bound: the sums and states of eight chunks are read at once (one token
+// over 8 chunks: 3.8 -> 3.0 us against sums first), joined in chunk order whatever
+// the order they were written in.
 template <int D, bool SHARED, bool IMAGE, typename Merge>
 __device__ __forceinline__ void merge_rows(const ChunkParams& p, const Merge& w) {
   constexpr int ROWS = 1024 / D;

@@ -1,6 +1,7 @@
 // Work planner of the chunk attention (chunk_attention.hip): which workgroup
 // takes which rows and which share of their keys.
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <cstdint>
 #include <functional>
@@ -623,12 +624,30 @@ std::vector<char> sharing(const ChunkPlanInput& in) {
   const double all = batch_us(in, use, 0, in.num_reqs);
   std::vector<char> kept = none;
   if (all < best) best = all, kept = use;
-  if (groups == 1) return kept;
-  std::vector<char> gain = use;
+  // (groups of about the same sizes are looked at once; of very many kinds, none is)
+  std::map<std::array<int, 4>, char> kinds;
+  auto kind_of = [&](int i) {
+    const int a = in.shared_indptr[i], b = in.shared_indptr[i + 1];
+    long long keys = 0;
+    for (int r = a; r < b; ++r) keys += in.kv_len[r];
+    auto about = [](long long x) {
+      int e = 0;
+      while (x >> e >= 8) ++e;
+      return (int)(x >> e << e);
+    };
+    return std::array<int, 4>{about(b - a), about(in.qo_indptr[b] - in.qo_indptr[a]), about(in.shared_len[i]), about(keys / (b - a))};
+  };
   for (int i = 0; i < in.num_groups; ++i)
-    if (use[i])
-      gain[i] = batch_us(in, use, in.shared_indptr[i], in.shared_indptr[i + 1]) <
-                batch_us(in, none, in.shared_indptr[i], in.shared_indptr[i + 1]);
+    if (use[i]) kinds[kind_of(i)] = 2;
+  if (kinds.size() == 1 || kinds.size() > 32) return kept;
+  std::vector<char> gain = use;
+  for (int i = 0; i < in.num_groups; ++i) {
+    if (!use[i]) continue;
+    char& known = kinds[kind_of(i)];
+    const int a = in.shared_indptr[i], b = in.shared_indptr[i + 1];
+    if (known == 2) known = batch_us(in, use, a, b) < batch_us(in, none, a, b);
+    gain[i] = known;
+  }
   if (gain != use && gain != none && batch_us(in, gain, 0, in.num_reqs) < best) kept = gain;
   return kept;
 }

@@ -456,7 +456,9 @@ void cache_append(const c10::optional<at::Tensor>& q, const at::Tensor& k, const
                         "d2sd: q and q_out must be [>= ", num_items, ", Hq, ", d, "] alike with a contiguous head_dim");
       same_device(*t, dev, "q / q_out");
     }
-    TORCH_CHECK_VALUE((q_out->size(0) < 2 || q_out->stride(0) >= d) && (q_out->size(1) < 2 || q_out->stride(1) >= d),
+    // (heads inside a token's, or tokens inside a head's)
+    const int64_t T = q_out->size(0), H = q_out->size(1), st = q_out->stride(0), sh = q_out->stride(1);
+    TORCH_CHECK_VALUE((T < 2 || st >= d) && (H < 2 || sh >= d) && (T < 2 || H < 2 || st >= (H - 1) * sh + d || sh >= (T - 1) * st + d),
                       "d2sd: the rows of q_out must lie apart");
     TORCH_CHECK_VALUE(q->size(1) <= INT32_MAX, "d2sd: too many heads");
     a.q = q->data_ptr();

@@ -52,7 +52,9 @@ EXPORTED_SYMBOLS = (
     "d2sd_rotary_embedding",
     "d2sd_cache_write",
     "d2sd_cache_read",
+    "d2sd_cache_append",
     "d2sd_chunk_plan",
+    "d2sd_chunk_plan_shared",
     "d2sd_chunk_run",
 )
 

@@ -26,7 +26,7 @@ def _args(**kw):
 @pytest.mark.parametrize("bad", [
     dict(items=None), dict(kv_len=None), dict(page_table=None), dict(q=None), dict(q_out=None), dict(k=None), dict(v=None),
     dict(inv_freq=None), dict(q=AT + 8), dict(q_out=AT + 2), dict(k=AT + 4), dict(v=AT + 8), dict(items=AT + 4),
-    dict(q_norm=AT + 2), dict(k_norm=AT + 8), dict(num_tokens=-1), dict(num_qo_heads=-1), dict(num_pairs=0),
+    dict(q_norm=AT + 2), dict(k_norm=AT + 8), dict(num_tokens=-1), dict(num_qo_heads=-1), dict(num_qo_heads=2 ** 31 - 1), dict(num_pairs=0),
     dict(num_pairs=65), dict(num_pairs=1 << 30), dict(num_pairs=-1), dict(scale=float("nan")), dict(scale=float("inf")),
     dict(q_norm=AT, eps=0.0), dict(k_norm=AT, eps=float("inf")), dict(k_norm=AT, eps=-1.0), dict(q_stride_n=4),
     dict(q_stride_h=-8), dict(qo_stride_n=12), dict(k_stride_n=1023), dict(k_stride_h=-128), dict(v_stride_n=2),

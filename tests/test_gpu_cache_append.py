@@ -332,6 +332,7 @@ def test_refusals():
                 lambda: run(q, k, z(2, 3, 64), p.batch, f), lambda: run(z(2, 4, 32), k, v, p.batch, f),
                 lambda: run(q, k, v, p.batch, f, q_out=z(2, 4, 65)), lambda: run(q, k, v, p.batch, f, q_out=z(3, 4, 64)),
                 lambda: run(q, k, v, p.batch, f, q_out=out[:, :1].expand(2, 4, 64)),
+                lambda: run(q, k, v, p.batch, f, q_out=z(8, 64).as_strided((2, 4, 64), (64, 64, 1))),
                 lambda: run(None, k, v, p.batch, f, q_out=out), lambda: run(q, k, v, p.batch, f.cpu()),
                 lambda: run(q, k, v, p.batch, torch.ones(33, dtype=torch.float64, device=DEV)),
                 lambda: run(q, k, v, p.batch, f, torch.zeros(1, dtype=torch.int32, device=DEV)),
