@@ -328,9 +328,9 @@ struct SharedPlanner {
     groups = std::move(other.groups);
   }
 
+  int most() const { return in.max_splits > 0 ? std::min(in.max_splits, kChunkMaxSplits) : kChunkMaxSplits; }
   int chunks_of(int kind, int units, double tiles, double own) const {
-    const int most = in.max_splits > 0 ? std::min(in.max_splits, kChunkMaxSplits) : kChunkMaxSplits;
-    return std::max(1, std::min(most, (int)std::ceil(units / (kind == CHUNK_TILE ? tiles : own) - 1e-6)));
+    return std::max(1, std::min(most(), (int)std::ceil(units / (kind == CHUNK_TILE ? tiles : own) - 1e-6)));
   }
 
   // Time until the last workgroup ends, those of tile items first, the longest before
@@ -394,7 +394,7 @@ struct SharedPlanner {
     const double longest = std::max(1, most_units);
     // (a coarse search first: the fine one then knows what need not be looked at)
     for (const auto& step : {std::pair<double, double>{1.6, 0.4}, {1.08, 0.62}})
-      for (double n = 1.0; n == 1.0 || longest / n >= 2.0; n = std::max(n + 1.0, std::floor(n * step.first)))
+      for (double n = 1.0; n == 1.0 || (n <= most() && longest / n >= 2.0); n = std::max(n + 1.0, std::floor(n * step.first)))
         for (double t = longest / n, o = std::max(4, most_own);; o = std::max(4.0, o * step.second)) {
           const double us = span(t, o, best * 0.995);
           if (us < best * 0.995) best = us, tile_limit = t, wave_limit = o;
