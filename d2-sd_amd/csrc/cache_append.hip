@@ -23,10 +23,10 @@
 // 66 us, 5.1 TB/s, where a large copy reaches 5.0.  (With paired dims read, unpacked
 // and normed again, library sines and each head's page address apart, vector
 // instructions bounded it: 81.)  5 prompts, 11.8K tokens of 64 + 16 heads of 64, into
-// mxfp4 with their read back, 247 MB, 54 us.  2500 tokens of 28 + 8 heads of 128 into fp8, 39
-// MB, 13: a round and a half of the waves that the device holds, each a chain of loads.
-// A decoding step is one launch's latency: a token 4 us (a call 5 to 6), 48 tokens of
-// 32 + 16 heads into mxfp8 5.
+// mxfp4 with their read back, 247 MB, 54 us.  2500 tokens of 28 + 8 heads of 128 into
+// fp8, 39 MB, 13: a round and a half of the waves that the device holds, each a chain
+// of loads.  A decoding step is one launch's latency: a token 4 us (a call 5 to 6), 48
+// tokens of 32 + 16 heads into mxfp8 5.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
