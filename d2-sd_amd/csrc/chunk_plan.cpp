@@ -507,20 +507,24 @@ void plan_shared(const ChunkPlanInput& in, const std::vector<Rows>& rows, const 
     it.heads = heads;
     it.slot = (int)slots[i];
     if (set.part == PART_SHARED) {
-      // The row tile's requests, where a wave's lanes can hold their lengths and their
-      // pages hold all that is shared and the tokens behind it.
+      // The row tile's requests, where a wave's lanes can hold their lengths, their pages
+      // hold all that is shared and the tokens behind it, and their rows see all of it
+      // (under the lengths planned for; others are found out at the end).
       const int t0 = set.q0 + g.row0 / group, t1 = set.q0 + (g.row0 + g.nrows - 1) / group;
       int first = set.req;
       while (in.qo_indptr[first + 1] <= t0) ++first;
       int last = first;
       long long room = 1ll << 40;
+      bool all = true;
       for (; last < set.last_req && in.qo_indptr[last] <= t1; ++last) {
         if (in.qo_indptr[last + 1] == in.qo_indptr[last]) continue;
-        it.back = std::max(it.back, in.qo_indptr[last + 1] - std::max(in.qo_indptr[last], t0));
+        const int back = in.qo_indptr[last + 1] - std::max(in.qo_indptr[last], t0);  // of the request's first row here
+        it.back = std::max(it.back, back);
+        all = all && in.kv_len[last] - back + 1 >= set.bound;
         room = std::min(room, (long long)(in.page_indptr[last + 1] - in.page_indptr[last]) * in.page_size);
       }
       it.nq = first;
-      it.heads = last - first <= 64 && room >= (long long)set.bound + it.back ? last - first : 0;
+      it.heads = all && last - first <= 64 && room >= (long long)set.bound + it.back ? last - first : 0;
     }
     return it;
   };

@@ -335,8 +335,9 @@ struct ChunkItem {                  // one workgroup (64 bytes)
   int bound;                        // keys [0, bound) are shared
   // token items of CHUNK_WAVES8 and CHUNK_WAVES4: a unit for each wave, from unit
   // `kvh` of the nchunks x heads ones on (unit = chunk * heads + kv head).
-  // PART_SHARED tile items: the rows' requests are nq .. nq + heads - 1 and the rows sit
-  // at most `back` tokens before their requests' ends (heads 0: no such promise).
+  // PART_SHARED tile items: the rows' requests are nq .. nq + heads - 1, the rows sit at
+  // most `back` tokens before their requests' ends and see all shared keys under the
+  // lengths planned for (heads 0: no such promise).
   int heads;
   int back;
 };

@@ -469,3 +469,40 @@ def test_sharing_that_does_not_pay_gives_the_same_result():
     torch.cuda.synchronize()
     p.check(*a)
     p.check(*b)
+
+
+def shared_states(p, ws):
+    """Partial states over shared keys of tile items: outputs and sums, in the items' order."""
+    i, d = p.attn.info, p.d
+    items = p.attn.plan_host[:16 * i.num_items].reshape(-1, 16)
+    room = i.workspace_bytes // ((d + 1) * 4)
+    f = ws.view(torch.int32)
+    o, lse = f[:room * d], f[room * d:room * (d + 1)]
+    got = []
+    for it in items[(items[:, 12] == 1) & (items[:, 11] == 0)].tolist():
+        n = -(-it[5] // 32) * 32
+        at = it[10] + it[8] * n
+        got.append((o[at * d:(at + it[5] // 32 * 32) * d].clone(), lse[at:at + it[5]].clone()))
+    return got
+
+
+@pytest.mark.parametrize("fmt,d", [("bf16", 128), ("mxfp8", 128), ("bf16", 64), ("fp8", 64)])
+def test_prompts_of_mixed_lengths_take_shared_keys_once(fmt, d):
+    """New prompts of 1 to 60 tokens behind one system prompt, an idle request among them: the states over the shared
+    keys are those that the same plan gives once every cache has grown far beyond them."""
+    rng = np.random.default_rng(5)
+    new = [int(n) for n in rng.integers(1, 61, 24)]
+    new[7] = 0
+    own = [max(n, 1) for n in new]
+    p = Problem([24], [1500], own, new, 8, 2, d, fmt, extra=64, num_cus=64)
+    ws = p.attn.workspace().fill_(0x7F)
+    out, lse = p.run(workspace=ws)
+    torch.cuda.synchronize()
+    p.check(out, lse)
+    planned = shared_states(p, ws)
+    assert len(planned) > 4
+    p.batch.set_kv_len([n + 60 for n in p.kv])
+    p.run(workspace=ws.fill_(0x7F))
+    torch.cuda.synchronize()
+    for (o, l), (o2, l2) in zip(planned, shared_states(p, ws)):
+        assert torch.equal(o, o2) and torch.equal(l, l2)

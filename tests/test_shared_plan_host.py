@@ -262,3 +262,21 @@ def test_every_row_sees_each_key_once_where_sharing_is_free(qo, kv, groups, pref
     else:
         apart = d2sd.PagedChunkAttention("cpu").plan(b, 8, 2, 128, num_cus=cus)
         assert np.array_equal(a.plan_host, apart.plan_host)
+
+
+def test_planned_lengths_keep_the_promise_of_shared_items():
+    """Items that look at their lengths last: under the planned lengths every row sees all shared keys, so that none is
+    computed again (requests cut back below what is shared among them, prompts of any length in one row tile)."""
+    rng = np.random.default_rng(8)
+    cut = ([1] * 70, [700 + i for i in range(60)] + [100, 690, 3] + [800] * 7, [70], [690])
+    mixed = [int(n) for n in rng.integers(1, 61, 64)]
+    for qo, kv, groups, prefix in (*CASES, cut, (mixed, [2000 + n for n in mixed], [64], [2000])):
+        for hq, hkv, d, fmt in ((8, 2, 128, "bf16"), (8, 1, 64, "fp8"), (20, 1, 128, "mxfp4")):
+            for window in (-1, 77):
+                a, b = plan(qo, kv, groups, prefix, hq, hkv, d, fmt=fmt, window=window, cus=64)
+                if not a.info.form & 8:
+                    continue
+                items, _, tokens = parts(a)
+                for it in items[(items[:, 12] == SHARED) & (items[:, 11] == 0) & (items[:, 14] > 0)]:
+                    t = tokens[it[2] + it[4] // (hq // hkv):it[2] + (it[4] + it[5] - 1) // (hq // hkv) + 1]
+                    assert (np.asarray(kv)[t[:, 0]] - t[:, 1] + 1 >= it[13]).all()
