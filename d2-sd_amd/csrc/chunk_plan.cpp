@@ -113,6 +113,14 @@ struct Planner {
     token_share = other.token_share;
   }
 
+  // Bytes of the partial states.
+  double states() const {
+    double rows = 0.0;
+    for (const Group& g : groups)
+      if (const int n = chunks(g); n > 1 || g.partial) rows += (double)n * g.nrows;
+    return rows * in.num_kv_heads * (in.head_dim + 1) * 4.0;
+  }
+
   int chunks(const Group& g) const {
     const int top = std::max(1, std::min(most, g.units / g.least));
     const double us = g.kind == CHUNK_TOKEN ? limit * token_share : limit;
@@ -326,6 +334,14 @@ struct SharedPlanner {
     form = other.form;
     waves = other.waves;
     groups = std::move(other.groups);
+  }
+
+  // Bytes of the partial states (planned).
+  double states() const {
+    double rows = 0.0;
+    for (const SharedGroup& g : groups)
+      if (g.chunks > 1 || rows_list[g.rows].part != PART_ALONE) rows += (double)g.chunks * g.nrows;
+    return rows * in.num_kv_heads * (in.head_dim + 1) * 4.0;
   }
 
   int most() const { return in.max_splits > 0 ? std::min(in.max_splits, kChunkMaxSplits) : kChunkMaxSplits; }
@@ -582,14 +598,18 @@ bool tokens_only(const ChunkPlanInput& in, const std::vector<Rows>& rows) {
   return true;
 }
 
-// Time of requests [r0, r1) with the keys of these groups shared.
-double batch_us(const ChunkPlanInput& in, const std::vector<char>& use, int r0, int r1) {
+// What requests [r0, r1) cost with the keys of these groups shared.
+struct Cost {
+  double us, states;  // time; bytes of the partial states
+};
+Cost batch_cost(const ChunkPlanInput& in, const std::vector<char>& use, int r0, int r1) {
   std::vector<Rows> rows;
   std::vector<int> shared_rows;
   const bool shared = batch_rows(in, use, r0, r1, rows, shared_rows), few = tokens_only(in, rows);
   if (shared && !few) {
     SharedPlanner pl(in, rows, shared_form(in));
-    return plan_waves(pl);
+    const double us = plan_waves(pl);
+    return {us, pl.states()};
   }
   Planner pl(in, rows, few ? CHUNK_TOKENS : CHUNK_WAVES4);
   if (!shared) {
@@ -605,15 +625,27 @@ double batch_us(const ChunkPlanInput& in, const std::vector<char>& use, int r0, 
     pl.read_rate = 1.0 / (again / keys / kAgainBytes + (1.0 - again / keys) / kHbmBytes);
     pl.wide_tokens = kWideTokens;
   }
-  return plan_waves(pl);
+  const double us = plan_waves(pl);
+  return {us, pl.states()};
 }
 
 // Groups whose keys are read once for all of their rows.  Sharing costs partial states
 // and a launch that joins them, so that it is not worth a few keys, nor many rows that
 // are bound by their products either way: all of the groups share, or those that gain
-// by themselves, or none, whichever ends soonest by the schedules' times.  (Of 135
-// batches of 2 to 64 requests of 1 to 200 tokens behind 64 to 4096 keys, shared they
-// took 0.26 to 2.4 times what they take apart.)
+// by themselves, or none, whichever ends soonest by the schedules' times.
+//
+// What is shared has to gain 1%, and 1% more for each 128 MB that its partial states are
+// larger: the caller holds them.  (330 batches of 2 to 64 requests of 1 to 400 tokens
+// behind 64 to 16384 keys took, shared, 0.28 to 2.5 times what they took apart; all of
+// them 31.2 ms apart, 25.6 shared, 24.5 as chosen and 24.4 by the better of the two.
+// Estimated ratios are off by 14%, to either side: with a margin of 5% the choice took
+// 24.75.  8 prompts of 8192 tokens behind 16384 bf16 keys would gain 1% by the
+// estimate, 6% measured, with 2.2 GB of states: apart; 1024 requests in 128 groups, 1.1
+// GB, 20% and 25%: shared.)
+constexpr double kShareGain = 0.01, kShareGainByte = 0.01 / (128 << 20);
+bool worth_sharing(const Cost& shared, const Cost& apart) {
+  return shared.us < apart.us * (1.0 - kShareGain - kShareGainByte * std::max(0.0, shared.states - apart.states));
+}
 std::vector<char> sharing(const ChunkPlanInput& in) {
   std::vector<char> use(in.num_groups, 0);
   int groups = 0;
@@ -624,10 +656,10 @@ std::vector<char> sharing(const ChunkPlanInput& in) {
   }
   if (groups == 0 || in.keep_shared) return use;
   const std::vector<char> none(in.num_groups, 0);
-  double best = batch_us(in, none, 0, in.num_reqs);
-  const double all = batch_us(in, use, 0, in.num_reqs);
+  const Cost apart = batch_cost(in, none, 0, in.num_reqs), all = batch_cost(in, use, 0, in.num_reqs);
+  double best = apart.us;
   std::vector<char> kept = none;
-  if (all < best) best = all, kept = use;
+  if (worth_sharing(all, apart)) best = all.us, kept = use;
   // (groups of about the same sizes are looked at once; of very many kinds, none is)
   std::map<std::array<int, 4>, char> kinds;
   auto kind_of = [&](int i) {
@@ -649,10 +681,11 @@ std::vector<char> sharing(const ChunkPlanInput& in) {
     if (!use[i]) continue;
     char& known = kinds[kind_of(i)];
     const int a = in.shared_indptr[i], b = in.shared_indptr[i + 1];
-    if (known == 2) known = batch_us(in, use, a, b) < batch_us(in, none, a, b);
+    if (known == 2) known = worth_sharing(batch_cost(in, use, a, b), batch_cost(in, none, a, b));
     gain[i] = known;
   }
-  if (gain != use && gain != none && batch_us(in, gain, 0, in.num_reqs) < best) kept = gain;
+  if (gain != use && gain != none)
+    if (const Cost some = batch_cost(in, gain, 0, in.num_reqs); some.us < best && worth_sharing(some, apart)) kept = gain;
   return kept;
 }
 

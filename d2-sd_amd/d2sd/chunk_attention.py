@@ -61,8 +61,10 @@ class PagedChunkAttention:
         are read once for all of them, through the first one's pages, where
         that is faster by the plan's estimate (joining partial states costs
         time; few shared keys, or many new tokens, do not repay it), else by
-        each request through its own.  keep_shared=True shares them in any
-        case; the others' pages of that range are then never looked at.
+        each request through its own.  The states take workspace too, 8 bytes
+        for each element of the output where nothing is split: they have to
+        gain 1%, and 1% more for each 128 MB.  keep_shared=True shares the keys
+        in any case; the others' pages of that range are then never looked at.
         shared_indptr starts at 0 and ends at the number of requests; a
         group's shared_len is any number that its first request's pages hold.
         The result is that of a plan without groups, whatever lengths the

@@ -280,3 +280,18 @@ def test_planned_lengths_keep_the_promise_of_shared_items():
                 for it in items[(items[:, 12] == SHARED) & (items[:, 11] == 0) & (items[:, 14] > 0)]:
                     t = tokens[it[2] + it[4] // (hq // hkv):it[2] + (it[4] + it[5] - 1) // (hq // hkv) + 1]
                     assert (np.asarray(kv)[t[:, 0]] - t[:, 1] + 1 >= it[13]).all()
+
+
+def test_states_that_weigh_more_than_they_gain_are_left():
+    """Long prompts behind a longer document: a per cent or two by the estimate, for gigabytes of partial states."""
+    for qo, prefix in (([8192] * 8, 16384), ([2048] * 16, 16384)):
+        kv = [prefix + n for n in qo]
+        kept, b = plan(qo, kv, [len(qo)], [prefix], hq=32, hkv=8)
+        left, _ = plan(qo, kv, [len(qo)], [prefix], hq=32, hkv=8, keep=False)
+        apart = d2sd.PagedChunkAttention("cpu").plan(b, 32, 8, 128, num_cus=256)
+        assert kept.info.form & 8 and kept.info.workspace_bytes > 2 ** 30
+        assert not left.info.form & 8 and left.info.workspace_bytes == apart.info.workspace_bytes
+    # as large ones that gain a fifth are taken
+    qo = [200 if i % 7 == 3 else 1 for i in range(1024)]
+    a, _ = plan(qo, [2048 + n + 50 + i % 150 for i, n in enumerate(qo)], [8] * 128, [2048] * 128, hq=32, hkv=8, keep=False)
+    assert a.info.form & 8 and a.info.workspace_bytes > 2 ** 29
