@@ -2,6 +2,7 @@
 it, gives every row each of its keys once, through the right pages, and every
 partial state to one merge; what a plan does not take is refused."""
 import ctypes as C
+import time
 
 import numpy as np
 import pytest
@@ -295,3 +296,40 @@ def test_states_that_weigh_more_than_they_gain_are_left():
     qo = [200 if i % 7 == 3 else 1 for i in range(1024)]
     a, _ = plan(qo, [2048 + n + 50 + i % 150 for i, n in enumerate(qo)], [8] * 128, [2048] * 128, hq=32, hkv=8, keep=False)
     assert a.info.form & 8 and a.info.workspace_bytes > 2 ** 29
+
+
+def test_planning_with_many_groups_costs_a_few_plans():
+    """What to share is found in a few times the time of a plan without groups, whatever the groups; and planned once."""
+    as_p = lambda x: x.ctypes.data_as(C.POINTER(C.c_int32))  # noqa: E731
+    rng = np.random.default_rng(3)
+    took = {0: 0.0, 1: 0.0}
+    for R, G, fmt in ((64, 4, 0), (256, 16, 0), (256, 26, 0), (256, 26, 2), (256, 30, 0)):
+        cuts = np.sort(rng.integers(0, R, G - 1)) if G > 16 else np.arange(1, G) * R // G
+        first = np.concatenate([[0], cuts, [R]]).astype(np.int32)
+        shared = rng.integers(64, 8192, G).astype(np.int32) if G > 16 else np.full(G, 4096, dtype=np.int32)
+        new = np.where(np.arange(R) % 7 == 3, 200, 1)
+        kv = (np.repeat(shared, np.diff(first)) + new + rng.integers(50, 4000, R)).astype(np.int32)
+        qo = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        pi = np.concatenate([[0], np.cumsum(-(-kv // 16))]).astype(np.int32)
+        desc, info = _lib.ChunkPlanDesc(), _lib.ChunkPlanInfo()
+        desc.num_reqs, desc.num_qo_heads, desc.num_kv_heads, desc.head_dim, desc.page_size = R, 32, 8, 128, 16
+        desc.qo_indptr, desc.kv_len, desc.page_indptr = as_p(qo), as_p(kv), as_p(pi)
+        desc.format, desc.window_left, desc.num_cus = fmt, -1, 256
+        for groups in took:
+            best = 1e9
+            for _ in range(7):
+                t = time.perf_counter()
+                assert _lib.lib.d2sd_chunk_plan_shared(C.byref(desc), G * groups, as_p(first), as_p(shared), 0, None, 0,
+                                                       C.byref(info)) == 0
+                best = min(best, time.perf_counter() - t)
+            took[groups] += best
+    assert took[1] < 9 * took[0], took
+
+
+def test_plans_of_some_thousand_rows_are_made_once(monkeypatch):
+    calls = []
+    fn = _lib.lib.d2sd_chunk_plan_shared
+    monkeypatch.setattr(_lib.lib, "d2sd_chunk_plan_shared", lambda *a: calls.append(1) or fn(*a))
+    qo = [200 if i % 7 == 3 else 1 for i in range(64)]
+    a, _ = plan(qo, [4096 + n + 60 * i for i, n in enumerate(qo)], [16] * 4, [4096] * 4, hq=32, hkv=8)
+    assert a.info.plan_ints > 2 ** 16 and len(calls) == 1
