@@ -1254,6 +1254,47 @@ int cache_params(const d2sd_cache_io_args* a, const char* who, d2sd::CacheParams
   return D2SD_OK;
 }
 
+// Rows of `width` elements: n tokens of h heads, strides not negative.
+struct RowSet {
+  int64_t at, n, h, sn, sh;  // element addresses
+  int64_t end(int64_t width) const { return at + (n - 1) * sn + (h - 1) * sh + width; }
+};
+
+// Heads inside a token's, or tokens inside a head's: no two rows meet.
+bool rows_apart(const RowSet& x, int64_t width) {
+  if ((x.n > 1 && x.sn < width) || (x.h > 1 && x.sh < width)) return false;
+  return x.n < 2 || x.h < 2 || x.sn >= (x.h - 1) * x.sh + width || x.sh >= (x.n - 1) * x.sn + width;
+}
+
+// Whether a row of y meets one of x, whose rows are apart.
+bool rows_meet(const RowSet& x, const RowSet& y, int64_t width) {
+  if (x.n <= 0 || x.h <= 0 || y.n <= 0 || y.h <= 0 || x.end(width) <= y.at || y.end(width) <= x.at) return false;
+  const bool by_token = x.n < 2 || x.h < 2 ? x.h < 2 || x.sn >= x.sh : x.sn > x.sh;  // heads inside a token's
+  const int64_t so = by_token ? x.sn : x.sh, no = by_token ? x.n : x.h, si = by_token ? x.sh : x.sn, ni = by_token ? x.h : x.n;
+  auto below = [](int64_t v, int64_t step) { return v >= 0 ? v / step : -((step - 1 - v) / step); };
+  // the inner rows of outer one i against the row that lies `off` behind x's first
+  auto inner = [&](int64_t off) {
+    const int64_t j = ni > 1 ? std::clamp<int64_t>(below(off, si), 0, ni - 1) : 0;
+    return std::abs(off - j * si) < width || (j + 1 < ni && std::abs(off - (j + 1) * si) < width);
+  };
+  if (by_token && x.n == y.n && x.n > 1 && x.sn == y.sn) {
+    // parts of one buffer: a head of y against x's tokens at one distance (or the next) from its own
+    for (int64_t g = 0; g < y.h; ++g) {
+      const int64_t off = y.at + g * y.sh - x.at, m = below(off, so);
+      for (int64_t i = m; i <= m + 1; ++i)
+        if (std::abs(i) < x.n && inner(off - i * so)) return true;
+    }
+    return false;
+  }
+  for (int64_t t = 0; t < y.n; ++t)
+    for (int64_t g = 0; g < y.h; ++g) {
+      const int64_t off = y.at + t * y.sn + g * y.sh - x.at, m = no > 1 ? below(off, so) : 0;
+      for (int64_t i = m; i <= m + 1; ++i)
+        if (i >= 0 && i < no && inner(off - i * so)) return true;
+    }
+  return false;
+}
+
 }  // namespace
 
 int d2sd_cache_write(const d2sd_cache_io_args* a, d2sd_stream_t stream) {
@@ -1304,6 +1345,19 @@ int d2sd_cache_append(const d2sd_cache_append_args* a, d2sd_stream_t stream) {
     if (!stride_ok(st) || st < 0) return fail(D2SD_ERR_INVALID_ARG, "cache_append: strides must be multiples of 8 elements");
   if (a->num_qo_heads > 0 && a->q == a->q_out && (a->q_stride_n != a->qo_stride_n || a->q_stride_h != a->qo_stride_h))
     return fail(D2SD_ERR_INVALID_ARG, "cache_append: in place needs the same strides");
+  if (a->num_qo_heads > 0) {
+    // (waves write queries while others still read)
+    const int64_t T = a->num_tokens, H = a->num_qo_heads, K = a->cache.num_kv_heads, width = a->cache.head_dim;
+    auto rows = [&](const void* at, int64_t heads, int64_t sn, int64_t sh) -> RowSet {
+      return {(int64_t)((uintptr_t)at / 2), T, heads, sn, sh};
+    };
+    const RowSet out = rows(a->q_out, H, a->qo_stride_n, a->qo_stride_h);
+    if (!rows_apart(out, width)) return fail(D2SD_ERR_INVALID_ARG, "cache_append: the rows of q_out must lie apart");
+    if ((a->q != a->q_out && rows_meet(out, rows(a->q, H, a->q_stride_n, a->q_stride_h), width)) ||
+        rows_meet(out, rows(a->k, K, a->k_stride_n, a->k_stride_h), width) ||
+        rows_meet(out, rows(a->v, K, a->v_stride_n, a->v_stride_h), width))
+      return fail(D2SD_ERR_INVALID_ARG, "cache_append: q_out must lie apart from k, v and q (or be q)");
+  }
   p.v_stride_n = a->v_stride_n;
   p.v_stride_h = a->v_stride_h;
   p.q = a->q;

@@ -267,9 +267,10 @@ class PagedKVCache:
 
         Everything is computed in 32 bits and rounded once, keys straight to the
         cache's elements (rotary_embedding and write() round them to bf16 in
-        between).  The rotated queries go to q_out (as large as q, its rows
-        apart), or back into q; k and v stay as they are.  Returns q_out.  Rows
-        behind the last request's are left alone."""
+        between).  The rotated queries go to q_out (as large as q; its rows
+        apart from each other and from those of q, k and v, or refused), or
+        back into q; k and v stay as they are.  Returns q_out.  Rows behind the
+        last request's are left alone."""
         self._check_batch(batch)
         if q_out is None:
             q_out = q

@@ -629,7 +629,9 @@ int d2sd_cache_read(const d2sd_cache_io_args* args, d2sd_stream_t stream);
  *   pairs, angles and scale as d2sd_rotary_embedding
  * in 32 bits, rounded once: queries to bf16, keys to the cache's elements.
  * Without positions a token's position is its place in its cache.  Rows: 16-byte
- * boundaries.  q_out may be q with the same strides, or lie apart. */
+ * boundaries.  q_out may be q with the same strides; else its rows lie apart from those
+ * of q, and always from those of k and v and from each other (heads inside a token's, or
+ * tokens inside a head's); other calls are refused. */
 typedef struct {
   d2sd_paged_cache cache;
   const d2sd_cache_token* items; /* device [num_tokens]; token i is row i of q, k and v */

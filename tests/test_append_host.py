@@ -77,3 +77,68 @@ def test_traced_by_meta_tensors():
     torch.ops.d2sd.cache_append(m(1, 32, 128), m(1, 8, 128), m(1, 8, 128), i, 1, i, i, pool, pool, None, None, 0, False,
                                 m(64, dt=torch.float64), None, None, None, 1e-6, 1.0, False, m(1, 32, 128))
     assert "append" in dir(d2sd.PagedKVCache)
+
+
+def _rows(base, tokens, heads, sn, sh, d):
+    return {base + t * sn + h * sh + i for t in range(tokens) for h in range(heads) for i in range(d)}
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="calls that are not refused would be launched, over no memory")
+def test_outputs_that_overlap_an_input_are_refused():
+    """q_out over a part of k, v or another place of q: refused; views of one buffer whose rows lie apart: not."""
+    import random
+    rng = random.Random(0)
+    d, seen = 32, {True: 0, False: 0}
+    for n in range(1500):
+        T, hq, hkv = rng.randint(1, 5), rng.randint(1, 4), rng.randint(1, 3)
+        style = rng.randrange(4)
+        width = (hq + 2 * hkv) * d + 8 * rng.randrange(3)
+        view = {  # token and head stride, start: of heads inside a token's row, or tokens inside a head's
+            0: lambda first: (width, d, first * d),
+            1: lambda first: (d, T * d, first * T * d),
+            2: lambda first: (width, d, first * d + 8 * rng.randint(-2, 2)),
+            3: lambda first: (8 * rng.randint(0, 40), 8 * rng.randint(0, 40), 8 * rng.randint(0, 200)),
+        }[style]
+        q, k, v = view(0), view(hq), view(hq + hkv)
+        out = rng.choice([q, q, view(0), view(rng.randint(0, hq + 2 * hkv)), (hq * d, d, 20000), (hq * d, d, 8 * rng.randint(0, 300))])
+        if out is q or out == q:
+            q = out
+        lo = min(x[2] for x in (q, k, v, out))
+        q, k, v, out = ((sn, sh, at - lo) for sn, sh, at in (q, k, v, out))
+        sets = {x: _rows(x[2], T, h, x[0], x[1], d) for x, h in ((k, hkv), (v, hkv), (q, hq))}
+        mine = _rows(out[2], T, hq, out[0], out[1], d)
+        apart = len(mine) == T * hq * d
+        nested = (T < 2 or out[0] >= d) and (hq < 2 or out[1] >= d) and \
+            (T < 2 or hq < 2 or out[0] >= (hq - 1) * out[1] + d or out[1] >= (T - 1) * out[0] + d)
+        if apart and not nested:
+            continue  # (rows of other orders are refused too)
+        bad = not apart or bool(mine & sets[k]) or bool(mine & sets[v]) or (out != q and bool(mine & sets[q]))
+        base = 1 << 30
+        a = _args(num_tokens=T, num_qo_heads=hq, num_pairs=16, cache=_cache(AT, head_dim=d, num_kv_heads=hkv), q=base + 2 * q[2],
+                  k=base + 2 * k[2], v=base + 2 * v[2], q_out=base + 2 * out[2], q_stride_n=q[0], q_stride_h=q[1],
+                  qo_stride_n=out[0], qo_stride_h=out[1], k_stride_n=k[0], k_stride_h=k[1], v_stride_n=v[0], v_stride_h=v[1])
+        assert _lib.lib.d2sd_cache_append(C.byref(a), None) != 0  # (no device: nothing is launched)
+        said = _lib.lib.d2sd_last_error()
+        if b"same strides" in said:
+            continue
+        assert (b"lie apart" in said) == bad, (n, style, T, hq, hkv, q, k, v, out, said)
+        seen[bad] += 1
+    assert min(seen.values()) > 200, seen
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="calls that are not refused would be launched, over no memory")
+def test_the_fused_projection_in_place_is_taken():
+    """A long prompt's queries rotated inside the projection that holds keys and values too: heads of all three side by side,
+    and the three behind each other."""
+    T, hq, hkv, d = 1 << 20, 64, 8, 128
+    base, row = 1 << 40, (hq + 2 * hkv) * d
+    one = dict(q=base, q_out=base, k=base + 2 * hq * d, v=base + 2 * (hq + hkv) * d, q_stride_n=row, qo_stride_n=row,
+               k_stride_n=row, v_stride_n=row)
+    three = dict(q=base, q_out=base, k=base + 2 * T * hq * d, v=base + 2 * T * (hq + hkv) * d, q_stride_n=hq * d, qo_stride_n=hq * d,
+                 k_stride_n=hkv * d, v_stride_n=hkv * d)
+    for kw in (one, three):
+        a = _args(num_tokens=T, num_qo_heads=hq, cache=_cache(AT, num_kv_heads=hkv), **kw)
+        assert _lib.lib.d2sd_cache_append(C.byref(a), None) != 0 and b"launch" in _lib.lib.d2sd_last_error()
+        for wrong in (dict(q_out=base + 16), dict(k=base + 2 * d * (hq - 1)), dict(v=base + 2 * (hq * d - 8))):
+            a = _args(num_tokens=T, num_qo_heads=hq, cache=_cache(AT, num_kv_heads=hkv), **{**kw, **wrong})
+            assert _lib.lib.d2sd_cache_append(C.byref(a), None) != 0 and b"lie apart" in _lib.lib.d2sd_last_error(), wrong

@@ -351,3 +351,23 @@ def test_refusals():
         run(q, k, v, d2sd.PagedBatch([0, 2], [5], [0, 1], [0], 32, device=DEV), f)
     torch.cuda.synchronize()
     assert bool((p.cache.k_pool.view(torch.uint8) == 0xA5).all())
+
+
+def test_queries_over_other_inputs_are_refused():
+    p = Problem([3, 2], [30, 9], 4, 4, 64, 64)
+    q, k, v = p.parts(p.dev)
+    hold = torch.zeros(p.T + 1, 12, 64, dtype=torch.bfloat16, device=DEV)
+    hold[:p.T] = p.dev
+    before = p.dev.clone()
+    for bad in (lambda: p.cache.append(q, k, v, p.batch, p.fd, q_out=k), lambda: p.cache.append(q, k, v, p.batch, p.fd, q_out=v),
+                lambda: p.cache.append(q, k, v, p.batch, p.fd, q_out=p.dev[:, 1:5]),
+                lambda: p.cache.append(hold[:-1, :4], hold[:-1, 4:8], hold[:-1, 8:], p.batch, p.fd, q_out=hold[1:, :4])):
+        with pytest.raises(RuntimeError, match="cache_append: .*lie apart"):
+            bad()
+    torch.cuda.synchronize()
+    assert torch.equal(p.dev, before) and bool((p.cache.k_pool.view(torch.uint8) == 0xA5).all())
+    # parts of one buffer that do lie apart
+    out = p.cache.append(hold[:-1, :4], hold[:-1, 4:8], hold[:-1, 8:], p.batch, p.fd, scale=p.s, q_norm=p.norms[0],
+                         k_norm=p.norms[1], q_out=hold[:-1, :4])
+    p.check_queries(out)
+    p.check_cache()
