@@ -1410,6 +1410,7 @@ int d2sd_chunk_plan_shared(const d2sd_chunk_plan_desc* d, int num_groups, const 
     if (d->num_reqs > 0 && (d->qo_indptr[0] != 0 || d->page_indptr[0] < 0))
       return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: qo_indptr starts at 0, page_indptr at 0 or above");
     int64_t room = 0, most_new = 0;  // tokens that a request's pages hold, that it brings: the largest
+    int64_t row_tiles = 0;           // at least, of each kv head
     for (int r = 0; r < d->num_reqs; ++r) {
       const int64_t n = (int64_t)d->qo_indptr[r + 1] - d->qo_indptr[r];
       const int64_t pages = (int64_t)d->page_indptr[r + 1] - d->page_indptr[r];
@@ -1421,7 +1422,12 @@ int d2sd_chunk_plan_shared(const d2sd_chunk_plan_desc* d, int num_groups, const 
         return fail(D2SD_ERR_UNSUPPORTED, "chunk_plan: request " + std::to_string(r) + " is too long");
       room = std::max(room, pages << lg);
       most_new = std::max(most_new, n);
+      row_tiles += (n * group + d2sd::chunk_rows(d2sd::CHUNK_WAVES8) - 1) / d2sd::chunk_rows(d2sd::CHUNK_WAVES8);
     }
+    // (an item for each, or a wave of one: before any of them takes memory)
+    const int64_t item_ints = sizeof(d2sd::ChunkItem) / 4 / (num_groups > 0 ? 8 : 1);
+    if (row_tiles > (int64_t)INT32_MAX / item_ints / d->num_kv_heads)
+      return fail(D2SD_ERR_UNSUPPORTED, "chunk_plan: the batch is too large for one plan");
     if (num_groups < 0) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: negative num_groups");
     if (num_groups > 0) {
       if (!shared_indptr || !shared_len) return fail(D2SD_ERR_INVALID_ARG, "chunk_plan: null pointer");

@@ -100,7 +100,8 @@ class PagedChunkAttention:
                 raise ValueError("shared_indptr must hold every request")
         info = _lib.ChunkPlanInfo()
         # (too small a buffer means planning twice: merges of 12 ints for 1024 elements of the output, and items)
-        host = np.empty((1 << 18) + 2 * 12 * (batch.total_q * max(num_qo_heads, 0) * max(head_dim, 0) >> 10), dtype=np.int32)
+        merges = 24 * (batch.total_q * max(num_qo_heads, 0) * max(head_dim, 0) >> 10)
+        host = np.empty((1 << 18) + min(merges, 1 << 24), dtype=np.int32)
         plan = lambda: lib.d2sd_chunk_plan_shared(C.byref(desc), groups, indptr, shared, bool(keep_shared), as_p(host),  # noqa: E731
                                                   host.size, C.byref(info))
         with torch.cuda.device(batch.device) if batch.device.type == "cuda" else torch.no_grad():

@@ -333,3 +333,10 @@ def test_plans_of_some_thousand_rows_are_made_once(monkeypatch):
     qo = [200 if i % 7 == 3 else 1 for i in range(64)]
     a, _ = plan(qo, [4096 + n + 60 * i for i, n in enumerate(qo)], [16] * 4, [4096] * 4, hq=32, hkv=8)
     assert a.info.plan_ints > 2 ** 16 and len(calls) == 1
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(2 ** 31 - 1, 1, 128), (2 ** 31 - 2, 2 ** 30 - 1, 128), (8, 2, 2 ** 30), (-8, 2, 128), (8, 2, -64)])
+def test_absurd_heads_are_refused_before_they_cost_memory(hq, hkv, d):
+    with pytest.raises(RuntimeError, match="chunk_plan"):
+        b = d2sd.PagedBatch([0, 40000, 80000], [40000, 40000], [0, 2500, 5000], np.zeros(5000), 16, device="cpu")
+        d2sd.PagedChunkAttention("cpu").plan(b, hq, hkv, d, num_cus=256, sm_scale=1.0, shared_indptr=[0, 2], shared_len=[16])
