@@ -111,7 +111,8 @@ class PagedChunkAttention:
                 rc = plan()
         check(rc, "chunk_plan")
         self.info, self.batch, self.sinks = info, batch, sinks
-        self.plan_host = host[:info.plan_ints]
+        # (a small plan does not hold the whole buffer)
+        self.plan_host = host[:info.plan_ints] if 2 * info.plan_ints > host.size else host[:info.plan_ints].copy()
         self.plan_dev = torch.from_numpy(self.plan_host).to(batch.device)
         self._home = home_stream(batch.device)
         self.kv_format, self.sm_scale, self.lse_base2 = kv_format, scale, bool(lse_base2)

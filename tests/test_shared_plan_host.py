@@ -340,3 +340,9 @@ def test_absurd_heads_are_refused_before_they_cost_memory(hq, hkv, d):
     with pytest.raises(RuntimeError, match="chunk_plan"):
         b = d2sd.PagedBatch([0, 40000, 80000], [40000, 40000], [0, 2500, 5000], np.zeros(5000), 16, device="cpu")
         d2sd.PagedChunkAttention("cpu").plan(b, hq, hkv, d, num_cus=256, sm_scale=1.0, shared_indptr=[0, 2], shared_len=[16])
+
+
+def test_a_plan_holds_no_more_host_memory_than_it_takes():
+    a, _ = plan([1, 1], [70, 90], [2], [64])
+    held = a.plan_host if a.plan_host.base is None else a.plan_host.base
+    assert held.size <= 2 * max(a.info.plan_ints, 1)
