@@ -180,6 +180,17 @@ __device__ __forceinline__ Span rows_span(const ChunkParams& p, const ChunkItem&
   return s;
 }
 
+// Keys [0, this) are visible to every row of the item, which is one of shared keys
+// without a window.  (Arguments and item are read again: nothing need be kept for here
+// over the tile loop.)
+__device__ __forceinline__ int seen_by_all_rows() {
+  auto at = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
+  __asm__ volatile("" : "+s"(at));
+  const ChunkParams& p = *(const ChunkParams*)at;
+  const ChunkItem w = p.items[blockIdx.x];
+  return rows_span<true>(p, w, 0, w.nrows - 1).all_hi;
+}
+
 // Keys that a row at `pos` sees: first and last of the item's.
 template <bool SHARED>
 __device__ __forceinline__ int row_first(const ChunkParams& p, const ChunkItem& w, int pos) {
@@ -1199,7 +1210,8 @@ __device__ __forceinline__ void chunk_work(const ChunkParams& p) {
           chunk_of(0, w.bound, from, to);
           if (from < to) {
             shared_tile<D, FMT, W>(p, w, (lds_char*)lds, from, to);
-            if (!__any(len < to + w.back - 1) || to <= rows_span<true>(p, w, 0, w.nrows - 1).all_hi) return;
+            if (!__any(len < to + w.back - 1)) return;
+            if (to <= seen_by_all_rows()) return;
             __syncthreads();  // (the tiles: all waves are done with them)
           }
         } else {
