@@ -264,7 +264,9 @@ struct SharedGroup {
 // below, all measured.  (A wave's 32-key tile takes 1.3; one of eight on a CU, which
 // wait for memory beside tile items, 1.7: 96 requests behind 32K mxfp8 keys 186 us
 // planned by 1.3, 158 by 1.7, 168 by 2; 64 behind 16K in bf16, of four waves, 42.8 by
-// 1.3, 44.1 by 1.7.  Without what reads and work cost beside each other, chunks
+// 1.3, 44.1 by 1.7.  By themselves, from 24 to 144 workgroups at 0.2 to 5 TB/s: 1.1 to 1.7
+// of four waves in bf16, 1.2 to 1.8 of eight in mxfp4 and mxfp8; heads of 64 0.6 to 1.1
+// in bf16, 0.6 to 0.9 quantised, taken as 0.7 of those of 128.  Without what reads and work cost beside each other, chunks
 // come out long where reads bound them: 48 behind 8K in bf16, heads of 64, 43 -> 35.)
 constexpr double kSharedItemUs = 6.0, kWaveItemUs = 6.0;  // a workgroup's start and end
 constexpr double kWaveTileUs = 1.3, kWaveTile8Us = 1.7;  // a 32-key tile of one of 4 waves, of 8
@@ -665,10 +667,10 @@ Cost batch_cost(const ChunkPlanInput& in, const std::vector<char>& use, int r0, 
 //
 // What is shared has to gain 1%, and 1% more for each 128 MB that its partial states are
 // larger: the caller holds them.  (330 batches of 2 to 64 requests of 1 to 400 tokens
-// behind 64 to 16384 keys took, shared, 0.28 to 2.5 times what they took apart; all of
-// them 31.2 ms apart, 25.6 shared, 24.5 as chosen and 24.4 by the better of the two.
+// behind 64 to 16384 keys took, shared, 0.26 to 2.5 times what they took apart; all of
+// them 31.5 ms apart, 25.8 shared, 24.73 as chosen and 24.64 by the better of the two.
 // Estimated ratios are off by 14%, to either side: with a margin of 5% the choice took
-// 24.75.  8 prompts of 8192 tokens behind 16384 bf16 keys would gain 1% by the
+// 24.96.  8 prompts of 8192 tokens behind 16384 bf16 keys would gain 1% by the
 // estimate, 6% measured, with 2.2 GB of states: apart; 1024 requests in 128 groups, 1.1
 // GB, 20% and 25%: shared.)
 constexpr double kShareGain = 0.01, kShareGainByte = 0.01 / (128 << 20);
