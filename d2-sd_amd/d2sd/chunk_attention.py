@@ -68,7 +68,9 @@ class PagedChunkAttention:
         shared_indptr starts at 0 and ends at the number of requests; a
         group's shared_len is any number that its first request's pages hold.
         The result is that of a plan without groups, whatever lengths the
-        caches have later."""
+        caches have later, as long as the first request's pages keep the shared
+        tokens (also where it is cut back below them: plan again before other
+        tokens are written there)."""
         if kv_format not in KV_FORMATS:
             raise ValueError(f"kv_format must be one of {sorted(KV_FORMATS)}")
         if self._want_device is not None and _device(self._want_device) != batch.device:

@@ -711,7 +711,7 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* desc, int32_t* host_plan, size_t
  * of these are read through the first request's pages, once for the rows of the
  * whole group; what a row sees, and the result, are those of d2sd_chunk_plan where
  * the tokens are indeed the same.  Lengths stay free: a request may be cut back
- * below what it shares.  Where the joining of partial states would cost more than
+ * below what it shares (the first one too, while its pages keep the shared tokens).  Where the joining of partial states would cost more than
  * that saves (few shared keys, or many rows), or saves less than 1% and 1% more for each
  * 128 MB of workspace that they take, requests are planned apart and read through pages
  * of their own, unless keep_shared != 0: then the others' pages of the shared range are
