@@ -264,10 +264,11 @@ struct SharedGroup {
 // below, all measured.  (A wave's 32-key tile takes 1.3; one of eight on a CU, which
 // wait for memory beside tile items, 1.7: 96 requests behind 32K mxfp8 keys 186 us
 // planned by 1.3, 158 by 1.7, 168 by 2; 64 behind 16K in bf16, of four waves, 42.8 by
-// 1.3, 44.1 by 1.7.  By themselves, from 24 to 144 workgroups at 0.2 to 5 TB/s: 1.1 to 1.7
+// 1.3, 44.1 by 1.7.  By themselves, in 24 to 144 workgroups at 0.2 to 5 TB/s: 1.1 to 1.7
 // of four waves in bf16, 1.2 to 1.8 of eight in mxfp4 and mxfp8; heads of 64 0.6 to 1.1
-// in bf16, 0.6 to 0.9 quantised, taken as 0.7 of those of 128.  Without what reads and work cost beside each other, chunks
-// come out long where reads bound them: 48 behind 8K in bf16, heads of 64, 43 -> 35.)
+// in bf16, 0.6 to 0.9 quantised, taken as 0.7 of those of 128.  Without what reads and
+// work cost beside each other, chunks come out long where reads bound them: 48 behind 8K
+// in bf16, heads of 64, 43 -> 35.)
 constexpr double kSharedItemUs = 6.0, kWaveItemUs = 6.0;  // a workgroup's start and end
 constexpr double kWaveTileUs = 1.3, kWaveTile8Us = 1.7;  // a 32-key tile of one of 4 waves, of 8
 constexpr double kReadBeside = 0.2;      // of reads and work, how much of the shorter is not hidden
@@ -496,7 +497,8 @@ void plan_shared(const ChunkPlanInput& in, const std::vector<Rows>& rows, const 
   std::vector<int> first_group(rows.size(), -1);
   size_t merges = 0;  // (some more where a merge would cross the border of two row tiles)
   for (const SharedGroup& g : pl.groups)
-    if (const int part = rows[g.rows].part; part == PART_OWN || (part == PART_ALONE && g.chunks > 1)) merges += (size_t)(g.nrows / merge_rows + 2) * heads;
+    if (const int part = rows[g.rows].part; part == PART_OWN || (part == PART_ALONE && g.chunks > 1))
+      merges += (size_t)(g.nrows / merge_rows + 2) * heads;
   out.shared_merges.reserve(merges);
   for (int i = 0; i < (int)pl.groups.size(); ++i) {
     const SharedGroup& g = pl.groups[i];

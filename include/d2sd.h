@@ -711,11 +711,12 @@ int d2sd_chunk_plan(const d2sd_chunk_plan_desc* desc, int32_t* host_plan, size_t
  * of these are read through the first request's pages, once for the rows of the
  * whole group; what a row sees, and the result, are those of d2sd_chunk_plan where
  * the tokens are indeed the same.  Lengths stay free: a request may be cut back
- * below what it shares (the first one too, while its pages keep the shared tokens).  Where the joining of partial states would cost more than
- * that saves (few shared keys, or many rows), or saves less than 1% and 1% more for each
- * 128 MB of workspace that they take, requests are planned apart and read through pages
- * of their own, unless keep_shared != 0: then the others' pages of the shared range are
- * never looked at. */
+ * below what it shares (the first one too, while its pages keep the shared tokens).
+ * Where the joining of partial states would cost more than that saves (few shared
+ * keys, or many rows), or saves less than 1% and 1% more for each 128 MB of workspace
+ * that they take, requests are planned apart and read through pages of their own,
+ * unless keep_shared != 0: then the others' pages of the shared range are never
+ * looked at. */
 int d2sd_chunk_plan_shared(const d2sd_chunk_plan_desc* desc, int num_groups, const int32_t* shared_indptr,
                            const int32_t* shared_len, int keep_shared, int32_t* host_plan, size_t host_plan_ints,
                            d2sd_chunk_plan_info* info);
