@@ -113,7 +113,7 @@ __device__ __forceinline__ void shared_tile(const ChunkParams& p, const ChunkIte
   // slot word_slot(w) on, counted from region 2's first; sums are in 32 bits, before
   // the probabilities are rounded to bf16 as the second product's operands (V is bf16 at
   // most, its product with 32-bit ones would take two MFMAs for one; outputs are 0.0020
-  // to 0.0023 from 64-bit ones in the mean, 0.0017 of it their own rounding).
+  // to 0.0024 from 64-bit ones in the mean, 0.0017 of it their own rounding).
   constexpr auto word_slot = [](int i) { return KS == 8 ? 3 * i / 2 : 2 * i / 3; };
   static_assert(word_slot(3) + 1 < KS && word_slot(7) + 1 < KS + MT, "words ready before their PV");
   auto words = [&](auto tc, f32x16& s) {
